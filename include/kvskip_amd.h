@@ -389,6 +389,97 @@ int kvskip_pv_select(const kvskip_attn_args* a, const kvskip_select_args* s, voi
 int kvskip_block_list(const uint8_t* keep, int32_t B, int32_t Hkv, int32_t nb, int32_t* block_idx,
                       int32_t* block_cnt, void* stream);
 
+/* ---- Caches held in 8 bits, and pages built on the device (none of it in the reference).
+ *
+ * A cache's type: e4m3 (1 sign, 4 exponent, 3 fraction bits, no infinities), int8, or bf16. In 8 bits each 64-token
+ * block (page) of a KV head has an fp32 scale for its keys and one for its values; a code stands for code * scale. */
+#define KVSKIP_E4M3 0
+#define KVSKIP_INT8 1
+#define KVSKIP_BF16 2
+
+/* Scales of a cache held in 8 bits, beside a kvskip_attn_args whose k and v point to the codes (strides in elements,
+ * multiples of 16, bases 16-byte aligned; 0 <= k_st, v_st < 2^24). Block blk of sequence b, KV head h has the scale
+ * k_scale[b * ks_sb + h * ks_sh + blk]; over pages, page pg has k_scale[pg * ks_sb + h * ks_sh]. */
+typedef struct kvskip_cache8_args {
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  int32_t format;              /* KVSKIP_E4M3 or KVSKIP_INT8 */
+} kvskip_cache8_args;
+
+/* kvskip_decode (with V) over a cache held in 8 bits: score s = scale * k_scale * q.k, out = sum softmax(s) v_scale v.
+ * Dense or block lists, statistics, split-K, seq_lens, paged caches and list_partition as in kvskip_decode; a sequence
+ * of length 0 (seq_lens: clamp(seq_lens[b], 0, T)) gets out 0 and lse -inf. D in {64, 128}, G = Hq / Hkv in 1..16. The
+ * p_out, key_sums and V-skip fields are refused or ignored; no limit on the blocks of a split. Statistics are
+ * those of the scores above. Always the MFMA engine, whatever KVSKIP_AMD_QK says. */
+int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int stats, void* stream);
+
+/* A step's block tables and slot map from the requests' lengths. Request b has n = seq_lens[b] tokens after the step
+ * (negative: 0), a = new_lens[b] of them new (clamped to [0, n]) and holds held[b] pages, entries [0, held[b]) of its
+ * table row; it needs ceil(n / 64). In this order:
+ *   1. entries [need, held) of every request that needs fewer (a finished one: n = 0) go on the free stack, request by
+ *      request: free_pages[*free_count ...]; avail = *free_count + those.
+ *   2. every request that needs more takes need - held pages, request by request; the k-th page taken by the step is
+ *      free_pages[avail - 1 - k], and goes into table entries [held, need) in order. The first request whose pages do
+ *      not suffice, and every later one that needs any, gets none; nor does one with n > 64 * width. Those are not
+ *      served: their held count stays, *short_out counts them.
+ *   3. row starts[b] + i (starts: the exclusive sums of new_lens; starts[B] all of them) is the request's position
+ *      p = n - a + i: slots[row] = page * 64 + p % 64 with page = entry p / 64; -1 where the request was not served, for
+ *      a page outside [0, num_pages), and for rows from starts[B] on. Rows past `rows` have no slot.
+ * held_out and free_count_out may be held and free_count (the step in place) or buffers of their own (the state before
+ * stays, but for table entries and stack positions that it does not count). Table entries past held_out are not cleared.
+ * B <= 4096; B * (rows + 1), B * width and 64 * num_pages below 2^31. work: kvskip_page_work_ints(B, rows) int32, or
+ * NULL where that is 0. No atomics: the same result every time. */
+typedef struct kvskip_page_args {
+  const int32_t* seq_lens;     /* [B] */
+  const int32_t* new_lens;     /* [B] */
+  const int32_t* held;         /* [B] */
+  int32_t* block_table;        /* [B, width], row stride bt_stride */
+  int64_t bt_stride;
+  int32_t* free_pages;         /* [num_pages] */
+  const int32_t* free_count;   /* one */
+  int32_t* slots;              /* [rows] out */
+  int32_t* starts;             /* [B + 1] out */
+  int32_t* held_out;           /* [B] out */
+  int32_t* free_count_out;     /* one, out */
+  int32_t* short_out;          /* one, out */
+  int32_t* work;
+  int32_t B, width, num_pages, rows;
+} kvskip_page_args;
+
+int kvskip_page_map(const kvskip_page_args* p, void* stream);
+
+/* int32 elements of kvskip_page_args.work (-1 for invalid sizes). */
+int64_t kvskip_page_work_ints(int32_t B, int32_t rows);
+
+/* Rows of new keys and values into the pages that a slot map names. k, v: bf16 [N, Hkv, D] (D contiguous, strides
+ * multiples of 8, 16-byte aligned); row i goes to token slot % 64 of page slot / 64 (slot = slot_map[i]); a slot outside
+ * [0, 64 * num_pages) leaves its row out. Pools [num_pages, Hkv, 64, D] of the format's type (D contiguous; strides and
+ * bases multiples of 16 bytes).
+ * In 8 bits, with scales k_scale[page * ks_sb + head * ks_sh]: let amax be the largest magnitude of the rows written to
+ * a page's head (an infinity counts as the largest finite bf16, NaN not). A page whose row 0 is written starts anew
+ * (scale 0 before). If amax > qmax * scale (qmax 448 for e4m3, 127 for int8) the scale becomes the smallest power of two
+ * s >= 2^-126 with amax <= qmax * s, and the page's other rows are moved to it: code' = round(code * old / s). Codes are
+ * round(x / scale), to nearest even, infinities at the largest code; NaN is NaN in e4m3 and 0 in int8. A scale that is
+ * not positive and finite counts as 0.
+ * The rows of a page must lie next to each other in the map (as kvskip_page_map has them): a page that two runs of rows
+ * name is written by both at once. Of rows with the same slot in one run the last is kept. */
+typedef struct kvskip_write_args {
+  const void* k;
+  const void* v;
+  int64_t k_sn, k_sh, v_sn, v_sh;
+  const int32_t* slot_map;     /* [N] */
+  void* k_pool;
+  void* v_pool;
+  int64_t kp_sb, kp_sh, kp_st, vp_sb, vp_sh, vp_st;   /* page, head and token strides, elements */
+  float* k_scale;              /* 8 bits only */
+  float* v_scale;
+  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  int32_t N, Hkv, D, num_pages, format;
+} kvskip_write_args;
+
+int kvskip_cache_write(const kvskip_write_args* p, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* kvskip_last_error(void);
 
@@ -396,7 +487,7 @@ const char* kvskip_last_error(void);
 const char* kvskip_version(void);
 
 /* sizeof of the argument blocks (0: kvskip_attn_args, 1: kvskip_plan_args, 2: kvskip_update_args,
- * 3: kvskip_select_args), -1 otherwise: lets a binding check its struct layout. Library utility, no
+ * 3: kvskip_select_args, 5: kvskip_cache8_args, 6: kvskip_page_args, 7: kvskip_write_args), -1 otherwise: lets a binding check its struct layout. Library utility, no
  * reference counterpart. */
 int kvskip_struct_size(int which);
 

@@ -78,6 +78,37 @@ class SelectArgs(ctypes.Structure):
     ]
 
 
+class Cache8Args(ctypes.Structure):
+    """kvskip_cache8_args."""
+    _fields_ = [
+        ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("ks_sb", c_int64), ("ks_sh", c_int64), ("vs_sb", c_int64), ("vs_sh", c_int64), ("format", c_int32),
+    ]
+
+
+class PageArgs(ctypes.Structure):
+    """kvskip_page_args."""
+    _fields_ = [
+        ("seq_lens", c_void_p), ("new_lens", c_void_p), ("held", c_void_p), ("block_table", c_void_p),
+        ("bt_stride", c_int64), ("free_pages", c_void_p), ("free_count", c_void_p), ("slots", c_void_p),
+        ("starts", c_void_p), ("held_out", c_void_p), ("free_count_out", c_void_p), ("short_out", c_void_p),
+        ("work", c_void_p), ("B", c_int32), ("width", c_int32), ("num_pages", c_int32), ("rows", c_int32),
+    ]
+
+
+class WriteArgs(ctypes.Structure):
+    """kvskip_write_args."""
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_sn", c_int64), ("k_sh", c_int64), ("v_sn", c_int64), ("v_sh", c_int64),
+        ("slot_map", c_void_p), ("k_pool", c_void_p), ("v_pool", c_void_p),
+        ("kp_sb", c_int64), ("kp_sh", c_int64), ("kp_st", c_int64),
+        ("vp_sb", c_int64), ("vp_sh", c_int64), ("vp_st", c_int64),
+        ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("ks_sb", c_int64), ("ks_sh", c_int64), ("vs_sb", c_int64), ("vs_sh", c_int64),
+        ("N", c_int32), ("Hkv", c_int32), ("D", c_int32), ("num_pages", c_int32), ("format", c_int32),
+    ]
+
+
 # Every entry point of include/kvskip_amd.h with its argument types.
 SIGNATURES = {
     "kvskip_decode": ([POINTER(AttnArgs), c_int, c_int, c_void_p], c_int),
@@ -100,6 +131,10 @@ SIGNATURES = {
     "kvskip_select": ([POINTER(SelectArgs), c_void_p], c_int),
     "kvskip_pv_select": ([POINTER(AttnArgs), POINTER(SelectArgs), c_void_p], c_int),
     "kvskip_block_list": ([c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p], c_int),
+    "kvskip_decode8": ([POINTER(AttnArgs), POINTER(Cache8Args), c_int, c_void_p], c_int),
+    "kvskip_page_map": ([POINTER(PageArgs), c_void_p], c_int),
+    "kvskip_page_work_ints": ([c_int32, c_int32], c_int64),
+    "kvskip_cache_write": ([POINTER(WriteArgs), c_void_p], c_int),
     "kvskip_last_error": ([], c_char_p),
     "kvskip_version": ([], c_char_p),
     "kvskip_struct_size": ([c_int], c_int),
@@ -126,7 +161,8 @@ def lib() -> ctypes.CDLL:
 
 # The entry points that the native host module calls, in the order of its table (csrc/host.cpp).
 HOST_CALLS = ("decode", "decode_splits", "merge_splits", "pv", "vskip1", "pv_select", "select", "plan", "plan_scores",
-              "update", "merge_update", "decode_splits_update", "decode_splits_planned", "plan_part_floats", "last_error")
+              "update", "merge_update", "decode_splits_update", "decode_splits_planned", "plan_part_floats", "decode8",
+              "page_map", "page_work_ints", "cache_write", "last_error")
 _HOST = None
 
 

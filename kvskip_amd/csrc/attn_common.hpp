@@ -98,12 +98,18 @@ __device__ __forceinline__ void work_coords(int S, int Hkv, int B, int& split, i
 }
 
 // ---- Ragged batches (seq_lens): sequence b attends tokens [0, clamp(seq_lens[b], 1, T)).
+// (A cache held in 8 bits: clamp(seq_lens[b], 0, T), an empty slot of the batch attends nothing; what reads
+// lengths below is written over the argument block's type P for that.)
 __device__ __forceinline__ int seq_len(const AttnP& p, int b) {
   return p.seq_lens != nullptr ? min(max(p.seq_lens[b], 1), p.T) : p.T;
 }
+__device__ __forceinline__ int seq_len(const Attn8P& p, int b) {
+  return p.seq_lens != nullptr ? min(max(p.seq_lens[b], 0), p.T) : p.T;
+}
 
 // Items of sequence b on KV head h: its blocks (dense) or its list entries (masked).
-__device__ __forceinline__ int ragged_items(const AttnP& p, int b, int h, bool masked) {
+template <class P>
+__device__ __forceinline__ int ragged_items(const P& p, int b, int h, bool masked) {
   if (masked) return min(max(p.block_cnt[b * p.Hkv + h], 0), p.max_blocks);
   return (seq_len(p, b) + BLK - 1) / BLK;
 }
@@ -152,7 +158,8 @@ __device__ __forceinline__ int fit_chunk_len(const AttnP& p, const int (&nv)[NR]
 // Returns C, uniform.
 constexpr int NRB = MAX_RAGGED_B / WAVE;
 
-__device__ __forceinline__ int ragged_chunk_len(const AttnP& p, int h, bool masked, int (&nv)[NRB]) {
+template <class P>
+__device__ __forceinline__ int ragged_chunk_len(const P& p, int h, bool masked, int (&nv)[NRB]) {
   const int lane = threadIdx.x % WAVE;
   int tot = 0, most = 0;
 #pragma unroll
@@ -172,7 +179,8 @@ __device__ __forceinline__ int ragged_chunk_len(const AttnP& p, int h, bool mask
 
 // Chunk number `it` of KV head h's ragged partition, uniform over the wavefront: b (-1 past the
 // head's last chunk), the chunk within b and b's item count. Returns C.
-__device__ int ragged_lookup(const AttnP& p, int h, int it, bool masked, int& b, int& chunk, int& items) {
+template <class P>
+__device__ int ragged_lookup(const P& p, int h, int it, bool masked, int& b, int& chunk, int& items) {
   const int lane = threadIdx.x % WAVE;
   int nv[NRB];
   const int C = ragged_chunk_len(p, h, masked, nv);
@@ -202,7 +210,8 @@ __device__ int ragged_lookup(const AttnP& p, int h, int it, bool masked, int& b,
 }
 
 // Chunks (split partials) of (b, KV head h) under the ragged partition.
-__device__ __forceinline__ int ragged_chunks(const AttnP& p, int b, int h, bool masked) {
+template <class P>
+__device__ __forceinline__ int ragged_chunks(const P& p, int b, int h, bool masked) {
   int nv[NRB];
   const int C = ragged_chunk_len(p, h, masked, nv);
   return (ragged_items(p, b, h, masked) + C - 1) / C;
@@ -1067,7 +1076,8 @@ __device__ __forceinline__ void merge_body(const AttnP& p, int plain, int64_t hq
 
 // Partials of query head hq: S, or in a ragged batch its (sequence, KV head)'s chunk count (0:
 // nothing attended, out 0 and lse -inf). Uniform over the workgroup.
-__device__ __forceinline__ int merge_count(const AttnP& p, int64_t hq) {
+template <class P>
+__device__ __forceinline__ int merge_count(const P& p, int64_t hq) {
   if (p.seq_lens == nullptr) return p.num_splits;
   const int b = static_cast<int>(hq / p.Hq), h = static_cast<int>(hq % p.Hq) / (p.Hq / p.Hkv);
   if (p.block_idx != nullptr && p.list_partition != 0) {
@@ -1095,8 +1105,8 @@ __device__ void merge_fit(const AttnP& p, int plain, int64_t hq, int slice, int 
 // Workgroup (x, y) of the (B Hq, D / 32) grid takes item xcd_remap(x + y B Hq) in (query head, dim
 // slice) order, so a KV head's merges run on the XCD that ran its splits (work_coords' mapping),
 // whose L2 still holds the partials just written (config 2's op 26.87 -> 26.52 us).
-template <int D, int U, bool WITH_V>
-__global__ void __launch_bounds__(256) combine_kernel(const AttnP p, int plain) {
+template <int D, int U, bool WITH_V, class P>
+__global__ void __launch_bounds__(256) combine_kernel(const P p, int plain) {
   const int nsl = gridDim.y;
   const int m = xcd_remap(blockIdx.x + blockIdx.y * gridDim.x, gridDim.x * nsl);
   const int64_t hq = m / nsl;
@@ -1109,18 +1119,19 @@ __device__ void merge_body_rt(const AttnP& p, int64_t hq, int slice) {
   merge_fit<D, MAX_SPLITS / 8, true>(p, 0, hq, slice, merge_count(p, hq));
 }
 
-template <int D, bool WITH_V>
-inline void launch_combine_u(const AttnP& p, dim3 grid, int plain, hipStream_t s) {
+template <int D, bool WITH_V, class P>
+inline void launch_combine_u(const P& p, dim3 grid, int plain, hipStream_t s) {
   const int u = (p.num_splits + 7) / 8;
-  if (u <= 1) hipLaunchKernelGGL((combine_kernel<D, 1, WITH_V>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 2) hipLaunchKernelGGL((combine_kernel<D, 2, WITH_V>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 4) hipLaunchKernelGGL((combine_kernel<D, 4, WITH_V>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 8) hipLaunchKernelGGL((combine_kernel<D, 8, WITH_V>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 16) hipLaunchKernelGGL((combine_kernel<D, 16, WITH_V>), grid, dim3(256), 0, s, p, plain);
-  else hipLaunchKernelGGL((combine_kernel<D, MAX_SPLITS / 8, WITH_V>), grid, dim3(256), 0, s, p, plain);
+  if (u <= 1) hipLaunchKernelGGL((combine_kernel<D, 1, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 2) hipLaunchKernelGGL((combine_kernel<D, 2, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 4) hipLaunchKernelGGL((combine_kernel<D, 4, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 8) hipLaunchKernelGGL((combine_kernel<D, 8, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 16) hipLaunchKernelGGL((combine_kernel<D, 16, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
+  else hipLaunchKernelGGL((combine_kernel<D, MAX_SPLITS / 8, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
 }
 
-inline hipError_t launch_combine(const AttnP& p, int D, bool plain, hipStream_t s) {
+template <class P>
+inline hipError_t launch_combine(const P& p, int D, bool plain, hipStream_t s) {
   const bool with_v = p.out != nullptr;
   const dim3 grid(p.B * p.Hq, with_v ? D / 32 : 1);
   const int pl = plain ? 1 : 0;

@@ -1,0 +1,523 @@
+// Split-K decode attention over a cache held in 8 bits (e4m3 or int8) with a scale for each 64-token block and KV
+// head: dense or over block lists, contiguous or paged, one length or a ragged batch, with optional block statistics.
+//
+//   s_t = scale ks[blk] (q . k_t),  p_t = exp(s_t - m),  out = sum_t p_t vs[blk] v_t / sum_t p_t
+//
+// The work is cut as the bf16 pass cuts it (attn_common.hpp: workgroups of four independent wavefronts, a block per
+// wavefront and step, the split merge a second launch); what differs is inside a block:
+//   codes     every e4m3 and int8 value is a value of fp16: codes become fp16 operands exactly (e4m3 by the hardware's
+//             conversion, int8 by placing the byte under the exponent of 1024 and taking 1152 off), and the block's two
+//             scales enter as scalars: ks with the softmax scale, vs with the block's factor of P V.
+//   q         bf16 as fp16 times a power of two of its head, chosen so that the head's largest value is near 2^15: what
+//             lies below 2^-39 of that is lost.
+//   weights   e = 2^(s - block maximum) in two fp16 parts (22 bits), which fill the operand rows that the group's heads
+//             leave free (up to 8 heads; 9 to 16 take two products). A block's P V starts from zero and is added as
+//             acc = acc * alpha + tmp * (2^(mt - m) vs), so the parts' exponents do not depend on the scales.
+//   items     lane l of a wavefront holds block, page and scales of the wavefront's step 64 i + l (one gather per 64
+//             steps, the next one fetched during this one in three stages, since a page needs its list entry and a
+//             scale its page); the loop takes them by readlane, so no step waits for them.
+//   memory    each block has a buffer resource of its own, based at the block's first row and ending with the
+//             sequence's last token: no offset of a cache of any length passes 32 bits, rows past the end read zeros
+//             (whatever codes a page holds there), and an empty block reads nothing.
+#include "attn_common.hpp"
+
+namespace kvs {
+namespace {
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// Four codes of a dword as fp16: codes 0, 1 and codes 2, 3.
+template <bool I8>
+__device__ __forceinline__ u32x2 widen4(uint32_t w) {
+  uint32_t lo, hi;
+  if constexpr (I8) {
+    const uint32_t u = w ^ 0x80808080u;  // x + 128
+    const f16x2_t off = {-1152.f16, -1152.f16};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+  } else {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
+  }
+  return u32x2{lo, hi};
+}
+
+__device__ __forceinline__ u32x2 bload8(rsrc_t r, uint32_t voff, uint32_t soff) {
+  return __builtin_amdgcn_raw_buffer_load_b64(r, static_cast<int>(voff), static_cast<int>(soff), BUF_NT);
+}
+
+// Sizes of a block's registers: K as 16-byte chunks of a row (lane r = lane % 16, j = lane / 16 holds bytes 16 j + 64 c
+// of row 16 nt + r, which are k-steps 2 c and 2 c + 1 of the scores' products; q is laid out alike), V as 8 bytes of a
+// row (D 128: a 16-lane group loads one row; D 64: two, and lanes c and c ^ 8 exchange halves).
+template <int D>
+struct Lay8 {
+  static constexpr int KC = D / 64;
+  static constexpr int KS = D / 32;
+  static constexpr int VN = BLK * D / (WAVE * 8);
+  static constexpr int VD = D / 16;
+};
+
+template <int D>
+__device__ __forceinline__ void load_k8(u32x4 (&kr)[4][Lay8<D>::KC], rsrc_t r, uint32_t koff, uint32_t st) {
+#pragma unroll
+  for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+    for (int c = 0; c < Lay8<D>::KC; ++c) kr[nt][c] = bload16<BUF_NT>(r, koff + 64 * c, 16 * nt * st);
+}
+
+template <int D>
+__device__ __forceinline__ void load_v8(u32x2 (&vr)[Lay8<D>::VN], rsrc_t r, uint32_t voff, uint32_t st) {
+#pragma unroll
+  for (int i = 0; i < Lay8<D>::VN; ++i) {
+    const int t = D == 128 ? mf_tok(i / 4, i % 4, 0) : mf_tok(i / 2, 2 * (i % 2), 0);
+    vr[i] = bload8(r, voff, t * st);
+  }
+}
+
+// Dword d (4 dims) of tokens (nt, i) and (nt, i + 1), i even, of this lane's column.
+template <int D>
+__device__ __forceinline__ void v_pair8(const u32x2 (&vr)[Lay8<D>::VN], int nt, int i, int d, bool up, uint32_t& a,
+                                        uint32_t& c) {
+  if constexpr (D == 128) {
+    a = vr[4 * nt + i][d];
+    c = vr[4 * nt + i + 1][d];
+  } else {  // up: lanes c >= 8, which loaded the second token's row
+    const u32x2 x = vr[2 * nt + i / 2];
+    const uint32_t other = dppu<DPP_ROR8>(up ? x.x : x.y);
+    a = up ? other : x.x;
+    c = up ? x.y : other;
+  }
+}
+
+// LDS of the epilogue: the wavefronts' accumulators by part and head, and their (m, l).
+template <int D, int GP>
+struct Merge8 {
+  static constexpr int NP = GP == 16 ? 1 : 2;
+  float acc[NWAVE * NP * GP * D];
+  float ml[NWAVE * GP * 2];
+};
+
+// The wavefronts' states merged: out / out_f32 / lse (one split) or the split partials. As finish_merge, with G at run
+// time and the two parts of a weight simply added (no code is infinite).
+template <int D, int GP>
+__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, const Merge8<D, GP>& L) {
+  constexpr int NP = Merge8<D, GP>::NP;
+  const int tid = threadIdx.x, S = p.num_splits;
+  __syncthreads();
+  const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G;
+  for (int o = tid; o < p.G * D; o += NT) {
+    const int g = o / D, d = o % D;
+    float M = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) M = fmaxf(M, L.ml[(w * GP + g) * 2]);
+    const float mu = M == NEG_INF ? 0.f : M;
+    float A = 0.f, Ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) {
+      const float f = fexp2(L.ml[(w * GP + g) * 2] - mu);
+      float x = L.acc[((w * NP) * GP + g) * D + d];
+      if constexpr (NP == 2) x += L.acc[((w * NP + 1) * GP + g) * D + d];
+      Ls += L.ml[(w * GP + g) * 2 + 1] * f;
+      A += x * f;
+    }
+    const int64_t hq = hq0 + g;
+    if (S == 1) {
+      // (a NaN sum, from a NaN of q or the cache, comes out as NaN)
+      const float r = Ls == 0.f ? 0.f : A / Ls;
+      p.out[hq * D + d] = f2bf(r);
+      if (p.out_f32) p.out_f32[hq * D + d] = r;
+      if (p.lse && d == 0) p.lse[hq] = Ls == 0.f ? NEG_INF : (M + flog2(Ls)) * LN2;
+    } else {
+      p.part_acc[(hq * S + split) * D + d] = A;
+      if (d == 0) {
+        p.part_ml[(hq * S + split) * 2] = M;
+        p.part_ml[(hq * S + split) * 2 + 1] = Ls;
+      }
+    }
+  }
+}
+
+// (-inf, 0) statistics of blocks a .. a + len - 1 of the KV head whose first query head is hq0: thread t of `stride`.
+__device__ __forceinline__ void empty_stats(const Attn8P& p, int64_t hq0, int a, int len, int t, int stride) {
+  for (int g = 0; g < p.G; ++g)
+    for (int x = t; x < len; x += stride) {
+      const int64_t i = (hq0 + g) * p.nb + a + x;
+      p.blk_max[i] = NEG_INF;
+      p.blk_sum[i] = 0.f;
+    }
+}
+
+// A wavefront's items of 64 steps, one per lane: block (-1: outside the sequence), page (0 of a contiguous cache; -1:
+// nothing to read, an empty block), scales.
+struct Items {
+  int blk, pg;
+  float ks, vs;
+};
+
+template <int D, int GP, bool I8, bool STATS>
+__global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
+  constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
+  __shared__ __attribute__((aligned(16))) Merge8<D, GP> sL;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
+  const int j4 = lane >> 4, c16 = lane & 15;
+  const bool masked = p.block_idx != nullptr, paged = p.block_table != nullptr, rag = p.seq_lens != nullptr;
+  const int G = p.G;
+
+  // ---- this workgroup's work, as decode_body finds it: list positions / blocks [i0, i0 + n) of the n_items of (b, h)
+  int split, h, b, n_items, i0, n, Tb = p.T, nbb = p.nb;
+  if (!rag) {
+    work_coords(blockIdx.x, p.num_splits, p.Hkv, p.B, split, h, b);
+    n_items = masked ? min(max(p.block_cnt[b * p.Hkv + h], 0), p.max_blocks) : p.nb;
+    const int per = (n_items + p.num_splits - 1) / p.num_splits;
+    i0 = min(n_items, split * per);
+    n = min(n_items, i0 + per) - i0;
+  } else {
+    const int W = p.num_splits + p.B;
+    const bool global = masked && p.list_partition != 0;
+    const int it = global ? static_cast<int>(blockIdx.x) : xcd_remap(blockIdx.x, W * p.Hkv);
+    int chunk, C;
+    if (global) {
+      C = global_lookup(p, it, b, h, chunk, n_items);
+    } else {
+      h = it / W;
+      C = ragged_lookup(p, h, it % W, masked, b, chunk, n_items);
+    }
+    if constexpr (STATS) {  // (sequence, KV head)s with nothing to read: written by one workgroup per KV head
+      const int eh = global ? (it < p.Hkv ? it : -1) : (it % W == 0 ? h : -1);
+      if (eh >= 0) {
+        for (int b0 = wave * WAVE; b0 < p.B; b0 += NT) {
+          const int bb = b0 + lane;
+          uint64_t none = __ballot(bb < p.B && ragged_items(p, bb, eh, masked) == 0);
+          while (none != 0) {
+            const int be = b0 + __builtin_ctzll(none);
+            none &= none - 1;
+            empty_stats(p, static_cast<int64_t>(be) * p.Hq + static_cast<int64_t>(eh) * G, 0, p.nb, lane, WAVE);
+          }
+        }
+      }
+    }
+    if (b < 0) return;
+    split = chunk;
+    if ((global && (G > 4 || grid_queued(p))) || p.B == 1) {
+      i0 = chunk * C;
+      n = min(n_items, i0 + C) - i0;
+    } else {
+      const int k = max(1, (n_items + C - 1) / C);
+      i0 = chunk * n_items / k;
+      n = (chunk + 1) * n_items / k - i0;
+    }
+    Tb = seq_len(p, b);
+    nbb = (Tb + BLK - 1) / BLK;
+  }
+  const int64_t bh = static_cast<int64_t>(b) * p.Hkv + h, hq0 = bh * G;
+  const int* list = masked ? p.block_idx + bh * p.max_blocks : nullptr;
+  const int* table = paged ? p.block_table + static_cast<int64_t>(b) * p.bt_stride : nullptr;
+  const int nw = n > wave ? (n - wave + NWAVE - 1) / NWAVE : 0;
+  const int rot = item_rotation(p, h, split + (rag && p.B > 1 ? n_items : 0), nw);
+
+  // ---- items of steps k0 .. k0 + 63, in three stages
+  auto item_block = [&](Items& x, int k0) {
+    const int k = k0 + lane;
+    x.blk = -1;
+    if (k < nw) {
+      const int pos = i0 + wave + NWAVE * rotated(k, rot, nw);
+      x.blk = masked ? list[pos] : pos;
+    }
+  };
+  auto item_page = [&](Items& x) {
+    if (x.blk < 0 || x.blk >= nbb) x.blk = -1;
+    x.pg = x.blk >= 0 ? 0 : -1;
+    if (paged && x.blk >= 0) x.pg = table[x.blk];
+  };
+  auto item_scales = [&](Items& x) {
+    if (paged && (x.pg < 0 || x.pg >= p.num_pages)) x.pg = -1;
+    x.ks = x.vs = 0.f;
+    if (x.pg >= 0) {
+      const int64_t i = paged ? x.pg : b;
+      const int e = paged ? 0 : x.blk;
+      x.ks = p.k_scale[i * p.ks_sb + h * p.ks_sh + e];
+      x.vs = p.v_scale[i * p.vs_sb + h * p.vs_sh + e];
+    }
+  };
+  Items cur, nxt;
+  item_block(cur, 0);
+  item_page(cur);
+  item_scales(cur);
+  nxt = cur;
+
+  const uint32_t k_st = static_cast<uint32_t>(p.k_st), v_st = static_cast<uint32_t>(p.v_st);
+  const uint32_t koff = c16 * k_st + 16 * j4;
+  const uint32_t voff = D == 128 ? 4 * j4 * v_st + 8 * c16 : (4 * j4 + (c16 >> 3)) * v_st + 8 * (c16 & 7);
+  const bool up = (lane & 8) != 0;
+  const char* kb = reinterpret_cast<const char*>(p.k) + h * p.k_sh;
+  const char* vb = reinterpret_cast<const char*>(p.v) + h * p.v_sh;
+  auto block_res = [&](const char* base, int64_t sb, uint32_t st, int blk, int pg) {
+    const int rows = pg >= 0 ? min(BLK, Tb - blk * BLK) : 0;
+    const char* at = base + (paged ? static_cast<int64_t>(pg) * sb : b * sb + static_cast<int64_t>(blk) * BLK * st);
+    return make_rsrc(rows > 0 ? at : base, rows > 0 ? (rows - 1) * st + D : 0u);
+  };
+
+  // ---- q as fp16: this lane's head's dims of every k-step, and the factor that takes its power of two out again
+  u32x4 qb[KS];
+  float qf;
+  {
+    const int g = c16 % GP;
+    float x[KS][8], amax = 0.f;
+    const uint16_t* qp = p.q + b * p.q_sb + (static_cast<int64_t>(h) * G + g) * p.q_sh + 16 * j4;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const u32x4 w = g < G ? ld16(qp + 64 * (ks / 2) + 8 * (ks % 2)) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[ks][2 * e] = bf_lo(w[e]);
+        x[ks][2 * e + 1] = bf_hi(w[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
+    }
+    amax = swap_max(amax);
+    const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -112), 127);  // 2^ex <= amax < 2^(ex + 1)
+    const float up_q = __uint_as_float(static_cast<uint32_t>(127 + 14 - ex) << 23);
+    qf = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + ex) << 23);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        qb[ks][e] = f2h(x[ks][2 * e] * up_q) | static_cast<uint32_t>(f2h(x[ks][2 * e + 1] * up_q)) << 16;
+  }
+
+  const uint32_t nb4 = 4u * static_cast<uint32_t>(p.nb);
+  const rsrc_t rs_max = make_rsrc(STATS ? p.blk_max + hq0 * p.nb : nullptr, STATS ? G * nb4 : 0);
+  const rsrc_t rs_sum = make_rsrc(STATS ? p.blk_sum + hq0 * p.nb : nullptr, STATS ? G * nb4 : 0);
+  constexpr uint32_t OOB = 0x80000000u;
+  const uint32_t v_stat = c16 < G && j4 == 0 ? c16 * nb4 : OOB;
+
+  float mr = NEG_INF, lr = 0.f;  // running (m, l) of this lane's head c16 % GP
+  f32x4_t acc[VD];
+#pragma unroll
+  for (int j = 0; j < VD; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (nw > 0) {
+    u32x4 kr[4][KC];
+    u32x2 vr[VN];
+    int blk = __builtin_amdgcn_readlane(cur.blk, 0), pg = __builtin_amdgcn_readlane(cur.pg, 0);
+    float ks = lane_value(cur.ks, 0), vs = lane_value(cur.vs, 0);
+    load_k8<D>(kr, block_res(kb, p.k_sb, k_st, blk, pg), koff, k_st);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v8<D>(vr, block_res(vb, p.v_sb, v_st, blk, pg), voff, v_st);
+    for (int k = 0; k < nw; ++k) {
+      // the next 64 steps' items, stage by stage
+      const int ph = k & 63;
+      if (k - ph + 64 < nw) {
+        if (ph == 0) item_block(nxt, k + 64);
+        if (ph == 16) item_page(nxt);
+        if (ph == 32) item_scales(nxt);
+        if (ph == 63) cur = nxt;
+      }
+      const int kn = (k + 1) & 63;
+      int blk_n = -1, pg_n = -1;
+      float ks_n = 0.f, vs_n = 0.f;
+      if (k + 1 < nw) {
+        blk_n = __builtin_amdgcn_readlane(cur.blk, kn);
+        pg_n = __builtin_amdgcn_readlane(cur.pg, kn);
+        ks_n = lane_value(cur.ks, kn);
+        vs_n = lane_value(cur.vs, kn);
+      }
+      const rsrc_t rk_n = block_res(kb, p.k_sb, k_st, blk_n, pg_n), rv_n = block_res(vb, p.v_sb, v_st, blk_n, pg_n);
+
+      // scores of this block in log2 units: s[nt][i] of head c16 % GP, token 16 nt + 4 j4 + i
+      float s[4][4], e[4][4];
+      const float f = qf * ks;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x2 w0 = widen4<I8>(kr[nt][c][2 * u]), w1 = widen4<I8>(kr[nt][c][2 * u + 1]);
+            const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w),
+                                                       __builtin_bit_cast(f16x8_t, qb[2 * c + u]), a, 0, 0, 0);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i] = a[i] * f;
+      }
+      const int t0 = blk * BLK, lim = pg >= 0 ? Tb : -BLK;
+      if (t0 + BLK > lim) {  // uniform: the block that the sequence's end cuts, or an empty one
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t0 + mf_tok(nt, i, j4) >= lim) s[nt][i] = NEG_INF;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_k8<D>(kr, rk_n, koff, k_st);
+      __builtin_amdgcn_sched_barrier(0);
+
+      const float mt = block_max_mf(s);
+      // e = 2^15 2^(s - mt): its low part stays a normal fp16 down to 2^-18 of the block's largest weight
+      const float mtu = mt == NEG_INF ? 0.f : mt - 15.f;
+      float r4[4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[nt][i] = fexp2(s[nt][i] - mtu);
+        r4[nt] = (e[nt][0] + e[nt][1]) + (e[nt][2] + e[nt][3]);
+      }
+      const float st = swap_sum((r4[0] + r4[1]) + (r4[2] + r4[3])) * 0x1p-15f;
+      const float m_new = fmaxf(mr, mt);
+      const float mu = m_new == NEG_INF ? 0.f : m_new;
+      const float alpha = fexp2(mr - mu);
+      const float cf = mt == NEG_INF ? 0.f : fexp2(mt - mu);
+      lr = lr * alpha + st * cf;
+      mr = m_new;
+      const float fv = cf * 0x1p-15f * vs;
+      if constexpr (STATS) {
+        const uint32_t blk4 = 4u * static_cast<uint32_t>(max(blk, 0));
+        const uint32_t at = blk >= 0 ? v_stat : OOB;
+        bstore_f32(mt * LN2, rs_max, at, blk4);
+        bstore_f32(st, rs_sum, at, blk4);
+      }
+
+      // the weights as operands: the high parts on rows of part 0, what they leave on the others
+      u32x4 ph_[2], pl_[2];
+      const bool low = GP < 16 && (c16 / GP) % 2 == 1;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float x = e[2 * q + u / 2][2 * (u % 2)], y = e[2 * q + u / 2][2 * (u % 2) + 1];
+          const auto hi = __builtin_amdgcn_cvt_pkrtz(x, y);
+          const auto lo = __builtin_amdgcn_cvt_pkrtz(x - static_cast<float>(hi.x), y - static_cast<float>(hi.y));
+          const uint32_t uh = __builtin_bit_cast(uint32_t, hi), ul = __builtin_bit_cast(uint32_t, lo);
+          if constexpr (GP == 16) {
+            ph_[q][u] = uh;
+            pl_[q][u] = ul;
+          } else {
+            ph_[q][u] = low ? ul : uh;
+          }
+        }
+      // alpha and fv of this lane's rows 4 j4 + i
+      float al[4], fr[4];
+      auto rows = [&](float (&r)[4], float x) {
+        if constexpr (GP == 16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = __shfl(x, 4 * j4 + i, WAVE);
+        } else {
+          r[0] = dpp<0x150>(x), r[1] = dpp<0x151>(x), r[2] = dpp<0x152>(x), r[3] = dpp<0x153>(x);  // row_newbcast
+          if constexpr (GP == 8) {
+            const bool odd = (lane & 16) != 0;  // rows 4 .. 7 of an 8-row part
+            r[0] = odd ? dpp<0x154>(x) : r[0], r[1] = odd ? dpp<0x155>(x) : r[1];
+            r[2] = odd ? dpp<0x156>(x) : r[2], r[3] = odd ? dpp<0x157>(x) : r[3];
+          }
+        }
+      };
+      rows(al, alpha);
+      rows(fr, fv);
+#pragma unroll
+      for (int d = 0; d < VD / 4; ++d) {
+        f32x4_t tmp[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmp[x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          u32x4 w[4];  // four dims, tokens in pairs
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t a, c;
+            v_pair8<D>(vr, 2 * q + u / 2, 2 * (u % 2), d, up, a, c);
+            const u32x2 w01 = widen4<I8>(__builtin_amdgcn_perm(c, a, 0x05010400u));
+            const u32x2 w23 = widen4<I8>(__builtin_amdgcn_perm(c, a, 0x07030602u));
+            w[0][u] = w01.x, w[1][u] = w01.y, w[2][u] = w23.x, w[3][u] = w23.y;
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            tmp[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, ph_[q]),
+                                                            __builtin_bit_cast(f16x8_t, w[x]), tmp[x], 0, 0, 0);
+            if constexpr (GP == 16)
+              tmp[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, pl_[q]),
+                                                              __builtin_bit_cast(f16x8_t, w[x]), tmp[x], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[4 * d + x][i] = fmaf(acc[4 * d + x][i], al[i], tmp[x][i] * fr[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_v8<D>(vr, rv_n, voff, v_st);
+      blk = blk_n;
+      pg = pg_n;
+      ks = ks_n;
+      vs = vs_n;
+    }
+  }
+
+  // ---- the wavefront's state into LDS (row 4 j4 + i of the products: part and head), then the merge
+  {
+    constexpr int NP = Merge8<D, GP>::NP;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * j4 + i, part = row / GP, g = row % GP;
+      if (part < NP && g < G) {
+        float* a = sL.acc + ((wave * NP + part) * GP + g) * D + mf_vdim<D>(c16);
+#pragma unroll
+        for (int j = 0; j < VD; j += 4)
+          *reinterpret_cast<float4*>(a + j) = make_float4(acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]);
+      }
+    }
+    if (lane < G) {
+      sL.ml[(wave * GP + lane) * 2] = mr;
+      sL.ml[(wave * GP + lane) * 2 + 1] = lr;
+    }
+  }
+  finish8<D, GP>(p, b, h, split, sL);
+
+  if constexpr (STATS) {
+    // the blocks that the list skips, and those past the sequence's end: the gap before each of this split's entries
+    // and, on the split of the last one, what follows it
+    if (masked) {
+      if (n_items == 0 && split == 0) empty_stats(p, hq0, 0, p.nb, tid, NT);
+      for (int k = i0 + wave; k < i0 + n; k += NWAVE) {
+        const int now = __builtin_amdgcn_readfirstlane(list[k]);
+        const int before = k > 0 ? __builtin_amdgcn_readfirstlane(list[k - 1]) : -1;
+        const int a = min(max(before, -1), p.nb - 1) + 1, len = min(max(now, 0), p.nb) - a;
+        empty_stats(p, hq0, a, len, lane, WAVE);
+      }
+    }
+    if (n > 0 && i0 + n == n_items) {
+      const int last = masked ? min(max(list[n_items - 1], -1), p.nb - 1) : nbb - 1;
+      empty_stats(p, hq0, last + 1, p.nb - last - 1, tid, NT);
+    }
+  }
+}
+
+template <int D, int GP, bool I8>
+void launch8(const Attn8P& p, bool stats, hipStream_t s) {
+  if (stats)
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, true>), attn_grid(p), dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, false>), attn_grid(p), dim3(NT), 0, s, p);
+}
+
+template <int D>
+void launch8_d(const Attn8P& p, bool i8, bool stats, hipStream_t s) {
+  if (p.G <= 4)
+    i8 ? launch8<D, 4, true>(p, stats, s) : launch8<D, 4, false>(p, stats, s);
+  else if (p.G <= 8)
+    i8 ? launch8<D, 8, true>(p, stats, s) : launch8<D, 8, false>(p, stats, s);
+  else
+    i8 ? launch8<D, 16, true>(p, stats, s) : launch8<D, 16, false>(p, stats, s);
+}
+
+}  // namespace
+
+hipError_t launch_decode8(const Attn8P& p, int D, bool i8, bool stats, hipStream_t s) {
+  D == 128 ? launch8_d<128>(p, i8, stats, s) : launch8_d<64>(p, i8, stats, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.num_splits == 1) return e;
+  return launch_combine(p, D, false, s);
+}
+
+}  // namespace kvs

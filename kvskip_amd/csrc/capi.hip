@@ -52,13 +52,14 @@ int check_kv(const void* ptr, int64_t sb, int64_t sh, int64_t st, const char* na
 }
 
 // Common checks of q/k/v and sizes; fills the derived parts of the kernel block.
-int prepare_attn(const kvskip_attn_args* a, bool need_q, bool need_k, bool need_v, kvs::AttnP* p) {
+// (eight_bit: the pass over a cache held in 8 bits, whose k and v its caller checks)
+int prepare_attn(const kvskip_attn_args* a, bool need_q, bool need_k, bool need_v, kvs::AttnP* p, bool eight_bit = false) {
   if (a == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
   if (a->B < 1 || a->Hq < 1 || a->Hkv < 1 || a->T < 1)
     return fail(KVSKIP_E_INVALID, "sizes must be positive (B=%d Hq=%d Hkv=%d T=%d)", a->B, a->Hq, a->Hkv, a->T);
   if (a->Hq % a->Hkv != 0) return fail(KVSKIP_E_INVALID, "Hq must be a multiple of Hkv");
   const int G = a->Hq / a->Hkv;
-  if (!kvs::attn_supported(a->D, G))
+  if (eight_bit ? !((a->D == 64 || a->D == 128) && G <= 16) : !kvs::attn_supported(a->D, G))
     return fail(KVSKIP_E_UNSUPPORTED, "kvskip: unsupported head dim / group size (D=%d, G=%d)", a->D, G);
   if (need_q) {
     if (a->q == nullptr) return fail(KVSKIP_E_INVALID, "q must be CUDA bf16 [B, Hq, D]");
@@ -130,6 +131,9 @@ int kvskip_struct_size(int which) {
     case 1: return static_cast<int>(sizeof(kvskip_plan_args));
     case 2: return static_cast<int>(sizeof(kvskip_update_args));
     case 3: return static_cast<int>(sizeof(kvskip_select_args));
+    case 5: return static_cast<int>(sizeof(kvskip_cache8_args));
+    case 6: return static_cast<int>(sizeof(kvskip_page_args));
+    case 7: return static_cast<int>(sizeof(kvskip_write_args));
     default: return -1;
   }
 }
@@ -526,6 +530,105 @@ int kvskip_token_index(const int32_t* ids, int64_t ids_stride, int32_t B, int32_
   if ((T + KVSKIP_BLOCK - 1) / KVSKIP_BLOCK > NBC) return fail(KVSKIP_E_INVALID, "block capacity exceeded");
   return launched(kvs::launch_token_index(ids, ids_stride, B, T, idx, NBC, seq_lens, static_cast<hipStream_t>(stream)),
                   "kvskip_token_index");
+}
+
+int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int stats, void* stream) {
+  kvs::Attn8P p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = prepare_attn(a, true, false, false, &p, true);
+  if (rc != KVSKIP_OK) return rc;
+  if (c == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
+  if (c->format != KVSKIP_E4M3 && c->format != KVSKIP_INT8)
+    return fail(KVSKIP_E_INVALID, "decode8: format e4m3 or int8 (got %d)", c->format);
+  const void* kv[2] = {a->k, a->v};
+  const int64_t st[2][3] = {{a->k_sb, a->k_sh, a->k_st}, {a->v_sb, a->v_sh, a->v_st}};
+  for (int i = 0; i < 2; ++i) {
+    const char* n = i == 0 ? "k" : "v";
+    if (kv[i] == nullptr || !aligned16(kv[i])) return fail(KVSKIP_E_INVALID, "%s must be 16-byte aligned", n);
+    if (st[i][0] % 16 != 0 || st[i][1] % 16 != 0 || st[i][2] % 16 != 0)
+      return fail(KVSKIP_E_INVALID, "%s strides must be multiples of 16 elements (16-byte rows)", n);
+    if (st[i][2] < 0 || st[i][2] >= (int64_t(1) << 24))
+      return fail(KVSKIP_E_UNSUPPORTED, "%s: token stride in [0, 2^24)", n);
+  }
+  if (c->k_scale == nullptr || c->v_scale == nullptr) return fail(KVSKIP_E_INVALID, "decode8: k_scale and v_scale");
+  if (a->out == nullptr) return fail(KVSKIP_E_INVALID, "out is required");
+  if (stats && (a->blk_max == nullptr || a->blk_sum == nullptr))
+    return fail(KVSKIP_E_INVALID, "stats needs blk_max and blk_sum");
+  if (a->num_splits > 1 && a->part_acc == nullptr)
+    return fail(KVSKIP_E_INVALID, "num_splits > 1 needs the split partial buffers");
+  if (a->p_out != nullptr || a->key_sums != nullptr)
+    return fail(KVSKIP_E_UNSUPPORTED, "decode8: no fp16 P and no key sums");
+  if (a->block_idx != nullptr) {
+    if (a->block_cnt == nullptr) return fail(KVSKIP_E_INVALID, "block_cnt is required with block_idx");
+    if (a->max_blocks < 0) return fail(KVSKIP_E_INVALID, "block_idx must be contiguous int32 [B, Hkv, max_blocks]");
+  }
+  if (a->seq_lens != nullptr) {
+    if (a->num_splits < 2) return fail(KVSKIP_E_INVALID, "seq_lens needs num_splits >= 2");
+    if (a->B > kvs::MAX_RAGGED_B) return fail(KVSKIP_E_UNSUPPORTED, "seq_lens: B <= %d", kvs::MAX_RAGGED_B);
+  }
+  if (a->list_partition != 0) {
+    if (a->list_partition != 1) return fail(KVSKIP_E_INVALID, "list_partition in {0, 1}");
+    if (a->block_idx == nullptr || a->seq_lens == nullptr)
+      return fail(KVSKIP_E_INVALID, "list_partition 1 partitions a masked ragged pass (block_idx and seq_lens)");
+    if (static_cast<int64_t>(a->B) * a->Hkv > kvs::MAX_GLOBAL_LISTS)
+      return fail(KVSKIP_E_UNSUPPORTED, "list_partition 1: B * Hkv <= %d", kvs::MAX_GLOBAL_LISTS);
+  }
+  if (a->block_table != nullptr && (a->num_pages < 1 || a->bt_stride < p.nb))
+    return fail(KVSKIP_E_INVALID, "paged cache: num_pages >= 1 and block_table rows of ceil(T / 64) pages");
+  p.k_scale = c->k_scale;
+  p.v_scale = c->v_scale;
+  p.ks_sb = c->ks_sb; p.ks_sh = c->ks_sh;
+  p.vs_sb = c->vs_sb; p.vs_sh = c->vs_sh;
+  p.G = a->Hq / a->Hkv;
+  return launched(kvs::launch_decode8(p, a->D, c->format == KVSKIP_INT8, stats != 0, static_cast<hipStream_t>(stream)),
+                  "kvskip_decode8");
+}
+
+int64_t kvskip_page_work_ints(int32_t B, int32_t rows) {
+  return B < 1 || B > kvs::MAX_PAGE_B || rows < 0 ? -1 : kvs::page_work_ints(B, rows);
+}
+
+int kvskip_page_map(const kvskip_page_args* p, void* stream) {
+  if (p == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
+  if (p->B < 1 || p->width < 1 || p->num_pages < 1 || p->rows < 0)
+    return fail(KVSKIP_E_INVALID, "page_map: sizes must be positive (B=%d width=%d num_pages=%d rows=%d)", p->B, p->width,
+                p->num_pages, p->rows);
+  if (p->B > kvs::MAX_PAGE_B) return fail(KVSKIP_E_UNSUPPORTED, "page_map: B <= %d", kvs::MAX_PAGE_B);
+  const int64_t most = int64_t(1) << 31;
+  if (p->B * (static_cast<int64_t>(p->rows) + 1) >= most || static_cast<int64_t>(p->B) * p->width >= most ||
+      static_cast<int64_t>(p->num_pages) * KVSKIP_BLOCK >= most)
+    return fail(KVSKIP_E_UNSUPPORTED, "page_map: B * (rows + 1), B * width and 64 * num_pages below 2^31");
+  if (p->bt_stride < p->width) return fail(KVSKIP_E_INVALID, "page_map: block_table rows must not overlap");
+  if (p->seq_lens == nullptr || p->new_lens == nullptr || p->held == nullptr || p->block_table == nullptr ||
+      p->free_pages == nullptr || p->free_count == nullptr || (p->slots == nullptr && p->rows > 0) ||
+      p->starts == nullptr || p->held_out == nullptr || p->free_count_out == nullptr || p->short_out == nullptr)
+    return fail(KVSKIP_E_INVALID, "page_map: null tensor");
+  if (p->work == nullptr && kvs::page_work_ints(p->B, p->rows) > 0)
+    return fail(KVSKIP_E_INVALID, "page_map: work of kvskip_page_work_ints(B, rows) int32");
+  return launched(kvs::launch_page_map(*p, static_cast<hipStream_t>(stream)), "kvskip_page_map");
+}
+
+int kvskip_cache_write(const kvskip_write_args* p, void* stream) {
+  if (p == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
+  if (p->N < 0 || p->Hkv < 1 || p->num_pages < 1) return fail(KVSKIP_E_INVALID, "cache_write: sizes must be positive");
+  if (p->D != 64 && p->D != 128) return fail(KVSKIP_E_UNSUPPORTED, "cache_write: D in {64, 128} (D=%d)", p->D);
+  if (p->Hkv > 65535) return fail(KVSKIP_E_UNSUPPORTED, "cache_write: Hkv <= 65535");
+  if (static_cast<int64_t>(p->num_pages) * KVSKIP_BLOCK >= (int64_t(1) << 31) || p->N > (1 << 30))
+    return fail(KVSKIP_E_UNSUPPORTED, "cache_write: 64 * num_pages below 2^31, N up to 2^30");
+  if (p->format != KVSKIP_E4M3 && p->format != KVSKIP_INT8 && p->format != KVSKIP_BF16)
+    return fail(KVSKIP_E_INVALID, "cache_write: format e4m3, int8 or bf16 (got %d)", p->format);
+  if (p->k_pool == nullptr || p->v_pool == nullptr || (p->N > 0 && (p->k == nullptr || p->v == nullptr || p->slot_map == nullptr)))
+    return fail(KVSKIP_E_INVALID, "cache_write: null tensor");
+  if (p->format != KVSKIP_BF16 && (p->k_scale == nullptr || p->v_scale == nullptr))
+    return fail(KVSKIP_E_INVALID, "cache_write: k_scale and v_scale with an 8-bit pool");
+  if (p->k_sn % 8 != 0 || p->k_sh % 8 != 0 || p->v_sn % 8 != 0 || p->v_sh % 8 != 0 || !aligned16(p->k) || !aligned16(p->v))
+    return fail(KVSKIP_E_INVALID, "cache_write: k, v rows must be 16-byte aligned");
+  const int m = p->format == KVSKIP_BF16 ? 8 : 16;
+  if (p->kp_sb % m != 0 || p->kp_sh % m != 0 || p->kp_st % m != 0 || p->vp_sb % m != 0 || p->vp_sh % m != 0 ||
+      p->vp_st % m != 0 || !aligned16(p->k_pool) || !aligned16(p->v_pool))
+    return fail(KVSKIP_E_INVALID, "cache_write: pool rows must be 16-byte aligned");
+  if (p->N == 0) return ok();
+  return launched(kvs::launch_cache_write(*p, static_cast<hipStream_t>(stream)), "kvskip_cache_write");
 }
 
 }  // extern "C"

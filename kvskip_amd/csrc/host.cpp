@@ -44,6 +44,10 @@ struct Api {
   int (*decode_splits_update)(const kvskip_attn_args*, const kvskip_update_args*, void*);
   int (*decode_splits_planned)(const kvskip_attn_args*, const kvskip_plan_args*, const kvskip_update_args*, void*);
   int64_t (*plan_part_floats)(int32_t, int32_t, int32_t, int32_t);
+  int (*decode8)(const kvskip_attn_args*, const kvskip_cache8_args*, int, void*);
+  int (*page_map)(const kvskip_page_args*, void*);
+  int64_t (*page_work_ints)(int32_t, int32_t);
+  int (*cache_write)(const kvskip_write_args*, void*);
   const char* (*last_error)();
 };
 constexpr int N_API = sizeof(Api) / sizeof(void*);
@@ -769,6 +773,160 @@ PyObject* update(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
+// ---- caches held in 8 bits, pages
+int cache_format(const at::Tensor& t, const std::string& n) {
+  const at::ScalarType ty = t.scalar_type();
+  if (!t.is_cuda() || (ty != at::kFloat8_e4m3fn && ty != at::kChar))
+    fail(n + " must be a CUDA float8_e4m3fn or int8 tensor");
+  return ty == at::kChar ? KVSKIP_INT8 : KVSKIP_E4M3;
+}
+void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> ts, const char* msg) {
+  for (const at::Tensor* t : ts)
+    if (t != nullptr && t->device() != a.device()) fail(msg);
+}
+
+// decode8(q, k, v, k_scale, v_scale, scale, block_idx, block_cnt, stats, num_splits, want_f32, seq_lens, block_table, T,
+//         list_partition)
+PyObject* decode8(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &ks = tensor(a[3], "k_scale"),
+                   &vs = tensor(a[4], "v_scale");
+  check_q(q);
+  kvskip_cache8_args c;
+  std::memset(&c, 0, sizeof(c));
+  c.format = cache_format(k, "k");
+  require(cache_format(v, "v") == c.format, "k and v must have one type");
+  for (const at::Tensor* t : {&k, &v}) {
+    require(t->dim() == 4 && t->stride(3) == 1, "k, v must be [B, Hkv, T, D] with a contiguous last dim");
+    require(t->stride(0) % 16 == 0 && t->stride(1) % 16 == 0 && t->stride(2) % 16 == 0 && aligned16(*t),
+            "k, v rows must be 16-byte aligned (strides multiples of 16 elements)");
+  }
+  const at::Tensor *bi = opt_tensor(a[6], "block_idx"), *bc = opt_tensor(a[7], "block_cnt"),
+                   *lens = opt_tensor(a[11], "seq_lens"), *bt = opt_tensor(a[12], "block_table");
+  same_device(q, {&k, &v, &ks, &vs, bi, bc, lens, bt}, "decode8: tensors on one device");
+  const Dims d = kv_dims(q, k, v, bt, a[13]);
+  require(d.B > 0 && d.T > 0, "sizes must be positive");
+  require(d.Hkv > 0 && d.Hq % d.Hkv == 0, "Hq must be a multiple of Hkv");
+  for (const at::Tensor* t : {&ks, &vs}) {
+    require(t->scalar_type() == at::kFloat, "k_scale, v_scale: fp32");
+    if (bt == nullptr)
+      require(t->dim() == 3 && t->size(0) == d.B && t->size(1) == d.Hkv && t->size(2) >= d.nb &&
+                  (t->size(2) == 1 || t->stride(2) == 1),
+              "k_scale, v_scale: [B, Hkv, >= ceil(T / 64)], blocks contiguous");
+    else
+      require(t->dim() == 2 && t->size(0) == k.size(0) && t->size(1) == d.Hkv, "paged cache: k_scale, v_scale [num_pages, Hkv]");
+  }
+  const bool stats = truth(a[8]), want_f32 = truth(a[10]);
+  const int64_t S = integer(a[9]);
+  require(1 <= S && S <= 256, "num_splits in 1..256");
+  const at::Device dev = q.device();
+  Outs o;
+  at::Tensor out = empty({d.B, d.Hq, d.D}, at::kBFloat16, dev), lse = empty({d.B, d.Hq}, at::kFloat, dev), out32, bmax,
+             bsum, part;
+  o.out = out.data_ptr(), o.lse = lse.data_ptr();
+  if (want_f32) o.out32 = (out32 = empty({d.B, d.Hq, d.D}, at::kFloat, dev)).data_ptr();
+  if (stats) {
+    o.bmax = (bmax = empty({d.B, d.Hq, d.nb}, at::kFloat, dev)).data_ptr();
+    o.bsum = (bsum = empty({d.B, d.Hq, d.nb}, at::kFloat, dev)).data_ptr();
+  }
+  if (S > 1) part = partials(o, d, S, true, dev);
+  kvskip_attn_args args;
+  set_decode(args, q, k, v, real(a[5]), bi, bc, S, o, lens, bt, a[13], int32(a[14]));
+  c.k_scale = static_cast<const float*>(ks.data_ptr()), c.ks_sb = ks.stride(0), c.ks_sh = ks.stride(1);
+  c.v_scale = static_cast<const float*>(vs.data_ptr()), c.vs_sb = vs.stride(0), c.vs_sh = vs.stride(1);
+  launch(dev, [&](void* s) { return api.decode8(&args, &c, stats, s); });
+  return list_of({out, lse, bmax, bsum, out32});
+}
+
+// page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts, short, held_out,
+//          free_count_out)
+PyObject* page_map(PyObject* const* a) {
+  const at::Tensor &lens = tensor(a[0], "seq_lens"), &add = tensor(a[1], "new_lens"), &held = tensor(a[2], "held"),
+                   &bt = tensor(a[3], "block_table"), &pool = tensor(a[4], "free_pages"), &cnt = tensor(a[5], "free_count"),
+                   &slots = tensor(a[6], "slot_map");
+  require(lens.is_cuda() && is(lens, at::kInt) && lens.dim() == 1 && lens.numel() > 0, "seq_lens: contiguous CUDA int32 [B]");
+  const int64_t B = lens.numel();
+  auto ints = [&](const at::Tensor& t, int64_t n, const char* name) {
+    if (!(t.device() == lens.device() && is(t, at::kInt) && t.numel() == n))
+      fail(std::string("page_map: ") + name + ": contiguous int32 of " + std::to_string(n) + " on seq_lens' device");
+    return static_cast<int32_t*>(t.data_ptr());
+  };
+  kvskip_page_args p;
+  std::memset(&p, 0, sizeof(p));
+  p.seq_lens = static_cast<const int32_t*>(lens.data_ptr());
+  p.new_lens = ints(add, B, "new_lens"), p.held = ints(held, B, "held");
+  require(bt.device() == lens.device() && bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) == B &&
+              bt.size(1) > 0 && (bt.size(1) == 1 || bt.stride(1) == 1) && (B == 1 || bt.stride(0) >= bt.size(1)),
+          "block_table: int32 [B, width] on the device, rows contiguous");
+  require(pool.numel() > 0 && pool.numel() < (int64_t(1) << 25) && slots.numel() < (int64_t(1) << 31) &&
+              bt.size(1) < (int64_t(1) << 31) && B < (int64_t(1) << 31),
+          "page_map: B * (rows + 1), B * width and 64 * num_pages below 2^31");
+  p.block_table = static_cast<int32_t*>(bt.data_ptr()), p.bt_stride = B == 1 ? bt.size(1) : bt.stride(0);
+  p.free_pages = ints(pool, pool.numel(), "free_pages"), p.free_count = ints(cnt, 1, "free_count");
+  p.slots = ints(slots, slots.numel(), "slot_map");
+  p.B = static_cast<int32_t>(B), p.width = static_cast<int32_t>(bt.size(1));
+  p.num_pages = static_cast<int32_t>(pool.numel()), p.rows = static_cast<int32_t>(slots.numel());
+  const at::Device dev = lens.device();
+  auto out = [&](PyObject* o, int64_t n, const char* name, at::Tensor& t) {
+    if (const at::Tensor* given = opt_tensor(o, name)) {
+      t = *given;
+      return ints(t, n, name);
+    }
+    t = empty({n}, at::kInt, dev);
+    return static_cast<int32_t*>(t.data_ptr());
+  };
+  at::Tensor starts, shrt, work;
+  p.starts = out(a[7], B + 1, "starts", starts);
+  p.short_out = out(a[8], 1, "short", shrt);
+  const at::Tensor *ho = opt_tensor(a[9], "held_out"), *co = opt_tensor(a[10], "free_count_out");
+  p.held_out = ho != nullptr ? ints(*ho, B, "held_out") : static_cast<int32_t*>(held.data_ptr());
+  p.free_count_out = co != nullptr ? ints(*co, 1, "free_count_out") : static_cast<int32_t*>(cnt.data_ptr());
+  const int64_t n_work = api.page_work_ints(p.B, p.rows);
+  if (n_work > 0) p.work = static_cast<int32_t*>((work = empty({n_work}, at::kInt, dev)).data_ptr());
+  launch(dev, [&](void* s) { return api.page_map(&p, s); });
+  return list_of({slots, starts, shrt});
+}
+
+// cache_write(k, v, slot_map, k_pool, v_pool, k_scale, v_scale)
+PyObject* cache_write(PyObject* const* a) {
+  const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &slots = tensor(a[2], "slot_map"),
+                   &kp = tensor(a[3], "k_pool"), &vp = tensor(a[4], "v_pool");
+  const at::Tensor *ks = opt_tensor(a[5], "k_scale"), *vs = opt_tensor(a[6], "v_scale");
+  kvskip_write_args p;
+  std::memset(&p, 0, sizeof(p));
+  for (const at::Tensor* t : {&k, &v})
+    require(is_bf16_cuda(*t) && t->dim() == 3 && (t->size(2) == 1 || t->stride(2) == 1) && t->sizes() == k.sizes(),
+            "k, v must be CUDA bf16 [N, Hkv, D] with a contiguous last dim");
+  const int64_t N = k.size(0), Hkv = k.size(1), D = k.size(2);
+  require(is(slots, at::kInt) && slots.numel() == N, "slot_map: contiguous int32 [N] on the device");
+  p.format = kp.scalar_type() == at::kBFloat16 ? KVSKIP_BF16 : cache_format(kp, "k_pool");
+  require(vp.scalar_type() == kp.scalar_type(), "k_pool and v_pool must have one type");
+  for (const at::Tensor* t : {&kp, &vp})
+    require(t->dim() == 4 && t->size(0) == kp.size(0) && t->size(1) == Hkv && t->size(2) == TILE && t->size(3) == D &&
+                t->stride(3) == 1,
+            "k_pool, v_pool must be page pools [num_pages, Hkv, 64, D] with a contiguous last dim");
+  require(p.format == KVSKIP_BF16 ? ks == nullptr && vs == nullptr : ks != nullptr && vs != nullptr,
+          "k_scale and v_scale belong to an 8-bit pool");
+  for (const at::Tensor* t : {ks, vs})
+    require(t == nullptr || (t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == kp.size(0) && t->size(1) == Hkv),
+            "k_scale, v_scale: fp32 [num_pages, Hkv]");
+  same_device(k, {&v, &slots, &kp, &vp, ks, vs}, "cache_write: tensors on one device");
+  require(N <= (int64_t(1) << 30) && kp.size(0) < (int64_t(1) << 25) && Hkv <= 65535,
+          "cache_write: 64 * num_pages below 2^31, N up to 2^30, Hkv <= 65535");
+  p.k = k.data_ptr(), p.k_sn = N > 1 ? k.stride(0) : 0, p.k_sh = Hkv > 1 ? k.stride(1) : 0;
+  p.v = v.data_ptr(), p.v_sn = N > 1 ? v.stride(0) : 0, p.v_sh = Hkv > 1 ? v.stride(1) : 0;
+  p.slot_map = static_cast<const int32_t*>(slots.data_ptr());
+  p.k_pool = kp.data_ptr(), p.kp_sb = kp.stride(0), p.kp_sh = kp.stride(1), p.kp_st = kp.stride(2);
+  p.v_pool = vp.data_ptr(), p.vp_sb = vp.stride(0), p.vp_sh = vp.stride(1), p.vp_st = vp.stride(2);
+  if (ks != nullptr) {
+    p.k_scale = static_cast<float*>(ks->data_ptr()), p.ks_sb = ks->stride(0), p.ks_sh = ks->stride(1);
+    p.v_scale = static_cast<float*>(vs->data_ptr()), p.vs_sb = vs->stride(0), p.vs_sh = vs->stride(1);
+  }
+  p.N = static_cast<int32_t>(N), p.Hkv = static_cast<int32_t>(Hkv), p.D = static_cast<int32_t>(D);
+  p.num_pages = static_cast<int32_t>(kp.size(0));
+  launch(k.device(), [&](void* s) { return api.cache_write(&p, s); });
+  Py_RETURN_NONE;
+}
+
 // num_splits(bh, n_tiles, slots, max_splits, min_tiles): kvskip.num_splits_for's rule over `slots`
 // resident workgroups, count by count in the same double arithmetic. In Python the scan took 45 us of a
 // decode call at 32k (63.8 us a call, 27 of them kernels) and 80 us of a planner layer-step.
@@ -869,6 +1027,7 @@ PyMethodDef methods[] = {
     KVS_FN(attn_block, 20), KVS_FN(vskip1, 13), KVS_FN(select, 10), KVS_FN(pv, 9), KVS_FN(pv_select, 13),
     KVS_FN(plan_block, 33), KVS_FN(update_block, 24), KVS_FN(plan, 2), KVS_FN(merge_update, 3), KVS_FN(plan_scores, 2),
     KVS_FN(update, 2), KVS_FN(num_splits, 5), KVS_FN(zeroed, 2),
+    KVS_FN(decode8, 15), KVS_FN(page_map, 11), KVS_FN(cache_write, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -46,6 +46,15 @@ struct AttnP {
   int list_partition;  // masked ragged pass: 0 per KV head, 1 over all B * Hkv lists
 };
 
+// Argument block of the pass over a cache held in 8 bits: k and v are bytes (strides in elements), with a
+// scale for each block and head; G = Hq / Hkv.
+struct Attn8P : AttnP {
+  const float* k_scale;  // block blk of (b, h): [b * ks_sb + h * ks_sh + blk]; paged: page pg: [pg * ks_sb + h * ks_sh]
+  const float* v_scale;
+  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  int G;
+};
+
 // The planned pass's argument segment (AttnP, kvskip_plan_args and, where an update is carried,
 // kvskip_update_args: 640 or 808 bytes, 10 or 13 lines of 64 bytes) loaded into the scalar cache
 // in one batch with one wait, as the kernel's first statement (the loaded words are unused). Read
@@ -125,6 +134,8 @@ hipError_t launch_planned_paged(const AttnP& a, const kvskip_plan_args& pa, cons
 // unfused carried update (its own translation unit).
 hipError_t launch_planned_ragged(const AttnP& a, const kvskip_plan_args& pa, const kvskip_update_args* u, int D,
                                  hipStream_t s);
+// The pass over a cache held in 8 bits and its merge (attn_decode8.hip); G = 1 .. 16.
+hipError_t launch_decode8(const Attn8P& p, int D, bool i8, bool stats, hipStream_t s);
 // The plan's first launch alone (the scores pass; needs part).
 hipError_t launch_plan_scores(const kvskip_plan_args& p, hipStream_t s);
 hipError_t launch_block_sums(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, int B, int Hkv, int T,
@@ -137,6 +148,12 @@ hipError_t launch_token_index(const int32_t* ids, int64_t ids_stride, int B, int
 hipError_t launch_select(const kvskip_select_args& a, hipStream_t s);
 hipError_t launch_block_list(const uint8_t* keep, int B, int Hkv, int nb, int32_t* block_idx, int32_t* block_cnt,
                              hipStream_t s);
+
+// Pages (pages.hip): a step's block tables and slot map; its rows into the pages.
+constexpr int MAX_PAGE_B = 4096;  // requests of a step (their sums are held in LDS)
+int page_work_ints(int B, int rows);
+hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s);
+hipError_t launch_cache_write(const kvskip_write_args& p, hipStream_t s);
 
 // Largest block count the planner kernels hold in LDS for a group of G query heads.
 int planner_max_blocks(int G);

@@ -6,7 +6,9 @@ with torch on the inputs' device; launches go to torch's current stream; nothing
 Absent outputs are returned as None (the reference returns undefined tensors).
 
 Extra operators with no counterpart in kvskip_ext: block_sums and token_index (the device-side
-planner initialisation and token index) and decode_into (decode into caller-owned buffers).
+planner initialisation and token index), decode_into (decode into caller-owned buffers), decode8
+(decode over a cache held in 8 bits), page_map and cache_write (a serving step's block tables, slot
+map and cache rows).
 
 Paged caches (block_table and T; not in the reference): k, v are page pools [num_pages, Hkv, 64, D]
 whose page block_table[b, j] (int32 [B, >= ceil(T / 64)] on the device) holds tokens 64 j .. 64 j + 63
@@ -118,6 +120,40 @@ def decode_into(q, k, v, scale, bufs: dict, block_idx=None, block_cnt=None, stat
     sequences' blocks there (kvskip_attn_args.key_sums; blocks past a sequence's end are left alone)."""
     _host().decode_into(q, k, v, scale, bufs, block_idx, block_cnt, stats, num_splits, seq_lens, phase, block_table, T,
                         list_partition, key_sums)
+
+
+def decode8(q, k, v, k_scale, v_scale, scale, block_idx=None, block_cnt=None, stats=False, num_splits=1, want_f32=False,
+            seq_lens=None, block_table=None, T=None, list_partition=0):
+    """Split-K decode attention over a cache held in 8 bits (kvskip_decode8; not in kvskip_ext): k, v are
+    float8_e4m3fn or int8 (one type), [B, Hkv, T, D] views with k_scale, v_scale fp32 [B, Hkv, >= ceil(T / 64)], or,
+    with block_table and T, page pools [num_pages, Hkv, 64, D] with scales [num_pages, Hkv]; a code stands for
+    code * its block's scale. Strides are multiples of 16 elements, D contiguous. The other arguments as decode's;
+    a sequence of length 0 gets out 0 and lse -inf. G = Hq / Hkv in 1..16, D in {64, 128}.
+    Returns [out bf16 [B, Hq, D], lse fp32 [B, Hq], blk_max, blk_sum ([B, Hq, nb] or None), out_f32 or None]."""
+    return _host().decode8(q, k, v, k_scale, v_scale, scale, block_idx, block_cnt, stats, num_splits, want_f32, seq_lens,
+                           block_table, T, list_partition)
+
+
+def page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts=None, short=None,
+             held_out=None, free_count_out=None):
+    """A serving step's block tables and slot map from the requests' lengths, on the device (kvskip_page_map; not in
+    kvskip_ext). All int32 on one device: seq_lens [B] (tokens after the step; 0: finished, its pages go back),
+    new_lens [B] (of them new), held [B] (pages of each table row), block_table [B, width], free_pages [num_pages] and
+    free_count [1] (the free stack), slot_map [rows]. Pages given back first, then taken request by request; a request
+    that cannot be served keeps what it holds and gets slots -1.
+    Updates block_table and free_pages, and held and free_count (or writes held_out, free_count_out). Row i of the
+    step's packed new tokens (request b's from starts[b] on) goes to slot_map[i] = page * 64 + offset; -1 past the last.
+    Returns [slot_map, starts int32 [B + 1], short int32 [1] (requests not served)]; starts, short: optional buffers."""
+    return _host().page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts, short,
+                            held_out, free_count_out)
+
+
+def cache_write(k, v, slot_map, k_pool, v_pool, k_scale=None, v_scale=None):
+    """New keys and values bf16 [N, Hkv, D] into page pools [num_pages, Hkv, 64, D] at the slots of slot_map (int32 [N];
+    -1 leaves a row out), in place (kvskip_cache_write; not in kvskip_ext). Pools are bf16, or float8_e4m3fn / int8 with
+    k_scale, v_scale fp32 [num_pages, Hkv], which grow by powers of two as rows need it (a page whose row 0 is written
+    starts anew). The rows of a page must lie next to each other in the map, as page_map's do."""
+    _host().cache_write(k, v, slot_map, k_pool, v_pool, k_scale, v_scale)
 
 
 class DecodeOp:

@@ -108,7 +108,8 @@ def _as_bhd(q: torch.Tensor) -> torch.Tensor:
 def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = False, load_v: bool = True,
            num_splits: int | None = None, stages: int = 2, out_f32: bool = False, write_p: bool = False,
            seq_lens: torch.Tensor | None = None, block_table: torch.Tensor | None = None,
-           T: int | None = None, merge: bool = True) -> dict:
+           T: int | None = None, merge: bool = True, k_scale: torch.Tensor | None = None,
+           v_scale: torch.Tensor | None = None) -> dict:
     """Decode attention of one layer (kernels/kvskip.py:88-113). Returns a dict with out [B, Hq, D]
     bf16 (None with load_v=False), lse [B, Hq] fp32, num_splits, and as asked blk_max / blk_sum
     [B, Hq, nb] fp32, out_f32, p (fp16 [B, Hq, nb*64] = exp(s - blk_max)).
@@ -116,7 +117,9 @@ def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = Fal
     capacity T, the split budget shared by the batch (with a plan, up to 512 lists, the lists of all
     KV heads cut by one chunk length: kvskip_attn_args.list_partition); block_table (int32 [B, >=
     ceil(T / 64)]) with T makes k, v page pools [num_pages, Hkv, 64, D]; merge=False (with
-    load_v=False) skips the split merge, leaving lse None."""
+    load_v=False) skips the split merge, leaving lse None; k_scale, v_scale (fp32 [B, Hkv, nb], or
+    [num_pages, Hkv] over pages) make k, v a cache held in 8 bits (float8_e4m3fn or int8, a scale for
+    each block and head: ext.decode8; G up to 16; with V only, no P)."""
     q = _as_bhd(q)
     B, Hkv = q.shape[0], k.shape[1]
     tokens = k.shape[2] if block_table is None else int(T)
@@ -127,9 +130,18 @@ def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = Fal
                       else num_splits_for(B * Hkv, items))
     lists = (None, None) if plan is None else (plan.block_idx, plan.block_cnt)
     lp = int(plan is not None and seq_lens is not None and B > 1 and B * Hkv <= 512)
-    out, lse, bmax, bsum, o32, p = ext().decode(q, k, v, float(scale), *lists, stats, load_v, int(num_splits),
-                                                int(stages), out_f32, write_p, seq_lens, **_paged(block_table, T),
-                                                merge=merge, list_partition=lp)
+    if (k_scale is None) != (v_scale is None):
+        raise RuntimeError("decode: k_scale and v_scale belong together")
+    if k_scale is not None:
+        if not load_v or write_p or not merge:
+            raise RuntimeError("decode: a cache held in 8 bits is read with V, without P, and merged")
+        out, lse, bmax, bsum, o32 = ext().decode8(q, k, v, k_scale, v_scale, float(scale), *lists, stats,
+                                                  int(num_splits), out_f32, seq_lens, block_table, T, lp)
+        p = None
+    else:
+        out, lse, bmax, bsum, o32, p = ext().decode(q, k, v, float(scale), *lists, stats, load_v, int(num_splits),
+                                                    int(stages), out_f32, write_p, seq_lens, **_paged(block_table, T),
+                                                    merge=merge, list_partition=lp)
     res = {"out": out, "lse": lse, "num_splits": num_splits}
     extra = {"blk_max": bmax, "blk_sum": bsum} if stats else {}
     if out_f32:
