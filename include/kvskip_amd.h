@@ -428,7 +428,7 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
  *      a page outside [0, num_pages), and for rows from starts[B] on. Rows past `rows` have no slot.
  * held_out and free_count_out may be held and free_count (the step in place) or buffers of their own (the state before
  * stays, but for table entries and stack positions that it does not count). Table entries past held_out are not cleared.
- * B <= 4096; B * (rows + 1), B * width and 64 * num_pages below 2^31. work: kvskip_page_work_ints(B, rows) int32, or
+ * B <= 2048; B * (rows + 1), B * width and 64 * num_pages below 2^31. work: kvskip_page_work_ints(B, rows) int32, or
  * NULL where that is 0. No atomics: the same result every time. */
 typedef struct kvskip_page_args {
   const int32_t* seq_lens;     /* [B] */

@@ -150,7 +150,7 @@ hipError_t launch_block_list(const uint8_t* keep, int B, int Hkv, int nb, int32_
                              hipStream_t s);
 
 // Pages (pages.hip): a step's block tables and slot map; its rows into the pages.
-constexpr int MAX_PAGE_B = 4096;  // requests of a step (their sums are held in LDS)
+constexpr int MAX_PAGE_B = 2048;  // requests of a step (their sums are held in LDS)
 int page_work_ints(int B, int rows);
 hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s);
 hipError_t launch_cache_write(const kvskip_write_args& p, hipStream_t s);

@@ -14,6 +14,7 @@
 // written an element. A scale is a power of two: dividing by it is exact, so a code depends on its value and scale
 // alone, and when a later row needs a larger scale, the rows that are there move to it without rounding again (e4m3:
 // but for subnormal codes; int8 rounds once more per doubling, less than the final step in sum).
+#include <cstdlib>
 #include "common.hpp"
 #include "internal.hpp"
 
@@ -24,20 +25,23 @@ namespace {
 constexpr int PT = 1024;  // threads of the summing workgroup
 constexpr int PF = 256;   // threads of a filling workgroup
 
-// A step's sums, in LDS: first row of each request (starts[B]: all rows), pages taken before it (or -1: not served),
-// pages held before it.
+// A step's sums, in LDS: first row of each request (starts[B]: all rows), pages given back before it, pages taken
+// before it (or -1: not served), pages held before the step.
 struct Step {
   int starts[MAX_PAGE_B + 1];
+  int given[MAX_PAGE_B];
   int taken[MAX_PAGE_B];
   int held[MAX_PAGE_B];
 };
+
+__device__ __forceinline__ int pages_of(int n) { return n / BLK + (n % BLK != 0); }
 
 // A request's sizes from its lengths: false if its tokens do not fit a table row.
 __device__ __forceinline__ bool page_need(const kvskip_page_args& p, int b, int& n, int& a, int& h, int& need) {
   n = max(p.seq_lens[b], 0);
   a = min(max(p.new_lens[b], 0), n);
   h = min(max(p.held[b], 0), p.width);
-  need = n / BLK + (n % BLK != 0);
+  need = pages_of(n);
   return need <= p.width;
 }
 
@@ -53,12 +57,12 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
   return incl - v + (wave > 0 ? __shfl(x, wave - 1, WAVE) : 0);
 }
 
-// Request of row i: the last b with starts[b] <= i (requests without rows share their start with the next).
-__device__ __forceinline__ int request_of(const int* starts, int B, int i) {
+// The last b with first[b] <= i (of requests with one value the last: the others have nothing there).
+__device__ __forceinline__ int request_of(const int* first, int B, int i) {
   int lo = 0, hi = B - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (starts[mid] <= i)
+    if (first[mid] <= i)
       lo = mid;
     else
       hi = mid - 1;
@@ -66,37 +70,68 @@ __device__ __forceinline__ int request_of(const int* starts, int B, int i) {
   return lo;
 }
 
+// The k-th page taken by the step: from the stack as it was, or of those given back by this step (position g of them).
+__device__ __forceinline__ int taken_page(const kvskip_page_args& p, const Step& s, int count, int avail, int k) {
+  const int g = avail - 1 - k - count;
+  if (g < 0) return p.free_pages[avail - 1 - k];
+  const int b = request_of(s.given, p.B, g);
+  return p.block_table[b * p.bt_stride + pages_of(max(p.seq_lens[b], 0)) + g - s.given[b]];
+}
+
 // Row i's slot, or -1.
-__device__ __forceinline__ int row_slot(const kvskip_page_args& p, const Step& s, int avail, int i) {
+__device__ __forceinline__ int row_slot(const kvskip_page_args& p, const Step& s, int count, int avail, int i) {
   if (i >= s.starts[p.B]) return -1;
   const int b = request_of(s.starts, p.B, i), before = s.taken[b];
   if (before < 0) return -1;
   const int n = max(p.seq_lens[b], 0), a = min(max(p.new_lens[b], 0), n);
   const int pos = n - a + (i - s.starts[b]), j = pos / BLK, h = s.held[b];
-  const int pg = j < h ? p.block_table[b * p.bt_stride + j] : p.free_pages[avail - 1 - (before + j - h)];
+  const int pg = j < h ? p.block_table[b * p.bt_stride + j] : taken_page(p, s, count, avail, before + j - h);
   return pg >= 0 && pg < p.num_pages ? pg * BLK + pos % BLK : -1;
 }
 
-// The sums; ONE: also the rows' slots and the tables' new entries (the whole operator in one launch).
+// The rows' slots and the pages that change hands, once the sums are in LDS: `threads` threads, this one number t; a
+// wavefront moves the pages of one request (of 64 at a time it skips those with none to move). Nothing that is written
+// is read here: entries given back are read below what a request keeps or in rows that take none, stack positions from
+// `count` on are not read.
+__device__ __forceinline__ void page_fill(const kvskip_page_args& p, const Step& s, int count, int avail, int t, int threads) {
+  for (int i = t; i < p.rows; i += threads) p.slots[i] = row_slot(p, s, count, avail, i);
+  const int lane = threadIdx.x % WAVE, w = __builtin_amdgcn_readfirstlane(t / WAVE), nw = threads / WAVE;
+  for (int b0 = w; b0 < p.B; b0 += nw * WAVE) {
+    const int mine = b0 + nw * lane;
+    bool any = false;
+    if (mine < p.B) {
+      const int need = pages_of(max(p.seq_lens[mine], 0));
+      any = s.taken[mine] >= 0 && need != s.held[mine];
+    }
+    for (uint64_t todo = __ballot(any); todo != 0; todo &= todo - 1) {
+      const int b = b0 + nw * __builtin_ctzll(todo), h = s.held[b], need = pages_of(max(p.seq_lens[b], 0));
+      int32_t* row = p.block_table + b * p.bt_stride;
+      for (int j = h + lane; j < need; j += WAVE) row[j] = taken_page(p, s, count, avail, s.taken[b] + j - h);
+      for (int j = need + lane; j < h; j += WAVE) {
+        const int at = count + s.given[b] + j - need;
+        if (at < p.num_pages) p.free_pages[at] = row[j];
+      }
+    }
+  }
+}
+
+// The sums; ONE: also page_fill (the whole operator in one launch).
 template <bool ONE>
 __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p) {
   __shared__ Step s;
   __shared__ int tmp[PT / WAVE];
   const int tid = threadIdx.x;
   const int count = min(max(*p.free_count, 0), p.num_pages);
-  // pages given back: table[b][need .. h) on the stack, request by request
   int given = 0;
   for (int b0 = 0; b0 < p.B; b0 += PT) {
     const int b = b0 + tid;
     int n, a, h, need, g = 0, all;
     if (b < p.B && page_need(p, b, n, a, h, need)) g = max(h - need, 0);
-    const int at = count + given + block_scan(g, tmp, all);
-    for (int j = 0; j < g; ++j)
-      if (at + j < p.num_pages) p.free_pages[at + j] = p.block_table[b * p.bt_stride + need + j];
+    const int at = given + block_scan(g, tmp, all);
+    if (b < p.B) s.given[b] = at;
     given += all;
   }
   const int avail = min(count + given, p.num_pages);
-  // pages taken and rows
   int taken = 0, rows = 0, short_ = 0, used = 0;
   for (int b0 = 0; b0 < p.B; b0 += PT) {
     const int b = b0 + tid;
@@ -115,8 +150,8 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
       p.starts[b] = start;
       p.held_out[b] = served ? need : h;
     }
-    block_scan(b < p.B && !served ? 1 : 0, tmp, all);
-    short_ += all;
+    // (not served, pages used: counts of at most 2^11 requests and 2^25 pages)
+    short_ += __syncthreads_count(b < p.B && !served);
     block_scan(served ? t : 0, tmp, all);
     used += all;
   }
@@ -126,51 +161,35 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
     *p.short_out = short_;
     *p.free_count_out = avail - used;
   }
-  if constexpr (!ONE) {
-    __syncthreads();
-    // what the filling launch needs: avail, then taken and held of each request
-    if (tid == 0) p.work[0] = avail;
+  __syncthreads();
+  if constexpr (ONE) {
+    page_fill(p, s, count, avail, tid, PT);
+  } else {  // what the filling launch needs beside starts
+    if (tid == 0) p.work[0] = count, p.work[1] = avail;
     for (int b = tid; b < p.B; b += PT) {
-      p.work[1 + b] = s.taken[b];
-      p.work[1 + p.B + b] = s.held[b];
-    }
-  } else {
-    __syncthreads();  // (the pages just given back are read below: same workgroup, same cache)
-    for (int i = tid; i < p.rows; i += PT) p.slots[i] = row_slot(p, s, avail, i);
-    for (int b = tid / 16; b < p.B; b += PT / 16) {
-      if (s.taken[b] < 0) continue;
-      const int n = max(p.seq_lens[b], 0), need = n / BLK + (n % BLK != 0), h = s.held[b];
-      for (int j = h + tid % 16; j < need; j += 16)
-        p.block_table[b * p.bt_stride + j] = p.free_pages[avail - 1 - (s.taken[b] + j - h)];
+      p.work[2 + b] = s.given[b];
+      p.work[2 + p.B + b] = s.taken[b];
+      p.work[2 + 2 * p.B + b] = s.held[b];
     }
   }
 }
 
-// Rows' slots and tables' new entries from the sums.
 __global__ void __launch_bounds__(PF) page_fill_kernel(const kvskip_page_args p) {
   __shared__ Step s;
   const int tid = threadIdx.x;
-  const int avail = p.work[0];
+  const int count = p.work[0], avail = p.work[1];
   for (int b = tid; b < p.B; b += PF) {
     s.starts[b] = p.starts[b];
-    s.taken[b] = p.work[1 + b];
-    s.held[b] = p.work[1 + p.B + b];
+    s.given[b] = p.work[2 + b];
+    s.taken[b] = p.work[2 + p.B + b];
+    s.held[b] = p.work[2 + 2 * p.B + b];
   }
   if (tid == 0) s.starts[p.B] = p.starts[p.B];
   __syncthreads();
-  const int stride = gridDim.x * PF, at = blockIdx.x * PF + tid;
-  for (int i = at; i < p.rows; i += stride) p.slots[i] = row_slot(p, s, avail, i);
-  for (int b = at / 16; b < p.B; b += stride / 16) {
-    if (s.taken[b] < 0) continue;
-    const int n = max(p.seq_lens[b], 0), need = n / BLK + (n % BLK != 0), h = s.held[b];
-    for (int j = h + at % 16; j < need; j += 16)
-      p.block_table[b * p.bt_stride + j] = p.free_pages[avail - 1 - (s.taken[b] + j - h)];
-  }
+  page_fill(p, s, count, avail, blockIdx.x * PF + tid, gridDim.x * PF);
 }
 
 // ------------------------------------------------------------------ cache_write
-constexpr int CT = 256;
-
 enum : int { FMT_E4M3 = 0, FMT_INT8 = 1, FMT_BF16 = 2 };
 
 // The smallest power of two s with amax <= qmax s (amax finite, > 0), at least 2^-126: qmax = (1 + f) 2^k, so s is
@@ -219,60 +238,76 @@ __device__ __forceinline__ void values4(uint32_t w, float (&x)[4]) {
   }
 }
 
-// Workgroup (window, KV head, keys or values): the runs that start in rows [win * w, + win) of the map.
+// One wavefront a workgroup: (window, KV head, keys or values), the runs that start in rows [w0, w0 + win) of the map.
 template <int FMT, int D>
-__global__ void __launch_bounds__(CT) cache_write_kernel(const kvskip_write_args p, int win) {
-  constexpr int LPR = D / 8, RPI = CT / LPR, NI = BLK / RPI;  // lanes a row, rows a pass, passes
-  __shared__ int sSrc[BLK];                                    // source row of each row of the page, or -1
-  __shared__ float sMax[CT / WAVE];
-  const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
+__global__ void __launch_bounds__(WAVE) cache_write_kernel(const kvskip_write_args p, int win) {
+  constexpr int LPR = D / 8, RPI = WAVE / LPR, NI = BLK / RPI;  // lanes a row, rows a load, loads a page
+  constexpr int EB = FMT == FMT_BF16 ? 2 : 1;
+  const int lane = threadIdx.x, c = lane % LPR, r0 = lane / LPR;
   const int h = blockIdx.y;
   const bool isv = blockIdx.z != 0;
-  const uint16_t* rows = static_cast<const uint16_t*>(isv ? p.v : p.k) + h * (isv ? p.v_sh : p.k_sh);
+  const uint16_t* rows = static_cast<const uint16_t*>(isv ? p.v : p.k) + h * (isv ? p.v_sh : p.k_sh) + 8 * c;
   const int64_t sn = isv ? p.v_sn : p.k_sn;
-  char* pool = static_cast<char*>(isv ? p.v_pool : p.k_pool);
-  constexpr int EB = FMT == FMT_BF16 ? 2 : 1;
-  const int64_t psb = (isv ? p.vp_sb : p.kp_sb) * EB, psh = (isv ? p.vp_sh : p.kp_sh) * EB,
-                pst = (isv ? p.vp_st : p.kp_st) * EB;
-  const int64_t slots = static_cast<int64_t>(p.num_pages) * BLK;
-  auto page_at = [&](int i) {
-    if (i < 0 || i >= p.N) return -1;
-    const int s = p.slot_map[i];
-    return s >= 0 && s < slots ? s / BLK : -1;
-  };
+  char* pool = static_cast<char*>(isv ? p.v_pool : p.k_pool) + h * (isv ? p.vp_sh : p.kp_sh) * EB + 8 * EB * c;
+  const int64_t psb = (isv ? p.vp_sb : p.kp_sb) * EB, pst = (isv ? p.vp_st : p.kp_st) * EB;
+  const int slots = p.num_pages * BLK;
+  // slots of the window's 64 rows, of the 64 after them and of the row before: -1 for none
   const int w0 = blockIdx.x * win;
-  const int mine = page_at(w0 + min(lane, win - 1)), prev = page_at(w0 + min(lane, win - 1) - 1);
-  uint64_t leaders = __ballot(lane < win && mine >= 0 && mine != prev);
-  while (leaders != 0) {  // uniform over the workgroup
+  auto slot_at = [&](int i) {
+    const int s = i >= 0 && i < p.N ? p.slot_map[i] : -1;
+    return s < slots ? max(s, -1) : -1;
+  };
+  int s0 = slot_at(w0 + lane), s1 = slot_at(w0 + WAVE + lane);
+  const int prev = slot_at(w0 + lane - 1);
+  uint64_t leaders = __ballot(lane < win && s0 >= 0 && (prev < 0 || s0 / BLK != prev / BLK));
+  while (leaders != 0) {
     const int l0 = __builtin_ctzll(leaders);
     leaders &= leaders - 1;
-    const int pg = __builtin_amdgcn_readlane(mine, l0);
-    // the run's rows, 64 at a time (a run is longer only where it names a slot twice: its later rows come later)
-    for (int rs = w0 + l0, len = WAVE; len == WAVE; rs += WAVE) {
-      const uint64_t on = __ballot(page_at(rs + lane) == pg);
-      len = on == ~0ull ? WAVE : __builtin_ctzll(~on);
+    const int pg = __builtin_amdgcn_readlane(s0, l0) / BLK;
+    // the run's slots, 64 rows at a time (it is longer only where it names a slot twice: later rows come later)
+    int rs = w0 + l0;
+    const int in0 = __shfl(s0, (l0 + lane) & 63, WAVE), in1 = __shfl(s1, (l0 + lane) & 63, WAVE);
+    int mine = l0 + lane < WAVE ? in0 : in1;
+    while (true) {
+      const uint64_t on = __ballot(mine >= 0 && mine / BLK == pg);
+      const int len = on == ~0ull ? WAVE : __builtin_ctzll(~on);
       if (len == 0) break;
-      __syncthreads();
-      if (tid < BLK) sSrc[tid] = -1;
-      __syncthreads();
-      if (tid < len) atomicMax(&sSrc[p.slot_map[rs + tid] % BLK], rs + tid);  // of rows with one slot the last
-      __syncthreads();
-      const int c = tid % LPR, r0 = tid / LPR;
-      int src[NI];
+      const int at = mine % BLK, first = __builtin_amdgcn_readfirstlane(at);
+      const uint64_t run = len == WAVE ? ~0ull : (1ull << len) - 1;
+      uint64_t keep = run, fresh = run << first;  // rows of the run that are kept; rows of the page they fill
+      if ((__ballot(at == first + lane) & run) != run) {  // not one after another: of rows with one slot the last
+        bool last = lane < len;
+        fresh = 0;
+        for (int l = 0; l < len; ++l) {
+          const int r = __builtin_amdgcn_readlane(at, l);
+          fresh |= 1ull << r;
+          last = last && !(l > lane && r == at);
+        }
+        keep = __ballot(last);
+      }
       u32x4 x[NI];
+      int to[NI];  // this lane's row of the page, or -1
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        src[i] = sSrc[r0 + RPI * i];
-        x[i] = src[i] >= 0 ? ld16(rows + src[i] * sn + 8 * c) : u32x4{0u, 0u, 0u, 0u};
+        const int r = RPI * i + r0;
+        to[i] = -1;
+        x[i] = u32x4{0u, 0u, 0u, 0u};
+        if (RPI * i < len) {  // uniform
+          const int row = __shfl(at, r, WAVE);
+          if (keep >> r & 1) {
+            to[i] = row;
+            x[i] = ld16_nt(rows + (rs + r) * sn);
+          }
+        }
       }
-      char* out = pool + pg * psb + h * psh + 8 * EB * c;
+      char* out = pool + pg * psb;
       if constexpr (FMT == FMT_BF16) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-          if (src[i] >= 0) *reinterpret_cast<u32x4*>(out + (r0 + RPI * i) * pst) = x[i];
+          if (to[i] >= 0) *reinterpret_cast<u32x4*>(out + to[i] * pst) = x[i];
       } else {
         float* scale = (isv ? p.v_scale : p.k_scale) + pg * (isv ? p.vs_sb : p.ks_sb) + h * (isv ? p.vs_sh : p.ks_sh);
-        const bool anew = sSrc[0] >= 0;
+        const bool anew = fresh & 1;
         const float held = *scale;
         const float was = !anew && held > 0.f && held < __builtin_huge_valf() ? held : 0.f;
         // the largest magnitude, of bf16 bits without the sign: an infinity counts as the largest finite value, NaN not
@@ -284,35 +319,42 @@ __global__ void __launch_bounds__(CT) cache_write_kernel(const kvskip_write_args
             const uint32_t lo = x[i][e] & 0x7fffu, hi = x[i][e] >> 16 & 0x7fffu;
             top = max(top, max(lo <= 0x7f80u ? lo : 0u, hi <= 0x7f80u ? hi : 0u));
           }
-        const float tw = wave_max(__uint_as_float(min(top, 0x7f7fu) << 16));
-        if (lane == 0) sMax[wave] = tw;
-        __syncthreads();
-        float amax = 0.f;
-#pragma unroll
-        for (int w = 0; w < CT / WAVE; ++w) amax = fmaxf(amax, sMax[w]);
+        const float amax = wave_max(__uint_as_float(min(top, 0x7f7fu) << 16));
         constexpr float QMAX = FMT == FMT_E4M3 ? 448.f : 127.f;
         const float now = amax > QMAX * was ? pow2_scale<FMT>(amax) : was;
         const float inv = now > 0.f ? 1.f / now : 0.f;  // exact where now is a power of two
-        const bool grown = now != was && !anew;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          u32x2* at = reinterpret_cast<u32x2*>(out + (r0 + RPI * i) * pst);
-          if (src[i] >= 0) {
+        for (int i = 0; i < NI; ++i)
+          if (to[i] >= 0) {
             const u32x4 w = x[i];
-            *at = u32x2{codes4<FMT>(bf_lo(w.x) * inv, bf_hi(w.x) * inv, bf_lo(w.y) * inv, bf_hi(w.y) * inv),
-                        codes4<FMT>(bf_lo(w.z) * inv, bf_hi(w.z) * inv, bf_lo(w.w) * inv, bf_hi(w.w) * inv)};
-          } else if (grown) {
-            const float f = was * inv;
-            const u32x2 w = *at;
-            float a[4], b[4];
-            values4<FMT>(w.x, a);
-            values4<FMT>(w.y, b);
-            *at = u32x2{codes4<FMT>(a[0] * f, a[1] * f, a[2] * f, a[3] * f),
-                        codes4<FMT>(b[0] * f, b[1] * f, b[2] * f, b[3] * f)};
+            *reinterpret_cast<u32x2*>(out + to[i] * pst) =
+                u32x2{codes4<FMT>(bf_lo(w.x) * inv, bf_hi(w.x) * inv, bf_lo(w.y) * inv, bf_hi(w.y) * inv),
+                      codes4<FMT>(bf_lo(w.z) * inv, bf_hi(w.z) * inv, bf_lo(w.w) * inv, bf_hi(w.w) * inv)};
           }
+        if (now != was && !anew) {  // uniform: the page's other rows move to the larger scale
+          const float f = was * inv;
+          u32x2 old[NI];
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+            if (!(fresh >> (RPI * i + r0) & 1)) old[i] = *reinterpret_cast<const u32x2*>(out + (RPI * i + r0) * pst);
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+            if (!(fresh >> (RPI * i + r0) & 1)) {
+              float a[4], b[4];
+              values4<FMT>(old[i].x, a);
+              values4<FMT>(old[i].y, b);
+              *reinterpret_cast<u32x2*>(out + (RPI * i + r0) * pst) =
+                  u32x2{codes4<FMT>(a[0] * f, a[1] * f, a[2] * f, a[3] * f),
+                        codes4<FMT>(b[0] * f, b[1] * f, b[2] * f, b[3] * f)};
+            }
         }
-        if (tid == 0 && !(now == held)) *scale = now;
+        if (lane == 0 && !(now == held)) *scale = now;
       }
+      if (len < WAVE) break;
+      rs += WAVE;
+      mine = slot_at(rs + lane);
+      // (the next 64 rows of the run read and write the same page and scale: after this chunk's stores)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     }
   }
 }
@@ -320,9 +362,9 @@ __global__ void __launch_bounds__(CT) cache_write_kernel(const kvskip_write_args
 template <int FMT>
 void launch_write_d(const kvskip_write_args& p, dim3 grid, int win, hipStream_t s) {
   if (p.D == 128)
-    hipLaunchKernelGGL((cache_write_kernel<FMT, 128>), grid, dim3(CT), 0, s, p, win);
+    hipLaunchKernelGGL((cache_write_kernel<FMT, 128>), grid, dim3(WAVE), 0, s, p, win);
   else
-    hipLaunchKernelGGL((cache_write_kernel<FMT, 64>), grid, dim3(CT), 0, s, p, win);
+    hipLaunchKernelGGL((cache_write_kernel<FMT, 64>), grid, dim3(WAVE), 0, s, p, win);
 }
 
 }  // namespace
@@ -330,7 +372,7 @@ void launch_write_d(const kvskip_write_args& p, dim3 grid, int win, hipStream_t 
 // One launch up to ONE_ROWS rows of the map, else the sums and a filling launch.
 constexpr int ONE_ROWS = 4096;
 
-int page_work_ints(int B, int rows) { return rows <= ONE_ROWS ? 0 : 1 + 2 * B; }
+int page_work_ints(int B, int rows) { return rows <= ONE_ROWS ? 0 : 2 + 3 * B; }
 
 hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s) {
   if (p.rows <= ONE_ROWS) {
@@ -345,7 +387,8 @@ hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s) {
 }
 
 hipError_t launch_cache_write(const kvskip_write_args& p, hipStream_t s) {
-  const int win = static_cast<int64_t>(p.N) * p.Hkv <= 16384 ? 1 : 16;
+  static const int wv = getenv("KVS_WIN") ? atoi(getenv("KVS_WIN")) : 16;
+  const int win = static_cast<int64_t>(p.N) * p.Hkv <= 16384 ? 1 : wv;
   const dim3 grid((p.N + win - 1) / win, p.Hkv, 2);
   if (p.format == KVSKIP_BF16)
     launch_write_d<FMT_BF16>(p, grid, win, s);

@@ -52,7 +52,7 @@ def _compare(lens, new, held, table, free, count, rows, in_place, stride=0):
 
 
 @pytest.mark.parametrize("B,width,rows", [(1, 1, 1), (1, 40, 64), (7, 30, 300), (64, 20, 4096), (65, 20, 4097),
-                                          (300, 12, 5000), (1025, 5, 2000), (4096, 3, 4096), (4096, 3, 9000)])
+                                          (300, 12, 5000), (1025, 5, 2000), (2048, 3, 4096), (2048, 3, 9000)])
 @pytest.mark.parametrize("tight", [False, True])
 def test_page_map(gpu, B, width, rows, tight):
     rng = random.Random(B * 31 + rows + tight)

@@ -83,8 +83,8 @@ def _page(**kw):
 @pytest.mark.parametrize("kw,code,msg", [
     (dict(B=0), -1, "sizes must be positive"), (dict(width=0), -1, "sizes must be positive"),
     (dict(num_pages=0), -1, "sizes must be positive"), (dict(rows=-1), -1, "sizes must be positive"),
-    (dict(B=4097), -2, "B <= 4096"), (dict(B=4096, rows=1 << 19), -2, "below 2^31"),
-    (dict(num_pages=1 << 25), -2, "below 2^31"), (dict(B=4096, width=1 << 19, bt_stride=1 << 19), -2, "below 2^31"),
+    (dict(B=2049), -2, "B <= 2048"), (dict(B=2048, rows=1 << 20), -2, "below 2^31"),
+    (dict(num_pages=1 << 25), -2, "below 2^31"), (dict(B=2048, width=1 << 20, bt_stride=1 << 20), -2, "below 2^31"),
     (dict(bt_stride=9), -1, "must not overlap"), (dict(starts=0), -1, "null tensor"), (dict(slots=0), -1, "null tensor"),
     (dict(rows=1 << 20), -1, "work of kvskip_page_work_ints"),
 ])
