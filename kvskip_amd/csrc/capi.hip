@@ -612,9 +612,9 @@ int kvskip_cache_write(const kvskip_write_args* p, void* stream) {
   if (p == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
   if (p->N < 0 || p->Hkv < 1 || p->num_pages < 1) return fail(KVSKIP_E_INVALID, "cache_write: sizes must be positive");
   if (p->D != 64 && p->D != 128) return fail(KVSKIP_E_UNSUPPORTED, "cache_write: D in {64, 128} (D=%d)", p->D);
-  if (p->Hkv > 65535) return fail(KVSKIP_E_UNSUPPORTED, "cache_write: Hkv <= 65535");
-  if (static_cast<int64_t>(p->num_pages) * KVSKIP_BLOCK >= (int64_t(1) << 31) || p->N > (1 << 30))
-    return fail(KVSKIP_E_UNSUPPORTED, "cache_write: 64 * num_pages below 2^31, N up to 2^30");
+  if (static_cast<int64_t>(p->num_pages) * KVSKIP_BLOCK >= (int64_t(1) << 31) || p->N > (1 << 21) ||
+      static_cast<int64_t>(p->N > 64 ? p->N : 64) * p->Hkv > (1 << 28))
+    return fail(KVSKIP_E_UNSUPPORTED, "cache_write: 64 * num_pages below 2^31, N up to 2^21, N * Hkv up to 2^28");
   if (p->format != KVSKIP_E4M3 && p->format != KVSKIP_INT8 && p->format != KVSKIP_BF16)
     return fail(KVSKIP_E_INVALID, "cache_write: format e4m3, int8 or bf16 (got %d)", p->format);
   if (p->k_pool == nullptr || p->v_pool == nullptr || (p->N > 0 && (p->k == nullptr || p->v == nullptr || p->slot_map == nullptr)))
@@ -623,6 +623,9 @@ int kvskip_cache_write(const kvskip_write_args* p, void* stream) {
     return fail(KVSKIP_E_INVALID, "cache_write: k_scale and v_scale with an 8-bit pool");
   if (p->k_sn % 8 != 0 || p->k_sh % 8 != 0 || p->v_sn % 8 != 0 || p->v_sh % 8 != 0 || !aligned16(p->k) || !aligned16(p->v))
     return fail(KVSKIP_E_INVALID, "cache_write: k, v rows must be 16-byte aligned");
+  const int64_t st[4] = {p->k_sn, p->v_sn, p->kp_st, p->vp_st};
+  for (const int64_t x : st)
+    if (x < 0 || x >= (int64_t(1) << 24)) return fail(KVSKIP_E_UNSUPPORTED, "cache_write: row strides in [0, 2^24)");
   const int m = p->format == KVSKIP_BF16 ? 8 : 16;
   if (p->kp_sb % m != 0 || p->kp_sh % m != 0 || p->kp_st % m != 0 || p->vp_sb % m != 0 || p->vp_sh % m != 0 ||
       p->vp_st % m != 0 || !aligned16(p->k_pool) || !aligned16(p->v_pool))

@@ -910,8 +910,8 @@ PyObject* cache_write(PyObject* const* a) {
     require(t == nullptr || (t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == kp.size(0) && t->size(1) == Hkv),
             "k_scale, v_scale: fp32 [num_pages, Hkv]");
   same_device(k, {&v, &slots, &kp, &vp, ks, vs}, "cache_write: tensors on one device");
-  require(N <= (int64_t(1) << 30) && kp.size(0) < (int64_t(1) << 25) && Hkv <= 65535,
-          "cache_write: 64 * num_pages below 2^31, N up to 2^30, Hkv <= 65535");
+  require(N <= (int64_t(1) << 21) && kp.size(0) < (int64_t(1) << 25) && Hkv <= (int64_t(1) << 28),
+          "cache_write: 64 * num_pages below 2^31, N up to 2^21, N * Hkv up to 2^28");
   p.k = k.data_ptr(), p.k_sn = N > 1 ? k.stride(0) : 0, p.k_sh = Hkv > 1 ? k.stride(1) : 0;
   p.v = v.data_ptr(), p.v_sn = N > 1 ? v.stride(0) : 0, p.v_sh = Hkv > 1 ? v.stride(1) : 0;
   p.slot_map = static_cast<const int32_t*>(slots.data_ptr());

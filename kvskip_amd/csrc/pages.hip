@@ -14,7 +14,6 @@
 // written an element. A scale is a power of two: dividing by it is exact, so a code depends on its value and scale
 // alone, and when a later row needs a larger scale, the rows that are there move to it without rounding again (e4m3:
 // but for subnormal codes; int8 rounds once more per doubling, less than the final step in sum).
-#include <cstdlib>
 #include "common.hpp"
 #include "internal.hpp"
 
@@ -43,18 +42,6 @@ __device__ __forceinline__ bool page_need(const kvskip_page_args& p, int b, int&
   h = min(max(p.held[b], 0), p.width);
   need = pages_of(n);
   return need <= p.width;
-}
-
-// Exclusive prefix of v over the workgroup's PT threads and its total; `tmp` holds one int a wavefront.
-__device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
-  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-  const int incl = wave_incl_scan(v);
-  __syncthreads();
-  if (lane == WAVE - 1) tmp[wave] = incl;
-  __syncthreads();
-  const int x = wave_incl_scan(lane < PT / WAVE ? tmp[lane] : 0);
-  total = __builtin_amdgcn_readlane(x, PT / WAVE - 1);
-  return incl - v + (wave > 0 ? __shfl(x, wave - 1, WAVE) : 0);
 }
 
 // The last b with first[b] <= i (of requests with one value the last: the others have nothing there).
@@ -115,53 +102,74 @@ __device__ __forceinline__ void page_fill(const kvskip_page_args& p, const Step&
   }
 }
 
-// The sums; ONE: also page_fill (the whole operator in one launch).
+// The sums; ONE: also page_fill (the whole operator in one launch). A thread holds two neighbouring requests; the three
+// prefix sums (pages given, pages taken, rows) meet in LDS together, once, and what needs the total of pages given back
+// (who is served, with how many pages) a second time.
 template <bool ONE>
 __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p) {
+  static_assert(MAX_PAGE_B == 2 * PT, "two requests a thread");
+  constexpr int NW = PT / WAVE;
   __shared__ Step s;
-  __shared__ int tmp[PT / WAVE];
-  const int tid = threadIdx.x;
+  __shared__ int tot[3][NW], tot2[2][NW];
+  const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
   const int count = min(max(*p.free_count, 0), p.num_pages);
-  int given = 0;
-  for (int b0 = 0; b0 < p.B; b0 += PT) {
-    const int b = b0 + tid;
-    int n, a, h, need, g = 0, all;
-    if (b < p.B && page_need(p, b, n, a, h, need)) g = max(h - need, 0);
-    const int at = given + block_scan(g, tmp, all);
-    if (b < p.B) s.given[b] = at;
-    given += all;
+  int v[2][3], h[2], need[2];  // of request 2 tid + r: pages given, pages taken, rows
+  bool fits[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int b = 2 * tid + r;
+    int n = 0, a = 0;
+    h[r] = need[r] = 0;
+    fits[r] = b < p.B && page_need(p, b, n, a, h[r], need[r]);
+    v[r][0] = fits[r] ? max(h[r] - need[r], 0) : 0;
+    v[r][1] = fits[r] ? max(need[r] - h[r], 0) : 0;
+    v[r][2] = min(a, p.rows + 1);
   }
-  const int avail = min(count + given, p.num_pages);
-  int taken = 0, rows = 0, short_ = 0, used = 0;
-  for (int b0 = 0; b0 < p.B; b0 += PT) {
-    const int b = b0 + tid;
-    int n = 0, a = 0, h = 0, need = 0, all;
-    const bool fits = b < p.B && page_need(p, b, n, a, h, need);
-    const int t = fits ? max(need - h, 0) : 0;
-    const int before = taken + block_scan(t, tmp, all);
-    taken += all;
-    const bool served = fits && (t == 0 || before + t <= avail);
-    const int start = rows + block_scan(min(a, p.rows + 1), tmp, all);
-    rows += all;
-    if (b < p.B) {
-      s.starts[b] = start;
-      s.taken[b] = served ? before : -1;
-      s.held[b] = h;
-      p.starts[b] = start;
-      p.held_out[b] = served ? need : h;
-    }
-    // (not served, pages used: counts of at most 2^11 requests and 2^25 pages)
-    short_ += __syncthreads_count(b < p.B && !served);
-    block_scan(served ? t : 0, tmp, all);
-    used += all;
-  }
-  if (tid == 0) {
-    s.starts[p.B] = rows;
-    p.starts[p.B] = rows;
-    *p.short_out = short_;
-    *p.free_count_out = avail - used;
+  int incl[3], all[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    incl[k] = wave_incl_scan(v[0][k] + v[1][k]);
+    if (lane == WAVE - 1) tot[k][wave] = incl[k];
   }
   __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const int x = wave_incl_scan(lane < NW ? tot[k][lane] : 0);
+    all[k] = __builtin_amdgcn_readlane(x, NW - 1);
+    incl[k] += (wave > 0 ? __shfl(x, wave - 1, WAVE) : 0) - v[0][k] - v[1][k];  // now exclusive
+  }
+  const int avail = min(count + all[0], p.num_pages);
+  int used = 0, left = 0;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int b = 2 * tid + r;
+    const bool served = fits[r] && (v[r][1] == 0 || incl[1] + v[r][1] <= avail);
+    if (b < p.B) {
+      s.starts[b] = incl[2];
+      s.given[b] = incl[0];
+      s.taken[b] = served ? incl[1] : -1;
+      s.held[b] = h[r];
+      p.starts[b] = incl[2];
+      p.held_out[b] = served ? need[r] : h[r];
+      used += served ? v[r][1] : 0;
+      left += served ? 0 : 1;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) incl[k] += v[r][k];
+  }
+  used = wave_sum_int(used);
+  left = wave_sum_int(left);
+  if (lane == 0) tot2[0][wave] = used, tot2[1][wave] = left;
+  if (tid == 0) s.starts[p.B] = p.starts[p.B] = all[2];
+  __syncthreads();
+  if (wave == NW - 1) {
+    used = wave_sum_int(lane < NW ? tot2[0][lane] : 0);
+    left = wave_sum_int(lane < NW ? tot2[1][lane] : 0);
+    if (lane == 0) {
+      *p.short_out = left;
+      *p.free_count_out = avail - used;
+    }
+  }
   if constexpr (ONE) {
     page_fill(p, s, count, avail, tid, PT);
   } else {  // what the filling launch needs beside starts
@@ -203,6 +211,13 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float(static_cast<uint32_t>(max(e, 1)) << 23);
 }
 
+__device__ __forceinline__ u32x2 bload8(rsrc_t r, uint32_t voff, uint32_t soff) {
+  return __builtin_amdgcn_raw_buffer_load_b64(r, static_cast<int>(voff), static_cast<int>(soff), 0);
+}
+__device__ __forceinline__ void bstore16(u32x4 v, rsrc_t r, uint32_t voff) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, static_cast<int>(voff), 0, 0);
+}
+
 // Two values (already divided by the scale) as codes in the low half; infinities at the largest value of their sign,
 // NaN as NaN (e4m3) or 0 (int8).
 template <int FMT>
@@ -238,123 +253,181 @@ __device__ __forceinline__ void values4(uint32_t w, float (&x)[4]) {
   }
 }
 
-// One wavefront a workgroup: (window, KV head, keys or values), the runs that start in rows [w0, w0 + win) of the map.
-template <int FMT, int D>
-__global__ void __launch_bounds__(WAVE) cache_write_kernel(const kvskip_write_args p, int win) {
-  constexpr int LPR = D / 8, RPI = WAVE / LPR, NI = BLK / RPI;  // lanes a row, rows a load, loads a page
+constexpr int CT = 256;
+
+// Keys or values of one KV head: what a run needs.
+struct Side {
+  const char* rows;  // row 0 of the head
+  char* pool;        // page 0 of the head
+  float* scale;
+  int64_t sn, psb, ssb;
+  uint32_t st, pst;
+};
+
+// One run of `len` rows (at most 64) from row rs of the map on, this lane's slot within the page `at`, by T threads: the
+// workgroup's (its wavefronts meet once, over `meet`), or one wavefront's for a run that one load takes.
+template <int FMT, int D, int T>
+__device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len, int at, float* meet) {
+  constexpr int LPR = D / 8, RPI = T / LPR;                     // lanes a row, rows a load
+  constexpr int NI = T == WAVE ? 1 : BLK / RPI, NO = BLK / RPI;  // loads of a run, of a page
   constexpr int EB = FMT == FMT_BF16 ? 2 : 1;
-  const int lane = threadIdx.x, c = lane % LPR, r0 = lane / LPR;
-  const int h = blockIdx.y;
-  const bool isv = blockIdx.z != 0;
-  const uint16_t* rows = static_cast<const uint16_t*>(isv ? p.v : p.k) + h * (isv ? p.v_sh : p.k_sh) + 8 * c;
-  const int64_t sn = isv ? p.v_sn : p.k_sn;
-  char* pool = static_cast<char*>(isv ? p.v_pool : p.k_pool) + h * (isv ? p.vp_sh : p.kp_sh) * EB + 8 * EB * c;
-  const int64_t psb = (isv ? p.vp_sb : p.kp_sb) * EB, pst = (isv ? p.vp_st : p.kp_st) * EB;
-  const int slots = p.num_pages * BLK;
-  // slots of the window's 64 rows, of the 64 after them and of the row before: -1 for none
-  const int w0 = blockIdx.x * win;
-  auto slot_at = [&](int i) {
-    const int s = i >= 0 && i < p.N ? p.slot_map[i] : -1;
-    return s < slots ? max(s, -1) : -1;
+  constexpr uint32_t OOB = 0xf0000000u;
+  const int lane = threadIdx.x % WAVE, t = threadIdx.x % T, c = t % LPR, r0 = t / LPR;
+  const int first = __builtin_amdgcn_readfirstlane(at);
+  const uint64_t run = len == WAVE ? ~0ull : (1ull << len) - 1;
+  uint64_t keep = run, fresh = run << first;  // rows of the run that are kept; rows of the page they fill
+  const bool linear = (__ballot(at == first + lane) & run) == run;
+  if (!linear) {  // not one after another: of rows with one slot the last
+    bool last = lane < len;
+    fresh = 0;
+    for (int l = 0; l < len; ++l) {
+      const int r = __builtin_amdgcn_readlane(at, l);
+      fresh |= 1ull << r;
+      last = last && !(l > lane && r == at);
+    }
+    keep = __ballot(last);
+  }
+  // Rows through buffer resources: the source's are consecutive and end with the run (rows past it read zero); so are the
+  // page's, but where a slot comes twice, which costs a shuffle a row.
+  const rsrc_t src = make_rsrc(s.rows + rs * s.sn, (len - 1) * s.st + 2 * D);
+  const rsrc_t dst = make_rsrc(s.pool + pg * s.psb, 63 * s.pst + EB * D);
+  u32x4 x[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) x[i] = bload16<BUF_NT>(src, r0 * s.st + 16 * c, RPI * i * s.st);
+  auto dst_off = [&](int i) -> uint32_t {
+    const int r = RPI * i + r0;
+    const int row = linear ? first + r : __shfl(at, r, WAVE);
+    return keep >> r & 1 ? row * s.pst + 8 * EB * c : OOB;
   };
-  int s0 = slot_at(w0 + lane), s1 = slot_at(w0 + WAVE + lane);
-  const int prev = slot_at(w0 + lane - 1);
-  uint64_t leaders = __ballot(lane < win && s0 >= 0 && (prev < 0 || s0 / BLK != prev / BLK));
-  while (leaders != 0) {
-    const int l0 = __builtin_ctzll(leaders);
-    leaders &= leaders - 1;
-    const int pg = __builtin_amdgcn_readlane(s0, l0) / BLK;
-    // the run's slots, 64 rows at a time (it is longer only where it names a slot twice: later rows come later)
-    int rs = w0 + l0;
+  if constexpr (FMT == FMT_BF16) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (RPI * i < len) bstore16(x[i], dst, dst_off(i));
+  } else {
+    float* scale = s.scale + pg * s.ssb;
+    const bool anew = fresh & 1;
+    const float held = *scale;
+    const float was = !anew && held > 0.f && held < __builtin_huge_valf() ? held : 0.f;
+    // the largest magnitude of the rows that are kept, of bf16 bits without the sign: an infinity counts as the largest
+    // finite value, NaN not
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = x[i][e] & 0x7fffu, hi = x[i][e] >> 16 & 0x7fffu;
+        m = max(m, max(lo <= 0x7f80u ? lo : 0u, hi <= 0x7f80u ? hi : 0u));
+      }
+      if (keep != run) m = keep >> (RPI * i + r0) & 1 ? m : 0u;
+      top = max(top, m);
+    }
+    float amax = wave_max(__uint_as_float(min(top, 0x7f7fu) << 16));
+    if constexpr (T > WAVE) {
+      if (lane == 0) meet[threadIdx.x / WAVE] = amax;
+      // a barrier for LDS alone: __syncthreads would wait for the stores of the run before too
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+#pragma unroll
+      for (int w = 0; w < T / WAVE; ++w) amax = fmaxf(amax, meet[w]);
+    }
+    constexpr float QMAX = FMT == FMT_E4M3 ? 448.f : 127.f;
+    const float now = amax > QMAX * was ? pow2_scale<FMT>(amax) : was;
+    const float inv = now > 0.f ? 1.f / now : 0.f;  // exact where now is a power of two
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (RPI * i < len) {  // uniform
+        const u32x4 w = x[i];
+        bstore_b64(u32x2{codes4<FMT>(bf_lo(w.x) * inv, bf_hi(w.x) * inv, bf_lo(w.y) * inv, bf_hi(w.y) * inv),
+                         codes4<FMT>(bf_lo(w.z) * inv, bf_hi(w.z) * inv, bf_lo(w.w) * inv, bf_hi(w.w) * inv)},
+                   dst, dst_off(i), 0);
+      }
+    if (now != was && !anew) {  // uniform: the page's other rows move to the larger scale
+      const float f = was * inv;
+#pragma unroll 1
+      for (int i0 = 0; i0 < NO; i0 += NO < 4 ? NO : 4) {
+        u32x2 old[NO < 4 ? NO : 4];
+#pragma unroll
+        for (int i = 0; i < (NO < 4 ? NO : 4); ++i) {
+          const int r = RPI * (i0 + i) + r0;
+          old[i] = bload8(dst, fresh >> r & 1 ? OOB : r * s.pst + 8 * c, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < (NO < 4 ? NO : 4); ++i) {
+          const int r = RPI * (i0 + i) + r0;
+          float a[4], b[4];
+          values4<FMT>(old[i].x, a);
+          values4<FMT>(old[i].y, b);
+          bstore_b64(u32x2{codes4<FMT>(a[0] * f, a[1] * f, a[2] * f, a[3] * f),
+                           codes4<FMT>(b[0] * f, b[1] * f, b[2] * f, b[3] * f)},
+                     dst, fresh >> r & 1 ? OOB : r * s.pst + 8 * c, 0);
+        }
+      }
+    }
+    if (t == 0 && !(now == held)) *scale = now;
+  }
+}
+
+// Workgroup (KV head's keys or values, window): the runs that start in rows [w0, w0 + win) of the map. Consecutive
+// workgroups take the heads, keys then values, of one window: together they read and write whole rows (heads by windows
+// instead: 72 us against 63 for 44 000 rows of 8 heads).
+template <int FMT, int D>
+__global__ void __launch_bounds__(CT, 4) cache_write_kernel(const kvskip_write_args p, int win) {
+  constexpr int EB = FMT == FMT_BF16 ? 2 : 1, RPW = WAVE / (D / 8);
+  __shared__ float sMax[2][CT / WAVE];
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const bool isv = static_cast<int>(blockIdx.x) >= p.Hkv;
+  const int h = blockIdx.x - (isv ? p.Hkv : 0);
+  Side s;
+  s.rows = static_cast<const char*>(isv ? p.v : p.k) + h * (isv ? p.v_sh : p.k_sh) * 2;
+  s.sn = (isv ? p.v_sn : p.k_sn) * 2;
+  s.st = static_cast<uint32_t>(s.sn);
+  s.pool = static_cast<char*>(isv ? p.v_pool : p.k_pool) + h * (isv ? p.vp_sh : p.kp_sh) * EB;
+  s.psb = (isv ? p.vp_sb : p.kp_sb) * EB;
+  s.pst = static_cast<uint32_t>((isv ? p.vp_st : p.kp_st) * EB);
+  s.scale = FMT == FMT_BF16 ? nullptr : (isv ? p.v_scale : p.k_scale) + h * (isv ? p.vs_sh : p.ks_sh);
+  s.ssb = isv ? p.vs_sb : p.ks_sb;
+  // slots of the window's 64 rows, of the 64 after them and of the row before: -1 for none
+  const int slots = p.num_pages * BLK;
+  const int w0 = blockIdx.y * win;
+  auto slot_at = [&](int i) {
+    const int x = i >= 0 && i < p.N ? p.slot_map[i] : -1;
+    return x < slots ? max(x, -1) : -1;
+  };
+  const int s0 = slot_at(w0 + lane), s1 = slot_at(w0 + WAVE + lane), before = slot_at(w0 + lane - 1);
+  uint64_t leaders = __ballot(lane < win && s0 >= 0 && (before < 0 || s0 / BLK != before / BLK));
+  auto run_slots = [&](int l0) {  // of the run that starts at row w0 + l0, 64 rows
     const int in0 = __shfl(s0, (l0 + lane) & 63, WAVE), in1 = __shfl(s1, (l0 + lane) & 63, WAVE);
-    int mine = l0 + lane < WAVE ? in0 : in1;
+    return l0 + lane < WAVE ? in0 : in1;
+  };
+  auto length = [&](int mine, int pg) {
+    const uint64_t on = __ballot(mine >= 0 && mine / BLK == pg);
+    return on == ~0ull ? WAVE : static_cast<int>(__builtin_ctzll(~on));
+  };
+  // Runs that one load of a wavefront takes (new tokens of many requests) go to the wavefronts one each; the others to
+  // the whole workgroup, in turn (4096 rows of as many pages, each run by the workgroup and with __syncthreads: 120 us,
+  // so 34).
+  int number = 0, turn = 0;
+  for (; leaders != 0; leaders &= leaders - 1) {
+    const int l0 = __builtin_ctzll(leaders);
+    const int pg = __builtin_amdgcn_readlane(s0, l0) / BLK;
+    int rs = w0 + l0, mine = run_slots(l0);
+    int len = length(mine, pg);
+    if (len <= RPW) {
+      if (number++ % (CT / WAVE) == wave) write_run<FMT, D, WAVE>(s, pg, rs, len, mine % BLK, nullptr);
+      continue;
+    }
+    // a run is longer than 64 rows only where it names a slot twice: its later rows come later
     while (true) {
-      const uint64_t on = __ballot(mine >= 0 && mine / BLK == pg);
-      const int len = on == ~0ull ? WAVE : __builtin_ctzll(~on);
-      if (len == 0) break;
-      const int at = mine % BLK, first = __builtin_amdgcn_readfirstlane(at);
-      const uint64_t run = len == WAVE ? ~0ull : (1ull << len) - 1;
-      uint64_t keep = run, fresh = run << first;  // rows of the run that are kept; rows of the page they fill
-      if ((__ballot(at == first + lane) & run) != run) {  // not one after another: of rows with one slot the last
-        bool last = lane < len;
-        fresh = 0;
-        for (int l = 0; l < len; ++l) {
-          const int r = __builtin_amdgcn_readlane(at, l);
-          fresh |= 1ull << r;
-          last = last && !(l > lane && r == at);
-        }
-        keep = __ballot(last);
-      }
-      u32x4 x[NI];
-      int to[NI];  // this lane's row of the page, or -1
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = RPI * i + r0;
-        to[i] = -1;
-        x[i] = u32x4{0u, 0u, 0u, 0u};
-        if (RPI * i < len) {  // uniform
-          const int row = __shfl(at, r, WAVE);
-          if (keep >> r & 1) {
-            to[i] = row;
-            x[i] = ld16_nt(rows + (rs + r) * sn);
-          }
-        }
-      }
-      char* out = pool + pg * psb;
-      if constexpr (FMT == FMT_BF16) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-          if (to[i] >= 0) *reinterpret_cast<u32x4*>(out + to[i] * pst) = x[i];
-      } else {
-        float* scale = (isv ? p.v_scale : p.k_scale) + pg * (isv ? p.vs_sb : p.ks_sb) + h * (isv ? p.vs_sh : p.ks_sh);
-        const bool anew = fresh & 1;
-        const float held = *scale;
-        const float was = !anew && held > 0.f && held < __builtin_huge_valf() ? held : 0.f;
-        // the largest magnitude, of bf16 bits without the sign: an infinity counts as the largest finite value, NaN not
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = x[i][e] & 0x7fffu, hi = x[i][e] >> 16 & 0x7fffu;
-            top = max(top, max(lo <= 0x7f80u ? lo : 0u, hi <= 0x7f80u ? hi : 0u));
-          }
-        const float amax = wave_max(__uint_as_float(min(top, 0x7f7fu) << 16));
-        constexpr float QMAX = FMT == FMT_E4M3 ? 448.f : 127.f;
-        const float now = amax > QMAX * was ? pow2_scale<FMT>(amax) : was;
-        const float inv = now > 0.f ? 1.f / now : 0.f;  // exact where now is a power of two
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-          if (to[i] >= 0) {
-            const u32x4 w = x[i];
-            *reinterpret_cast<u32x2*>(out + to[i] * pst) =
-                u32x2{codes4<FMT>(bf_lo(w.x) * inv, bf_hi(w.x) * inv, bf_lo(w.y) * inv, bf_hi(w.y) * inv),
-                      codes4<FMT>(bf_lo(w.z) * inv, bf_hi(w.z) * inv, bf_lo(w.w) * inv, bf_hi(w.w) * inv)};
-          }
-        if (now != was && !anew) {  // uniform: the page's other rows move to the larger scale
-          const float f = was * inv;
-          u32x2 old[NI];
-#pragma unroll
-          for (int i = 0; i < NI; ++i)
-            if (!(fresh >> (RPI * i + r0) & 1)) old[i] = *reinterpret_cast<const u32x2*>(out + (RPI * i + r0) * pst);
-#pragma unroll
-          for (int i = 0; i < NI; ++i)
-            if (!(fresh >> (RPI * i + r0) & 1)) {
-              float a[4], b[4];
-              values4<FMT>(old[i].x, a);
-              values4<FMT>(old[i].y, b);
-              *reinterpret_cast<u32x2*>(out + (RPI * i + r0) * pst) =
-                  u32x2{codes4<FMT>(a[0] * f, a[1] * f, a[2] * f, a[3] * f),
-                        codes4<FMT>(b[0] * f, b[1] * f, b[2] * f, b[3] * f)};
-            }
-        }
-        if (lane == 0 && !(now == held)) *scale = now;
-      }
+      turn ^= 1;
+      write_run<FMT, D, CT>(s, pg, rs, len, mine % BLK, sMax[turn]);
       if (len < WAVE) break;
       rs += WAVE;
       mine = slot_at(rs + lane);
-      // (the next 64 rows of the run read and write the same page and scale: after this chunk's stores)
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      len = length(mine, pg);
+      if (len == 0) break;
+      __syncthreads();  // the next 64 rows of the run read and write the same page and scale
     }
   }
 }
@@ -362,14 +435,15 @@ __global__ void __launch_bounds__(WAVE) cache_write_kernel(const kvskip_write_ar
 template <int FMT>
 void launch_write_d(const kvskip_write_args& p, dim3 grid, int win, hipStream_t s) {
   if (p.D == 128)
-    hipLaunchKernelGGL((cache_write_kernel<FMT, 128>), grid, dim3(WAVE), 0, s, p, win);
+    hipLaunchKernelGGL((cache_write_kernel<FMT, 128>), grid, dim3(CT), 0, s, p, win);
   else
-    hipLaunchKernelGGL((cache_write_kernel<FMT, 64>), grid, dim3(WAVE), 0, s, p, win);
+    hipLaunchKernelGGL((cache_write_kernel<FMT, 64>), grid, dim3(CT), 0, s, p, win);
 }
 
 }  // namespace
 
-// One launch up to ONE_ROWS rows of the map, else the sums and a filling launch.
+// One launch up to ONE_ROWS rows of the map, else the sums and a filling launch. us, one launch / two: 24 requests of one
+// new token 5.1 / 8.6, 2048 of one 8.3 / 12.8, 4 of 1024 6.3 / 8.1, 16 of 512 9.8 / 8.1, 64 of 2048 114 / 11.7.
 constexpr int ONE_ROWS = 4096;
 
 int page_work_ints(int B, int rows) { return rows <= ONE_ROWS ? 0 : 2 + 3 * B; }
@@ -387,9 +461,12 @@ hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s) {
 }
 
 hipError_t launch_cache_write(const kvskip_write_args& p, hipStream_t s) {
-  static const int wv = getenv("KVS_WIN") ? atoi(getenv("KVS_WIN")) : 16;
-  const int win = static_cast<int64_t>(p.N) * p.Hkv <= 16384 ? 1 : wv;
-  const dim3 grid((p.N + win - 1) / win, p.Hkv, 2);
+  // Rows of the map a workgroup looks at: few enough that 4096 workgroups find work, at most 64 (a page of a prompt then
+  // is one or two workgroups' and none ends with nothing to do), at least four (one new token a wavefront). 44 000 rows of
+  // prompts, 8 heads, us: 4096 workgroups 51, with windows of 16 rows 83; 4096 single rows 34, by windows of 64 35.
+  int win = 4;
+  while (win < WAVE && static_cast<int64_t>(p.N) * 2 * p.Hkv > 4096 * win) win *= 2;
+  const dim3 grid(2 * p.Hkv, (p.N + win - 1) / win);
   if (p.format == KVSKIP_BF16)
     launch_write_d<FMT_BF16>(p, grid, win, s);
   else if (p.format == KVSKIP_INT8)

@@ -122,7 +122,8 @@ def _write(**kw):
     (dict(slot_map=0), -1, "null tensor"), (dict(k_scale=0), -1, "k_scale and v_scale"),
     (dict(k=0x1008), -1, "k, v rows must be 16-byte aligned"), (dict(v_sh=100), -1, "k, v rows must be 16-byte aligned"),
     (dict(kp_st=136), -1, "pool rows must be 16-byte aligned"), (dict(v_pool=0x1004), -1, "pool rows must be 16-byte"),
-    (dict(Hkv=70000), -2, "Hkv <= 65535"),
+    (dict(N=(1 << 21) + 1), -2, "N up to 2^21"), (dict(N=1 << 20, Hkv=257), -2, "N * Hkv up to 2^28"),
+    (dict(Hkv=1 << 23), -2, "N * Hkv up to 2^28"), (dict(k_sn=1 << 24), -2, "row strides"), (dict(vp_st=-16), -2, "row strides"),
 ])
 def test_cache_write_refusals(kw, code, msg):
     lib = _native.lib()
