@@ -155,18 +155,18 @@ struct Items {
   float ks, vs;
 };
 
-template <int D, int GP, bool I8, bool STATS>
+template <int D, int GP, bool I8, bool STATS, bool RAG>
 __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
   __shared__ __attribute__((aligned(16))) Merge8<D, GP> sL;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
   const int j4 = lane >> 4, c16 = lane & 15;
-  const bool masked = p.block_idx != nullptr, paged = p.block_table != nullptr, rag = p.seq_lens != nullptr;
+  const bool masked = p.block_idx != nullptr, paged = p.block_table != nullptr;
   const int G = p.G;
 
   // ---- this workgroup's work, as decode_body finds it: list positions / blocks [i0, i0 + n) of the n_items of (b, h)
   int split, h, b, n_items, i0, n, Tb = p.T, nbb = p.nb;
-  if (!rag) {
+  if constexpr (!RAG) {
     work_coords(blockIdx.x, p.num_splits, p.Hkv, p.B, split, h, b);
     n_items = masked ? min(max(p.block_cnt[b * p.Hkv + h], 0), p.max_blocks) : p.nb;
     const int per = (n_items + p.num_splits - 1) / p.num_splits;
@@ -210,11 +210,15 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
     Tb = seq_len(p, b);
     nbb = (Tb + BLK - 1) / BLK;
   }
+  // scalar registers for the addressing that follows
+  split = __builtin_amdgcn_readfirstlane(split), h = __builtin_amdgcn_readfirstlane(h), b = __builtin_amdgcn_readfirstlane(b);
+  n_items = __builtin_amdgcn_readfirstlane(n_items), i0 = __builtin_amdgcn_readfirstlane(i0), n = __builtin_amdgcn_readfirstlane(n);
+  Tb = __builtin_amdgcn_readfirstlane(Tb), nbb = __builtin_amdgcn_readfirstlane(nbb);
   const int64_t bh = static_cast<int64_t>(b) * p.Hkv + h, hq0 = bh * G;
   const int* list = masked ? p.block_idx + bh * p.max_blocks : nullptr;
   const int* table = paged ? p.block_table + static_cast<int64_t>(b) * p.bt_stride : nullptr;
   const int nw = n > wave ? (n - wave + NWAVE - 1) / NWAVE : 0;
-  const int rot = item_rotation(p, h, split + (rag && p.B > 1 ? n_items : 0), nw);
+  const int rot = item_rotation(p, h, split + (RAG && p.B > 1 ? n_items : 0), nw);
 
   // ---- items of steps k0 .. k0 + 63, in three stages
   auto item_block = [&](Items& x, int k0) {
@@ -252,10 +256,15 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
   const bool up = (lane & 8) != 0;
   const char* kb = reinterpret_cast<const char*>(p.k) + h * p.k_sh;
   const char* vb = reinterpret_cast<const char*>(p.v) + h * p.v_sh;
+  // (through readfirstlane: left to itself the compiler added the offset up in vector registers and wrapped every load in
+  // a loop over the resource's values)
   auto block_res = [&](const char* base, int64_t sb, uint32_t st, int blk, int pg) {
     const int rows = pg >= 0 ? min(BLK, Tb - blk * BLK) : 0;
-    const char* at = base + (paged ? static_cast<int64_t>(pg) * sb : b * sb + static_cast<int64_t>(blk) * BLK * st);
-    return make_rsrc(rows > 0 ? at : base, rows > 0 ? (rows - 1) * st + D : 0u);
+    const int64_t off = paged ? max(pg, 0) * sb : b * sb + static_cast<int64_t>(max(blk, 0)) * BLK * st;
+    const uint64_t at = reinterpret_cast<uint64_t>(base) + off;
+    const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32)));
+    return make_rsrc(reinterpret_cast<const void*>(hi << 32 | lo), rows > 0 ? (rows - 1) * st + D : 0u);
   };
 
   // ---- q as fp16: this lane's head's dims of every k-step, and the factor that takes its power of two out again
@@ -493,12 +502,17 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
   }
 }
 
+template <int D, int GP, bool I8, bool STATS>
+void launch8_r(const Attn8P& p, hipStream_t s) {
+  if (p.seq_lens != nullptr)
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, true>), attn_grid(p), dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, false>), attn_grid(p), dim3(NT), 0, s, p);
+}
+
 template <int D, int GP, bool I8>
 void launch8(const Attn8P& p, bool stats, hipStream_t s) {
-  if (stats)
-    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, true>), attn_grid(p), dim3(NT), 0, s, p);
-  else
-    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, false>), attn_grid(p), dim3(NT), 0, s, p);
+  stats ? launch8_r<D, GP, I8, true>(p, s) : launch8_r<D, GP, I8, false>(p, s);
 }
 
 template <int D>
