@@ -1017,8 +1017,9 @@ __device__ __forceinline__ void finish_mf(const AttnP& p, float m, float l, cons
 // Body of one merge workgroup (query head hq, dims [32 slice, 32 slice + 32)) over its Sv <= 8 U
 // partials. A workgroup wider than 256 threads (the fused merge + update launch) runs it with its
 // first 256; the others only pass the barriers.
-template <int D, int U, bool WITH_V>
-__device__ __forceinline__ void merge_body(const AttnP& p, int plain, int64_t hq, int slice, int Sv) {
+// (A cache held in 8 bits, P = Attn8P: a NaN of its passes comes out as NaN; the others' merge makes 0 of it.)
+template <int D, int U, bool WITH_V, class P>
+__device__ __forceinline__ void merge_body(const P& p, int plain, int64_t hq, int slice, int Sv) {
   constexpr int NC = 8;
   const int tid = threadIdx.x, cls = (tid / 32) % NC, dl = tid % 32;
   const bool act = tid < 256;
@@ -1048,7 +1049,7 @@ __device__ __forceinline__ void merge_body(const AttnP& p, int plain, int64_t hq
   float A = 0.f, L = 0.f;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (cls + NC * u < Sv && (plain || ls[u] > 0.f)) {  // an empty partial (l = 0) adds nothing
+    if (cls + NC * u < Sv && (plain || (std::is_same_v<P, Attn8P> ? ls[u] != 0.f : ls[u] > 0.f))) {  // an empty partial (l = 0) adds nothing
       const float w = plain ? 1.f : fexp2(ms[u] - mu);
       L += ls[u] * w;
       if constexpr (WITH_V) A += as[u] * w;
@@ -1066,11 +1067,12 @@ __device__ __forceinline__ void merge_body(const AttnP& p, int plain, int64_t hq
     }
     if (plain) l = 1.f;
     if constexpr (WITH_V) {
-      const float o = l > 0.f ? a / l : 0.f;
+      const bool some = std::is_same_v<P, Attn8P> ? l != 0.f : l > 0.f;
+      const float o = some ? a / l : 0.f;
       p.out[hq * D + d] = f2bf(o);
       if (p.out_f32) p.out_f32[hq * D + d] = o;
     }
-    if (!plain && tid == 0 && slice == 0 && p.lse) p.lse[hq] = l > 0.f ? (M + flog2(l)) * LN2 : NEG_INF;
+    if (!plain && tid == 0 && slice == 0 && p.lse) p.lse[hq] = (std::is_same_v<P, Attn8P> ? l != 0.f : l > 0.f) ? (M + flog2(l)) * LN2 : NEG_INF;
   }
 }
 
@@ -1091,8 +1093,8 @@ __device__ __forceinline__ int merge_count(const P& p, int64_t hq) {
 // merge_body with the fewest slots that hold Sv partials (U halved while 4 U still does): a ragged
 // head with few chunks issues no loads for slots it does not have (at S = 128 most heads have a
 // handful of chunks). Sv is uniform, so the choice is a uniform branch.
-template <int D, int U, bool WITH_V>
-__device__ void merge_fit(const AttnP& p, int plain, int64_t hq, int slice, int Sv) {
+template <int D, int U, bool WITH_V, class P>
+__device__ void merge_fit(const P& p, int plain, int64_t hq, int slice, int Sv) {
   if constexpr (U > 1) {
     if (Sv <= 8 * (U / 2)) {
       merge_fit<D, U / 2, WITH_V>(p, plain, hq, slice, Sv);

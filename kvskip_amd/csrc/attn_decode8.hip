@@ -5,20 +5,26 @@
 //
 // The work is cut as the bf16 pass cuts it (attn_common.hpp: workgroups of four independent wavefronts, a block per
 // wavefront and step, the split merge a second launch); what differs is inside a block:
-//   codes     every e4m3 and int8 value is a value of fp16: codes become fp16 operands exactly (e4m3 by the hardware's
-//             conversion, int8 by placing the byte under the exponent of 1024 and taking 1152 off), and the block's two
-//             scales enter as scalars: ks with the softmax scale, vs with the block's factor of P V.
-//   q         bf16 as fp16 times a power of two of its head, chosen so that the head's largest value is near 2^15: what
-//             lies below 2^-39 of that is lost.
-//   weights   e = 2^(s - block maximum) in two fp16 parts (22 bits), which fill the operand rows that the group's heads
-//             leave free (up to 8 heads; 9 to 16 take two products). A block's P V starts from zero and is added as
-//             acc = acc * alpha + tmp * (2^(mt - m) vs), so the parts' exponents do not depend on the scales.
+//   scores    e4m3  codes to fp16, exactly (the hardware's conversion), and products with q on v_mfma_f32_16x16x32_f16, q
+//                   in fp16 times a power of two of its head, so that its largest value is near 2^15: whole, but for what
+//                   lies below 2^-39 of that. (The matrix unit also takes e4m3 itself, q cut to two parts of it: a
+//                   quarter of the products and no conversions, but it sums them to 12 to 16 bits of the largest only,
+//                   measured, where fp16 products are summed in fp32.)
+//             int8  K's codes as they lie in memory, q in three digits of 8 bits, together in steps of 2^-22 of its head's
+//                   largest value (v_mfma_i32_16x16x64_i8, exact sums), the digits on the columns that the group's heads
+//                   leave free.
+//   weights   e = 2^(s - block maximum) times 2^(mt - r) vs, rounded to fp16 (2^-11 of a weight, a quarter of a bf16 output's
+//             own half step; softmax sums are taken before the rounding, in fp32). r is the accumulators' reference, at
+//             most 2^7 below the largest weight times |vs| so far: they are rescaled only when a block passes that.
+//   V         codes to fp16, exactly (e4m3 by the hardware's conversion, int8 by placing the byte under the exponent of 1024
+//             and taking 1152 off), rows paired by byte permutation, and P V on v_mfma_f32_16x16x32_f16.
 //   items     lane l of a wavefront holds block, page and scales of the wavefront's step 64 i + l (one gather per 64
 //             steps, the next one fetched during this one in three stages, since a page needs its list entry and a
 //             scale its page); the loop takes them by readlane, so no step waits for them.
 //   memory    each block has a buffer resource of its own, based at the block's first row and ending with the
 //             sequence's last token: no offset of a cache of any length passes 32 bits, rows past the end read zeros
 //             (whatever codes a page holds there), and an empty block reads nothing.
+#include <cstdlib>
 #include "attn_common.hpp"
 
 namespace kvs {
@@ -90,36 +96,150 @@ __device__ __forceinline__ void v_pair8(const u32x2 (&vr)[Lay8<D>::VN], int nt, 
   }
 }
 
-// LDS of the epilogue: the wavefronts' accumulators by part and head, and their (m, l).
+// Two values as fp16, to nearest even, the first in the low half.
+__device__ __forceinline__ uint32_t pack_h(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), f16x2_t));
+}
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+// q as the B operands of the scores' products: column c is head c % GP.
+//   e4m3  x[ks]: fp16 of the dims of k-step ks, 64 (ks / 2) + 16 j + 8 (ks % 2) .. + 7
+//   int8  y[n][c]: dims 64 c + 16 j .. + 15 of one digit: GP 4 the digits on column groups 0, 1, 2 (3: none), GP 8 on
+//         two groups and a second product, GP 16 three products. z: the digit's weight on this lane's column.
+template <int D, int GP, bool I8>
+struct Q8 {
+  static constexpr int NY = GP == 4 ? 1 : GP == 8 ? 2 : 3, KC = D / 64, KS = D / 32;
+  u32x4 x[I8 ? 1 : KS];
+  u32x4 y[I8 ? NY : 1][KC];
+  float z[NY];
+};
+
+template <int D, int GP, bool I8>
+__device__ __forceinline__ void make_q8(Q8<D, GP, I8>& qb, const u32x4 (&qr)[D / 32], float up, int lane) {
+  typedef Q8<D, GP, I8> Q;
+  const int c = lane & 15;
+  if constexpr (I8) {
+#pragma unroll
+    for (int n = 0; n < Q::NY; ++n) {
+      // digit 0 (weight 2^16) .. 2 (1), 3: none
+      const int digit = GP == 4 ? c / 4 : GP == 8 ? (n == 0 ? c / 8 : c < 8 ? 2 : 3) : n;
+      qb.z[n] = digit == 0 ? 65536.f : digit == 1 ? 256.f : 1.f;
+#pragma unroll
+      for (int k = 0; k < Q::KC; ++k)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int o = 0; o < 4; ++o) {
+            const uint32_t two = qr[2 * k + u / 2][2 * (u % 2) + o / 2];
+            int v = static_cast<int>(__builtin_rintf((o % 2 ? bf_hi(two) : bf_lo(two)) * up));
+            int d[3];
+            d[2] = static_cast<int8_t>(v), v = (v - d[2]) >> 8;
+            d[1] = static_cast<int8_t>(v), v = (v - d[1]) >> 8;
+            d[0] = v;
+            const int mine = digit == 0 ? d[0] : digit == 1 ? d[1] : digit == 2 ? d[2] : 0;
+            w |= (static_cast<uint32_t>(mine) & 0xffu) << (8 * o);
+          }
+          qb.y[n][k][u] = w;
+        }
+    }
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < Q::KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qb.x[ks][e] = pack_h(bf_lo(qr[ks][e]) * up, bf_hi(qr[ks][e]) * up);
+  }
+}
+
+// Scores of a block's tokens from K's codes (times the power of two of q): s[nt][i] of head c % GP on every lane.
+template <int D, int GP, bool I8>
+__device__ __forceinline__ void qk8(float (&s)[4][4], const u32x4 (&kr)[4][D / 64], const Q8<D, GP, I8>& qb, int lane) {
+  typedef Q8<D, GP, I8> Q;
+#pragma unroll
+  for (int nt = 0; nt < 4; ++nt) {
+    if constexpr (I8) {
+#pragma unroll
+      for (int n = 0; n < Q::NY; ++n) {
+        i32x4_t a = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < Q::KC; ++k)
+          a = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, kr[nt][k]),
+                                                    __builtin_bit_cast(i32x4_t, qb.y[n][k]), a, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = static_cast<float>(a[i]);
+          s[nt][i] = n == 0 ? x * qb.z[0] : fmaf(x, qb.z[n], s[nt][i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (GP <= 8) s[nt][i] += dpp<DPP_ROR8>(s[nt][i]);
+        if constexpr (GP == 4) s[nt][i] += dpp<0x124>(s[nt][i]);  // row_ror:4
+      }
+    } else {
+      f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < Q::KS; ++ks) {
+        const u32x2 w0 = widen4<I8>(kr[nt][ks / 2][2 * (ks % 2)]), w1 = widen4<I8>(kr[nt][ks / 2][2 * (ks % 2) + 1]);
+        const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, qb.x[ks]), a,
+                                                   0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] = a[i];
+    }
+  }
+}
+
+// acc *= alpha of each row's head (alpha: this lane's head's).
 template <int D, int GP>
+__device__ __forceinline__ void rescale8(f32x4_t (&acc)[D / 16], float alpha, int lane) {
+  float r[4];
+  if constexpr (GP == 16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __shfl(alpha, 4 * (lane >> 4) + i, WAVE);
+  } else {
+    r[0] = dpp<0x150>(alpha), r[1] = dpp<0x151>(alpha), r[2] = dpp<0x152>(alpha), r[3] = dpp<0x153>(alpha);  // row_newbcast
+    if constexpr (GP == 8) {
+      const bool odd = (lane & 16) != 0;  // rows 4 .. 7
+      r[0] = odd ? dpp<0x154>(alpha) : r[0], r[1] = odd ? dpp<0x155>(alpha) : r[1];
+      r[2] = odd ? dpp<0x156>(alpha) : r[2], r[3] = odd ? dpp<0x157>(alpha) : r[3];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] *= r[i];
+}
+
+// LDS of the epilogue: the wavefronts' accumulators by head, and their (m, l, reference of the accumulators).
+template <int D, int GP, int NW>
 struct Merge8 {
-  static constexpr int NP = GP == 16 ? 1 : 2;
-  float acc[NWAVE * NP * GP * D];
-  float ml[NWAVE * GP * 2];
+  float acc[NW * GP * D];
+  float ml[NW * GP * 3];
 };
 
 // The wavefronts' states merged: out / out_f32 / lse (one split) or the split partials. As finish_merge, with G at run
-// time and the two parts of a weight simply added (no code is infinite).
-template <int D, int GP>
-__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, const Merge8<D, GP>& L) {
-  constexpr int NP = Merge8<D, GP>::NP;
+// time.
+template <int D, int GP, int NW>
+__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, const Merge8<D, GP, NW>& L) {
   const int tid = threadIdx.x, S = p.num_splits;
   __syncthreads();
   const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G;
-  for (int o = tid; o < p.G * D; o += NT) {
+  for (int o = tid; o < p.G * D; o += NW * WAVE) {
     const int g = o / D, d = o % D;
     float M = NEG_INF;
 #pragma unroll
-    for (int w = 0; w < NWAVE; ++w) M = fmaxf(M, L.ml[(w * GP + g) * 2]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, L.ml[(w * GP + g) * 3]);
     const float mu = M == NEG_INF ? 0.f : M;
     float A = 0.f, Ls = 0.f;
 #pragma unroll
-    for (int w = 0; w < NWAVE; ++w) {
-      const float f = fexp2(L.ml[(w * GP + g) * 2] - mu);
-      float x = L.acc[((w * NP) * GP + g) * D + d];
-      if constexpr (NP == 2) x += L.acc[((w * NP + 1) * GP + g) * D + d];
-      Ls += L.ml[(w * GP + g) * 2 + 1] * f;
-      A += x * f;
+    for (int w = 0; w < NW; ++w) {
+      const float* ml = L.ml + (w * GP + g) * 3;
+      Ls += ml[1] * fexp2(ml[0] - mu);
+      A += L.acc[(w * GP + g) * D + d] * fexp2(ml[2] - mu - 7.f);
     }
     const int64_t hq = hq0 + g;
     if (S == 1) {
@@ -155,10 +275,11 @@ struct Items {
   float ks, vs;
 };
 
-template <int D, int GP, bool I8, bool STATS, bool RAG>
-__global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
+template <int D, int GP, bool I8, bool STATS, bool RAG, int NW>
+__global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
-  __shared__ __attribute__((aligned(16))) Merge8<D, GP> sL;
+  constexpr int NT = NW * WAVE, NWAVE = NW;
+  __shared__ __attribute__((aligned(16))) Merge8<D, GP, NW> sL;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
   const int j4 = lane >> 4, c16 = lane & 15;
   const bool masked = p.block_idx != nullptr, paged = p.block_table != nullptr;
@@ -244,12 +365,6 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
       x.vs = p.v_scale[i * p.vs_sb + h * p.vs_sh + e];
     }
   };
-  Items cur, nxt;
-  item_block(cur, 0);
-  item_page(cur);
-  item_scales(cur);
-  nxt = cur;
-
   const uint32_t k_st = static_cast<uint32_t>(p.k_st), v_st = static_cast<uint32_t>(p.v_st);
   const uint32_t koff = c16 * k_st + 16 * j4;
   const uint32_t voff = D == 128 ? 4 * j4 * v_st + 8 * c16 : (4 * j4 + (c16 >> 3)) * v_st + 8 * (c16 & 7);
@@ -267,33 +382,47 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
     return make_rsrc(reinterpret_cast<const void*>(hi << 32 | lo), rows > 0 ? (rows - 1) * st + D : 0u);
   };
 
-  // ---- q as fp16: this lane's head's dims of every k-step, and the factor that takes its power of two out again
-  u32x4 qb[KS];
+  // ---- the first block and q: nothing is waited for before the first block's loads but its page
+  Items cur, nxt;
+  item_block(cur, 0);
+  item_page(cur);
+  item_scales(cur);
+  nxt = cur;
+  u32x4 qr[KS];
+  const int qg = c16 % GP;
+  const uint16_t* qp = p.q + b * p.q_sb + (static_cast<int64_t>(h) * G + min(qg, G - 1)) * p.q_sh + 16 * j4;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qr[ks] = ld16(qp + 64 * (ks / 2) + 8 * (ks % 2));
+  u32x4 kr[4][KC];
+  u32x2 vr[VN];
+  int blk = __builtin_amdgcn_readlane(cur.blk, 0), pg = nw > 0 ? __builtin_amdgcn_readlane(cur.pg, 0) : -1;
+  __builtin_amdgcn_sched_barrier(0);
+  load_k8<D>(kr, block_res(kb, p.k_sb, k_st, blk, pg), koff, k_st);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v8<D>(vr, block_res(vb, p.v_sb, v_st, blk, pg), voff, v_st);
+  __builtin_amdgcn_sched_barrier(0);
+
+  // ---- q in the codes' type, and the factor that takes its power of two out again
+  Q8<D, GP, I8> qb;
   float qf;
   {
-    const int g = c16 % GP;
-    float x[KS][8], amax = 0.f;
-    const uint16_t* qp = p.q + b * p.q_sb + (static_cast<int64_t>(h) * G + g) * p.q_sh + 16 * j4;
+    float amax = 0.f, bad = 0.f;  // bad: NaN where q has an infinity or NaN
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const u32x4 w = g < G ? ld16(qp + 64 * (ks / 2) + 8 * (ks % 2)) : u32x4{0u, 0u, 0u, 0u};
+      if (qg >= G) qr[ks] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[ks][2 * e] = bf_lo(w[e]);
-        x[ks][2 * e + 1] = bf_hi(w[e]);
+        const float x = bf_lo(qr[ks][e]), y = bf_hi(qr[ks][e]);
+        amax = fmaxf(amax, fmaxf(fabsf(x), fabsf(y)));
+        bad = fmaf(x, 0.f, fmaf(y, 0.f, bad));
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
     }
     amax = swap_max(amax);
-    const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -112), 127);  // 2^ex <= amax < 2^(ex + 1)
-    const float up_q = __uint_as_float(static_cast<uint32_t>(127 + 14 - ex) << 23);
-    qf = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + ex) << 23);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        qb[ks][e] = f2h(x[ks][2 * e] * up_q) | static_cast<uint32_t>(f2h(x[ks][2 * e + 1] * up_q)) << 16;
+    bad = swap_sum(bad);
+    constexpr int TOP = I8 ? 21 : 14;                               // 2^TOP <= q's largest value < 2^(TOP + 1)
+    const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, TOP - 126), 127);
+    qf = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - TOP + ex) << 23) + bad;
+    make_q8<D, GP, I8>(qb, qr, __uint_as_float(static_cast<uint32_t>(127 + TOP - ex) << 23), lane);
   }
 
   const uint32_t nb4 = 4u * static_cast<uint32_t>(p.nb);
@@ -302,21 +431,15 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
   constexpr uint32_t OOB = 0x80000000u;
   const uint32_t v_stat = c16 < G && j4 == 0 ? c16 * nb4 : OOB;
 
-  float mr = NEG_INF, lr = 0.f;  // running (m, l) of this lane's head c16 % GP
+  float mr = NEG_INF, lr = 0.f, ar = NEG_INF;  // running (m, l) of this lane's head c16 % GP, its accumulators' reference
   f32x4_t acc[VD];
 #pragma unroll
   for (int j = 0; j < VD; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (nw > 0) {
-    u32x4 kr[4][KC];
-    u32x2 vr[VN];
-    int blk = __builtin_amdgcn_readlane(cur.blk, 0), pg = __builtin_amdgcn_readlane(cur.pg, 0);
-    float ks = lane_value(cur.ks, 0), vs = lane_value(cur.vs, 0);
-    load_k8<D>(kr, block_res(kb, p.k_sb, k_st, blk, pg), koff, k_st);
-    __builtin_amdgcn_sched_barrier(0);
-    load_v8<D>(vr, block_res(vb, p.v_sb, v_st, blk, pg), voff, v_st);
     for (int k = 0; k < nw; ++k) {
       // the next 64 steps' items, stage by stage
       const int ph = k & 63;
+      const float ks = lane_value(cur.ks, ph), vs = lane_value(cur.vs, ph);
       if (k - ph + 64 < nw) {
         if (ph == 0) item_block(nxt, k + 64);
         if (ph == 16) item_page(nxt);
@@ -325,63 +448,57 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
       }
       const int kn = (k + 1) & 63;
       int blk_n = -1, pg_n = -1;
-      float ks_n = 0.f, vs_n = 0.f;
       if (k + 1 < nw) {
         blk_n = __builtin_amdgcn_readlane(cur.blk, kn);
         pg_n = __builtin_amdgcn_readlane(cur.pg, kn);
-        ks_n = lane_value(cur.ks, kn);
-        vs_n = lane_value(cur.vs, kn);
       }
       const rsrc_t rk_n = block_res(kb, p.k_sb, k_st, blk_n, pg_n), rv_n = block_res(vb, p.v_sb, v_st, blk_n, pg_n);
 
-      // scores of this block in log2 units: s[nt][i] of head c16 % GP, token 16 nt + 4 j4 + i
+      // scores of this block, s[nt][i] of head c16 % GP, token 16 nt + 4 j4 + i: in log2 units times 1 / f
       float s[4][4], e[4][4];
-      const float f = qf * ks;
+      float f = qf * ks;
+      qk8<D, GP, I8>(s, kr, qb, lane);
+      if ((__float_as_int(ks) ^ __float_as_int(p.scale_log2)) < 0) {  // uniform: a negative scale, f made positive
+        f = -f;
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const u32x2 w0 = widen4<I8>(kr[nt][c][2 * u]), w1 = widen4<I8>(kr[nt][c][2 * u + 1]);
-            const u32x4 w = {w0.x, w0.y, w1.x, w1.y};
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w),
-                                                       __builtin_bit_cast(f16x8_t, qb[2 * c + u]), a, 0, 0, 0);
-          }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] = a[i] * f;
+        for (int t = 0; t < 16; ++t) s[t / 4][t % 4] = -s[t / 4][t % 4];
       }
       const int t0 = blk * BLK, lim = pg >= 0 ? Tb : -BLK;
       if (t0 + BLK > lim) {  // uniform: the block that the sequence's end cuts, or an empty one
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (t0 + mf_tok(nt, i, j4) >= lim) s[nt][i] = NEG_INF;
+          for (int i = 0; i < 4; ++i) s[nt][i] = t0 + mf_tok(nt, i, j4) >= lim ? NEG_INF : s[nt][i] * f;
+        f = 1.f;
       }
       __builtin_amdgcn_sched_barrier(0);
       load_k8<D>(kr, rk_n, koff, k_st);
       __builtin_amdgcn_sched_barrier(0);
 
-      const float mt = block_max_mf(s);
-      // e = 2^15 2^(s - mt): its low part stays a normal fp16 down to 2^-18 of the block's largest weight
-      const float mtu = mt == NEG_INF ? 0.f : mt - 15.f;
+      const float mt = block_max_mf(s) * f;  // f >= 0
+      const float mtu = mt == NEG_INF ? 0.f : mt;
       float r4[4];
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[nt][i] = fexp2(s[nt][i] - mtu);
+        for (int i = 0; i < 4; ++i) e[nt][i] = fexp2(fmaf(s[nt][i], f, -mtu));
         r4[nt] = (e[nt][0] + e[nt][1]) + (e[nt][2] + e[nt][3]);
       }
-      const float st = swap_sum((r4[0] + r4[1]) + (r4[2] + r4[3])) * 0x1p-15f;
+      const float st = swap_sum((r4[0] + r4[1]) + (r4[2] + r4[3]));
       const float m_new = fmaxf(mr, mt);
       const float mu = m_new == NEG_INF ? 0.f : m_new;
-      const float alpha = fexp2(mr - mu);
       const float cf = mt == NEG_INF ? 0.f : fexp2(mt - mu);
-      lr = lr * alpha + st * cf;
+      lr = lr * fexp2(mr - mu) + st * cf;
       mr = m_new;
-      const float fv = cf * 0x1p-15f * vs;
+      // the accumulators' reference: mt + log2 |vs| (its whole part) of the largest block so far, left where it is for as
+      // long as a block passes it by at most 2^7
+      const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(vs) >> 23 & 0xffu) - 127, -100));
+      if (__ballot(mt + ev > ar + 7.f) != 0) {
+        const float an = fmaxf(ar, mt + ev);
+        rescale8<D, GP>(acc, fexp2(ar - (an == NEG_INF ? 0.f : an)), lane);
+        ar = an;
+      }
+      const float fv = vs * fexp2(mt - (ar == NEG_INF ? 0.f : ar)) * 0x1p7f;  // below 2^15
       if constexpr (STATS) {
         const uint32_t blk4 = 4u * static_cast<uint32_t>(max(blk, 0));
         const uint32_t at = blk >= 0 ? v_stat : OOB;
@@ -389,46 +506,15 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
         bstore_f32(st, rs_sum, at, blk4);
       }
 
-      // the weights as operands: the high parts on rows of part 0, what they leave on the others
-      u32x4 ph_[2], pl_[2];
-      const bool low = GP < 16 && (c16 / GP) % 2 == 1;
+      // the weights as operands: row c of a product is head c % GP (rows from GP on are not read)
+      u32x4 w8[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float x = e[2 * q + u / 2][2 * (u % 2)], y = e[2 * q + u / 2][2 * (u % 2) + 1];
-          const auto hi = __builtin_amdgcn_cvt_pkrtz(x, y);
-          const auto lo = __builtin_amdgcn_cvt_pkrtz(x - static_cast<float>(hi.x), y - static_cast<float>(hi.y));
-          const uint32_t uh = __builtin_bit_cast(uint32_t, hi), ul = __builtin_bit_cast(uint32_t, lo);
-          if constexpr (GP == 16) {
-            ph_[q][u] = uh;
-            pl_[q][u] = ul;
-          } else {
-            ph_[q][u] = low ? ul : uh;
-          }
-        }
-      // alpha and fv of this lane's rows 4 j4 + i
-      float al[4], fr[4];
-      auto rows = [&](float (&r)[4], float x) {
-        if constexpr (GP == 16) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[i] = __shfl(x, 4 * j4 + i, WAVE);
-        } else {
-          r[0] = dpp<0x150>(x), r[1] = dpp<0x151>(x), r[2] = dpp<0x152>(x), r[3] = dpp<0x153>(x);  // row_newbcast
-          if constexpr (GP == 8) {
-            const bool odd = (lane & 16) != 0;  // rows 4 .. 7 of an 8-row part
-            r[0] = odd ? dpp<0x154>(x) : r[0], r[1] = odd ? dpp<0x155>(x) : r[1];
-            r[2] = odd ? dpp<0x156>(x) : r[2], r[3] = odd ? dpp<0x157>(x) : r[3];
-          }
-        }
-      };
-      rows(al, alpha);
-      rows(fr, fv);
+        for (int u = 0; u < 4; ++u)
+          w8[q][u] = pack_h(e[2 * q + u / 2][2 * (u % 2)] * fv, e[2 * q + u / 2][2 * (u % 2) + 1] * fv);
 #pragma unroll
       for (int d = 0; d < VD / 4; ++d) {
-        f32x4_t tmp[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tmp[x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           u32x4 w[4];  // four dims, tokens in pairs
@@ -441,47 +527,36 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
             w[0][u] = w01.x, w[1][u] = w01.y, w[2][u] = w23.x, w[3][u] = w23.y;
           }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            tmp[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, ph_[q]),
-                                                            __builtin_bit_cast(f16x8_t, w[x]), tmp[x], 0, 0, 0);
-            if constexpr (GP == 16)
-              tmp[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, pl_[q]),
-                                                              __builtin_bit_cast(f16x8_t, w[x]), tmp[x], 0, 0, 0);
-          }
+          for (int x = 0; x < 4; ++x)
+            acc[4 * d + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w8[q]),
+                                                                    __builtin_bit_cast(f16x8_t, w[x]), acc[4 * d + x], 0, 0, 0);
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[4 * d + x][i] = fmaf(acc[4 * d + x][i], al[i], tmp[x][i] * fr[i]);
       }
       __builtin_amdgcn_sched_barrier(0);
       load_v8<D>(vr, rv_n, voff, v_st);
       blk = blk_n;
       pg = pg_n;
-      ks = ks_n;
-      vs = vs_n;
     }
   }
 
-  // ---- the wavefront's state into LDS (row 4 j4 + i of the products: part and head), then the merge
+  // ---- the wavefront's state into LDS (row 4 j4 + i of the products is head 4 j4 + i), then the merge
   {
-    constexpr int NP = Merge8<D, GP>::NP;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 4 * j4 + i, part = row / GP, g = row % GP;
-      if (part < NP && g < G) {
-        float* a = sL.acc + ((wave * NP + part) * GP + g) * D + mf_vdim<D>(c16);
+      const int g = 4 * j4 + i;
+      if (g < G) {
+        float* a = sL.acc + (wave * GP + g) * D + mf_vdim<D>(c16);
 #pragma unroll
         for (int j = 0; j < VD; j += 4)
           *reinterpret_cast<float4*>(a + j) = make_float4(acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]);
       }
     }
     if (lane < G) {
-      sL.ml[(wave * GP + lane) * 2] = mr;
-      sL.ml[(wave * GP + lane) * 2 + 1] = lr;
+      float* ml = sL.ml + (wave * GP + lane) * 3;
+      ml[0] = mr, ml[1] = lr, ml[2] = ar;
     }
   }
-  finish8<D, GP>(p, b, h, split, sL);
+  finish8<D, GP, NW>(p, b, h, split, sL);
 
   if constexpr (STATS) {
     // the blocks that the list skips, and those past the sequence's end: the gap before each of this split's entries
@@ -502,12 +577,19 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
   }
 }
 
+template <int D, int GP, bool I8, bool STATS, bool RAG>
+void launch8_n(const Attn8P& p, hipStream_t s) {
+  const dim3 grid = attn_grid(p);
+  static const int lim = getenv("KVS_LIM") ? atoi(getenv("KVS_LIM")) : 256;
+  if (static_cast<int>(grid.x) <= lim)
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, RAG, 8>), grid, dim3(8 * WAVE), 0, s, p);
+  else
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, RAG, 4>), grid, dim3(4 * WAVE), 0, s, p);
+}
+
 template <int D, int GP, bool I8, bool STATS>
 void launch8_r(const Attn8P& p, hipStream_t s) {
-  if (p.seq_lens != nullptr)
-    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, true>), attn_grid(p), dim3(NT), 0, s, p);
-  else
-    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, false>), attn_grid(p), dim3(NT), 0, s, p);
+  p.seq_lens != nullptr ? launch8_n<D, GP, I8, STATS, true>(p, s) : launch8_n<D, GP, I8, STATS, false>(p, s);
 }
 
 template <int D, int GP, bool I8>

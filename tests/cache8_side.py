@@ -28,20 +28,23 @@ def typed(codes, fmt, device="cuda"):
 
 def check_out(r, ref, q, k, v, scale, keep=None, what=""):
     """r: K.decode's dict (on the CPU), ref: (out, lse) in 64 bits of q, k, v (values, [B, Hkv, T, D]).
-    Bounds. A score is a sum of D exact products in fp32 times two fp32 factors: |ds| <= (D + 8) 2^-24 A with A the
-    largest scale sum |q_d k_d|. A weight is off by its score's error, twice (its own and the normaliser's), by 2^-21
-    where it is cut to two fp16 parts, and by 2^-22 for v_exp_f32 and the block's factor, taken together as 2^-20; the
-    sums over tokens are fp32 sums of at most 2 x 64 terms a block, then one a block and a split: 2^-17 of the sum of
-    magnitudes for up to 128 terms in a row. So |out - ref| <= (2 ds + 2^-16) sum p |v|, plus half a bf16 step 2^-8 |ref|."""
+    Bounds. q is held in steps of at most 2^-21 of its head's largest element where it is not exact: off by 2^-22 of it.
+    A score is then a sum of D products, each cut at 2^-23 of the largest at worst in the matrix unit, times two fp32
+    factors: |ds| <= (D + 8) 2^-23 A + 2^-22 A' with A the largest scale sum |q_d k_d| and A' that of the head's largest
+    |q| in every place. A weight is off by its score's error, twice (its own and the normaliser's), by 2^-11 where it is
+    rounded to fp16 (with its block's scale), and by 2^-20 for v_exp_f32 and the block's factors; the sums over tokens are
+    fp32 sums: 2^-17 of the sum of magnitudes for up to 128 terms in a row. So |out - ref| <= (2 ds + 2^-11 + 2^-16)
+    sum p |v|, plus half a bf16 step 2^-8 |ref|."""
     out, lse = ref
     B, Hq, D = q.shape
     G = Hq // k.shape[1]
     from oracle import attention as O
 
     A = (O.scores(q.double().abs(), k.abs(), abs(scale))).amax(-1)                     # [B, Hq]
-    ds = (D + 8) * 2.0 ** -24 * A
+    top = q.double().abs().amax(-1, keepdim=True).expand(B, Hq, D)
+    ds = (D + 8) * 2.0 ** -23 * A + 2.0 ** -22 * O.scores(top, k.abs(), abs(scale)).amax(-1)
     absv = O.decode(q.double(), k, v.abs(), scale, keep=keep)[0]
-    tol = (2 * ds[..., None] + 2.0 ** -16) * absv
+    tol = (2 * ds[..., None] + 2.0 ** -11 + 2.0 ** -16) * absv
     got = r["out"].double()
     bad = (got - out).abs() > tol + 2.0 ** -8 * out.abs()
     assert not bad.any(), (what, "out", (got - out).abs().max().item())

@@ -276,8 +276,11 @@ def test_every_code(gpu):
 
         want = OPG.decode_values(codes, fmt) * float(vs[0])
         got = r["out_f32"].double().cpu()[:, 0, 0]
-        # the value is exact in fp16; its weight 2^15 is exact; one product by the scale's factor and one division
-        assert ((got - want).abs() <= 2.0 ** -22 * want.abs()).all(), fmt
+        # the value is exact in fp16; its weight times the scale is rounded to fp16 (2^-11), the rest is fp32
+        assert ((got - want).abs() <= (2.0 ** -11 + 2.0 ** -20) * want.abs()).all(), fmt
+        r = K.decode(_q(n, 2, 64, 1).cuda(), typed(torch.zeros_like(vc), fmt), typed(vc, fmt), 1.0, k_scale=ks.cuda(),
+                     v_scale=torch.full((n, 1, 1), 0.25).cuda(), out_f32=True)
+        assert torch.equal(r["out_f32"].double().cpu()[:, 0, 0], OPG.decode_values(codes, fmt) * 0.25), fmt
 
 
 def test_query_range(gpu):
@@ -296,6 +299,19 @@ def test_query_range(gpu):
         if float(A) * 72 * 2.0 ** -24 < 1:              # else the scores' own rounding decides (fp32 has no more)
             check_out(r, O.decode(one, c.k, c.v, scale), one, c.k, c.v, scale, what=scale)
         assert torch.isfinite(r["out_f32"]).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_query_not_finite(gpu, fmt):
+    """An infinity or NaN in a head's query makes that head NaN, and no other."""
+    c = Case(1, 4, 1, 64, 200, fmt, 3)
+    for bad in (math.inf, -math.inf, math.nan):
+        c.q = _q(1, 4, 64, 3)
+        c.q[0, 2, 60] = bad
+        for S in (1, 2):
+            r = _cpu(c.decode(num_splits=S, out_f32=True))
+            assert torch.isnan(r["out_f32"][0, 2]).all() and torch.isnan(r["lse"][0, 2])
+            assert torch.isfinite(r["out_f32"][0, [0, 1, 3]]).all()
 
 
 def test_scale_range(gpu):
