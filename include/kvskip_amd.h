@@ -404,6 +404,7 @@ typedef struct kvskip_cache8_args {
   const float* k_scale;
   const float* v_scale;
   int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  int32_t* counts;             /* [B, Hkv] workspace, needed with seq_lens (the merge finds each list's partials there) */
   int32_t format;              /* KVSKIP_E4M3 or KVSKIP_INT8 */
 } kvskip_cache8_args;
 
@@ -427,7 +428,8 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
  *      p = n - a + i: slots[row] = page * 64 + p % 64 with page = entry p / 64; -1 where the request was not served, for
  *      a page outside [0, num_pages), and for rows from starts[B] on. Rows past `rows` have no slot.
  * held_out and free_count_out may be held and free_count (the step in place) or buffers of their own (the state before
- * stays, but for table entries and stack positions that it does not count). Table entries past held_out are not cleared.
+ * stays, but for table entries and stack positions that it does not count); with buffers of their own a step of many rows
+ * is one launch instead of two. Table entries past held_out are not cleared.
  * B <= 2048; B * (rows + 1), B * width and 64 * num_pages below 2^31. work: kvskip_page_work_ints(B, rows) int32, or
  * NULL where that is 0. No atomics: the same result every time. */
 typedef struct kvskip_page_args {

@@ -82,7 +82,8 @@ class Cache8Args(ctypes.Structure):
     """kvskip_cache8_args."""
     _fields_ = [
         ("k_scale", c_void_p), ("v_scale", c_void_p),
-        ("ks_sb", c_int64), ("ks_sh", c_int64), ("vs_sb", c_int64), ("vs_sh", c_int64), ("format", c_int32),
+        ("ks_sb", c_int64), ("ks_sh", c_int64), ("vs_sb", c_int64), ("vs_sh", c_int64), ("counts", c_void_p),
+        ("format", c_int32),
     ]
 
 

@@ -1082,6 +1082,7 @@ template <class P>
 __device__ __forceinline__ int merge_count(const P& p, int64_t hq) {
   if (p.seq_lens == nullptr) return p.num_splits;
   const int b = static_cast<int>(hq / p.Hq), h = static_cast<int>(hq % p.Hq) / (p.Hq / p.Hkv);
+  if constexpr (std::is_same_v<P, Attn8P>) return p.counts[b * p.Hkv + h];
   if (p.block_idx != nullptr && p.list_partition != 0) {
     int nv[NRG];
     const int C = global_chunk_len(p, nv);

@@ -24,7 +24,6 @@
 //   memory    each block has a buffer resource of its own, based at the block's first row and ending with the
 //             sequence's last token: no offset of a cache of any length passes 32 bits, rows past the end read zeros
 //             (whatever codes a page holds there), and an empty block reads nothing.
-#include <cstdlib>
 #include "attn_common.hpp"
 
 namespace kvs {
@@ -215,28 +214,28 @@ __device__ __forceinline__ void rescale8(f32x4_t (&acc)[D / 16], float alpha, in
 }
 
 // LDS of the epilogue: the wavefronts' accumulators by head, and their (m, l, reference of the accumulators).
-template <int D, int GP, int NW>
+template <int D, int GP>
 struct Merge8 {
-  float acc[NW * GP * D];
-  float ml[NW * GP * 3];
+  float acc[NWAVE * GP * D];
+  float ml[NWAVE * GP * 3];
 };
 
 // The wavefronts' states merged: out / out_f32 / lse (one split) or the split partials. As finish_merge, with G at run
 // time.
-template <int D, int GP, int NW>
-__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, const Merge8<D, GP, NW>& L) {
+template <int D, int GP>
+__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, const Merge8<D, GP>& L) {
   const int tid = threadIdx.x, S = p.num_splits;
   __syncthreads();
   const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G;
-  for (int o = tid; o < p.G * D; o += NW * WAVE) {
+  for (int o = tid; o < p.G * D; o += NT) {
     const int g = o / D, d = o % D;
     float M = NEG_INF;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, L.ml[(w * GP + g) * 3]);
+    for (int w = 0; w < NWAVE; ++w) M = fmaxf(M, L.ml[(w * GP + g) * 3]);
     const float mu = M == NEG_INF ? 0.f : M;
     float A = 0.f, Ls = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int w = 0; w < NWAVE; ++w) {
       const float* ml = L.ml + (w * GP + g) * 3;
       Ls += ml[1] * fexp2(ml[0] - mu);
       A += L.acc[(w * GP + g) * D + d] * fexp2(ml[2] - mu - 7.f);
@@ -275,11 +274,10 @@ struct Items {
   float ks, vs;
 };
 
-template <int D, int GP, bool I8, bool STATS, bool RAG, int NW>
-__global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
+template <int D, int GP, bool I8, bool STATS, bool RAG>
+__global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
-  constexpr int NT = NW * WAVE, NWAVE = NW;
-  __shared__ __attribute__((aligned(16))) Merge8<D, GP, NW> sL;
+  __shared__ __attribute__((aligned(16))) Merge8<D, GP> sL;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
   const int j4 = lane >> 4, c16 = lane & 15;
   const bool masked = p.block_idx != nullptr, paged = p.block_table != nullptr;
@@ -304,7 +302,7 @@ __global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
       h = it / W;
       C = ragged_lookup(p, h, it % W, masked, b, chunk, n_items);
     }
-    if constexpr (STATS) {  // (sequence, KV head)s with nothing to read: written by one workgroup per KV head
+    {  // (sequence, KV head)s with nothing to read: no partials, statistics written by one workgroup per KV head
       const int eh = global ? (it < p.Hkv ? it : -1) : (it % W == 0 ? h : -1);
       if (eh >= 0) {
         for (int b0 = wave * WAVE; b0 < p.B; b0 += NT) {
@@ -313,13 +311,15 @@ __global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
           while (none != 0) {
             const int be = b0 + __builtin_ctzll(none);
             none &= none - 1;
-            empty_stats(p, static_cast<int64_t>(be) * p.Hq + static_cast<int64_t>(eh) * G, 0, p.nb, lane, WAVE);
+            if (lane == 0) p.counts[be * p.Hkv + eh] = 0;
+            if constexpr (STATS) empty_stats(p, static_cast<int64_t>(be) * p.Hq + static_cast<int64_t>(eh) * G, 0, p.nb, lane, WAVE);
           }
         }
       }
     }
     if (b < 0) return;
     split = chunk;
+    if (chunk == 0 && tid == 0) p.counts[b * p.Hkv + h] = (n_items + C - 1) / C;
     if ((global && (G > 4 || grid_queued(p))) || p.B == 1) {
       i0 = chunk * C;
       n = min(n_items, i0 + C) - i0;
@@ -382,6 +382,14 @@ __global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
     return make_rsrc(reinterpret_cast<const void*>(hi << 32 | lo), rows > 0 ? (rows - 1) * st + D : 0u);
   };
 
+  int gap_prev = -1, gap_cur = 0;  // masked statistics: the list entries around this lane's gap
+  if constexpr (STATS) {
+    const int t = wave + NWAVE * lane;
+    if (masked && t < n) {
+      gap_cur = list[i0 + t];
+      gap_prev = i0 + t > 0 ? list[i0 + t - 1] : -1;
+    }
+  }
   // ---- the first block and q: nothing is waited for before the first block's loads but its page
   Items cur, nxt;
   item_block(cur, 0);
@@ -556,16 +564,23 @@ __global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
       ml[0] = mr, ml[1] = lr, ml[2] = ar;
     }
   }
-  finish8<D, GP, NW>(p, b, h, split, sL);
+  finish8<D, GP>(p, b, h, split, sL);
 
   if constexpr (STATS) {
     // the blocks that the list skips, and those past the sequence's end: the gap before each of this split's entries
     // and, on the split of the last one, what follows it
     if (masked) {
       if (n_items == 0 && split == 0) empty_stats(p, hq0, 0, p.nb, tid, NT);
-      for (int k = i0 + wave; k < i0 + n; k += NWAVE) {
-        const int now = __builtin_amdgcn_readfirstlane(list[k]);
-        const int before = k > 0 ? __builtin_amdgcn_readfirstlane(list[k - 1]) : -1;
+      for (int j = 0; wave + NWAVE * j < n; ++j) {  // uniform over the wavefront
+        int before, now;
+        if (j < WAVE) {
+          before = __builtin_amdgcn_readlane(gap_prev, j);
+          now = __builtin_amdgcn_readlane(gap_cur, j);
+        } else {
+          const int k = i0 + wave + NWAVE * j;
+          now = __builtin_amdgcn_readfirstlane(list[k]);
+          before = __builtin_amdgcn_readfirstlane(list[k - 1]);
+        }
         const int a = min(max(before, -1), p.nb - 1) + 1, len = min(max(now, 0), p.nb) - a;
         empty_stats(p, hq0, a, len, lane, WAVE);
       }
@@ -577,19 +592,12 @@ __global__ void __launch_bounds__(NW * WAVE, 2) decode8_kernel(const Attn8P p) {
   }
 }
 
-template <int D, int GP, bool I8, bool STATS, bool RAG>
-void launch8_n(const Attn8P& p, hipStream_t s) {
-  const dim3 grid = attn_grid(p);
-  static const int lim = getenv("KVS_LIM") ? atoi(getenv("KVS_LIM")) : 256;
-  if (static_cast<int>(grid.x) <= lim)
-    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, RAG, 8>), grid, dim3(8 * WAVE), 0, s, p);
-  else
-    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, RAG, 4>), grid, dim3(4 * WAVE), 0, s, p);
-}
-
 template <int D, int GP, bool I8, bool STATS>
 void launch8_r(const Attn8P& p, hipStream_t s) {
-  p.seq_lens != nullptr ? launch8_n<D, GP, I8, STATS, true>(p, s) : launch8_n<D, GP, I8, STATS, false>(p, s);
+  if (p.seq_lens != nullptr)
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, true>), attn_grid(p), dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL((decode8_kernel<D, GP, I8, STATS, false>), attn_grid(p), dim3(NT), 0, s, p);
 }
 
 template <int D, int GP, bool I8>

@@ -565,6 +565,7 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
   if (a->seq_lens != nullptr) {
     if (a->num_splits < 2) return fail(KVSKIP_E_INVALID, "seq_lens needs num_splits >= 2");
     if (a->B > kvs::MAX_RAGGED_B) return fail(KVSKIP_E_UNSUPPORTED, "seq_lens: B <= %d", kvs::MAX_RAGGED_B);
+    if (c->counts == nullptr) return fail(KVSKIP_E_INVALID, "decode8: seq_lens needs counts [B, Hkv]");
   }
   if (a->list_partition != 0) {
     if (a->list_partition != 1) return fail(KVSKIP_E_INVALID, "list_partition in {0, 1}");
@@ -579,6 +580,7 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
   p.v_scale = c->v_scale;
   p.ks_sb = c->ks_sb; p.ks_sh = c->ks_sh;
   p.vs_sb = c->vs_sb; p.vs_sh = c->vs_sh;
+  p.counts = c->counts;
   p.G = a->Hq / a->Hkv;
   return launched(kvs::launch_decode8(p, a->D, c->format == KVSKIP_INT8, stats != 0, static_cast<hipStream_t>(stream)),
                   "kvskip_decode8");

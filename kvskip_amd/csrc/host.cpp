@@ -785,8 +785,33 @@ void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> t
     if (t != nullptr && t->device() != a.device()) fail(msg);
 }
 
+// kvskip.num_splits_for's rule over `slots` resident workgroups, count by count in the same double arithmetic.
+int64_t split_rule(int64_t bh, int64_t n, int64_t slots, int64_t cap, int64_t least) {
+  auto score = [&](int64_t s) {
+    const double waves = static_cast<double>(bh * s) / static_cast<double>(slots);
+    return waves / std::ceil(waves) - 0.002 * static_cast<double>(s);
+  };
+  int64_t most = 1;  // ceil(n / s) only falls as s grows
+  while (most < cap && std::ceil(static_cast<double>(n) / static_cast<double>(most + 1)) >= static_cast<double>(least))
+    ++most;
+  int64_t best = 1;
+  double best_score = score(1);
+  for (int64_t s = 2; s <= most; ++s) {
+    const double x = score(s);
+    if (x > best_score + 1e-9) best = s, best_score = x;
+  }
+  return best;
+}
+
+// kvskip.ragged_splits' rule (no carried update) over `cus` compute units.
+int64_t ragged_rule(int64_t B, int64_t Hkv, int64_t nb, int64_t cus, int64_t G) {
+  const int64_t per = G <= 4 ? cus * 2 / Hkv - cus / (4 * Hkv) : cus * 2 / Hkv - B;
+  return std::max<int64_t>(2, std::min({int64_t(256), per, std::max<int64_t>(1, B * nb / 8)}));
+}
+
 // decode8(q, k, v, k_scale, v_scale, scale, block_idx, block_cnt, stats, num_splits, want_f32, seq_lens, block_table, T,
-//         list_partition)
+//         list_partition, items, slots): num_splits 0: by kvskip's rules over `slots` workgroup slots for lists of up to
+// `items` blocks (0: every block); list_partition -1: kvskip.decode's choice. Returns the outputs and the split count.
 PyObject* decode8(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &ks = tensor(a[3], "k_scale"),
                    &vs = tensor(a[4], "v_scale");
@@ -816,8 +841,14 @@ PyObject* decode8(PyObject* const* a) {
       require(t->dim() == 2 && t->size(0) == k.size(0) && t->size(1) == d.Hkv, "paged cache: k_scale, v_scale [num_pages, Hkv]");
   }
   const bool stats = truth(a[8]), want_f32 = truth(a[10]);
-  const int64_t S = integer(a[9]);
+  int64_t S = integer(a[9]);
+  if (const int64_t slots = integer(a[16]); S == 0 && slots > 0) {
+    const int64_t items = bi != nullptr ? integer(a[15]) : d.nb;
+    S = lens != nullptr ? ragged_rule(d.B, d.Hkv, items, slots, d.Hq / d.Hkv) : split_rule(d.B * d.Hkv, items, slots, 256, 4);
+  }
   require(1 <= S && S <= 256, "num_splits in 1..256");
+  int32_t lp = int32(a[14]);
+  if (lp < 0) lp = bi != nullptr && lens != nullptr && d.B > 1 && d.B * d.Hkv <= 512;
   const at::Device dev = q.device();
   Outs o;
   at::Tensor out = empty({d.B, d.Hq, d.D}, at::kBFloat16, dev), lse = empty({d.B, d.Hq}, at::kFloat, dev), out32, bmax,
@@ -828,13 +859,27 @@ PyObject* decode8(PyObject* const* a) {
     o.bmax = (bmax = empty({d.B, d.Hq, d.nb}, at::kFloat, dev)).data_ptr();
     o.bsum = (bsum = empty({d.B, d.Hq, d.nb}, at::kFloat, dev)).data_ptr();
   }
-  if (S > 1) part = partials(o, d, S, true, dev);
+  if (S > 1) {  // partials in one allocation, the ragged merge's counts behind them
+    const int64_t acc = d.B * d.Hq * S * d.D, ml = d.B * d.Hq * S * 2;
+    part = empty({acc + ml + (lens != nullptr ? d.B * d.Hkv : 0)}, at::kFloat, dev);
+    float* f = static_cast<float*>(part.data_ptr());
+    o.part_acc = f, o.part_ml = f + acc;
+    if (lens != nullptr) c.counts = reinterpret_cast<int32_t*>(f + acc + ml);
+  }
   kvskip_attn_args args;
-  set_decode(args, q, k, v, real(a[5]), bi, bc, S, o, lens, bt, a[13], int32(a[14]));
+  set_decode(args, q, k, v, real(a[5]), bi, bc, S, o, lens, bt, a[13], lp);
   c.k_scale = static_cast<const float*>(ks.data_ptr()), c.ks_sb = ks.stride(0), c.ks_sh = ks.stride(1);
   c.v_scale = static_cast<const float*>(vs.data_ptr()), c.vs_sb = vs.stride(0), c.vs_sh = vs.stride(1);
   launch(dev, [&](void* s) { return api.decode8(&args, &c, stats, s); });
-  return list_of({out, lse, bmax, bsum, out32});
+  PyObject* l = list_of({out, lse, bmax, bsum, out32});
+  PyObject* n = PyLong_FromLongLong(S);
+  if (n == nullptr || PyList_Append(l, n) != 0) {
+    Py_XDECREF(n);
+    Py_DECREF(l);
+    throw PyErr{};
+  }
+  Py_DECREF(n);
+  return l;
 }
 
 // page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts, short, held_out,
@@ -927,26 +972,12 @@ PyObject* cache_write(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
-// num_splits(bh, n_tiles, slots, max_splits, min_tiles): kvskip.num_splits_for's rule over `slots`
-// resident workgroups, count by count in the same double arithmetic. In Python the scan took 45 us of a
+// num_splits(bh, n_tiles, slots, max_splits, min_tiles): split_rule. In Python the scan took 45 us of a
 // decode call at 32k (63.8 us a call, 27 of them kernels) and 80 us of a planner layer-step.
 PyObject* num_splits(PyObject* const* a) {
   const int64_t bh = integer(a[0]), n = integer(a[1]), slots = integer(a[2]), cap = integer(a[3]), least = integer(a[4]);
   require(bh > 0 && slots > 0, "num_splits_for: bh >= 1 and at least one workgroup slot");
-  auto score = [&](int64_t s) {
-    const double waves = static_cast<double>(bh * s) / static_cast<double>(slots);
-    return waves / std::ceil(waves) - 0.002 * static_cast<double>(s);
-  };
-  int64_t most = 1;  // ceil(n / s) only falls as s grows
-  while (most < cap && std::ceil(static_cast<double>(n) / static_cast<double>(most + 1)) >= static_cast<double>(least))
-    ++most;
-  int64_t best = 1;
-  double best_score = score(1);
-  for (int64_t s = 2; s <= most; ++s) {
-    const double x = score(s);
-    if (x > best_score + 1e-9) best = s, best_score = x;
-  }
-  return PyLong_FromLongLong(best);
+  return PyLong_FromLongLong(split_rule(bh, n, slots, cap, least));
 }
 
 // zeroed(dtype-named shapes, tensor): tensors of zeros on the tensor's device, carved from one zeroed
@@ -1027,7 +1058,7 @@ PyMethodDef methods[] = {
     KVS_FN(attn_block, 20), KVS_FN(vskip1, 13), KVS_FN(select, 10), KVS_FN(pv, 9), KVS_FN(pv_select, 13),
     KVS_FN(plan_block, 33), KVS_FN(update_block, 24), KVS_FN(plan, 2), KVS_FN(merge_update, 3), KVS_FN(plan_scores, 2),
     KVS_FN(update, 2), KVS_FN(num_splits, 5), KVS_FN(zeroed, 2),
-    KVS_FN(decode8, 15), KVS_FN(page_map, 11), KVS_FN(cache_write, 7),
+    KVS_FN(decode8, 17), KVS_FN(page_map, 11), KVS_FN(cache_write, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -52,6 +52,7 @@ struct Attn8P : AttnP {
   const float* k_scale;  // block blk of (b, h): [b * ks_sb + h * ks_sh + blk]; paged: page pg: [pg * ks_sb + h * ks_sh]
   const float* v_scale;
   int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  int* counts;  // with seq_lens: [B, Hkv] partials of each list, written by the split pass for the merge
   int G;
 };
 

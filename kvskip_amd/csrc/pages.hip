@@ -102,7 +102,8 @@ __device__ __forceinline__ void page_fill(const kvskip_page_args& p, const Step&
   }
 }
 
-// The sums; ONE: also page_fill (the whole operator in one launch). A thread holds two neighbouring requests; the three
+// The sums; ONE: also page_fill (the whole operator in one launch: of one workgroup, or of several that all make the sums,
+// the first of which writes them). A thread holds two neighbouring requests; the three
 // prefix sums (pages given, pages taken, rows) meet in LDS together, once, and what needs the total of pages given back
 // (who is served, with how many pages) a second time.
 template <bool ONE>
@@ -149,8 +150,10 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
       s.given[b] = incl[0];
       s.taken[b] = served ? incl[1] : -1;
       s.held[b] = h[r];
-      p.starts[b] = incl[2];
-      p.held_out[b] = served ? need[r] : h[r];
+      if (!ONE || blockIdx.x == 0) {
+        p.starts[b] = incl[2];
+        p.held_out[b] = served ? need[r] : h[r];
+      }
       used += served ? v[r][1] : 0;
       left += served ? 0 : 1;
     }
@@ -160,9 +163,12 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
   used = wave_sum_int(used);
   left = wave_sum_int(left);
   if (lane == 0) tot2[0][wave] = used, tot2[1][wave] = left;
-  if (tid == 0) s.starts[p.B] = p.starts[p.B] = all[2];
+  if (tid == 0) {
+    s.starts[p.B] = all[2];
+    if (!ONE || blockIdx.x == 0) p.starts[p.B] = all[2];
+  }
   __syncthreads();
-  if (wave == NW - 1) {
+  if ((!ONE || blockIdx.x == 0) && wave == NW - 1) {
     used = wave_sum_int(lane < NW ? tot2[0][lane] : 0);
     left = wave_sum_int(lane < NW ? tot2[1][lane] : 0);
     if (lane == 0) {
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
     }
   }
   if constexpr (ONE) {
-    page_fill(p, s, count, avail, tid, PT);
+    page_fill(p, s, count, avail, blockIdx.x * PT + tid, gridDim.x * PT);
   } else {  // what the filling launch needs beside starts
     if (tid == 0) p.work[0] = count, p.work[1] = avail;
     for (int b = tid; b < p.B; b += PT) {
@@ -442,15 +448,30 @@ void launch_write_d(const kvskip_write_args& p, dim3 grid, int win, hipStream_t 
 
 }  // namespace
 
-// One launch up to ONE_ROWS rows of the map, else the sums and a filling launch. us, one launch / two: 24 requests of one
-// new token 5.1 / 8.6, 2048 of one 8.3 / 12.8, 4 of 1024 6.3 / 8.1, 16 of 512 9.8 / 8.1, 64 of 2048 114 / 11.7.
+// One launch of one workgroup up to ONE_ROWS rows of the map. Above, one launch of many workgroups where what they write
+// is none of what the others read (the state's outputs are buffers of their own), else the sums and a filling launch. us,
+// one workgroup / two launches: 24 requests of one new token 5.1 / 8.6, 2048 of one 8.3 / 12.8, 4 of 1024 6.3 / 8.1, 16 of
+// 512 9.8 / 8.1, 64 of 2048 114 / 11.7; two launches / one of many workgroups: MANY_US.
 constexpr int ONE_ROWS = 4096;
 
 int page_work_ints(int B, int rows) { return rows <= ONE_ROWS ? 0 : 2 + 3 * B; }
 
+static bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x + 4 * na <= y || y + 4 * nb <= x;
+}
+
 hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s) {
-  if (p.rows <= ONE_ROWS) {
-    hipLaunchKernelGGL((page_sums_kernel<true>), dim3(1), dim3(PT), 0, s, p);
+  const void* in[] = {p.seq_lens, p.new_lens, p.held, p.free_count};
+  const int64_t n_in[] = {p.B, p.B, p.B, 1};
+  const void* out[] = {p.starts, p.held_out, p.free_count_out, p.short_out};
+  const int64_t n_out[] = {p.B + 1, p.B, 1, 1};
+  bool own = true;
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) own = own && apart(in[i], n_in[i], out[j], n_out[j]);
+  if (p.rows <= ONE_ROWS || own) {
+    const int wgs = p.rows <= ONE_ROWS ? 1 : min(256, (p.rows + PT - 1) / PT);
+    hipLaunchKernelGGL((page_sums_kernel<true>), dim3(wgs), dim3(PT), 0, s, p);
     return hipGetLastError();
   }
   hipLaunchKernelGGL((page_sums_kernel<false>), dim3(1), dim3(PT), 0, s, p);

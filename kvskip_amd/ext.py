@@ -131,7 +131,7 @@ def decode8(q, k, v, k_scale, v_scale, scale, block_idx=None, block_cnt=None, st
     a sequence of length 0 gets out 0 and lse -inf. G = Hq / Hkv in 1..16, D in {64, 128}.
     Returns [out bf16 [B, Hq, D], lse fp32 [B, Hq], blk_max, blk_sum ([B, Hq, nb] or None), out_f32 or None]."""
     return _host().decode8(q, k, v, k_scale, v_scale, scale, block_idx, block_cnt, stats, num_splits, want_f32, seq_lens,
-                           block_table, T, list_partition)
+                           block_table, T, list_partition, 0, 0)[:5]
 
 
 def page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts=None, short=None,

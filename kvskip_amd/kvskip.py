@@ -120,6 +120,12 @@ def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = Fal
     load_v=False) skips the split merge, leaving lse None; k_scale, v_scale (fp32 [B, Hkv, nb], or
     [num_pages, Hkv] over pages) make k, v a cache held in 8 bits (float8_e4m3fn or int8, a scale for
     each block and head: ext.decode8; G up to 16; with V only, no P)."""
+    if k_scale is not None or v_scale is not None:
+        if k_scale is None or v_scale is None:
+            raise RuntimeError("decode: k_scale and v_scale belong together")
+        if not load_v or write_p or not merge:
+            raise RuntimeError("decode: a cache held in 8 bits is read with V, without P, and merged")
+        return _decode8(q, k, v, k_scale, v_scale, scale, plan, stats, num_splits, out_f32, seq_lens, block_table, T)
     q = _as_bhd(q)
     B, Hkv = q.shape[0], k.shape[1]
     tokens = k.shape[2] if block_table is None else int(T)
@@ -130,18 +136,9 @@ def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = Fal
                       else num_splits_for(B * Hkv, items))
     lists = (None, None) if plan is None else (plan.block_idx, plan.block_cnt)
     lp = int(plan is not None and seq_lens is not None and B > 1 and B * Hkv <= 512)
-    if (k_scale is None) != (v_scale is None):
-        raise RuntimeError("decode: k_scale and v_scale belong together")
-    if k_scale is not None:
-        if not load_v or write_p or not merge:
-            raise RuntimeError("decode: a cache held in 8 bits is read with V, without P, and merged")
-        out, lse, bmax, bsum, o32 = ext().decode8(q, k, v, k_scale, v_scale, float(scale), *lists, stats,
-                                                  int(num_splits), out_f32, seq_lens, block_table, T, lp)
-        p = None
-    else:
-        out, lse, bmax, bsum, o32, p = ext().decode(q, k, v, float(scale), *lists, stats, load_v, int(num_splits),
-                                                    int(stages), out_f32, write_p, seq_lens, **_paged(block_table, T),
-                                                    merge=merge, list_partition=lp)
+    out, lse, bmax, bsum, o32, p = ext().decode(q, k, v, float(scale), *lists, stats, load_v, int(num_splits),
+                                                int(stages), out_f32, write_p, seq_lens, **_paged(block_table, T),
+                                                merge=merge, list_partition=lp)
     res = {"out": out, "lse": lse, "num_splits": num_splits}
     extra = {"blk_max": bmax, "blk_sum": bsum} if stats else {}
     if out_f32:
@@ -149,6 +146,24 @@ def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = Fal
     if write_p:
         extra["p"] = p
     res.update(extra)
+    return res
+
+
+def _decode8(q, k, v, k_scale, v_scale, scale, plan, stats, num_splits, out_f32, seq_lens, block_table, T) -> dict:
+    """decode() over a cache held in 8 bits; the split rules above, made up natively where num_splits is not given (the
+    Python around a small call took as long as its kernel: 200 tokens HOST_US us a call)."""
+    idx = cnt = None
+    items = 0
+    if plan is not None:
+        idx, cnt, items = plan.block_idx, plan.block_cnt, plan.max_cnt
+    out, lse, bmax, bsum, o32, splits = _ops._host().decode8(
+        q[:, :, 0] if q.dim() == 4 else q, k, v, k_scale, v_scale, scale, idx, cnt, stats, num_splits or 0, out_f32, seq_lens,
+        block_table, T, -1, items, 0 if num_splits else num_sms() * WG_PER_CU)
+    res = {"out": out, "lse": lse, "num_splits": splits}
+    if stats:
+        res["blk_max"], res["blk_sum"] = bmax, bsum
+    if out_f32:
+        res["out_f32"] = o32
     return res
 
 

@@ -50,6 +50,7 @@ def _attn(**kw):
     (dict(block_idx=0x100), {}, 0, -1, "block_cnt is required"),
     (dict(seq_lens=0x100), {}, 0, -1, "seq_lens needs num_splits >= 2"),
     (dict(seq_lens=0x100, num_splits=2, part_acc=0x10, part_ml=0x10, B=257), {}, 0, -2, "seq_lens: B <= 256"),
+    (dict(seq_lens=0x100, num_splits=2, part_acc=0x10, part_ml=0x10), {}, 0, -1, "seq_lens needs counts"),
     (dict(list_partition=1), {}, 0, -1, "list_partition 1 partitions"),
     (dict(block_table=0x100, num_pages=4, bt_stride=63), {}, 0, -1, "paged cache"),
 ])
