@@ -130,8 +130,10 @@ __device__ __forceinline__ bool grid_queued(const AttnP& p) {
   return (p.num_splits + p.B) * p.Hkv > RESIDENT_SLOTS;
 }
 
-template <int NR>
-__device__ __forceinline__ int fit_chunk_len(const AttnP& p, const int (&nv)[NR], int n_lists, int lo, int c0,
+__device__ __forceinline__ bool grid_queued(const Attn8P& p) { return (p.num_splits + p.B) * p.Hkv > p.resident; }
+
+template <int NR, class P>
+__device__ __forceinline__ int fit_chunk_len(const P& p, const int (&nv)[NR], int n_lists, int lo, int c0,
                                              int slots) {
   if (grid_queued(p) || c0 < 32) return c0;
   int hi = c0;
@@ -210,8 +212,7 @@ __device__ int ragged_lookup(const P& p, int h, int it, bool masked, int& b, int
 }
 
 // Chunks (split partials) of (b, KV head h) under the ragged partition.
-template <class P>
-__device__ __forceinline__ int ragged_chunks(const P& p, int b, int h, bool masked) {
+__device__ __forceinline__ int ragged_chunks(const AttnP& p, int b, int h, bool masked) {
   int nv[NRB];
   const int C = ragged_chunk_len(p, h, masked, nv);
   return (ragged_items(p, b, h, masked) + C - 1) / C;
@@ -227,7 +228,8 @@ __device__ __forceinline__ int ragged_chunks(const P& p, int b, int h, bool mask
 // +0.4 us and B 32 at 64k +3.5 us). Lane j holds lists j + 64 r in nv. Returns C, uniform.
 constexpr int NRG = MAX_GLOBAL_LISTS / WAVE;
 
-__device__ __forceinline__ int global_chunk_len(const AttnP& p, int (&nv)[NRG]) {
+template <class P>
+__device__ __forceinline__ int global_chunk_len(const P& p, int (&nv)[NRG]) {
   const int lane = threadIdx.x % WAVE, nl = p.B * p.Hkv;
   int tot = 0, most = 0;
 #pragma unroll
@@ -252,7 +254,8 @@ __device__ __forceinline__ int global_chunk_len(const AttnP& p, int (&nv)[NRG]) 
 // on its shortest chunks (B 32 at 64k, stable queries: 592.4 -> 579.8 us per layer-step, and
 // 580.2-582.0 -> 577.6-578.1 with the two classes of partial chunks); a resident grid takes them
 // list by list.
-__device__ int global_lookup(const AttnP& p, int it, int& b, int& h, int& chunk, int& items) {
+template <class P>
+__device__ int global_lookup(const P& p, int it, int& b, int& h, int& chunk, int& items) {
   const int lane = threadIdx.x % WAVE, nl = p.B * p.Hkv;
   int nv[NRG];
   const int C = global_chunk_len(p, nv);
@@ -1017,9 +1020,8 @@ __device__ __forceinline__ void finish_mf(const AttnP& p, float m, float l, cons
 // Body of one merge workgroup (query head hq, dims [32 slice, 32 slice + 32)) over its Sv <= 8 U
 // partials. A workgroup wider than 256 threads (the fused merge + update launch) runs it with its
 // first 256; the others only pass the barriers.
-// (A cache held in 8 bits, P = Attn8P: a NaN of its passes comes out as NaN; the others' merge makes 0 of it.)
-template <int D, int U, bool WITH_V, class P>
-__device__ __forceinline__ void merge_body(const P& p, int plain, int64_t hq, int slice, int Sv) {
+template <int D, int U, bool WITH_V>
+__device__ __forceinline__ void merge_body(const AttnP& p, int plain, int64_t hq, int slice, int Sv) {
   constexpr int NC = 8;
   const int tid = threadIdx.x, cls = (tid / 32) % NC, dl = tid % 32;
   const bool act = tid < 256;
@@ -1049,7 +1051,7 @@ __device__ __forceinline__ void merge_body(const P& p, int plain, int64_t hq, in
   float A = 0.f, L = 0.f;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (cls + NC * u < Sv && (plain || (std::is_same_v<P, Attn8P> ? ls[u] != 0.f : ls[u] > 0.f))) {  // an empty partial (l = 0) adds nothing
+    if (cls + NC * u < Sv && (plain || ls[u] > 0.f)) {  // an empty partial (l = 0) adds nothing
       const float w = plain ? 1.f : fexp2(ms[u] - mu);
       L += ls[u] * w;
       if constexpr (WITH_V) A += as[u] * w;
@@ -1067,22 +1069,19 @@ __device__ __forceinline__ void merge_body(const P& p, int plain, int64_t hq, in
     }
     if (plain) l = 1.f;
     if constexpr (WITH_V) {
-      const bool some = std::is_same_v<P, Attn8P> ? l != 0.f : l > 0.f;
-      const float o = some ? a / l : 0.f;
+      const float o = l > 0.f ? a / l : 0.f;
       p.out[hq * D + d] = f2bf(o);
       if (p.out_f32) p.out_f32[hq * D + d] = o;
     }
-    if (!plain && tid == 0 && slice == 0 && p.lse) p.lse[hq] = (std::is_same_v<P, Attn8P> ? l != 0.f : l > 0.f) ? (M + flog2(l)) * LN2 : NEG_INF;
+    if (!plain && tid == 0 && slice == 0 && p.lse) p.lse[hq] = l > 0.f ? (M + flog2(l)) * LN2 : NEG_INF;
   }
 }
 
 // Partials of query head hq: S, or in a ragged batch its (sequence, KV head)'s chunk count (0:
 // nothing attended, out 0 and lse -inf). Uniform over the workgroup.
-template <class P>
-__device__ __forceinline__ int merge_count(const P& p, int64_t hq) {
+__device__ __forceinline__ int merge_count(const AttnP& p, int64_t hq) {
   if (p.seq_lens == nullptr) return p.num_splits;
   const int b = static_cast<int>(hq / p.Hq), h = static_cast<int>(hq % p.Hq) / (p.Hq / p.Hkv);
-  if constexpr (std::is_same_v<P, Attn8P>) return p.counts[b * p.Hkv + h];
   if (p.block_idx != nullptr && p.list_partition != 0) {
     int nv[NRG];
     const int C = global_chunk_len(p, nv);
@@ -1094,8 +1093,8 @@ __device__ __forceinline__ int merge_count(const P& p, int64_t hq) {
 // merge_body with the fewest slots that hold Sv partials (U halved while 4 U still does): a ragged
 // head with few chunks issues no loads for slots it does not have (at S = 128 most heads have a
 // handful of chunks). Sv is uniform, so the choice is a uniform branch.
-template <int D, int U, bool WITH_V, class P>
-__device__ void merge_fit(const P& p, int plain, int64_t hq, int slice, int Sv) {
+template <int D, int U, bool WITH_V>
+__device__ void merge_fit(const AttnP& p, int plain, int64_t hq, int slice, int Sv) {
   if constexpr (U > 1) {
     if (Sv <= 8 * (U / 2)) {
       merge_fit<D, U / 2, WITH_V>(p, plain, hq, slice, Sv);
@@ -1108,8 +1107,8 @@ __device__ void merge_fit(const P& p, int plain, int64_t hq, int slice, int Sv) 
 // Workgroup (x, y) of the (B Hq, D / 32) grid takes item xcd_remap(x + y B Hq) in (query head, dim
 // slice) order, so a KV head's merges run on the XCD that ran its splits (work_coords' mapping),
 // whose L2 still holds the partials just written (config 2's op 26.87 -> 26.52 us).
-template <int D, int U, bool WITH_V, class P>
-__global__ void __launch_bounds__(256) combine_kernel(const P p, int plain) {
+template <int D, int U, bool WITH_V>
+__global__ void __launch_bounds__(256) combine_kernel(const AttnP p, int plain) {
   const int nsl = gridDim.y;
   const int m = xcd_remap(blockIdx.x + blockIdx.y * gridDim.x, gridDim.x * nsl);
   const int64_t hq = m / nsl;
@@ -1122,19 +1121,18 @@ __device__ void merge_body_rt(const AttnP& p, int64_t hq, int slice) {
   merge_fit<D, MAX_SPLITS / 8, true>(p, 0, hq, slice, merge_count(p, hq));
 }
 
-template <int D, bool WITH_V, class P>
-inline void launch_combine_u(const P& p, dim3 grid, int plain, hipStream_t s) {
+template <int D, bool WITH_V>
+inline void launch_combine_u(const AttnP& p, dim3 grid, int plain, hipStream_t s) {
   const int u = (p.num_splits + 7) / 8;
-  if (u <= 1) hipLaunchKernelGGL((combine_kernel<D, 1, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 2) hipLaunchKernelGGL((combine_kernel<D, 2, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 4) hipLaunchKernelGGL((combine_kernel<D, 4, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 8) hipLaunchKernelGGL((combine_kernel<D, 8, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
-  else if (u <= 16) hipLaunchKernelGGL((combine_kernel<D, 16, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
-  else hipLaunchKernelGGL((combine_kernel<D, MAX_SPLITS / 8, WITH_V, P>), grid, dim3(256), 0, s, p, plain);
+  if (u <= 1) hipLaunchKernelGGL((combine_kernel<D, 1, WITH_V>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 2) hipLaunchKernelGGL((combine_kernel<D, 2, WITH_V>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 4) hipLaunchKernelGGL((combine_kernel<D, 4, WITH_V>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 8) hipLaunchKernelGGL((combine_kernel<D, 8, WITH_V>), grid, dim3(256), 0, s, p, plain);
+  else if (u <= 16) hipLaunchKernelGGL((combine_kernel<D, 16, WITH_V>), grid, dim3(256), 0, s, p, plain);
+  else hipLaunchKernelGGL((combine_kernel<D, MAX_SPLITS / 8, WITH_V>), grid, dim3(256), 0, s, p, plain);
 }
 
-template <class P>
-inline hipError_t launch_combine(const P& p, int D, bool plain, hipStream_t s) {
+inline hipError_t launch_combine(const AttnP& p, int D, bool plain, hipStream_t s) {
   const bool with_v = p.out != nullptr;
   const dim3 grid(p.B * p.Hq, with_v ? D / 32 : 1);
   const int pl = plain ? 1 : 0;

@@ -13,9 +13,10 @@
 //             int8  K's codes as they lie in memory, q in three digits of 8 bits, together in steps of 2^-22 of its head's
 //                   largest value (v_mfma_i32_16x16x64_i8, exact sums), the digits on the columns that the group's heads
 //                   leave free.
-//   weights   e = 2^(s - block maximum) times 2^(mt - r) vs, rounded to fp16 (2^-11 of a weight, a quarter of a bf16 output's
+//   weights   e = 2^(s - block maximum) times 2^(mt - r) vs, rounded to fp16 (2^-11 of a weight, an eighth of a bf16 output's
 //             own half step; softmax sums are taken before the rounding, in fp32). r is the accumulators' reference, at
 //             most 2^7 below the largest weight times |vs| so far: they are rescaled only when a block passes that.
+//             (fp16 holds nothing finer than 2^-24, so a weight is off by up to 2^-32 of the largest p |vs| of the wavefront.)
 //   V         codes to fp16, exactly (e4m3 by the hardware's conversion, int8 by placing the byte under the exponent of 1024
 //             and taking 1152 off), rows paired by byte permutation, and P V on v_mfma_f32_16x16x32_f16.
 //   items     lane l of a wavefront holds block, page and scales of the wavefront's step 64 i + l (one gather per 64
@@ -220,10 +221,10 @@ struct Merge8 {
   float ml[NWAVE * GP * 3];
 };
 
-// The wavefronts' states merged: out / out_f32 / lse (one split) or the split partials. As finish_merge, with G at run
-// time.
+// The wavefronts' states merged: out / out_f32 / lse (whole: all of the list) or the split partials. As finish_merge, with
+// G at run time.
 template <int D, int GP>
-__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, const Merge8<D, GP>& L) {
+__device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, bool whole, const Merge8<D, GP>& L) {
   const int tid = threadIdx.x, S = p.num_splits;
   __syncthreads();
   const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split
       A += L.acc[(w * GP + g) * D + d] * fexp2(ml[2] - mu - 7.f);
     }
     const int64_t hq = hq0 + g;
-    if (S == 1) {
+    if (whole) {
       // (a NaN sum, from a NaN of q or the cache, comes out as NaN)
       const float r = Ls == 0.f ? 0.f : A / Ls;
       p.out[hq * D + d] = f2bf(r);
@@ -267,15 +268,20 @@ __device__ __forceinline__ void empty_stats(const Attn8P& p, int64_t hq0, int a,
     }
 }
 
-// A wavefront's items of 64 steps, one per lane: block (-1: outside the sequence), page (0 of a contiguous cache; -1:
+// A wavefront's items of 64 steps, one per lane: block (-1: none of the cache's), page (0 of a contiguous cache; -1:
 // nothing to read, an empty block), scales.
 struct Items {
   int blk, pg;
   float ks, vs;
 };
 
+// Workgroups per CU that the registers are to allow: a ragged batch's hide each other's starts and ends (48 sequences of
+// up to 16384 tokens at 4 a CU, two of them running at a time 96.9 us, three 89.1). 16 heads of 128 dims would spill.
+template <int D, int GP>
+constexpr int WG8 = D == 64 ? 4 : GP == 16 ? 2 : 3;
+
 template <int D, int GP, bool I8, bool STATS, bool RAG>
-__global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
+__global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P p) {
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
   __shared__ __attribute__((aligned(16))) Merge8<D, GP> sL;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
@@ -285,6 +291,7 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
 
   // ---- this workgroup's work, as decode_body finds it: list positions / blocks [i0, i0 + n) of the n_items of (b, h)
   int split, h, b, n_items, i0, n, Tb = p.T, nbb = p.nb;
+  bool whole = p.num_splits == 1;
   if constexpr (!RAG) {
     work_coords(blockIdx.x, p.num_splits, p.Hkv, p.B, split, h, b);
     n_items = masked ? min(max(p.block_cnt[b * p.Hkv + h], 0), p.max_blocks) : p.nb;
@@ -319,6 +326,9 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
     }
     if (b < 0) return;
     split = chunk;
+    // (a list of one chunk is finished here, and the merge has nothing to do: 64 sequences of up to 4096 tokens 53.5 us,
+    // 50.2 so)
+    whole = n_items <= C;
     if (chunk == 0 && tid == 0) p.counts[b * p.Hkv + h] = (n_items + C - 1) / C;
     if ((global && (G > 4 || grid_queued(p))) || p.B == 1) {
       i0 = chunk * C;
@@ -351,9 +361,9 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
     }
   };
   auto item_page = [&](Items& x) {
-    if (x.blk < 0 || x.blk >= nbb) x.blk = -1;
-    x.pg = x.blk >= 0 ? 0 : -1;
-    if (paged && x.blk >= 0) x.pg = table[x.blk];
+    if (x.blk < 0 || x.blk >= p.nb) x.blk = -1;
+    x.pg = x.blk >= 0 && x.blk < nbb ? 0 : -1;
+    if (paged && x.pg == 0) x.pg = table[x.blk];
   };
   auto item_scales = [&](Items& x) {
     if (paged && (x.pg < 0 || x.pg >= p.num_pages)) x.pg = -1;
@@ -564,7 +574,7 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
       ml[0] = mr, ml[1] = lr, ml[2] = ar;
     }
   }
-  finish8<D, GP>(p, b, h, split, sL);
+  finish8<D, GP>(p, b, h, split, whole, sL);
 
   if constexpr (STATS) {
     // the blocks that the list skips, and those past the sequence's end: the gap before each of this split's entries
@@ -589,6 +599,81 @@ __global__ void __launch_bounds__(NT, 2) decode8_kernel(const Attn8P p) {
       const int last = masked ? min(max(list[n_items - 1], -1), p.nb - 1) : nbb - 1;
       empty_stats(p, hq0, last + 1, p.nb - last - 1, tid, NT);
     }
+  }
+}
+
+// Split merge: workgroup (b, query head), a thread four dims of a class of splits. A wavefront takes the partials'
+// maxima and sums a split a lane, so the weights 2^(m_s - M) are in LDS after one barrier, under which the accumulators
+// are already on their way. Its workgroup takes the place (xcd_remap) of its KV head's splits, whose L2 holds the partials.
+// A ragged list's partials are counted by the pass; one of a single chunk has its result already. (The merge of the bf16
+// passes, four workgroups a head that count chunks anew, took 10.5 us for 64 sequences of up to 4096 tokens, 8.4 for 16 of
+// up to 32000 of 28 heads; this one 4.6 and 4.8, of which a launch alone is 3.3. Of a dim a thread: 4.7 and 4.8, and one
+// sequence of 32768 tokens in 32 splits 18.1 us a call for 17.2 with four.)
+template <int D>
+__global__ void __launch_bounds__(NT) combine8_kernel(const Attn8P p) {
+  constexpr int NC = NT * 4 / D, U = 4;
+  __shared__ float sW[MAX_SPLITS];
+  __shared__ __attribute__((aligned(16))) float sA[NC * D];
+  const int tid = threadIdx.x, lane = tid % WAVE, cls = tid / (D / 4), d = tid % (D / 4) * 4;
+  const int hq = xcd_remap(blockIdx.x, p.B * p.Hq), S = p.num_splits;
+  const int n = p.seq_lens == nullptr ? S : __builtin_amdgcn_readfirstlane(p.counts[hq / p.Hq * p.Hkv + hq % p.Hq / p.G]);
+  if (p.seq_lens != nullptr && n == 1) return;
+  const float* ml = p.part_ml + static_cast<int64_t>(hq) * S * 2;
+  const float* acc = p.part_acc + static_cast<int64_t>(hq) * S * D + d;
+  auto load = [&](int s) {
+    return s < n ? *reinterpret_cast<const f32x4_t*>(acc + s * D) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  float ms[MAX_SPLITS / WAVE], ls[MAX_SPLITS / WAVE];
+#pragma unroll
+  for (int r = 0; r < MAX_SPLITS / WAVE; ++r) {
+    const int s = lane + WAVE * r;
+    ms[r] = NEG_INF, ls[r] = 0.f;
+    if (s < n) {
+      const float2 t = *reinterpret_cast<const float2*>(ml + 2 * s);
+      ms[r] = t.x, ls[r] = t.y;
+    }
+  }
+  f32x4_t x[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) x[u] = load(cls + NC * u);
+  float M = NEG_INF, L = 0.f;
+#pragma unroll
+  for (int r = 0; r < MAX_SPLITS / WAVE; ++r) M = fmaxf(M, ms[r]);
+  M = wave_max(M);
+  const float mu = M == NEG_INF ? 0.f : M;
+#pragma unroll
+  for (int r = 0; r < MAX_SPLITS / WAVE; ++r) {
+    // (an empty partial, l = 0, may hold anything in its accumulators and counts for nothing; a NaN counts)
+    const float w = ls[r] == 0.f ? 0.f : fexp2(ms[r] - mu);
+    L += ls[r] * w;
+    if (tid < WAVE && lane + WAVE * r < n) sW[lane + WAVE * r] = ls[r] == 0.f ? -1.f : w;
+  }
+  L = wave_sum(L);
+  __syncthreads();
+  f32x4_t A = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = cls; s0 < n; s0 += NC * U) {
+    f32x4_t y[U];  // the next round's, asked for before this one's are added
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = load(s0 + NC * (U + u));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = s0 + NC * u < n ? sW[s0 + NC * u] : -1.f;
+      if (w != -1.f) A += x[u] * w;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = y[u];
+  }
+  *reinterpret_cast<f32x4_t*>(sA + cls * D + d) = A;
+  __syncthreads();
+  if (tid < D) {
+    float a = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) a += sA[c * D + tid];
+    const float o = L == 0.f ? 0.f : a / L;
+    const int64_t at = static_cast<int64_t>(hq) * D + tid;
+    p.out[at] = f2bf(o);
+    if (p.out_f32) p.out_f32[at] = o;
+    if (p.lse && tid == 0) p.lse[hq] = L == 0.f ? NEG_INF : (M + flog2(L)) * LN2;
   }
 }
 
@@ -621,7 +706,11 @@ hipError_t launch_decode8(const Attn8P& p, int D, bool i8, bool stats, hipStream
   D == 128 ? launch8_d<128>(p, i8, stats, s) : launch8_d<64>(p, i8, stats, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.num_splits == 1) return e;
-  return launch_combine(p, D, false, s);
+  if (D == 128)
+    hipLaunchKernelGGL(combine8_kernel<128>, dim3(p.B * p.Hq), dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL(combine8_kernel<64>, dim3(p.B * p.Hq), dim3(NT), 0, s, p);
+  return hipGetLastError();
 }
 
 }  // namespace kvs

@@ -582,6 +582,7 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
   p.vs_sb = c->vs_sb; p.vs_sh = c->vs_sh;
   p.counts = c->counts;
   p.G = a->Hq / a->Hkv;
+  p.resident = 1024;  // (four workgroups per CU; of 128 dims three run at a time, but cut alike they end alike too)
   return launched(kvs::launch_decode8(p, a->D, c->format == KVSKIP_INT8, stats != 0, static_cast<hipStream_t>(stream)),
                   "kvskip_decode8");
 }

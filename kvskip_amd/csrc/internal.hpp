@@ -54,6 +54,7 @@ struct Attn8P : AttnP {
   int64_t ks_sb, ks_sh, vs_sb, vs_sh;
   int* counts;  // with seq_lens: [B, Hkv] partials of each list, written by the split pass for the merge
   int G;
+  int resident;  // workgroups of a ragged grid that run at once
 };
 
 // The planned pass's argument segment (AttnP, kvskip_plan_args and, where an update is carried,

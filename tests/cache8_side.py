@@ -26,7 +26,7 @@ def typed(codes, fmt, device="cuda"):
     return codes.to(device).view(DTYPE[fmt])
 
 
-def check_out(r, ref, q, k, v, scale, keep=None, what=""):
+def check_out(r, ref, q, k, v, scale, keep=None, what="", v_scale=None):
     """r: K.decode's dict (on the CPU), ref: (out, lse) in 64 bits of q, k, v (values, [B, Hkv, T, D]).
     Bounds. q is held in steps of at most 2^-21 of its head's largest element where it is not exact: off by 2^-22 of it.
     A score is then a sum of D products, each cut at 2^-23 of the largest at worst in the matrix unit, times two fp32
@@ -34,7 +34,11 @@ def check_out(r, ref, q, k, v, scale, keep=None, what=""):
     |q| in every place. A weight is off by its score's error, twice (its own and the normaliser's), by 2^-11 where it is
     rounded to fp16 (with its block's scale), and by 2^-20 for v_exp_f32 and the block's factors; the sums over tokens are
     fp32 sums: 2^-17 of the sum of magnitudes for up to 128 terms in a row. So |out - ref| <= (2 ds + 2^-11 + 2^-16)
-    sum p |v|, plus half a bf16 step 2^-8 |ref|."""
+    sum p |v|, plus half a bf16 step 2^-8 |ref|.
+    With v_scale ([B, Hkv, T], each token's, powers of two) also the spacing of fp16 below 2^-14, which no relative error
+    covers where the heaviest tokens hold exact zeros: a weight p vs times 2^7 / 2^r is off by 2^-25 there, and the
+    reference r is log2 of the largest p vs of the wavefront or at most 2^7 below it, so by 2^-32 max(p vs) of a weight, for
+    each |code| = |v| / vs of the sum."""
     out, lse = ref
     B, Hq, D = q.shape
     G = Hq // k.shape[1]
@@ -45,6 +49,10 @@ def check_out(r, ref, q, k, v, scale, keep=None, what=""):
     ds = (D + 8) * 2.0 ** -23 * A + 2.0 ** -22 * O.scores(top, k.abs(), abs(scale)).amax(-1)
     absv = O.decode(q.double(), k, v.abs(), scale, keep=keep)[0]
     tol = (2 * ds[..., None] + 2.0 ** -11 + 2.0 ** -16) * absv
+    if v_scale is not None:
+        vs = v_scale.double().repeat_interleave(G, 1)
+        top = (torch.softmax(O.scores(q.double(), k, scale), -1) * vs).amax(-1, keepdim=True)
+        tol = tol + 2.0 ** -32 * top * (v.abs().repeat_interleave(G, 1) / vs[..., None]).sum(2)
     got = r["out"].double()
     bad = (got - out).abs() > tol + 2.0 ** -8 * out.abs()
     assert not bad.any(), (what, "out", (got - out).abs().max().item())

@@ -176,7 +176,9 @@ def test_ragged_lists(gpu, fmt, lp, Hq, Hkv):
     for b, n in enumerate(lens):
         keep[b, :, math.ceil(n / 64):] = False
     keep[3, 1] = False
-    p = K.make_plan(keep.cuda())
+    past = keep.clone()
+    past[2, 0, 15] = True                               # an entry past the sequence's end: an empty block
+    p = K.make_plan(past.cuda())
     k, v = c.views()
     ks, vs = c.scales()
     out, lse, m, s, o32 = E.decode8(c.q.cuda(), k, v, ks, vs, c.scale, p.block_idx, p.block_cnt, True, 9, True,
@@ -312,6 +314,38 @@ def test_query_not_finite(gpu, fmt):
             r = _cpu(c.decode(num_splits=S, out_f32=True))
             assert torch.isnan(r["out_f32"][0, 2]).all() and torch.isnan(r["lse"][0, 2])
             assert torch.isfinite(r["out_f32"][0, [0, 1, 3]]).all()
+
+
+def test_split_counts(gpu):
+    """The counts made up natively: kvskip.num_splits_for's for one length; grids of whole CUs for a ragged batch."""
+    for B, Hq, Hkv, D, T in ((1, 8, 8, 64, 300), (1, 32, 8, 128, 9000), (3, 14, 2, 64, 5000)):
+        c = Case(B, Hq, Hkv, D, T, "int8", 1)
+        nb = math.ceil(T / 64)
+        assert c.decode()["num_splits"] == K.num_splits_for(B * Hkv, nb)
+        keep = W.random_block_list(B, Hkv, nb, 0.3, 2)
+        p = K.make_plan(keep.cuda())
+        assert c.decode(plan=p)["num_splits"] == K.num_splits_for(B * Hkv, p.max_cnt)
+        S = c.decode(seq_lens=torch.full((B,), T, dtype=torch.int32, device="cuda"))["num_splits"]
+        assert 2 <= S <= 256 and S <= max(2, B * nb // 16)
+        with pytest.raises(RuntimeError, match="num_splits in 1..256"):
+            c.decode(num_splits=257)
+
+
+def test_refusals_on_the_device(gpu):
+    c = Case(2, 8, 2, 64, 130, "e4m3", 1)
+    k, v = c.views()
+    ks, vs = c.scales()
+    q = c.q.cuda()
+    call = lambda q=q, k=k, v=v, ks=ks, vs=vs, **kw: K.decode(q, k, v, 1.0, k_scale=ks, v_scale=vs, **kw)
+    for kw, msg in ((dict(k=k.view(torch.uint8)), "float8_e4m3fn or int8"), (dict(v=v.view(torch.int8)), "one type"),
+                    (dict(k=k[..., :-1]), "shape mismatch|16-byte"), (dict(k=k[:, :, :-1]), "shape mismatch"),
+                    (dict(ks=ks[:, :, :2]), r"ceil\(T / 64\)"), (dict(ks=ks.double()), "fp32"), (dict(ks=ks[0]), "ceil"),
+                    (dict(ks=ks.cpu()), "one device"), (dict(q=q[:, :7]), "multiple of Hkv"),
+                    (dict(seq_lens=torch.ones(2, device="cuda")), "int32"),
+                    (dict(block_table=torch.zeros(2, 3, dtype=torch.int32, device="cuda")), "T .tokens"),
+                    (dict(block_table=torch.zeros(2, 3, dtype=torch.int32, device="cuda"), T=130), "page pools")):
+        with pytest.raises(RuntimeError, match=msg):
+            call(**kw)
 
 
 def test_scale_range(gpu):
