@@ -535,6 +535,7 @@ int kvskip_token_index(const int32_t* ids, int64_t ids_stride, int32_t B, int32_
 int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int stats, void* stream) {
   kvs::Attn8P p;
   std::memset(&p, 0, sizeof(p));
+  if (a != nullptr && a->T > INT32_MAX - 127) return fail(KVSKIP_E_UNSUPPORTED, "decode8: T up to 2^31 - 128");
   int rc = prepare_attn(a, true, false, false, &p, true);
   if (rc != KVSKIP_OK) return rc;
   if (c == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");

@@ -834,6 +834,7 @@ PyObject* decode8(PyObject* const* a) {
   same_device(q, {&k, &v, &ks, &vs, bi, bc, lens, bt}, "decode8: tensors on one device");
   const Dims d = kv_dims(q, k, v, bt, a[13]);
   require(d.B > 0 && d.T > 0, "sizes must be positive");
+  require(d.T <= INT32_MAX - 127, "decode8: T up to 2^31 - 128");
   require(d.Hkv > 0 && d.Hq % d.Hkv == 0, "Hq must be a multiple of Hkv");
   for (const at::Tensor* t : {&ks, &vs}) {
     require(t->scalar_type() == at::kFloat, "k_scale, v_scale: fp32");

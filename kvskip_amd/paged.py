@@ -9,8 +9,7 @@ layers in 8 bits, one block table for all of them, and the free pages.
 
 Nothing synchronises and, but for decode's outputs, nothing is allocated after the construction: a step can be captured in a
 HIP graph and replayed. cache.short (int32 [1], on the device) counts the requests that the last step had no pages for: their
-rows are not written and their lengths end with the pages they hold, so a caller that admits requests without counting pages
-reads it now and then."""
+rows are not written, and a caller that admits requests without counting pages reads it now and then. (Such a request keeps the tokens it had.)"""
 
 from __future__ import annotations
 
@@ -31,6 +30,8 @@ class PagedCache:
                  device="cuda"):
         if fmt not in FORMATS:
             raise ValueError(f"fmt in {sorted(FORMATS)} (got {fmt!r})")
+        if not 1 <= requests <= 256:
+            raise ValueError(f"requests in 1..256, a decode batch's bound (got {requests})")
         i32 = dict(dtype=torch.int32, device=device)
         self.T = (tokens + PAGE - 1) // PAGE * PAGE
         self.pools = [[torch.zeros(pages, Hkv, PAGE, D, dtype=FORMATS[fmt], device=device) for _ in "kv"]
@@ -46,15 +47,19 @@ class PagedCache:
         self.short = torch.zeros(1, **i32)
 
     def step(self, new_lens: torch.Tensor, drop: torch.Tensor | None = None):
-        """Makes room for the step's new tokens (int32 [requests]); the requests that drop marks (bool [requests]) end
-        first, and give their pages back unless they bring new tokens of another request. Updates lens, block_table,
-        slot_map and starts."""
+        """Makes room for the step's new tokens (int32 [requests], in sum at most `rows`; a negative number takes a
+        request's last tokens off, down to none); the requests that drop marks (bool [requests]) end first, and give
+        their pages back, but for those that the place's next request fills at once. Updates lens, block_table, slot_map
+        and starts."""
+        if new_lens.dtype != torch.int32 or new_lens.shape != self.lens.shape or (drop is not None and (
+                drop.dtype != torch.bool or drop.shape != self.lens.shape)):
+            raise RuntimeError("step: new_lens int32 [requests], drop bool [requests]")
         if drop is not None:
             self.lens.masked_fill_(drop, 0)
         self.lens.add_(new_lens)
         K.ext().page_map(self.lens, new_lens, self.held, self.block_table, self.free_pages, self.free_count, self.slot_map,
                          self.starts, self.short)
-        torch.minimum(self.lens, self.held * PAGE, out=self.lens)
+        self.lens.clamp_(min=0).sub_(new_lens * (self.lens > self.held * PAGE))  # not served: as before
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor):
         """The step's keys and values of a layer, bf16 [n, Hkv, D] with n rows, at most the map's (rows past starts' last are

@@ -15,18 +15,18 @@ from oracle import pages as OPG
 
 pytestmark = pytest.mark.gpu
 
-LAYERS, PAGES, HKV, HQ, D, B, TOKENS, ROWS = 2, 40, 2, 6, 64, 5, 640, 256
+LAYERS, HKV, HQ, D, B, TOKENS, ROWS = 2, 2, 6, 64, 5, 640, 512
 
 
 class Beside:
     """The oracle's cache: pages by lists, codes and scales by the oracle's writer, and the rows as they went in."""
 
-    def __init__(self, fmt):
+    def __init__(self, fmt, pages):
         self.fmt = fmt
         self.lens, self.held = [0] * B, [0] * B
-        self.table, self.free, self.count = [[-1] * (TOKENS // 64) for _ in range(B)], list(range(PAGES)), PAGES
-        self.pools = [[torch.zeros(PAGES, HKV, 64, D, dtype=torch.uint8) for _ in "kv"] for _ in range(LAYERS)]
-        self.scales = [[torch.zeros(PAGES, HKV) for _ in "kv"] for _ in range(LAYERS)]
+        self.table, self.free, self.count = [[-1] * (TOKENS // 64) for _ in range(B)], list(range(pages)), pages
+        self.pools = [[torch.zeros(pages, HKV, 64, D, dtype=torch.uint8) for _ in "kv"] for _ in range(LAYERS)]
+        self.scales = [[torch.zeros(pages, HKV) for _ in "kv"] for _ in range(LAYERS)]
         self.rows = [[[[], []] for _ in range(B)] for _ in range(LAYERS)]
 
     def step(self, new, drop):
@@ -38,7 +38,7 @@ class Beside:
         self.lens = [n + a for n, a in zip(self.lens, new)]
         self.slots, self.starts, short, self.table, self.free, self.held, self.count = OPG.page_map(
             self.lens, new, self.held, self.table, self.free, self.count, ROWS)
-        self.lens = [min(n, 64 * h) for n, h in zip(self.lens, self.held)]
+        self.lens = [n - (a if n > 64 * h else 0) for n, h, a in zip(self.lens, self.held, new)]
         return short
 
     def write(self, l, k, v):
@@ -84,10 +84,11 @@ def _script(rng, steps):
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("captured", [False, True])
-def test_serving(gpu, fmt, captured):
+@pytest.mark.parametrize("pages", [40, 6])
+def test_serving(gpu, fmt, captured, pages):
     rng = random.Random(7)
     g = torch.Generator().manual_seed(3)
-    cache, beside = PagedCache(LAYERS, PAGES, HKV, D, B, TOKENS, ROWS, fmt), Beside(fmt)
+    cache, beside = PagedCache(LAYERS, pages, HKV, D, B, TOKENS, ROWS, fmt), Beside(fmt, pages)
     dev = "cuda"
     new_d, drop_d = torch.zeros(B, dtype=torch.int32, device=dev), torch.zeros(B, dtype=torch.bool, device=dev)
     k_d, v_d = (torch.zeros(LAYERS, ROWS, HKV, D, dtype=torch.bfloat16, device=dev) for _ in "kv")
@@ -101,7 +102,7 @@ def test_serving(gpu, fmt, captured):
             outs.append(cache.decode(l, q_d, D ** -0.5))
         return outs
 
-    graph = None
+    shorts = 0
     if captured:
         step()                                          # nothing new: no page, no row
         torch.cuda.synchronize()
@@ -120,6 +121,7 @@ def test_serving(gpu, fmt, captured):
             outs = step()
         torch.cuda.synchronize()
         short = beside.step(new, drop)
+        shorts += short
         assert cache.lens.tolist() == beside.lens and cache.slot_map.tolist() == beside.slots and int(cache.short) == short
         for l in range(LAYERS):
             beside.write(l, k[l], v[l])
@@ -134,8 +136,14 @@ def test_serving(gpu, fmt, captured):
                 r = {x: outs[l][x][b:b + 1].cpu() for x in ("out", "lse")}
                 check_out(r, O.decode(q[b:b + 1], kk, vv, D ** -0.5), q[b:b + 1], kk, vv, D ** -0.5, what=(t, l, b),
                           v_scale=vs)
+    assert (shorts > 0) == (pages == 6)
 
 
-def test_format_refused():
-    with pytest.raises(ValueError, match="fmt in"):
-        PagedCache(1, 1, 1, 64, 1, 64, 1, "bf16", device="cpu")
+def test_take_off(gpu):
+    """A negative count takes tokens off the end, and their pages back; the next ones go in their place."""
+    c = PagedCache(1, 4, 1, 64, 2, 192, 160, "int8")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for new, lens, held in (((130, 5), [130, 5], [3, 1]), ((-70, 1), [60, 6], [1, 1]), ((-100, 0), [0, 6], [0, 1]),
+                            ((64, -6), [64, 0], [1, 0])):
+        c.step(i32(*new))
+        assert c.lens.tolist() == lens and c.held.tolist() == held and int(c.free_count) == 4 - sum(held)

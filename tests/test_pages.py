@@ -35,6 +35,7 @@ def _attn(**kw):
     (dict(Hq=136), {}, 0, -2, "unsupported head dim / group size"),
     (dict(Hq=30), {}, 0, -1, "Hq must be a multiple of Hkv"),
     (dict(T=0), {}, 0, -1, "sizes must be positive"),
+    (dict(T=2 ** 31 - 127), {}, 0, -2, "T up to 2^31 - 128"),
     (dict(k_st=136), {}, 0, -1, "k strides must be multiples of 16"),
     (dict(v=0x3008), {}, 0, -1, "v must be 16-byte aligned"),
     (dict(k=0), {}, 0, -1, "k must be 16-byte aligned"),
