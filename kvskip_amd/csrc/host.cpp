@@ -803,18 +803,34 @@ int64_t split_rule(int64_t bh, int64_t n, int64_t slots, int64_t cap, int64_t le
   return best;
 }
 
+// The splits of a (b, KV head) over a cache held in 8 bits: one while the merge's launch costs more than the steps it saves
+// (8 blocks, 12 of 64 dims; us a call, one / three blocks a split: 512 tokens of 28 heads 9.6 / 10.5, 520 of 64 dims 7.6 /
+// 9.6), then three blocks a workgroup for as long as the workgroups have a CU each (a CU's own rate bounds a short split:
+// one sequence of 6000 tokens over 8 heads in 31 splits of four blocks 10.3, in 32 of three 9.6; of 2050 tokens 9.7 / 9.4),
+// then by split_rule.
+int64_t split_rule8(int64_t bh, int64_t n, int64_t D, int64_t slots) {
+  const int64_t thin = (n + 2) / 3;
+  if (n <= (D == 64 ? 12 : 8)) return 1;
+  return thin * bh <= slots && thin <= 256 ? thin : split_rule(bh, n, slots, 256, 4);
+}
+
 // The split budget of a KV head for a ragged batch over a cache held in 8 bits: the grid's S + B chunk slots a KV head
-// fill a whole number of workgroups per CU, two or as many more as leave S at seven eighths of two (at most four), at
-// least 16 blocks a chunk at full length. Measured, us (e4m3, pages), the bf16 rule's S / this one's: 24 sequences to 20011
-// tokens 72 / 67, 48 to 16384 97 / 89, 6 to 9001 16.7 / 14.6; of 64 dims 24 to 20011 37.2 / 36.3, 48 to 16384 51 / 48.
-int64_t ragged_rule8(int64_t B, int64_t Hkv, int64_t nb, int64_t cus) {
-  int64_t k = 2;
-  while (k < 4 && (cus * k / Hkv - B) * Hkv * 8 < cus * 2 * 7) ++k;
-  return std::max<int64_t>(2, std::min({int64_t(256), cus * k / Hkv - B, std::max<int64_t>(1, B * nb / 16)}));
+// fill a whole number of workgroups per CU. One where that leaves at most 128 blocks a workgroup (64 where S is small beside
+// B, so that the lists' ends weigh more), else two or as many more as leave S at seven eighths of two (at most four).
+// Measured, us (pages), at least 16 blocks a chunk and any fill / this: 3 sequences to 1540 tokens 13.4 / 10.8, to 12000
+// 18.4 / 15.8, 6 to 12000 20.1 / 15.5, to 16000 24.7 / 20.3, of 64 dims 8 to 2050 11.1 / 9.8; one / two to four a CU: 20 to
+// 9001 24.0 / 25.9, 5 of 64 dims to 32000 16.0 / 17.2, but 16 of 28 heads to 32000 (167 blocks) 50.5 / 47.4, 28 to 1500
+// over 8 heads (S 4) 16.8 / 15.0; the bf16 rule's S / this one's: 24 to 20011 72 / 67, 48 to 16384 97 / 89.
+int64_t ragged_rule8(int64_t B, int64_t Hkv, int64_t n, int64_t cus) {
+  auto fill = [&](int64_t k) { return cus * k / Hkv - B; };
+  int64_t k = 1;
+  if (B * n > (2 * fill(1) >= B ? 128 : 64) * fill(1))
+    for (k = 2; k < 4 && fill(k) * Hkv * 8 < cus * 2 * 7;) ++k;
+  return std::max<int64_t>(2, std::min({int64_t(256), fill(k), (B * n + 1) / 2}));
 }
 
 // decode8(q, k, v, k_scale, v_scale, scale, block_idx, block_cnt, stats, num_splits, want_f32, seq_lens, block_table, T,
-//         list_partition, items, slots): num_splits 0: by kvskip's rules over `slots` workgroup slots for lists of up to
+//         list_partition, items, slots): num_splits 0: by the rules above over `slots` workgroup slots for lists of up to
 // `items` blocks (0: every block); list_partition -1: kvskip.decode's choice. Returns the outputs and the split count.
 PyObject* decode8(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &ks = tensor(a[3], "k_scale"),
@@ -849,7 +865,7 @@ PyObject* decode8(PyObject* const* a) {
   int64_t S = integer(a[9]);
   if (const int64_t slots = integer(a[16]); S == 0 && slots > 0) {
     const int64_t items = bi != nullptr ? integer(a[15]) : d.nb;
-    S = lens != nullptr ? ragged_rule8(d.B, d.Hkv, items, slots) : split_rule(d.B * d.Hkv, items, slots, 256, 4);
+    S = lens != nullptr ? ragged_rule8(d.B, d.Hkv, items, slots) : split_rule8(d.B * d.Hkv, items, d.D, slots);
   }
   require(1 <= S && S <= 256, "num_splits in 1..256");
   int32_t lp = int32(a[14]);

@@ -150,7 +150,7 @@ def decode(q, k, v, scale: float, *, plan: Plan | None = None, stats: bool = Fal
 
 
 def _decode8(q, k, v, k_scale, v_scale, scale, plan, stats, num_splits, out_f32, seq_lens, block_table, T) -> dict:
-    """decode() over a cache held in 8 bits; the split rules above, made up natively where num_splits is not given (the
+    """decode() over a cache held in 8 bits; split rules of its own, made up natively where num_splits is not given (the
     Python around a small call took as long as its kernel: 200 tokens 7.9 us a call, 7.2 so)."""
     idx = cnt = None
     items = 0

@@ -317,16 +317,19 @@ def test_query_not_finite(gpu, fmt):
 
 
 def test_split_counts(gpu):
-    """The counts made up natively: kvskip.num_splits_for's for one length; grids of whole CUs for a ragged batch."""
-    for B, Hq, Hkv, D, T in ((1, 8, 8, 64, 300), (1, 32, 8, 128, 9000), (3, 14, 2, 64, 5000)):
+    """The counts made up natively: one split up to 8 blocks (12 of 64 dims), then three blocks each while every split has a CU, then
+    kvskip.num_splits_for's; a ragged batch's fill whole workgroups per CU."""
+    for B, Hq, Hkv, D, T in ((1, 8, 8, 64, 300), (1, 16, 2, 128, 513), (1, 32, 8, 128, 9000), (3, 14, 2, 64, 5000)):
         c = Case(B, Hq, Hkv, D, T, "int8", 1)
         nb = math.ceil(T / 64)
-        assert c.decode()["num_splits"] == K.num_splits_for(B * Hkv, nb)
         keep = W.random_block_list(B, Hkv, nb, 0.3, 2)
         p = K.make_plan(keep.cuda())
-        assert c.decode(plan=p)["num_splits"] == K.num_splits_for(B * Hkv, p.max_cnt)
+        for n, r in ((nb, c.decode()), (p.max_cnt, c.decode(plan=p))):
+            thin = math.ceil(n / 3)
+            assert r["num_splits"] == (1 if n <= (12 if D == 64 else 8) else thin if thin * B * Hkv <= K.num_sms() else
+                                       K.num_splits_for(B * Hkv, n))
         S = c.decode(seq_lens=torch.full((B,), T, dtype=torch.int32, device="cuda"))["num_splits"]
-        assert 2 <= S <= 256 and S <= max(2, B * nb // 16)
+        assert 2 <= S <= max(2, (B * nb + 1) // 2) and (S == (B * nb + 1) // 2 or (S + B) * Hkv % K.num_sms() == 0 or S == 2)
         with pytest.raises(RuntimeError, match="num_splits in 1..256"):
             c.decode(num_splits=257)
 
