@@ -557,6 +557,8 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
     return fail(KVSKIP_E_INVALID, "stats needs blk_max and blk_sum");
   if (a->num_splits > 1 && a->part_acc == nullptr)
     return fail(KVSKIP_E_INVALID, "num_splits > 1 needs the split partial buffers");
+  if (!aligned16(a->out) || !aligned16(a->out_f32) || !aligned16(a->part_acc) || !aligned16(a->part_ml))
+    return fail(KVSKIP_E_INVALID, "decode8: out, out_f32, part_acc, part_ml must be 16-byte aligned");
   if (a->p_out != nullptr || a->key_sums != nullptr)
     return fail(KVSKIP_E_UNSUPPORTED, "decode8: no fp16 P and no key sums");
   if (a->block_idx != nullptr) {

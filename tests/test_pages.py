@@ -44,6 +44,10 @@ def _attn(**kw):
     ({}, dict(format=2), 0, -1, "format e4m3 or int8"),
     ({}, dict(k_scale=0), 0, -1, "k_scale and v_scale"),
     (dict(out=0), {}, 0, -1, "out is required"),
+    (dict(out=0x4008), {}, 0, -1, "must be 16-byte aligned"),
+    (dict(out_f32=0x4008), {}, 0, -1, "must be 16-byte aligned"),
+    (dict(num_splits=4, part_acc=0x4004, part_ml=0x4000), {}, 0, -1, "must be 16-byte aligned"),
+    (dict(num_splits=4, part_acc=0x4000, part_ml=0x4008), {}, 0, -1, "must be 16-byte aligned"),
     ({}, {}, 1, -1, "stats needs blk_max"),
     (dict(num_splits=4), {}, 0, -1, "split partial buffers"),
     (dict(num_splits=257), {}, 0, -1, "num_splits <= 256"),
