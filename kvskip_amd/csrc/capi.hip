@@ -569,6 +569,9 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
     if (a->num_splits < 2) return fail(KVSKIP_E_INVALID, "seq_lens needs num_splits >= 2");
     if (a->B > kvs::MAX_RAGGED_B) return fail(KVSKIP_E_UNSUPPORTED, "seq_lens: B <= %d", kvs::MAX_RAGGED_B);
     if (c->counts == nullptr) return fail(KVSKIP_E_INVALID, "decode8: seq_lens needs counts [B, Hkv]");
+    // (the cut's sums over a batch, and chunk times blocks, stay in 31 bits)
+    if (a->T > (1 << 27) || (a->block_idx != nullptr && a->max_blocks > (1 << 21)))
+      return fail(KVSKIP_E_UNSUPPORTED, "decode8: with seq_lens T up to 2^27, max_blocks up to 2^21");
   }
   if (a->list_partition != 0) {
     if (a->list_partition != 1) return fail(KVSKIP_E_INVALID, "list_partition in {0, 1}");

@@ -56,6 +56,9 @@ def _attn(**kw):
     (dict(seq_lens=0x100), {}, 0, -1, "seq_lens needs num_splits >= 2"),
     (dict(seq_lens=0x100, num_splits=2, part_acc=0x10, part_ml=0x10, B=257), {}, 0, -2, "seq_lens: B <= 256"),
     (dict(seq_lens=0x100, num_splits=2, part_acc=0x10, part_ml=0x10), {}, 0, -1, "seq_lens needs counts"),
+    (dict(seq_lens=0x100, num_splits=2, part_acc=0x10, part_ml=0x10, T=(1 << 27) + 1), dict(counts=0x10), 0, -2, "T up to 2^27"),
+    (dict(seq_lens=0x100, num_splits=2, part_acc=0x10, part_ml=0x10, block_idx=0x100, block_cnt=0x100,
+          max_blocks=(1 << 21) + 1), dict(counts=0x10), 0, -2, "max_blocks up to 2^21"),
     (dict(list_partition=1), {}, 0, -1, "list_partition 1 partitions"),
     (dict(block_table=0x100, num_pages=4, bt_stride=63), {}, 0, -1, "paged cache"),
 ])
