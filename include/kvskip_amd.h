@@ -412,7 +412,8 @@ typedef struct kvskip_cache8_args {
  * Dense or block lists, statistics, split-K, seq_lens, paged caches and list_partition as in kvskip_decode; a sequence
  * of length 0 (seq_lens: clamp(seq_lens[b], 0, T)) gets out 0 and lse -inf. D in {64, 128}, G = Hq / Hkv in 1..16, T up
  * to 2^31 - 128 (with seq_lens to 2^27, and max_blocks to 2^21). out, out_f32, part_acc and part_ml are 16-byte aligned. p_out and key_sums are refused, the V-skip
- * fields ignored. Statistics are those of the scores above. Always the MFMA engine, whatever KVSKIP_AMD_QK says. */
+ * fields ignored. Statistics are those of the scores above. q is exact to 2^-30 of its head's largest element, a weight
+ * holds 22 bits, sums are fp32. Always the MFMA engine, whatever KVSKIP_AMD_QK says. */
 int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int stats, void* stream);
 
 /* A step's block tables and slot map from the requests' lengths. Request b has n = seq_lens[b] tokens after the step

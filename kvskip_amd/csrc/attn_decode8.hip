@@ -10,13 +10,16 @@
 //                   lies below 2^-39 of that. (The matrix unit also takes e4m3 itself, q cut to two parts of it: a
 //                   quarter of the products and no conversions, but it sums them to 12 to 16 bits of the largest only,
 //                   measured, where fp16 products are summed in fp32.)
-//             int8  K's codes as they lie in memory, q in three digits of 8 bits, together in steps of 2^-22 of its head's
+//             int8  K's codes as they lie in memory, q in four digits of 8 bits, together in steps of 2^-29 of its head's
 //                   largest value (v_mfma_i32_16x16x64_i8, exact sums), the digits on the columns that the group's heads
 //                   leave free.
-//   weights   e = 2^(s - block maximum) times 2^(mt - r) vs, rounded to fp16 (2^-11 of a weight, an eighth of a bf16 output's
-//             own half step; softmax sums are taken before the rounding, in fp32). r is the accumulators' reference, at
-//             most 2^7 below the largest weight times |vs| so far: they are rescaled only when a block passes that.
-//             (fp16 holds nothing finer than 2^-24, so a weight is off by up to 2^-32 of the largest p |vs| of the wavefront.)
+//   weights   e = 2^(s - block maximum) times 2^(mt - r) vs in two fp16 parts, 22 bits (softmax sums are taken before, in
+//             fp32). Up to 8 heads the low parts, times 2^11, are the operand rows that the group's heads leave free, with
+//             accumulators of their own (no further product); 9 to 16 heads take a second product for them, onto the same
+//             accumulators. r is the accumulators' reference, at most 2^7 below the largest weight times |vs| so far: they
+//             are rescaled only when a block passes that. (fp16 holds nothing finer than 2^-24, so beside its 2^-22 a weight
+//             is off by up to 2^-43 of the largest p |vs| of the wavefront, of 9 to 16 heads 2^-32.) One part: 32 sequences
+//             of 65536 tokens 607.9 us for 609.0, a ragged batch of 24 of 64 dims 34.9 for 35.4.
 //   V         codes to fp16, exactly (e4m3 by the hardware's conversion, int8 by placing the byte under the exponent of 1024
 //             and taking 1152 off), rows paired by byte permutation, and P V on v_mfma_f32_16x16x32_f16.
 //   items     lane l of a wavefront holds block, page and scales of the wavefront's step 64 i + l (one gather per 64
@@ -102,18 +105,25 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), f16x2_t));
 }
 
+// h c + (a, b) as fp16, rounded once (v_fma_mixlo_f16, v_fma_mixhi_f16).
+__device__ __forceinline__ uint32_t mix_h(f16x2_t h, float c, float a, float b) {
+  return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(fmaf(static_cast<float>(h.x), c, a)),
+                                              static_cast<_Float16>(fmaf(static_cast<float>(h.y), c, b))});
+}
+
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 // q as the B operands of the scores' products: column c is head c % GP.
 //   e4m3  x[ks]: fp16 of the dims of k-step ks, 64 (ks / 2) + 16 j + 8 (ks % 2) .. + 7
-//   int8  y[n][c]: dims 64 c + 16 j .. + 15 of one digit: GP 4 the digits on column groups 0, 1, 2 (3: none), GP 8 on
-//         two groups and a second product, GP 16 three products. z: the digit's weight on this lane's column.
+//   int8  y[n][c]: dims 64 c + 16 j .. + 15 of one digit: GP 4 the digits on the four column groups, GP 8 on two groups of
+//         two products, GP 16 four products. z: the weight of this lane's column in the last one
+//         (the digits of a product before it weigh 2^(8 digits a product) more).
 template <int D, int GP, bool I8>
 struct Q8 {
-  static constexpr int NY = GP == 4 ? 1 : GP == 8 ? 2 : 3, KC = D / 64, KS = D / 32;
+  static constexpr int NY = GP / 4, KC = D / 64, KS = D / 32;
   u32x4 x[I8 ? 1 : KS];
   u32x4 y[I8 ? NY : 1][KC];
-  float z[NY];
+  float z;
 };
 
 template <int D, int GP, bool I8>
@@ -123,26 +133,23 @@ __device__ __forceinline__ void make_q8(Q8<D, GP, I8>& qb, const u32x4 (&qr)[D /
   if constexpr (I8) {
 #pragma unroll
     for (int n = 0; n < Q::NY; ++n) {
-      // digit 0 (weight 2^16) .. 2 (1), 3: none
-      const int digit = GP == 4 ? c / 4 : GP == 8 ? (n == 0 ? c / 8 : c < 8 ? 2 : 3) : n;
-      qb.z[n] = digit == 0 ? 65536.f : digit == 1 ? 256.f : 1.f;
+      const int digit = GP == 4 ? c / 4 : GP == 8 ? 2 * n + c / 8 : n;  // 0 (weight 2^24) .. 3 (1)
+      if (n == Q::NY - 1) qb.z = __uint_as_float((127u + 24u - 8u * digit) << 23);
+      // a digit's byte of each of two values; the lower three are held with 128 added
+      const uint32_t pick = 0x0c0c0000u | (7u - digit) << 8 | (3u - digit), flip = digit == 0 ? 0u : 0x80808080u;
 #pragma unroll
       for (int k = 0; k < Q::KC; ++k)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          uint32_t w = 0;
+          uint32_t v[4];
 #pragma unroll
           for (int o = 0; o < 4; ++o) {
             const uint32_t two = qr[2 * k + u / 2][2 * (u % 2) + o / 2];
-            int v = static_cast<int>(__builtin_rintf((o % 2 ? bf_hi(two) : bf_lo(two)) * up));
-            int d[3];
-            d[2] = static_cast<int8_t>(v), v = (v - d[2]) >> 8;
-            d[1] = static_cast<int8_t>(v), v = (v - d[1]) >> 8;
-            d[0] = v;
-            const int mine = digit == 0 ? d[0] : digit == 1 ? d[1] : digit == 2 ? d[2] : 0;
-            w |= (static_cast<uint32_t>(mine) & 0xffu) << (8 * o);
+            // (below 2^30: the top digit is within +-64)
+            v[o] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf((o % 2 ? bf_hi(two) : bf_lo(two)) * up))) + 0x00808080u;
           }
-          qb.y[n][k][u] = w;
+          qb.y[n][k][u] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], pick), __builtin_amdgcn_perm(v[1], v[0], pick),
+                                                0x05040100u) ^ flip;
         }
     }
   } else {
@@ -170,11 +177,12 @@ __device__ __forceinline__ void qk8(float (&s)[4][4], const u32x4 (&kr)[4][D / 6
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float x = static_cast<float>(a[i]);
-          s[nt][i] = n == 0 ? x * qb.z[0] : fmaf(x, qb.z[n], s[nt][i]);
+          s[nt][i] = n == 0 ? x : fmaf(s[nt][i], GP == 8 ? 65536.f : 256.f, x);
         }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        if constexpr (GP <= 8) s[nt][i] *= qb.z;
         if constexpr (GP <= 8) s[nt][i] += dpp<DPP_ROR8>(s[nt][i]);
         if constexpr (GP == 4) s[nt][i] += dpp<0x124>(s[nt][i]);  // row_ror:4
       }
@@ -214,11 +222,12 @@ __device__ __forceinline__ void rescale8(f32x4_t (&acc)[D / 16], float alpha, in
     for (int i = 0; i < 4; ++i) acc[j][i] *= r[i];
 }
 
-// LDS of the epilogue: the wavefronts' accumulators by head, and each head's (m, l, reference of the accumulators) of all
+// LDS of the epilogue: the wavefronts' accumulators by part and head, and each head's (m, l, reference of the accumulators) of all
 // wavefronts.
 template <int D, int GP>
 struct Merge8 {
-  float acc[NWAVE * GP * D];
+  static constexpr int NP = GP == 16 ? 1 : 2;  // parts of the weights with accumulators of their own
+  float acc[NWAVE * NP * GP * D];
   f32x4_t m[GP], l[GP], r[GP];
 };
 
@@ -227,6 +236,7 @@ struct Merge8 {
 template <int D, int GP>
 __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split, bool whole, const Merge8<D, GP>& L) {
   static_assert(NWAVE == 4, "a vector holds a value of each wavefront");
+  constexpr int NP = Merge8<D, GP>::NP;
   const int S = p.num_splits;
   __syncthreads();
   const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G;
@@ -240,7 +250,9 @@ __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split
 #pragma unroll
     for (int w = 0; w < NWAVE; ++w) {
       Ls += l[w] * fexp2(m[w] - mu);
-      A += *reinterpret_cast<const f32x4_t*>(L.acc + (w * GP + g) * D + d) * fexp2(r[w] - mu - 7.f);
+      f32x4_t x = *reinterpret_cast<const f32x4_t*>(L.acc + (w * NP * GP + g) * D + d);
+      if constexpr (NP == 2) x += *reinterpret_cast<const f32x4_t*>(L.acc + ((w * NP + 1) * GP + g) * D + d) * 0x1p-11f;
+      A += x * fexp2(r[w] - mu - 7.f);
     }
     const int64_t hq = hq0 + g;
     if (whole) {
@@ -379,6 +391,8 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
   const uint32_t koff = c16 * k_st + 16 * j4;
   const uint32_t voff = D == 128 ? 4 * j4 * v_st + 8 * c16 : (4 * j4 + (c16 >> 3)) * v_st + 8 * (c16 & 7);
   const bool up = (lane & 8) != 0;
+  // up to 8 heads: this lane's operand row takes high or low parts of the weights
+  const float part = (c16 / GP) % 2 == 1 ? 0x1p11f : 0.f;
   const char* kb = reinterpret_cast<const char*>(p.k) + h * p.k_sh;
   const char* vb = reinterpret_cast<const char*>(p.v) + h * p.v_sh;
   // (through readfirstlane: left to itself the compiler added the offset up in vector registers and wrapped every load in
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
     }
     amax = swap_max(amax);
     bad = swap_sum(bad);
-    constexpr int TOP = I8 ? 21 : 14;                               // 2^TOP <= q's largest value < 2^(TOP + 1)
+    constexpr int TOP = I8 ? 29 : 14;                               // 2^TOP <= q's largest value < 2^(TOP + 1)
     const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, TOP - 126), 127);
     qf = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - TOP + ex) << 23) + bad;
     make_q8<D, GP, I8>(qb, qr, __uint_as_float(static_cast<uint32_t>(127 + TOP - ex) << 23), lane);
@@ -524,13 +538,24 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
         bstore_f32(st, rs_sum, at, blk4);
       }
 
-      // the weights as operands: row c of a product is head c % GP (rows from GP on are not read)
-      u32x4 w8[2];
+      // the weights as operands: row c of a product is head c % GP, up to 8 heads the high parts in rows below GP and the
+      // low ones in the GP rows after them (the rows from 2 GP on are not read)
+      u32x4 w8[2], wl[2];
+      const float fl = fv * part, fh = fmaf(part, -1.f - 0x1p-11f, 1.f);  // -2^11 or 1
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          w8[q][u] = pack_h(e[2 * q + u / 2][2 * (u % 2)] * fv, e[2 * q + u / 2][2 * (u % 2) + 1] * fv);
+        for (int u = 0; u < 4; ++u) {
+          const float x = e[2 * q + u / 2][2 * (u % 2)], y = e[2 * q + u / 2][2 * (u % 2) + 1];
+          const uint32_t hi = pack_h(x * fv, y * fv);
+          const f16x2_t hf = __builtin_bit_cast(f16x2_t, hi);
+          if constexpr (GP == 16) {
+            w8[q][u] = hi;
+            wl[q][u] = mix_h(hf, -1.f, x * fv, y * fv);
+          } else {  // high rows hi + 0 x, low ones -2^11 hi + 2^11 x
+            w8[q][u] = mix_h(hf, fh, x * fl, y * fl);
+          }
+        }
 #pragma unroll
       for (int d = 0; d < VD / 4; ++d) {
 #pragma unroll
@@ -545,9 +570,13 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
             w[0][u] = w01.x, w[1][u] = w01.y, w[2][u] = w23.x, w[3][u] = w23.y;
           }
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x) {
             acc[4 * d + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w8[q]),
                                                                     __builtin_bit_cast(f16x8_t, w[x]), acc[4 * d + x], 0, 0, 0);
+            if constexpr (GP == 16)
+              acc[4 * d + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(f16x8_t, wl[q]), __builtin_bit_cast(f16x8_t, w[x]), acc[4 * d + x], 0, 0, 0);
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -557,13 +586,14 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
     }
   }
 
-  // ---- the wavefront's state into LDS (row 4 j4 + i of the products is head 4 j4 + i), then the merge
+  // ---- the wavefront's state into LDS (row 4 j4 + i of the products is part and head of Merge8), then the merge
   {
+    constexpr int NP = Merge8<D, GP>::NP;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int g = 4 * j4 + i;
-      if (g < G) {
-        float* a = sL.acc + (wave * GP + g) * D + mf_vdim<D>(c16);
+      const int row = 4 * j4 + i;
+      if (row < NP * GP && row % GP < G) {
+        float* a = sL.acc + (wave * NP * GP + row) * D + mf_vdim<D>(c16);
 #pragma unroll
         for (int j = 0; j < VD; j += 4)
           *reinterpret_cast<float4*>(a + j) = make_float4(acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]);
