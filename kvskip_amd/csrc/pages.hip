@@ -271,7 +271,9 @@ struct Side {
 };
 
 // One run of `len` rows (at most 64) from row rs of the map on, this lane's slot within the page `at`, by T threads: the
-// workgroup's (its wavefronts meet once, over `meet`), or one wavefront's for a run that one load takes.
+// workgroup's (its wavefronts meet once, over `meet`: their maxima and, from the thread that will store the new one, the
+// scale that the page holds, so that no wavefront loads it while that thread may have passed the barrier), or one
+// wavefront's for a run that one load takes.
 template <int FMT, int D, int T>
 __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len, int at, float* meet) {
   constexpr int LPR = D / 8, RPI = T / LPR;                     // lanes a row, rows a load
@@ -297,6 +299,9 @@ __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len
   // page's, but where a slot comes twice, which costs a shuffle a row.
   const rsrc_t src = make_rsrc(s.rows + rs * s.sn, (len - 1) * s.st + 2 * D);
   const rsrc_t dst = make_rsrc(s.pool + pg * s.psb, 63 * s.pst + EB * D);
+  float* scale = FMT == FMT_BF16 ? nullptr : s.scale + pg * s.ssb;
+  float held = 0.f;  // asked for before the rows: whoever waits for those has it
+  if (FMT != FMT_BF16 && (T == WAVE || t == 0)) held = *scale;
   u32x4 x[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) x[i] = bload16<BUF_NT>(src, r0 * s.st + 16 * c, RPI * i * s.st);
@@ -310,10 +315,6 @@ __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len
     for (int i = 0; i < NI; ++i)
       if (RPI * i < len) bstore16(x[i], dst, dst_off(i));
   } else {
-    float* scale = s.scale + pg * s.ssb;
-    const bool anew = fresh & 1;
-    const float held = *scale;
-    const float was = !anew && held > 0.f && held < __builtin_huge_valf() ? held : 0.f;
     // the largest magnitude of the rows that are kept, of bf16 bits without the sign: an infinity counts as the largest
     // finite value, NaN not
     uint32_t top = 0;
@@ -330,14 +331,18 @@ __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len
     }
     float amax = wave_max(__uint_as_float(min(top, 0x7f7fu) << 16));
     if constexpr (T > WAVE) {
-      if (lane == 0) meet[threadIdx.x / WAVE] = amax;
+      if (lane == 0) meet[t / WAVE] = amax;
+      if (t == 0) meet[T / WAVE] = held;
       // a barrier for LDS alone: __syncthreads would wait for the stores of the run before too
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 #pragma unroll
       for (int w = 0; w < T / WAVE; ++w) amax = fmaxf(amax, meet[w]);
+      held = meet[T / WAVE];
     }
+    const bool anew = fresh & 1;
+    const float was = !anew && held > 0.f && held < __builtin_huge_valf() ? held : 0.f;
     constexpr float QMAX = FMT == FMT_E4M3 ? 448.f : 127.f;
     const float now = amax > QMAX * was ? pow2_scale<FMT>(amax) : was;
     const float inv = now > 0.f ? 1.f / now : 0.f;  // exact where now is a power of two
@@ -383,7 +388,7 @@ __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len
 template <int FMT, int D>
 __global__ void __launch_bounds__(CT, (D == 64 ? 8 : 4)) cache_write_kernel(const kvskip_write_args p, int win) {
   constexpr int EB = FMT == FMT_BF16 ? 2 : 1, RPW = WAVE / (D / 8);
-  __shared__ float sMax[2][CT / WAVE];
+  __shared__ float sMax[2][CT / WAVE + 1];
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const bool isv = static_cast<int>(blockIdx.x) >= p.Hkv;
   const int h = blockIdx.x - (isv ? p.Hkv : 0);
