@@ -425,9 +425,13 @@ int kvskip_decode8(const kvskip_attn_args* a, const kvskip_cache8_args* c, int s
  *      free_pages[avail - 1 - k], and goes into table entries [held, need) in order. The first request whose pages do
  *      not suffice, and every later one that needs any, gets none; nor does one with n > 64 * width. Those are not
  *      served: their held count stays, *short_out counts them.
- *   3. row starts[b] + i (starts: the exclusive sums of new_lens; starts[B] all of them) is the request's position
+ *   3. row starts[b] + i (starts: the exclusive sums of min(a, rows + 1); starts[B] all of them) is the request's position
  *      p = n - a + i: slots[row] = page * 64 + p % 64 with page = entry p / 64; -1 where the request was not served, for
  *      a page outside [0, num_pages), and for rows from starts[B] on. Rows past `rows` have no slot.
+ * With lens_out a request is served only if all of its rows have a slot as well (starts[b] + a <= rows; one that does not,
+ * and so every later one with rows, moves no pages), and lens_out[b], which may be seq_lens, is its length after the step:
+ * n where it is served, else n - a as before. (A sum of old length and new tokens that passed 31 bits counts as one whose
+ * rows do not fit.)
  * held_out and free_count_out may be held and free_count (the step in place) or buffers of their own (the state before
  * stays, but for table entries and stack positions that it does not count); with buffers of their own a step of many rows
  * is one launch instead of two. Table entries past held_out are not cleared.
@@ -448,6 +452,7 @@ typedef struct kvskip_page_args {
   int32_t* short_out;          /* one, out */
   int32_t* work;
   int32_t B, width, num_pages, rows;
+  int32_t* lens_out;           /* [B] out, or NULL */
 } kvskip_page_args;
 
 int kvskip_page_map(const kvskip_page_args* p, void* stream);

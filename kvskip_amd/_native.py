@@ -94,6 +94,7 @@ class PageArgs(ctypes.Structure):
         ("bt_stride", c_int64), ("free_pages", c_void_p), ("free_count", c_void_p), ("slots", c_void_p),
         ("starts", c_void_p), ("held_out", c_void_p), ("free_count_out", c_void_p), ("short_out", c_void_p),
         ("work", c_void_p), ("B", c_int32), ("width", c_int32), ("num_pages", c_int32), ("rows", c_int32),
+        ("lens_out", c_void_p),
     ]
 
 

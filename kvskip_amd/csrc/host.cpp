@@ -904,7 +904,7 @@ PyObject* decode8(PyObject* const* a) {
 }
 
 // page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts, short, held_out,
-//          free_count_out)
+//          free_count_out, lens_out)
 PyObject* page_map(PyObject* const* a) {
   const at::Tensor &lens = tensor(a[0], "seq_lens"), &add = tensor(a[1], "new_lens"), &held = tensor(a[2], "held"),
                    &bt = tensor(a[3], "block_table"), &pool = tensor(a[4], "free_pages"), &cnt = tensor(a[5], "free_count"),
@@ -946,6 +946,7 @@ PyObject* page_map(PyObject* const* a) {
   const at::Tensor *ho = opt_tensor(a[9], "held_out"), *co = opt_tensor(a[10], "free_count_out");
   p.held_out = ho != nullptr ? ints(*ho, B, "held_out") : static_cast<int32_t*>(held.data_ptr());
   p.free_count_out = co != nullptr ? ints(*co, 1, "free_count_out") : static_cast<int32_t*>(cnt.data_ptr());
+  if (const at::Tensor* lo = opt_tensor(a[11], "lens_out")) p.lens_out = ints(*lo, B, "lens_out");
   const int64_t n_work = api.page_work_ints(p.B, p.rows);
   if (n_work > 0) p.work = static_cast<int32_t*>((work = empty({n_work}, at::kInt, dev)).data_ptr());
   launch(dev, [&](void* s) { return api.page_map(&p, s); });
@@ -1079,7 +1080,7 @@ PyMethodDef methods[] = {
     KVS_FN(attn_block, 20), KVS_FN(vskip1, 13), KVS_FN(select, 10), KVS_FN(pv, 9), KVS_FN(pv_select, 13),
     KVS_FN(plan_block, 33), KVS_FN(update_block, 24), KVS_FN(plan, 2), KVS_FN(merge_update, 3), KVS_FN(plan_scores, 2),
     KVS_FN(update, 2), KVS_FN(num_splits, 5), KVS_FN(zeroed, 2),
-    KVS_FN(decode8, 17), KVS_FN(page_map, 11), KVS_FN(cache_write, 7),
+    KVS_FN(decode8, 17), KVS_FN(page_map, 12), KVS_FN(cache_write, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -14,6 +14,8 @@
 // written an element. A scale is a power of two: dividing by it is exact, so a code depends on its value and scale
 // alone, and when a later row needs a larger scale, the rows that are there move to it without rounding again (e4m3:
 // but for subnormal codes; int8 rounds once more per doubling, less than the final step in sum).
+#include <type_traits>
+
 #include "common.hpp"
 #include "internal.hpp"
 
@@ -78,7 +80,8 @@ __device__ __forceinline__ int row_slot(const kvskip_page_args& p, const Step& s
 
 // The rows' slots and the pages that change hands, once the sums are in LDS: `threads` threads, this one number t; a
 // wavefront moves the pages of one request (of 64 at a time it skips those with none to move). Nothing that is written
-// is read here: entries given back are read below what a request keeps or in rows that take none, stack positions from
+// is read here (a request's length after the step, where lens_out replaces it, is the same if it is served, and not used
+// if it is not): entries given back are read below what a request keeps or in rows that take none, stack positions from
 // `count` on are not read.
 __device__ __forceinline__ void page_fill(const kvskip_page_args& p, const Step& s, int count, int avail, int t, int threads) {
   for (int i = t; i < p.rows; i += threads) p.slots[i] = row_slot(p, s, count, avail, i);
@@ -115,29 +118,62 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
   const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
   const int count = min(max(*p.free_count, 0), p.num_pages);
   int v[2][3], h[2], need[2];  // of request 2 tid + r: pages given, pages taken, rows
+  int n[2], was[2];     // tokens after the step; before it
   bool fits[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int b = 2 * tid + r;
-    int n = 0, a = 0;
-    h[r] = need[r] = 0;
-    fits[r] = b < p.B && page_need(p, b, n, a, h[r], need[r]);
-    v[r][0] = fits[r] ? max(h[r] - need[r], 0) : 0;
-    v[r][1] = fits[r] ? max(need[r] - h[r], 0) : 0;
+    int a = 0;
+    h[r] = need[r] = n[r] = was[r] = 0;
+    fits[r] = b < p.B && page_need(p, b, n[r], a, h[r], need[r]);
+    was[r] = n[r] - a;
     v[r][2] = min(a, p.rows + 1);
+    if (p.lens_out != nullptr && b < p.B) {
+      const int sum = p.seq_lens[b], add = p.new_lens[b];
+      if (sum < 0 && add > 0) {  // past 31 bits: more rows than any map has
+        was[r] = static_cast<int>(static_cast<uint32_t>(sum) - static_cast<uint32_t>(add));
+        v[r][2] = p.rows + 1;
+      }
+    }
   }
   int incl[3], all[3];
+  auto sums = [&](auto k0, auto k1) {
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    incl[k] = wave_incl_scan(v[0][k] + v[1][k]);
-    if (lane == WAVE - 1) tot[k][wave] = incl[k];
-  }
-  __syncthreads();
+    for (int k = k0; k < k1; ++k) {
+      incl[k] = wave_incl_scan(v[0][k] + v[1][k]);
+      if (lane == WAVE - 1) tot[k][wave] = incl[k];
+    }
+    __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const int x = wave_incl_scan(lane < NW ? tot[k][lane] : 0);
-    all[k] = __builtin_amdgcn_readlane(x, NW - 1);
-    incl[k] += (wave > 0 ? __shfl(x, wave - 1, WAVE) : 0) - v[0][k] - v[1][k];  // now exclusive
+    for (int k = k0; k < k1; ++k) {
+      const int x = wave_incl_scan(lane < NW ? tot[k][lane] : 0);
+      all[k] = __builtin_amdgcn_readlane(x, NW - 1);
+      incl[k] += (wave > 0 ? __shfl(x, wave - 1, WAVE) : 0) - v[0][k] - v[1][k];  // now exclusive
+    }
+  };
+  auto pages = [&] {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      v[r][0] = fits[r] ? max(h[r] - need[r], 0) : 0;
+      v[r][1] = fits[r] ? max(need[r] - h[r], 0) : 0;
+    }
+  };
+  typedef std::integral_constant<int, 0> I0;
+  typedef std::integral_constant<int, 2> I2;
+  typedef std::integral_constant<int, 3> I3;
+  if (p.lens_out == nullptr) {  // uniform
+    pages();
+    sums(I0{}, I3{});
+  } else {  // a request whose rows do not all fit the map moves no pages: rows first
+    sums(I2{}, I3{});
+    int before = incl[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      before += v[r][2];
+      fits[r] = fits[r] && (v[r][2] == 0 || before <= p.rows);
+    }
+    pages();
+    sums(I0{}, I2{});
   }
   const int avail = min(count + all[0], p.num_pages);
   int used = 0, left = 0;
@@ -153,6 +189,7 @@ __global__ void __launch_bounds__(PT) page_sums_kernel(const kvskip_page_args p)
       if (!ONE || blockIdx.x == 0) {
         p.starts[b] = incl[2];
         p.held_out[b] = served ? need[r] : h[r];
+        if (p.lens_out != nullptr) p.lens_out[b] = served ? n[r] : was[r];
       }
       used += served ? v[r][1] : 0;
       left += served ? 0 : 1;
@@ -472,11 +509,11 @@ static bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
 hipError_t launch_page_map(const kvskip_page_args& p, hipStream_t s) {
   const void* in[] = {p.seq_lens, p.new_lens, p.held, p.free_count};
   const int64_t n_in[] = {p.B, p.B, p.B, 1};
-  const void* out[] = {p.starts, p.held_out, p.free_count_out, p.short_out};
-  const int64_t n_out[] = {p.B + 1, p.B, 1, 1};
+  const void* out[] = {p.starts, p.held_out, p.free_count_out, p.short_out, p.lens_out};
+  const int64_t n_out[] = {p.B + 1, p.B, 1, 1, p.B};
   bool own = true;
   for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) own = own && apart(in[i], n_in[i], out[j], n_out[j]);
+    for (int j = 0; j < 4 + (p.lens_out != nullptr); ++j) own = own && apart(in[i], n_in[i], out[j], n_out[j]);
   if (p.rows <= ONE_ROWS || own) {
     const int wgs = p.rows <= ONE_ROWS ? 1 : min(256, (p.rows + PT - 1) / PT);
     hipLaunchKernelGGL((page_sums_kernel<true>), dim3(wgs), dim3(PT), 0, s, p);

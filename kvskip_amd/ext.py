@@ -135,7 +135,7 @@ def decode8(q, k, v, k_scale, v_scale, scale, block_idx=None, block_cnt=None, st
 
 
 def page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts=None, short=None,
-             held_out=None, free_count_out=None):
+             held_out=None, free_count_out=None, lens_out=None):
     """A serving step's block tables and slot map from the requests' lengths, on the device (kvskip_page_map; not in
     kvskip_ext). All int32 on one device: seq_lens [B] (tokens after the step; 0: finished, its pages go back),
     new_lens [B] (of them new), held [B] (pages of each table row), block_table [B, width], free_pages [num_pages] and
@@ -143,9 +143,11 @@ def page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot
     that cannot be served keeps what it holds and gets slots -1.
     Updates block_table and free_pages, and held and free_count (or writes held_out, free_count_out). Row i of the
     step's packed new tokens (request b's from starts[b] on) goes to slot_map[i] = page * 64 + offset; -1 past the last.
+    With lens_out (int32 [B], may be seq_lens) a request is not served either where its rows do not all fit slot_map, and
+    lens_out gets the lengths after the step, those of requests not served as before it.
     Returns [slot_map, starts int32 [B + 1], short int32 [1] (requests not served)]; starts, short: optional buffers."""
     return _host().page_map(seq_lens, new_lens, held, block_table, free_pages, free_count, slot_map, starts, short,
-                            held_out, free_count_out)
+                            held_out, free_count_out, lens_out)
 
 
 def cache_write(k, v, slot_map, k_pool, v_pool, k_scale=None, v_scale=None):

@@ -47,8 +47,9 @@ class PagedCache:
         self.short = torch.zeros(1, **i32)
 
     def step(self, new_lens: torch.Tensor, drop: torch.Tensor | None = None):
-        """Makes room for the step's new tokens (int32 [requests], in sum at most `rows`; a negative number takes a
-        request's last tokens off, down to none); the requests that drop marks (bool [requests]) end first, and give
+        """Makes room for the step's new tokens (int32 [requests]; a negative number takes a request's last tokens off, down to
+        none); a request whose rows pass the map's `rows`, or for which there are no pages, gets none, keeps the tokens it
+        had and counts in `short`. The requests that drop marks (bool [requests]) end first, and give
         their pages back, but for those that the place's next request fills at once. Updates lens, block_table, slot_map
         and starts."""
         if new_lens.dtype != torch.int32 or new_lens.shape != self.lens.shape or (drop is not None and (
@@ -58,8 +59,7 @@ class PagedCache:
             self.lens.masked_fill_(drop, 0)
         self.lens.add_(new_lens)
         K.ext().page_map(self.lens, new_lens, self.held, self.block_table, self.free_pages, self.free_count, self.slot_map,
-                         self.starts, self.short)
-        self.lens.clamp_(min=0).sub_(new_lens * (self.lens > self.held * PAGE))  # not served: as before
+                         self.starts, self.short, lens_out=self.lens)
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor):
         """The step's keys and values of a layer, bf16 [n, Hkv, D] with n rows, at most the map's (rows past starts' last are

@@ -11,22 +11,30 @@ BLOCK = 64
 QMAX = {"e4m3": 448.0, "int8": 127.0}
 
 
-def page_map(lens, new, held, table, free, count, rows):
-    """kvskip_page_map on lists: (slots, starts, short, table, free, held_out, count_out)."""
+def page_map(lens, new, held, table, free, count, rows, whole=False):
+    """kvskip_page_map on lists: (slots, starts, short, table, free, held_out, count_out); whole: with lens_out, the lengths
+    after the step last."""
     table, free, kept = [list(r) for r in table], list(free), list(held)
     width, pages = len(table[0]), len(free)
     n = [max(x, 0) for x in lens]
     a = [min(max(x, 0), y) for x, y in zip(new, n)]
     need = [math.ceil(x / BLOCK) for x in n]
+    over, before, at = [False] * len(n), [y - x for x, y in zip(a, n)], 0
+    for b in range(len(n) if whole else 0):
+        if lens[b] < 0 < new[b]:                  # a sum of 32 bits that passed 31
+            over[b], before[b], at = True, (lens[b] - new[b] + 2 ** 31) % 2 ** 32 - 2 ** 31, rows + 1
+        elif a[b] > 0:
+            at += a[b]
+            over[b] = at > rows
     for b, h in enumerate(held):
-        if need[b] <= width:
+        if need[b] <= width and not over[b]:
             for j in range(need[b], h):
                 free[count] = table[b][j]
                 count += 1
-    slots, starts, short, out_of_pages = [], [0], 0, False
+    slots, starts, short, out_of_pages, n_after = [], [0], 0, False, list(n)
     for b, h in enumerate(held):
         want = max(need[b] - h, 0)
-        fits = need[b] <= width
+        fits = need[b] <= width and not over[b]
         if fits and want > 0 and (out_of_pages or want > count):
             out_of_pages = True
         served = fits and (want == 0 or not out_of_pages)
@@ -37,14 +45,16 @@ def page_map(lens, new, held, table, free, count, rows):
             kept[b] = need[b]
         else:
             short += 1
+            n_after[b] = before[b]
         for p in range(n[b] - a[b], n[b]):
             if len(slots) >= rows:
                 break
             page = table[b][p // BLOCK] if served else -1
             slots.append(page * BLOCK + p % BLOCK if 0 <= page < pages else -1)
-        starts.append(starts[-1] + min(a[b], rows + 1))
+        starts.append(starts[-1] + (rows + 1 if whole and lens[b] < 0 < new[b] else min(a[b], rows + 1)))
     slots += [-1] * (rows - len(slots))
-    return slots[:rows], starts, short, table, free, kept, count
+    res = slots[:rows], starts, short, table, free, kept, count
+    return (*res, n_after) if whole else res
 
 
 def pow2_scale(amax: float, fmt: str) -> float:
