@@ -52,9 +52,10 @@ class PagedCache:
         had and counts in `short`. The requests that drop marks (bool [requests]) end first, and give
         their pages back, but for those that the place's next request fills at once. Updates lens, block_table, slot_map
         and starts."""
-        if new_lens.dtype != torch.int32 or new_lens.shape != self.lens.shape or (drop is not None and (
-                drop.dtype != torch.bool or drop.shape != self.lens.shape)):
-            raise RuntimeError("step: new_lens int32 [requests], drop bool [requests]")
+        for t, ty in ((new_lens, torch.int32), (drop, torch.bool)):
+            if t is not None and (t.dtype != ty or t.shape != self.lens.shape or not t.is_contiguous() or not t.is_cuda
+                                  or t.device != self.lens.device):
+                raise RuntimeError("step: new_lens int32 [requests], drop bool [requests], contiguous on the cache's device")
         if drop is not None:
             self.lens.masked_fill_(drop, 0)
         self.lens.add_(new_lens)
