@@ -7,9 +7,10 @@ layers in 8 bits, one block table for all of them, and the free pages.
         cache.write(l, k, v)                     # bf16 [rows, Hkv, D], request b's rows from cache.starts[b] on
         out = cache.decode(l, q, scale)["out"]   # q [requests, Hq, D]; every request's tokens, new ones included
 
-Nothing synchronises and, but for decode's outputs, nothing is allocated after the construction: a step can be captured in a
-HIP graph and replayed. cache.short (int32 [1], on the device) counts the requests that the last step had no pages for: their
-rows are not written, and a caller that admits requests without counting pages reads it now and then. (Such a request keeps the tokens it had.)"""
+Nothing synchronises: a step can be captured in a HIP graph and replayed. What is allocated after the construction comes from
+torch's allocator: decode's outputs and split partials, and in a step of more than 4096 rows page_map's workspace. cache.short
+(int32 [1], on the device) counts the requests that the last step had no pages or rows for: their rows are not written, they
+keep the tokens they had, and a caller that admits requests without counting pages reads it now and then."""
 
 from __future__ import annotations
 
