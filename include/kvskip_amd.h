@@ -466,7 +466,7 @@ int64_t kvskip_page_work_ints(int32_t B, int32_t rows);
  * bases multiples of 16 bytes).
  * In 8 bits, with scales k_scale[page * ks_sb + head * ks_sh]: let amax be the largest magnitude of the rows written to
  * a page's head (an infinity counts as the largest finite bf16, NaN not). A page whose row 0 is written starts anew
- * (scale 0 before). If amax > qmax * scale (qmax 448 for e4m3, 127 for int8) the scale becomes the smallest power of two
+ * (scale 0 before). If amax > qmax * scale (qmax 448 for e4m3, 127 for int8; the product in fp32) the scale becomes the smallest power of two
  * s >= 2^-126 with amax <= qmax * s, and the page's other rows are moved to it: code' = round(code * old / s). Codes are
  * round(x / scale), to nearest even, infinities at the largest code; NaN is NaN in e4m3 and 0 in int8. A scale that is
  * not positive and finite counts as 0.

@@ -11,8 +11,8 @@
 // cache_write. The rows of one page lie next to each other in the slot map (a run). A workgroup takes a run of one KV
 // head's keys or values: its rows are loaded once, into registers, the largest magnitude goes through LDS, and the codes
 // are stored 8 bytes a lane in the page's order (a head's page is one contiguous piece). Bound by HBM: 2 bytes read and 1
-// written an element. A scale is a power of two: dividing by it is exact, so a code depends on its value and scale
-// alone, and when a later row needs a larger scale, the rows that are there move to it without rounding again (e4m3:
+// written an element. A scale is a power of two (or what a caller brought, as long as it suffices: its quotients are
+// rounded once too): dividing by it is exact, so a code depends on its value and scale alone, and when a later row needs a larger scale, the rows that are there move to it without rounding again (e4m3:
 // but for subnormal codes; int8 rounds once more per doubling, less than the final step in sum).
 #include <type_traits>
 
@@ -257,6 +257,12 @@ __device__ __forceinline__ float pow2_scale(float amax) {
 __device__ __forceinline__ u32x2 bload8(rsrc_t r, uint32_t voff, uint32_t soff) {
   return __builtin_amdgcn_raw_buffer_load_b64(r, static_cast<int>(voff), static_cast<int>(soff), 0);
 }
+__device__ __forceinline__ uint32_t bload4(rsrc_t r, uint32_t voff) {
+  return static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b32(r, static_cast<int>(voff), 0, 0));
+}
+__device__ __forceinline__ void bstore4(uint32_t v, rsrc_t r, uint32_t voff) {
+  __builtin_amdgcn_raw_buffer_store_b32(v, r, static_cast<int>(voff), 0, 0);
+}
 __device__ __forceinline__ void bstore16(u32x4 v, rsrc_t r, uint32_t voff) {
   __builtin_amdgcn_raw_buffer_store_b128(v, r, static_cast<int>(voff), 0, 0);
 }
@@ -294,6 +300,21 @@ __device__ __forceinline__ void values4(uint32_t w, float (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i) & 0xffu));
   }
+}
+
+// A quotient or product y, rounded to fp32, whose exact value lies off it towards the sign of r: rounded to odd instead, so
+// that rounding it once more, to a code, gives the code of the exact value. (Far from every code's border y stays: below
+// 2^-20 the code is 0, past 2^10 the largest.)
+__device__ __forceinline__ float to_odd(float y, float r) {
+  const uint32_t u = __float_as_uint(y);
+  const bool off = r != 0.f && (u & 1u) == 0u && fabsf(y) >= 0x1p-20f && fabsf(y) <= 0x1p10f;
+  return off ? __uint_as_float((r > 0.f) == (y > 0.f) ? u + 1u : u - 1u) : y;
+}
+
+// Powers of two (normal ones): dividing by them is multiplying by their reciprocal.
+__device__ __forceinline__ bool is_pow2(float s) {
+  const uint32_t u = __float_as_uint(s);
+  return (u & 0x7fffffu) == 0u && u != 0u;
 }
 
 constexpr int CT = 256;
@@ -382,17 +403,47 @@ __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len
     const float was = !anew && held > 0.f && held < __builtin_huge_valf() ? held : 0.f;
     constexpr float QMAX = FMT == FMT_E4M3 ? 448.f : 127.f;
     const float now = amax > QMAX * was ? pow2_scale<FMT>(amax) : was;
-    const float inv = now > 0.f ? 1.f / now : 0.f;  // exact where now is a power of two
+    const float inv = now > 0.f ? 1.f / now : 0.f;
+    if (__builtin_expect(now == 0.f || is_pow2(now), 1)) {  // uniform; the reciprocal is exact
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (RPI * i < len) {  // uniform
-        const u32x4 w = x[i];
-        bstore_b64(u32x2{codes4<FMT>(bf_lo(w.x) * inv, bf_hi(w.x) * inv, bf_lo(w.y) * inv, bf_hi(w.y) * inv),
-                         codes4<FMT>(bf_lo(w.z) * inv, bf_hi(w.z) * inv, bf_lo(w.w) * inv, bf_hi(w.w) * inv)},
-                   dst, dst_off(i), 0);
+      for (int i = 0; i < NI; ++i)
+        if (RPI * i < len) {  // uniform
+          const u32x4 w = x[i];
+          bstore_b64(u32x2{codes4<FMT>(bf_lo(w.x) * inv, bf_hi(w.x) * inv, bf_lo(w.y) * inv, bf_hi(w.y) * inv),
+                           codes4<FMT>(bf_lo(w.z) * inv, bf_hi(w.z) * inv, bf_lo(w.w) * inv, bf_hi(w.w) * inv)},
+                     dst, dst_off(i), 0);
+        }
+    } else {
+      // a scale that the caller brought: quotients to odd (both sides times 2^80 where the remainder could underflow; the
+      // product with the reciprocal, improved once, is within a step of the quotient, which is what to_odd needs). A rare path
+      // that is to cost the others no registers: four values at a time, loaded again
+      const float lift = now < 0x1p-60f ? 0x1p80f : 1.f, den = now * lift, rec = 1.f / den;
+      auto over = [&](uint32_t bits) {
+        const float num = __uint_as_float(bits) * lift, q0 = num * rec, q = fmaf(fmaf(-q0, den, num), rec, q0);
+        // (infinities, NaN and zeros of either sign as they are)
+        return fabsf(q0) >= 0x1p-20f && fabsf(q0) <= 0x1p10f ? to_odd(q, fmaf(-q, den, num)) : q0;
+      };
+#pragma unroll 1
+      for (int i = 0; i < 2 * NI; ++i) {
+        const int r = RPI * (i / 2) + r0, half = i % 2;
+        const u32x2 w = bload8(src, r * s.st + 16 * c + 8 * half, 0);
+        const uint32_t off = dst_off(i / 2) + 4 * half;
+        bstore4(codes4<FMT>(over(w.x << 16), over(w.x & 0xffff0000u), over(w.y << 16), over(w.y & 0xffff0000u)), dst, off);
       }
-    if (now != was && !anew) {  // uniform: the page's other rows move to the larger scale
-      const float f = was * inv;
+    }
+    if (__builtin_expect(now != was && !anew, 0)) {  // uniform: the page's other rows move to the larger scale
+      const float f = was * inv;  // exact: a scale that grows is a power of two
+      if (__builtin_expect(was != 0.f && !is_pow2(was), 0)) {  // as above
+        auto moved = [&](float code) { return to_odd(code * f, fmaf(code, f, -(code * f))); };
+#pragma unroll 1
+        for (int i = 0; i < 2 * NO; ++i) {
+          const int r = RPI * (i / 2) + r0;
+          const uint32_t off = fresh >> r & 1 ? OOB : r * s.pst + 8 * c + 4 * (i % 2);
+          float a[4];
+          values4<FMT>(bload4(dst, off), a);
+          bstore4(codes4<FMT>(moved(a[0]), moved(a[1]), moved(a[2]), moved(a[3])), dst, off);
+        }
+      } else
 #pragma unroll 1
       for (int i0 = 0; i0 < NO; i0 += NO < 4 ? NO : 4) {
         u32x2 old[NO < 4 ? NO : 4];
@@ -421,9 +472,10 @@ __device__ __forceinline__ void write_run(const Side& s, int pg, int rs, int len
 // workgroups take the heads, keys then values, of one window: together they read and write whole rows (heads by windows
 // instead: 72 us against 63 for 44 000 rows of 8 heads). Workgroups per CU, four (the compiler's choice of registers) /
 // eight, us: prompts of 44 000 rows of 64 dims 39 / 33 in int8, 35 / 32 in e4m3, of 512 rows 6.2 / 7.3 and 5.9 / 6.1; of
-// 128 dims and very different lengths 51.1 / 53.4, of 512 rows 7.4 / 9.2 and 7.2 / 8.5 (4096 single rows 34.7 / 30.9).
+// 128 dims and very different lengths 51.1 / 53.4, of 512 rows 7.4 / 9.2 and 7.2 / 8.5 (4096 single rows 34.7 / 30.9). Five of
+// 128 dims is what 96 registers allow; with 97 to 128, four resident, the prompts take 55.2 for 51.5.
 template <int FMT, int D>
-__global__ void __launch_bounds__(CT, (D == 64 ? 8 : 4)) cache_write_kernel(const kvskip_write_args p, int win) {
+__global__ void __launch_bounds__(CT, (D == 64 ? 8 : 5)) cache_write_kernel(const kvskip_write_args p, int win) {
   constexpr int EB = FMT == FMT_BF16 ? 2 : 1, RPW = WAVE / (D / 8);
   __shared__ float sMax[2][CT / WAVE + 1];
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);

@@ -106,7 +106,7 @@ def cache_write(rows, slots, codes, scales, fmt):
             was = float(scales[page[i], h])
             if 0 in last or not (0 < was < math.inf):
                 was = 0.0
-            now = pow2_scale(amax, fmt) if amax > QMAX[fmt] * was else was
+            now = pow2_scale(amax, fmt) if amax > float(torch.tensor(QMAX[fmt] * was).float()) else was   # (the product in fp32)
             if now != was and 0 not in last:
                 others = [r for r in range(BLOCK) if r not in last]
                 codes[page[i], h, others] = encode(decode_values(codes[page[i], h, others].clone(), fmt) * was / now, fmt)
