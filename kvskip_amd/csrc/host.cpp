@@ -816,16 +816,21 @@ int64_t split_rule8(int64_t bh, int64_t n, int64_t D, int64_t slots) {
 
 // The split budget of a KV head for a ragged batch over a cache held in 8 bits: the grid's S + B chunk slots a KV head
 // fill a whole number of workgroups per CU. One where that leaves at most 128 blocks a workgroup (64 where S is small beside
-// B, so that the lists' ends weigh more), else two or as many more as leave S at seven eighths of two (at most four).
+// B, so that the lists' ends weigh more), else two or as many more as leave S at seven eighths of two: at most four
+// while those leave it at seven eighths of one, else however many (what passes the CUs waits, slots without a chunk end at
+// once), so that the longest list is cut to about an even share in a batch of any size.
 // Measured, us (pages), at least 16 blocks a chunk and any fill / this: 3 sequences to 1540 tokens 13.4 / 10.8, to 12000
 // 18.4 / 15.8, 6 to 12000 20.1 / 15.5, to 16000 24.7 / 20.3, of 64 dims 8 to 2050 11.1 / 9.8; one / two to four a CU: 20 to
 // 9001 24.0 / 25.9, 5 of 64 dims to 32000 16.0 / 17.2, but 16 of 28 heads to 32000 (167 blocks) 50.5 / 47.4, 28 to 1500
-// over 8 heads (S 4) 16.8 / 15.0; the bf16 rule's S / this one's: 24 to 20011 72 / 67, 48 to 16384 97 / 89.
+// over 8 heads (S 4) 16.8 / 15.0; the bf16 rule's S / this one's: 24 to 20011 72 / 67, 48 to 16384 97 / 89. At most four a CU (S 2 from
+// 128 sequences over 8 heads on) / this: 128 to 8192 181 / 160, one of 131072 beside 127 of 2048 1089 / 164, one of 32768
+// in 128 places 119 / 24.6, in 256 124 / 33, 64 to 8192 over 16 heads 153 / 141, 256 of 8192 each 647 / 646, but 128 of 64
+// dims to 16000 131 / 137; 96 to 8192 (S 32 with four) 120, with five 129.
 int64_t ragged_rule8(int64_t B, int64_t Hkv, int64_t n, int64_t cus) {
   auto fill = [&](int64_t k) { return cus * k / Hkv - B; };
   int64_t k = 1;
   if (B * n > (2 * fill(1) >= B ? 128 : 64) * fill(1))
-    for (k = 2; k < 4 && fill(k) * Hkv * 8 < cus * 2 * 7;) ++k;
+    for (k = 2; fill(k) * Hkv * 8 < cus * 2 * 7 && (k < 4 || fill(4) * Hkv * 8 < cus * 7);) ++k;
   return std::max<int64_t>(2, std::min({int64_t(256), fill(k), (B * n + 1) / 2}));
 }
 
