@@ -14,11 +14,11 @@
 //                   largest value (v_mfma_i32_16x16x64_i8, exact sums), the digits on the columns that the group's heads
 //                   leave free.
 //   weights   e = 2^(s - block maximum) times 2^(mt - r) vs in two fp16 parts, 22 bits (softmax sums are taken before, in
-//             fp32). Up to 8 heads the low parts, times 2^11, are the operand rows that the group's heads leave free, with
-//             accumulators of their own (no further product); 9 to 16 heads take a second product for them, onto the same
-//             accumulators. r is the accumulators' reference, at most 2^7 below the largest weight times |vs| so far: they
-//             are rescaled only when a block passes that. (fp16 holds nothing finer than 2^-24, so beside its 2^-22 a weight
-//             is off by up to 2^-43 of the largest p |vs| of the wavefront, of 9 to 16 heads 2^-32.) One part: 32 sequences
+//             fp32). Up to 8 heads the low parts are the operand rows that the group's heads leave free, with accumulators
+//             of their own (no further product); 9 to 16 heads take a second product for them, onto the same accumulators.
+//             r is the accumulators' reference, at most 2^7 below the largest weight times |vs| so far: they are rescaled
+//             only when a block passes that. (fp16 holds nothing finer than 2^-24, so beside its 2^-22 a weight is off by up
+//             to 2^-32 of the largest p |vs| of the wavefront.) One part: 32 sequences
 //             of 65536 tokens 607.9 us for 609.0, a ragged batch of 24 of 64 dims 34.9 for 35.4.
 //   V         codes to fp16, exactly (e4m3 by the hardware's conversion, int8 by placing the byte under the exponent of 1024
 //             and taking 1152 off), rows paired by byte permutation, and P V on v_mfma_f32_16x16x32_f16.
@@ -105,10 +105,10 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), f16x2_t));
 }
 
-// h c + (a, b) as fp16, rounded once (v_fma_mixlo_f16, v_fma_mixhi_f16).
-__device__ __forceinline__ uint32_t mix_h(f16x2_t h, float c, float a, float b) {
-  return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(fmaf(static_cast<float>(h.x), c, a)),
-                                              static_cast<_Float16>(fmaf(static_cast<float>(h.y), c, b))});
+// (a, b) c + h as fp16, rounded once (v_fma_mixlo_f16, v_fma_mixhi_f16).
+__device__ __forceinline__ uint32_t mix_h(float a, float b, float c, f16x2_t h) {
+  return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(fmaf(a, c, static_cast<float>(h.x))),
+                                              static_cast<_Float16>(fmaf(b, c, static_cast<float>(h.y)))});
 }
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
@@ -251,7 +251,7 @@ __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split
     for (int w = 0; w < NWAVE; ++w) {
       Ls += l[w] * fexp2(m[w] - mu);
       f32x4_t x = *reinterpret_cast<const f32x4_t*>(L.acc + (w * NP * GP + g) * D + d);
-      if constexpr (NP == 2) x += *reinterpret_cast<const f32x4_t*>(L.acc + ((w * NP + 1) * GP + g) * D + d) * 0x1p-11f;
+      if constexpr (NP == 2) x -= *reinterpret_cast<const f32x4_t*>(L.acc + ((w * NP + 1) * GP + g) * D + d);
       A += x * fexp2(r[w] - mu - 7.f);
     }
     const int64_t hq = hq0 + g;
@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
   const uint32_t koff = c16 * k_st + 16 * j4;
   const uint32_t voff = D == 128 ? 4 * j4 * v_st + 8 * c16 : (4 * j4 + (c16 >> 3)) * v_st + 8 * (c16 & 7);
   const bool up = (lane & 8) != 0;
-  // up to 8 heads: this lane's operand row takes high or low parts of the weights
-  const float part = (c16 / GP) % 2 == 1 ? 0x1p11f : 0.f;
+  // up to 8 heads: this lane's operand row takes the weights' high parts (0) or, negative, their low ones (-1)
+  const float part = (c16 / GP) % 2 == 1 ? -1.f : 0.f;
   const char* kb = reinterpret_cast<const char*>(p.k) + h * p.k_sh;
   const char* vb = reinterpret_cast<const char*>(p.v) + h * p.v_sh;
   // (through readfirstlane: left to itself the compiler added the offset up in vector registers and wrapped every load in
@@ -406,12 +406,13 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
     return make_rsrc(reinterpret_cast<const void*>(hi << 32 | lo), rows > 0 ? (rows - 1) * st + D : 0u);
   };
 
-  int gap_prev = -1, gap_cur = 0;  // masked statistics: the list entries around this lane's gap
+  __shared__ int2 sGap[STATS ? NT : 1];  // masked statistics: the list entries around a lane's gap
+  int2 gap = make_int2(-1, 0);
   if constexpr (STATS) {
     const int t = wave + NWAVE * lane;
     if (masked && t < n) {
-      gap_cur = list[i0 + t];
-      gap_prev = i0 + t > 0 ? list[i0 + t - 1] : -1;
+      gap.y = list[i0 + t];
+      if (i0 + t > 0) gap.x = list[i0 + t - 1];
     }
   }
   // ---- the first block and q: nothing is waited for before the first block's loads but its page
@@ -457,6 +458,7 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
     make_q8<D, GP, I8>(qb, qr, __uint_as_float(static_cast<uint32_t>(127 + TOP - ex) << 23), lane);
   }
 
+  if constexpr (STATS) sGap[tid] = gap;  // (registers are short in the loop)
   const uint32_t nb4 = 4u * static_cast<uint32_t>(p.nb);
   const rsrc_t rs_max = make_rsrc(STATS ? p.blk_max + hq0 * p.nb : nullptr, STATS ? G * nb4 : 0);
   const rsrc_t rs_sum = make_rsrc(STATS ? p.blk_sum + hq0 * p.nb : nullptr, STATS ? G * nb4 : 0);
@@ -541,19 +543,17 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
       // the weights as operands: row c of a product is head c % GP, up to 8 heads the high parts in rows below GP and the
       // low ones in the GP rows after them (the rows from 2 GP on are not read)
       u32x4 w8[2], wl[2];
-      const float fl = fv * part, fh = fmaf(part, -1.f - 0x1p-11f, 1.f);  // -2^11 or 1
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const float x = e[2 * q + u / 2][2 * (u % 2)], y = e[2 * q + u / 2][2 * (u % 2) + 1];
-          const uint32_t hi = pack_h(x * fv, y * fv);
-          const f16x2_t hf = __builtin_bit_cast(f16x2_t, hi);
+          const float x = e[2 * q + u / 2][2 * (u % 2)] * fv, y = e[2 * q + u / 2][2 * (u % 2) + 1] * fv;
+          const f16x2_t hi = __builtin_bit_cast(f16x2_t, pack_h(x, y));
           if constexpr (GP == 16) {
-            w8[q][u] = hi;
-            wl[q][u] = mix_h(hf, -1.f, x * fv, y * fv);
-          } else {  // high rows hi + 0 x, low ones -2^11 hi + 2^11 x
-            w8[q][u] = mix_h(hf, fh, x * fl, y * fl);
+            w8[q][u] = __builtin_bit_cast(uint32_t, hi);
+            wl[q][u] = mix_h(x, y, 1.f, -hi);
+          } else {  // high rows hi - 0 x, low ones hi - x
+            w8[q][u] = mix_h(x, y, part, hi);
           }
         }
 #pragma unroll
@@ -613,8 +613,9 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
       for (int j = 0; wave + NWAVE * j < n; ++j) {  // uniform over the wavefront
         int before, now;
         if (j < WAVE) {
-          before = __builtin_amdgcn_readlane(gap_prev, j);
-          now = __builtin_amdgcn_readlane(gap_cur, j);
+          const int2 g = sGap[wave * WAVE + j];  // this wavefront's own
+          before = __builtin_amdgcn_readfirstlane(g.x);
+          now = __builtin_amdgcn_readfirstlane(g.y);
         } else {
           const int k = i0 + wave + NWAVE * j;
           now = __builtin_amdgcn_readfirstlane(list[k]);
