@@ -222,13 +222,13 @@ __device__ __forceinline__ void rescale8(f32x4_t (&acc)[D / 16], float alpha, in
     for (int i = 0; i < 4; ++i) acc[j][i] *= r[i];
 }
 
-// LDS of the epilogue: the wavefronts' accumulators by part and head, and each head's (m, l, reference of the accumulators) of all
-// wavefronts.
+// LDS of the epilogue: the wavefronts' accumulators by part and head, and each head's (m, l, reference of the accumulators, its
+// two parts) of all wavefronts.
 template <int D, int GP>
 struct Merge8 {
   static constexpr int NP = GP == 16 ? 1 : 2;  // parts of the weights with accumulators of their own
   float acc[NWAVE * NP * GP * D];
-  f32x4_t m[GP], l[GP], r[GP];
+  f32x4_t m[GP], l[GP], r[GP], x[GP];
 };
 
 // The wavefronts' states merged: out / out_f32 / lse (whole: all of the list) or the split partials; a thread four dims of
@@ -242,7 +242,7 @@ __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split
   const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + static_cast<int64_t>(h) * p.G;
   for (int o = threadIdx.x; o < p.G * (D / 4); o += NT) {
     const int g = o / (D / 4), d = o % (D / 4) * 4;
-    const f32x4_t m = L.m[g], l = L.l[g], r = L.r[g];
+    const f32x4_t m = L.m[g], l = L.l[g], r = L.r[g], rx = L.x[g];
     const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     const float mu = M == NEG_INF ? 0.f : M;
     f32x4_t A = {0.f, 0.f, 0.f, 0.f};
@@ -252,7 +252,7 @@ __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split
       Ls += l[w] * fexp2(m[w] - mu);
       f32x4_t x = *reinterpret_cast<const f32x4_t*>(L.acc + (w * NP * GP + g) * D + d);
       if constexpr (NP == 2) x -= *reinterpret_cast<const f32x4_t*>(L.acc + ((w * NP + 1) * GP + g) * D + d);
-      A += x * fexp2(r[w] - mu - 7.f);
+      A += x * fexp2((r[w] - mu) + (rx[w] - 7.f));
     }
     const int64_t hq = hq0 + g;
     if (whole) {
@@ -465,7 +465,9 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
   constexpr uint32_t OOB = 0x80000000u;
   const uint32_t v_stat = c16 < G && j4 == 0 ? c16 * nb4 : OOB;
 
-  float mr = NEG_INF, lr = 0.f, ar = NEG_INF;  // running (m, l) of this lane's head c16 % GP, its accumulators' reference
+  // running (m, l) of this lane's head c16 % GP, its accumulators' reference ar + ax: a block's maximum and the exponent of
+  // its vs (apart, since in one float a large maximum takes the exponent's bits)
+  float mr = NEG_INF, lr = 0.f, ar = NEG_INF, ax = 0.f;
   f32x4_t acc[VD];
 #pragma unroll
   for (int j = 0; j < VD; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -511,6 +513,13 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
 
       const float mt = block_max_mf(s) * f;  // f >= 0
       const float mtu = mt == NEG_INF ? 0.f : mt;
+      // (scores so large that mt's rounding would show, or overflow, in s f - mt: rounded alike instead, so that the largest
+      // weight is 1 whatever the scores are)
+      if (__ballot(fabsf(mtu) > 0x1p17f) != 0) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) s[t / 4][t % 4] *= f;
+        f = 1.f;
+      }
       float r4[4];
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) {
@@ -527,12 +536,14 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
       // the accumulators' reference: mt + log2 |vs| (its whole part) of the largest block so far, left where it is for as
       // long as a block passes it by at most 2^7
       const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(vs) >> 23 & 0xffu) - 127, -100));
-      if (__ballot(mt + ev > ar + 7.f) != 0) {
-        const float an = fmaxf(ar, mt + ev);
-        rescale8<D, GP>(acc, fexp2(ar - (an == NEG_INF ? 0.f : an)), lane);
-        ar = an;
+      const float past = (mt - ar) + (ev - ax);  // (NaN, which passes nothing, where nothing came yet)
+      if (__ballot(past > 7.f) != 0) {
+        const bool on = past > 0.f;
+        rescale8<D, GP>(acc, on ? fexp2(-past) : 1.f, lane);
+        ar = on ? mt : ar;
+        ax = on ? ev : ax;
       }
-      const float fv = vs * fexp2(mt - (ar == NEG_INF ? 0.f : ar)) * 0x1p7f;  // below 2^15
+      const float fv = vs * fexp2((mt - (ar == NEG_INF ? 0.f : ar)) - ax) * 0x1p7f;  // below 2^15
       if constexpr (STATS) {
         const uint32_t blk4 = 4u * static_cast<uint32_t>(max(blk, 0));
         const uint32_t at = blk >= 0 ? v_stat : OOB;
@@ -600,7 +611,7 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
       }
     }
     if (lane < G) {
-      sL.m[lane][wave] = mr, sL.l[lane][wave] = lr, sL.r[lane][wave] = ar;
+      sL.m[lane][wave] = mr, sL.l[lane][wave] = lr, sL.r[lane][wave] = ar, sL.x[lane][wave] = ax;
     }
   }
   finish8<D, GP>(p, b, h, split, whole, sL);
