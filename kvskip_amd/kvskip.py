@@ -157,8 +157,8 @@ def _decode8(q, k, v, k_scale, v_scale, scale, plan, stats, num_splits, out_f32,
     if plan is not None:
         idx, cnt, items = plan.block_idx, plan.block_cnt, plan.max_cnt
     out, lse, bmax, bsum, o32, splits = _ops._host().decode8(
-        q[:, :, 0] if q.dim() == 4 else q, k, v, k_scale, v_scale, scale, idx, cnt, stats, num_splits or 0, out_f32, seq_lens,
-        block_table, T, -1, items, 0 if num_splits else num_sms() * WG_PER_CU)
+        _as_bhd(q), k, v, k_scale, v_scale, scale, idx, cnt, stats, 0 if num_splits is None else num_splits, out_f32, seq_lens,
+        block_table, T, -1, items, num_sms() * WG_PER_CU if num_splits is None else 0)
     res = {"out": out, "lse": lse, "num_splits": splits}
     if stats:
         res["blk_max"], res["blk_sum"] = bmax, bsum
