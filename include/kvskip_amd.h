@@ -463,7 +463,7 @@ int64_t kvskip_page_work_ints(int32_t B, int32_t rows);
 /* Rows of new keys and values into the pages that a slot map names. k, v: bf16 [N, Hkv, D] (D contiguous, strides
  * multiples of 8, 16-byte aligned); row i goes to token slot % 64 of page slot / 64 (slot = slot_map[i]); a slot outside
  * [0, 64 * num_pages) leaves its row out. Pools [num_pages, Hkv, 64, D] of the format's type (D contiguous; strides and
- * bases multiples of 16 bytes).
+ * bases multiples of 16 bytes, token strides at least D).
  * In 8 bits, with scales k_scale[page * ks_sb + head * ks_sh]: let amax be the largest magnitude of the rows written to
  * a page's head (an infinity counts as the largest finite bf16, NaN not). A page whose row 0 is written starts anew
  * (scale 0 before). If amax > qmax * scale (qmax 448 for e4m3, 127 for int8; the product in fp32) the scale becomes the smallest power of two

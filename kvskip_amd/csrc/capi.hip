@@ -639,6 +639,7 @@ int kvskip_cache_write(const kvskip_write_args* p, void* stream) {
   if (p->kp_sb % m != 0 || p->kp_sh % m != 0 || p->kp_st % m != 0 || p->vp_sb % m != 0 || p->vp_sh % m != 0 ||
       p->vp_st % m != 0 || !aligned16(p->k_pool) || !aligned16(p->v_pool))
     return fail(KVSKIP_E_INVALID, "cache_write: pool rows must be 16-byte aligned");
+  if (p->kp_st < p->D || p->vp_st < p->D) return fail(KVSKIP_E_INVALID, "cache_write: pool rows must not overlap");
   if (p->N == 0) return ok();
   return launched(kvs::launch_cache_write(*p, static_cast<hipStream_t>(stream)), "kvskip_cache_write");
 }
