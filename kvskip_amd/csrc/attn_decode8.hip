@@ -19,7 +19,7 @@
 //             r is the accumulators' reference, at most 2^7 below the largest weight times |vs| so far: they are rescaled
 //             only when a block passes that. (fp16 holds nothing finer than 2^-24, so beside its 2^-22 a weight is off by up
 //             to 2^-32 of the largest p |vs| of the wavefront.) One part: 32 sequences
-//             of 65536 tokens 607.9 us for 609.0, a ragged batch of 24 of 64 dims 34.9 for 35.4.
+//             of 65536 tokens 612.5 us for 613.8, a ragged batch of 24 of 64 dims 35.1 for 35.5.
 //   V         codes to fp16, exactly (e4m3 by the hardware's conversion, int8 by placing the byte under the exponent of 1024
 //             and taking 1152 off), rows paired by byte permutation, and P V on v_mfma_f32_16x16x32_f16.
 //   items     lane l of a wavefront holds block, page and scales of the wavefront's step 64 i + l (one gather per 64
