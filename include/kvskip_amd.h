@@ -488,6 +488,101 @@ typedef struct kvskip_write_args {
 
 int kvskip_cache_write(const kvskip_write_args* p, void* stream);
 
+/* ---- Attention of the rows that a step brings, over 8-bit pages (none of it in the reference).
+ *
+ * Request b brings the rows [starts[b], starts[b + 1]) of the call's `rows` rows (clamped to them), the last of its
+ * seq_lens[b] tokens (clamped to [0, T]); its tokens lie in the pages of its block table row, T / 64 of them at most. Where
+ * shared_of[b] is in [0, shared), the shared_lens[shared_of[b]] tokens (clamped to [0, shared_T]) of that prefix come before
+ * them, in the pages of the prefix's own table row. Position 0 is the first token of all. A row at position p sees the key at
+ * position j of its request where
+ *   j < prefix_lens[b]  or  (j <= p and (window == 0 or j > p - window)),
+ * and nothing of any other request; a row at a negative position (more rows than tokens) sees only what prefix_lens gives it.
+ *
+ * kvskip_attend_plan cuts that work for the launches of kvskip_attend, once for all layers of a step. It reads the arrays
+ * named here and writes work and positions ([rows]: the position of each row, -1 of a row that no request brings); work is
+ * self-contained, so the arrays may change after it. max_rows: the most rows that one request is expected to bring (0: all);
+ * it chooses the tiles, and a request that brings more is served all the same, at a lower rate. Hq, Hkv, rows, T, shared,
+ * shared_T, max_rows and B are the same in both calls. The unit order in work differs from run to run, results do not. */
+typedef struct kvskip_attend_plan_args {
+  const int32_t* starts;       /* [B + 1], rising */
+  const int32_t* seq_lens;     /* [B] */
+  const int32_t* prefix_lens;  /* [B] or NULL */
+  const int32_t* shared_lens;  /* [shared] */
+  const int32_t* shared_of;    /* [B] */
+  int32_t* work;               /* kvskip_attend_work_ints int32, 16-byte aligned */
+  int32_t* positions;          /* [rows] out */
+  int32_t B, rows, Hq, Hkv, T; /* B <= 2048, rows <= 2^21, rows * Hq < 2^28, T <= 2^27 */
+  int32_t shared, shared_T;    /* shared prefixes (0: none; at most 64) and the capacity of one, <= 2^27 */
+  int32_t max_rows, window;
+} kvskip_attend_plan_args;
+
+int kvskip_attend_plan(const kvskip_attend_plan_args* p, void* stream);
+
+/* int32 elements of kvskip_attend_plan_args.work, and rows of the partial results of kvskip_attend (-1 for invalid sizes). */
+int64_t kvskip_attend_work_ints(const kvskip_attend_plan_args* p);
+int64_t kvskip_attend_part_rows(const kvskip_attend_plan_args* p);
+
+/* out [rows, Hq, D] (bf16) and lse [rows, Hq] (natural log) of a plan's rows: with key and value codes times their page's
+ * scale,
+ *   s = scale * q.k;  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s -= slopes[head] * |p - j|
+ *   out = sum over the keys seen of softmax(s) v,
+ * 0 and -inf for a row that sees nothing and for rows that no request brings. q: bf16 [rows, Hq, D] (strides multiples of 8,
+ * 16-byte aligned). Pools [num_pages, Hkv, 64, D] of codes (strides multiples of 16, 16-byte aligned, token strides below
+ * 2^24), scales [num_pages, Hkv]; a page outside [0, num_pages) holds no keys. D in {64, 128}, any Hq / Hkv. q is exact to
+ * 2^-25 of its row's largest element, a weight holds 11 bits, scores and sums are fp32. Keys that a row does not see do not
+ * reach it, whatever they hold. part_acc [part_rows, Hkv, D] and part_ml [part_rows, Hkv, 2] fp32, 16-byte aligned. */
+typedef struct kvskip_attend_args {
+  kvskip_attend_plan_args plan;  /* sizes and work; its other pointers are not read */
+  const void* q;
+  int64_t q_sn, q_sh;
+  const void* k;
+  const void* v;
+  int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  const int32_t* block_table;    /* [B, >= ceil(T / 64)] */
+  const int32_t* shared_table;   /* [shared, >= ceil(shared_T / 64)] */
+  int64_t bt_stride, st_stride;
+  const float* slopes;           /* [Hq] or NULL */
+  void* out;
+  float* lse;
+  float* part_acc;
+  float* part_ml;
+  float scale, softcap;          /* softcap 0: none */
+  int32_t D, num_pages, format;
+} kvskip_attend_args;
+
+int kvskip_attend(const kvskip_attend_args* a, void* stream);
+
+/* Norms of queries and keys for each head, and their rotation, in one pass. For each row n and head of q [rows, Hq, D] and
+ * k [rows, Hkv, D] (bf16), in fp32, rounded once at the end:
+ *   y = x / sqrt(mean(x^2) + eps) * weight        (weight NULL: y = x)
+ *   pair i < rot / 2 of y: (y[i], y[i + rot / 2]), with pairs = 1 (y[2 i], y[2 i + 1]);
+ *   angle = positions[axis(i), n] * inv_freq[i], the product in 64 bits;
+ *   (a, b) -> mscale * (a cos - b sin, b cos + a sin); elements from rot on stay y.
+ * axis(i): the first sections[0] pairs belong to axis 0, the next sections[1] to axis 1, ... (their sum is rot / 2).
+ * Outputs may be the inputs themselves (same pointer and strides), and must not overlap them otherwise. D a multiple of 8 up
+ * to 256, rot a multiple of 8 up to D (0: no rotation); strides multiples of 4 elements, bases 8-byte aligned. Hkv 0: no k. */
+typedef struct kvskip_rope_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_sn, q_sh, k_sn, k_sh, qo_sn, qo_sh, ko_sn, ko_sh;
+  const int32_t* positions;      /* [axes, rows], rows contiguous */
+  int64_t pos_stride;
+  const float* inv_freq;         /* [rot / 2] */
+  const void* q_weight;          /* [D] or NULL */
+  const void* k_weight;
+  int32_t rows, Hq, Hkv, D, rot, axes, pairs;
+  int32_t sections[4];
+  int32_t q_weight_f32, k_weight_f32;  /* weights in fp32 (else bf16) */
+  float eps, mscale;
+} kvskip_rope_args;
+
+int kvskip_norm_rope(const kvskip_rope_args* a, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* kvskip_last_error(void);
 
@@ -495,7 +590,8 @@ const char* kvskip_last_error(void);
 const char* kvskip_version(void);
 
 /* sizeof of the argument blocks (0: kvskip_attn_args, 1: kvskip_plan_args, 2: kvskip_update_args,
- * 3: kvskip_select_args, 5: kvskip_cache8_args, 6: kvskip_page_args, 7: kvskip_write_args), -1 otherwise: lets a binding
+ * 3: kvskip_select_args, 5: kvskip_cache8_args, 6: kvskip_page_args, 7: kvskip_write_args, 8: kvskip_attend_plan_args,
+ * 9: kvskip_attend_args, 10: kvskip_rope_args), -1 otherwise: lets a binding
  * check its struct layout. Library utility, no reference counterpart. */
 int kvskip_struct_size(int which);
 

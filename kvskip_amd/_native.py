@@ -111,6 +111,43 @@ class WriteArgs(ctypes.Structure):
     ]
 
 
+class AttendPlanArgs(ctypes.Structure):
+    """kvskip_attend_plan_args."""
+    _fields_ = [
+        ("starts", c_void_p), ("seq_lens", c_void_p), ("prefix_lens", c_void_p), ("shared_lens", c_void_p),
+        ("shared_of", c_void_p), ("work", c_void_p), ("positions", c_void_p),
+        ("B", c_int32), ("rows", c_int32), ("Hq", c_int32), ("Hkv", c_int32), ("T", c_int32),
+        ("shared", c_int32), ("shared_T", c_int32), ("max_rows", c_int32), ("window", c_int32),
+    ]
+
+
+class AttendArgs(ctypes.Structure):
+    """kvskip_attend_args."""
+    _fields_ = [
+        ("plan", AttendPlanArgs), ("q", c_void_p), ("q_sn", c_int64), ("q_sh", c_int64), ("k", c_void_p), ("v", c_void_p),
+        ("k_sb", c_int64), ("k_sh", c_int64), ("k_st", c_int64), ("v_sb", c_int64), ("v_sh", c_int64), ("v_st", c_int64),
+        ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("ks_sb", c_int64), ("ks_sh", c_int64), ("vs_sb", c_int64), ("vs_sh", c_int64),
+        ("block_table", c_void_p), ("shared_table", c_void_p), ("bt_stride", c_int64), ("st_stride", c_int64),
+        ("slopes", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("part_acc", c_void_p), ("part_ml", c_void_p),
+        ("scale", c_float), ("softcap", c_float), ("D", c_int32), ("num_pages", c_int32), ("format", c_int32),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    """kvskip_rope_args."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+        ("q_sn", c_int64), ("q_sh", c_int64), ("k_sn", c_int64), ("k_sh", c_int64),
+        ("qo_sn", c_int64), ("qo_sh", c_int64), ("ko_sn", c_int64), ("ko_sh", c_int64),
+        ("positions", c_void_p), ("pos_stride", c_int64), ("inv_freq", c_void_p),
+        ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("rows", c_int32), ("Hq", c_int32), ("Hkv", c_int32), ("D", c_int32), ("rot", c_int32), ("axes", c_int32),
+        ("pairs", c_int32), ("sections", c_int32 * 4), ("q_weight_f32", c_int32), ("k_weight_f32", c_int32),
+        ("eps", c_float), ("mscale", c_float),
+    ]
+
+
 # Every entry point of include/kvskip_amd.h with its argument types.
 SIGNATURES = {
     "kvskip_decode": ([POINTER(AttnArgs), c_int, c_int, c_void_p], c_int),
@@ -137,6 +174,11 @@ SIGNATURES = {
     "kvskip_page_map": ([POINTER(PageArgs), c_void_p], c_int),
     "kvskip_page_work_ints": ([c_int32, c_int32], c_int64),
     "kvskip_cache_write": ([POINTER(WriteArgs), c_void_p], c_int),
+    "kvskip_attend_plan": ([POINTER(AttendPlanArgs), c_void_p], c_int),
+    "kvskip_attend_work_ints": ([POINTER(AttendPlanArgs)], c_int64),
+    "kvskip_attend_part_rows": ([POINTER(AttendPlanArgs)], c_int64),
+    "kvskip_attend": ([POINTER(AttendArgs), c_void_p], c_int),
+    "kvskip_norm_rope": ([POINTER(RopeArgs), c_void_p], c_int),
     "kvskip_last_error": ([], c_char_p),
     "kvskip_version": ([], c_char_p),
     "kvskip_struct_size": ([c_int], c_int),
@@ -164,7 +206,8 @@ def lib() -> ctypes.CDLL:
 # The entry points that the native host module calls, in the order of its table (csrc/host.cpp).
 HOST_CALLS = ("decode", "decode_splits", "merge_splits", "pv", "vskip1", "pv_select", "select", "plan", "plan_scores",
               "update", "merge_update", "decode_splits_update", "decode_splits_planned", "plan_part_floats", "decode8",
-              "page_map", "page_work_ints", "cache_write", "last_error")
+              "page_map", "page_work_ints", "cache_write", "attend_plan", "attend_work_ints", "attend_part_rows", "attend",
+              "norm_rope", "last_error")
 _HOST = None
 
 

@@ -1,0 +1,919 @@
+// Attention of a step's rows over 8-bit pages: the units of a plan (attend.hpp), and the join of their partial results.
+//
+//   s = scale ks (q . k), capped and biased as asked;  out = sum softmax(s) vs v
+//
+// Both bodies hold scores transposed, S^T = K Q^T: a lane has scores of ONE virtual row, so its softmax is arithmetic in its
+// own registers and one or two lane swaps, and its weights are already the operand of O^T = V^T P^T (any order of the
+// keys will do inside a product, as long as V's operand has the same). Codes become fp16, which holds them exactly; q is
+// fp16 times a power of two of its row (2^14 <= largest < 2^15: exact, but for what lies below 2^-39 of that); weights
+// are one fp16 part, 2^-12 of each, taken relative to a reference that is within 2^7 of the largest weight times |vs|
+// so far (as in attn_decode8.hip: accumulators are rescaled only when a page passes it); sums and statistics are fp32.
+#include "codes8.hpp"
+#include "attend.hpp"
+
+namespace kvs {
+namespace {
+
+struct AttendP {
+  const uint16_t* q;
+  int64_t q_sn, q_sh;
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t k_sb, k_sh, v_sb, v_sh;
+  uint32_t k_st, v_st;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  const int* block_table;
+  const int* shared_table;
+  int64_t bt_stride, st_stride;
+  const float* slopes;
+  uint16_t* out;
+  float* lse;
+  float* part_acc;
+  float* part_ml;
+  const int* head;
+  const AttendUnit* units;
+  const AttendJoin* joins;
+  const AttendTile* tiles;
+  const AttendRow* rows;
+  int n_rows, Hq, Hkv, G, num_pages, window, chunks;
+  float scale, softcap;
+};
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 fp16x4_t;
+
+__device__ __forceinline__ float swap32_max(float v) {
+  const uint32_t a = __float_as_uint(v);
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ float swap32_sum(float v) {
+  const uint32_t a = __float_as_uint(v);
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+// A virtual row: its row of q and out, query head, position, prefix.
+struct Row {
+  int n, hq, pos, pre;
+};
+__device__ __forceinline__ Row virtual_row(const AttendP& p, const AttendUnit& u, int h, int i) {
+  // (rows past the tile's last are that one again: computed and not stored)
+  const int v = u.v0 + min(i, u.nv - 1), r = v / p.G;
+  Row x;
+  x.hq = h * p.G + (v - r * p.G);
+  if (u.kind & 2) {
+    const AttendRow y = p.rows[u.row0 + r];
+    x.n = y.row, x.pos = y.pos, x.pre = y.pre;
+  } else {
+    x.n = u.row0 + r, x.pos = u.p0 + r, x.pre = u.pre;
+  }
+  return x;
+}
+
+// What a row sees of the unit's keys, as indices: t < pre or lo < t <= hi (and t < the unit's len).
+struct Sight {
+  int lo, hi, pre;
+};
+__device__ __forceinline__ Sight sight(const AttendP& p, const AttendUnit& u, const Row& r) {
+  Sight s;
+  s.hi = r.pos - u.base;
+  s.lo = p.window > 0 ? s.hi - p.window : INT32_MIN;
+  s.pre = r.pre - u.base;
+  return s;
+}
+__device__ __forceinline__ bool sees(const Sight& s, int t) { return t < s.pre || (t <= s.hi && t > s.lo); }
+
+template <int W>  // over all lanes
+__device__ __forceinline__ int wave_min_int(int v) {
+#pragma unroll
+  for (int m = 1; m < W; m *= 2) v = min(v, __shfl_xor(v, m, WAVE));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// The rows of a wavefront together: a page of keys [t0, t0 + 64) is whole (every row sees all of it), cut, or empty.
+struct Reach {
+  int hi_min, hi_max, lo_min, lo_max, pre_min, pre_max;
+};
+__device__ __forceinline__ Reach reach(const Sight& s) {
+  Reach r;
+  r.hi_min = wave_min_int<WAVE>(s.hi), r.hi_max = -wave_min_int<WAVE>(-s.hi);
+  r.lo_min = wave_min_int<WAVE>(s.lo);
+  r.lo_max = ~wave_min_int<WAVE>(~s.lo);
+  r.pre_min = wave_min_int<WAVE>(s.pre), r.pre_max = -wave_min_int<WAVE>(-s.pre);
+  return r;
+}
+__device__ __forceinline__ Reach both(const Reach& a, const Reach& b) {
+  return Reach{min(a.hi_min, b.hi_min), max(a.hi_max, b.hi_max), min(a.lo_min, b.lo_min), max(a.lo_max, b.lo_max),
+               min(a.pre_min, b.pre_min), max(a.pre_max, b.pre_max)};
+}
+// Every row sees all of a page's keys (there are none from len on, where its rows read as zeros).
+__device__ __forceinline__ bool sees_keys(const Reach& r, int t0, int len) {
+  const int t1 = min(t0 + BLK, len) - 1;
+  return t1 < r.pre_min || (t1 <= r.hi_min && t0 > r.lo_max);
+}
+__device__ __forceinline__ bool sees_all(const Reach& r, int t0, int len) { return t0 + BLK <= len && sees_keys(r, t0, len); }
+__device__ __forceinline__ bool sees_none(const Reach& r, int t0, int len) {
+  const int t1 = t0 + BLK - 1;
+  return t0 >= len || (t0 >= r.pre_max && (t0 > r.hi_max || t1 <= r.lo_min));
+}
+
+// A NaN among V's codes (e4m3's 0x7f and 0xff) must reach the rows that see its key and no others, but a weight of 0 times NaN
+// is NaN. So where a page is cut, its NaN codes are made zeros before the product and put into the accumulators of the
+// rows that see them after it. Returns the bytes with a NaN as 0x80, and clears them.
+__device__ __forceinline__ uint32_t take_nan(uint32_t& w) {
+  const uint32_t z = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  w &= ~((z >> 7) * 0xffu);
+  return z;
+}
+// 0x80 of four bytes as four bits.
+__device__ __forceinline__ uint32_t four_bits(uint32_t z) { return ((z >> 7) * 0x01020408u) >> 24; }
+
+// Running state of a row: maximum and sum (log2 units; the sum is this lane's part), and the accumulators' reference ar + ax.
+struct State {
+  float m = NEG_INF, l = 0.f, ar = NEG_INF, ax = 0.f;
+};
+
+// Capped and biased scores, in log2 units, of raw products s times f (a score in natural units): tanh y as
+// 1 - 2 / (e^2y + 1), off by 2^-24 of the cap, or where the wavefront's scores are all below an eighth of the cap as
+// y - y^3 / 3 + 2 y^5 / 15 - 17 y^7 / 315, off by 2^-29 of y. d0: distance of key t0 (|t - t0| below 64), or its negative.
+template <int N, class T>
+__device__ __forceinline__ void modify(float (&s)[N], float f, float cap, bool biased, float slope, float d0, T&& at) {
+  if (cap > 0.f) {
+    const float g = f / cap;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(s[i]));
+    if (__ballot(!(top * fabsf(g) <= 0.125f)) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = s[i] * g, z = y * y;
+        s[i] = fmaf(y * z, fmaf(z, fmaf(z, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), y);
+      }
+    } else {
+      const float g2 = 2.f * LOG2E * g;
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] = fmaf(__builtin_amdgcn_rcpf(fexp2(s[i] * g2) + 1.f), -2.f, 1.f);
+    }
+    f = cap;
+  }
+  if (biased) {
+    const float a = f * LOG2E, b = slope * LOG2E;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = fmaf(s[i], a, -b * fabsf(d0 - at(i)));
+  } else {
+    const float a = f * LOG2E;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] *= a;
+  }
+}
+
+// One page of a row: s in, e = weights relative to the reference out (as fp16 pairs, tokens in order). f >= 0: s f is the
+// score in log2 units. The row's maximum is taken over `swap`'s lanes. Returns the factor of the accumulators.
+template <int N, class F>
+__device__ __forceinline__ bool soften(float (&s)[N], float f, float vs, State& st, float& alpha, uint32_t (&w)[N / 2], F&& swap) {
+  float x = s[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) x = fmaxf(x, s[i]);
+  const float mt = swap(x) * f;
+  const float mtu = mt == NEG_INF ? 0.f : mt;
+  // (scores so large that mt's rounding would show in s f - mt: rounded alike)
+  if (__ballot(fabsf(mtu) > 0x1p17f) != 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] *= f;
+    f = 1.f;
+  }
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] = fexp2(fmaf(s[i], f, -mtu));
+    sum[i % 4] += s[i];
+  }
+  const float m_new = fmaxf(st.m, mt);
+  const float mu = m_new == NEG_INF ? 0.f : m_new;
+  const float cf = mt == NEG_INF ? 0.f : fexp2(mt - mu);
+  st.l = st.l * fexp2(st.m - mu) + ((sum[0] + sum[1]) + (sum[2] + sum[3])) * cf;
+  st.m = m_new;
+  const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(vs) >> 23 & 0xffu) - 127, -100));
+  const float past = (mt - st.ar) + (ev - st.ax);  // (NaN, which passes nothing, where nothing came yet)
+  const bool move = __ballot(past > 7.f) != 0;
+  alpha = 1.f;
+  if (move) {
+    const bool on = past > 0.f;
+    alpha = on ? fexp2(-past) : 1.f;
+    st.ar = on ? mt : st.ar;
+    st.ax = on ? ev : st.ax;
+  }
+  // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
+  const float fv = mt == NEG_INF ? 0.f : vs * fexp2((mt - st.ar) - st.ax) * 0x1p7f;
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) w[i] = pack_h(s[2 * i] * fv, s[2 * i + 1] * fv);
+  return move;
+}
+
+// q of a row in fp16: its power of two taken out, the factor of its scores.
+__device__ __forceinline__ float q_factor(float amax, float bad, float& up) {
+  constexpr int TOP = 14;
+  const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, TOP - 126), 127);
+  up = __uint_as_float(static_cast<uint32_t>(127 + TOP - ex) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 - TOP + ex) << 23) + bad;
+}
+__device__ __forceinline__ void q_extent(const u32x4& x, float& amax, float& bad) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = bf_lo(x[e]), b = bf_hi(x[e]);
+    amax = fmaxf(amax, fmaxf(fabsf(a), fabsf(b)));
+    bad = fmaf(a, 0.f, fmaf(b, 0.f, bad));  // NaN of an infinity or NaN
+  }
+}
+__device__ __forceinline__ u32x4 q_half(const u32x4& x, float up) {
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = pack_h(bf_lo(x[e]) * up, bf_hi(x[e]) * up);
+  return r;
+}
+
+// Pages of 64 steps of a unit, one a lane: table entry (-1: past the unit's), page (-1: none) and scales, gathered in three
+// stages while the 64 before them run.
+struct Pages {
+  int blk, pg;
+  float ks, vs;
+};
+template <int STRIDE>
+struct PageList {
+  const AttendP& p;
+  const AttendUnit& u;
+  const int* table;
+  int h, first, n;
+  Pages cur, nxt;
+  __device__ PageList(const AttendP& p_, const AttendUnit& u_, int h_, int first_, int n_)
+      : p(p_), u(u_), h(h_), first(first_), n(n_) {
+    table = (u.kind & 2) ? p.shared_table + u.table * p.st_stride : p.block_table + u.table * p.bt_stride;
+    block(cur, 0), page(cur), scales(cur);
+    nxt = cur;
+  }
+  __device__ __forceinline__ void block(Pages& x, int k0) {
+    const int k = k0 + static_cast<int>(threadIdx.x % WAVE);
+    x.blk = -1;
+    if (k < n) {
+      const int i = u.i0 + first + STRIDE * k;
+      x.blk = i < u.a1 ? i : i - u.a1 + u.b0;
+    }
+  }
+  __device__ __forceinline__ void page(Pages& x) { x.pg = x.blk >= 0 ? table[x.blk] : -1; }
+  __device__ __forceinline__ void scales(Pages& x) {
+    if (x.pg < 0 || x.pg >= p.num_pages) x.pg = -1;
+    x.ks = x.vs = 0.f;
+    if (x.pg >= 0) {
+      x.ks = p.k_scale[x.pg * p.ks_sb + h * p.ks_sh];
+      x.vs = p.v_scale[x.pg * p.vs_sb + h * p.vs_sh];
+    }
+  }
+  // Before step k's own use of the list: what is to be had for the steps 64 on.
+  __device__ __forceinline__ void advance(int k) {
+    const int ph = k & 63;
+    if (k - ph + 64 < n) {
+      if (ph == 0) block(nxt, k + 64);
+      if (ph == 16) page(nxt);
+      if (ph == 32) scales(nxt);
+    }
+  }
+  __device__ __forceinline__ void turn(int k) {  // after the last read of step k's scales
+    if ((k & 63) == 63) cur = nxt;
+  }
+  __device__ __forceinline__ int blk(int k) const { return __builtin_amdgcn_readlane(cur.blk, k & 63); }
+  __device__ __forceinline__ int pg(int k) const { return __builtin_amdgcn_readlane(cur.pg, k & 63); }
+  __device__ __forceinline__ float ks(int k) const { return lane_value(cur.ks, k & 63); }
+  __device__ __forceinline__ float vs(int k) const { return lane_value(cur.vs, k & 63); }
+};
+
+// The rows of a page that hold keys, as a buffer resource: rows past the sequence's last read zeros.
+template <int D>
+__device__ __forceinline__ rsrc_t page_res(const uint8_t* base, int64_t sb, uint32_t st, int pg, int rows) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base) + max(pg, 0) * sb;
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32)));
+  return make_rsrc(reinterpret_cast<const void*>(hi << 32 | lo), rows > 0 ? (rows - 1) * st + D : 0u);
+}
+
+// A row's result, or its partial result: four dims.
+__device__ __forceinline__ void store4(const AttendP& p, const AttendUnit& u, int h, int i, const Row& r, int d, int D, f32x4_t a,
+                                       float m, float l) {
+  if (u.part >= 0) {
+    const int64_t at = static_cast<int64_t>(u.part + i) * p.Hkv + h;
+    *reinterpret_cast<f32x4_t*>(p.part_acc + at * D + d) = a;
+    if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
+    return;
+  }
+  const int64_t at = static_cast<int64_t>(r.n) * p.Hq + r.hq;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] = l == 0.f ? 0.f : a[e] / l;
+  *reinterpret_cast<u32x2*>(p.out + at * D + d) =
+      u32x2{f2bf(a[0]) | static_cast<uint32_t>(f2bf(a[1])) << 16, f2bf(a[2]) | static_cast<uint32_t>(f2bf(a[3])) << 16};
+  if (d == 0) p.lse[at] = l == 0.f ? NEG_INF : (m + flog2(l)) * LN2;
+}
+
+// ---- Few rows: four independent wavefronts, a page a step each, no barrier but the one before their states are joined. Keys
+// come from memory as operands and become fp16 in registers (the layouts of attn_decode8.hip), 16 rows a product.
+template <int D, int NQ>
+struct Few {
+  float acc[NWAVE][16 * NQ][D];
+  float m[NWAVE][16 * NQ], l[NWAVE][16 * NQ], x[NWAVE][16 * NQ];
+};
+
+// The NaNs of a page's V in registers: cleared, noted in LDS as a bit a dim (D / 8 bytes a key), and the keys that have any.
+template <int D>
+__device__ __forceinline__ uint64_t nan_of_page(u32x2 (&vr)[Lay8<D>::VN], uint8_t* nan, int lane) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < Lay8<D>::VN; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      uint32_t w = vr[i][e];
+      any |= take_nan(w);
+    }
+  if (__ballot(any != 0) == 0) return 0;
+  const int j4 = lane >> 4, c16 = lane & 15;
+#pragma unroll
+  for (int i = 0; i < Lay8<D>::VN; ++i) {
+    const int t = D == 128 ? mf_tok(i / 4, i % 4, j4) : mf_tok(i / 2, 2 * (i % 2), j4) + (c16 >> 3);
+    uint32_t lo = vr[i].x, hi = vr[i].y;
+    const uint32_t b = four_bits(take_nan(lo)) | four_bits(take_nan(hi)) << 4;
+    nan[t * (D / 8) + c16 % (D / 8)] = static_cast<uint8_t>(b);
+    vr[i] = u32x2{lo, hi};
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  uint32_t of = 0;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) of |= *reinterpret_cast<const uint32_t*>(nan + lane * (D / 8) + 4 * e);
+  return __ballot(of != 0);
+}
+// Bit 8 i + x: a NaN of key t at dim mf_vdim(4 j4 + i) + x.
+template <int D>
+__device__ __forceinline__ uint32_t nan_bits(const uint8_t* nan, int t, int j4) {
+  const uint32_t* b = reinterpret_cast<const uint32_t*>(nan + t * (D / 8));
+  if constexpr (D == 128) return b[j4];
+  return b[j4 & 1] >> (j4 >= 2 ? 4 : 0) & 0x0f0f0f0fu;
+}
+
+template <int D, int NQ, bool I8, bool MOD>
+__device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, int h, Few<D, NQ>& L) {
+  constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
+  const int j4 = lane >> 4, c16 = lane & 15;
+  const int nw = u.n > wave ? (u.n - wave + NWAVE - 1) / NWAVE : 0;
+  PageList<NWAVE> list(p, u, h, wave, nw);
+  const uint32_t koff = c16 * p.k_st + 16 * j4;
+  const uint32_t voff = D == 128 ? 4 * j4 * p.v_st + 8 * c16 : (4 * j4 + (c16 >> 3)) * p.v_st + 8 * (c16 & 7);
+  const bool up_half = (lane & 8) != 0;
+  const uint8_t* kb = p.k + h * p.k_sh;
+  const uint8_t* vb = p.v + h * p.v_sh;
+  auto res = [&](const uint8_t* base, int64_t sb, uint32_t st, int blk, int pg) {
+    return page_res<D>(base, sb, st, pg, pg >= 0 ? min(BLK, u.len - blk * BLK) : 0);
+  };
+  u32x4 kr[4][KC];
+  u32x2 vr[VN];
+  int blk = list.blk(0), pg = nw > 0 ? list.pg(0) : -1;
+  load_k8<D>(kr, res(kb, p.k_sb, p.k_st, blk, pg), koff, p.k_st);
+  load_v8<D>(vr, res(vb, p.v_sb, p.v_st, blk, pg), voff, p.v_st);
+
+  u32x4 qh[NQ][KS];
+  float qf[NQ], slope[NQ];
+  Sight see[NQ];
+  State st[NQ];
+  Reach re;
+#pragma unroll
+  for (int a = 0; a < NQ; ++a) {
+    const Row r = virtual_row(p, u, h, 16 * a + c16);
+    const uint16_t* qp = p.q + r.n * p.q_sn + r.hq * p.q_sh + 16 * j4;
+    float amax = 0.f, bad = 0.f, up;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qh[a][ks] = ld16(qp + 64 * (ks / 2) + 8 * (ks % 2));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q_extent(qh[a][ks], amax, bad);
+    qf[a] = q_factor(swap_max(amax), swap_sum(bad), up) * (MOD ? p.scale : p.scale * LOG2E);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qh[a][ks] = q_half(qh[a][ks], up);
+    see[a] = sight(p, u, r);
+    slope[a] = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
+    re = a == 0 ? reach(see[a]) : both(re, reach(see[a]));
+  }
+  uint8_t* nan = reinterpret_cast<uint8_t*>(L.acc[wave]);  // (free until the loop's end)
+  uint32_t poison[NQ] = {};                                // accumulators that are NaN
+  f32x4_t acc[NQ][VD];
+#pragma unroll
+  for (int a = 0; a < NQ; ++a)
+#pragma unroll
+    for (int j = 0; j < VD; ++j) acc[a][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (int k = 0; k < nw; ++k) {
+    list.advance(k);
+    const float ks = list.ks(k), vs = list.vs(k);
+    list.turn(k);
+    int blk_n = -1, pg_n = -1;
+    if (k + 1 < nw) blk_n = list.blk(k + 1), pg_n = list.pg(k + 1);
+    float s[NQ][16];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      u32x4 w[KS];
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const u32x2 w0 = widen4<I8>(kr[nt][x / 2][2 * (x % 2)]), w1 = widen4<I8>(kr[nt][x / 2][2 * (x % 2) + 1]);
+        w[x] = u32x4{w0.x, w0.y, w1.x, w1.y};
+      }
+#pragma unroll
+      for (int a = 0; a < NQ; ++a) {
+        f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < KS; ++x)
+          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[x]), __builtin_bit_cast(f16x8_t, qh[a][x]), c,
+                                                     0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[a][4 * nt + i] = c[i];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k8<D>(kr, res(kb, p.k_sb, p.k_st, blk_n, pg_n), koff, p.k_st);
+    __builtin_amdgcn_sched_barrier(0);
+
+    const int t0 = blk * BLK, len = pg >= 0 ? u.len : 0;
+    const bool whole = sees_all(re, t0, len);
+    uint64_t bad = 0;  // keys of a cut page with a NaN in V
+    if constexpr (!I8)
+      if (!sees_keys(re, t0, len)) bad = nan_of_page<D>(vr, nan, lane);
+    uint32_t w[NQ][8];
+#pragma unroll
+    for (int a = 0; a < NQ; ++a) {
+      float f = qf[a] * ks;
+      if constexpr (MOD) {
+        modify(s[a], f, p.softcap, p.slopes != nullptr, slope[a], static_cast<float>(see[a].hi - t0 - 4 * j4),
+               [](int i) { return static_cast<float>(16 * (i / 4) + i % 4); });
+        f = 1.f;
+      } else if ((__float_as_int(ks) ^ __float_as_int(p.scale)) < 0) {  // uniform: f made positive
+        f = -f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[a][i] = -s[a][i];
+      }
+      if (!whole) {  // uniform
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int t = t0 + mf_tok(i / 4, i % 4, j4);
+          s[a][i] = t < len && sees(see[a], t) ? s[a][i] * f : NEG_INF;
+        }
+        f = 1.f;
+      }
+      float alpha;
+      if (soften(s[a], f, vs, st[a], alpha, w[a], [](float x) { return swap_max(x); }))
+#pragma unroll
+        for (int j = 0; j < VD; ++j) acc[a][j] *= alpha;
+    }
+#pragma unroll
+    for (int d = 0; d < VD / 4; ++d)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        u32x4 x[4];  // four dims, tokens in pairs
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          uint32_t a, c;
+          v_pair8<D>(vr, 2 * q + y / 2, 2 * (y % 2), d, up_half, a, c);
+          const u32x2 w01 = widen4<I8>(__builtin_amdgcn_perm(c, a, 0x05010400u));
+          const u32x2 w23 = widen4<I8>(__builtin_amdgcn_perm(c, a, 0x07030602u));
+          x[0][y] = w01.x, x[1][y] = w01.y, x[2][y] = w23.x, x[3][y] = w23.y;
+        }
+#pragma unroll
+        for (int a = 0; a < NQ; ++a) {
+          const u32x4 pw = {w[a][4 * q], w[a][4 * q + 1], w[a][4 * q + 2], w[a][4 * q + 3]};
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            acc[a][4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                __builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pw), acc[a][4 * d + y], 0, 0, 0);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v8<D>(vr, res(vb, p.v_sb, p.v_st, blk_n, pg_n), voff, p.v_st);
+    if constexpr (!I8)
+      for (; bad != 0; bad &= bad - 1) {  // uniform
+        const int t = __builtin_ctzll(bad);
+#pragma unroll
+        for (int a = 0; a < NQ; ++a) poison[a] |= sees(see[a], t0 + t) ? nan_bits<D>(nan, t, j4) : 0u;
+      }
+    blk = blk_n;
+    pg = pg_n;
+  }
+
+  // ---- the four states joined: lane (c16, j4) holds row c16's dims mf_vdim(4 j4 + i) + j
+#pragma unroll
+  for (int a = 0; a < NQ; ++a) {
+    const int row = 16 * a + c16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* o = L.acc[wave][row] + mf_vdim<D>(4 * j4 + i);
+#pragma unroll
+      for (int j = 0; j < VD; ++j)
+        if (!I8 && (poison[a] >> (8 * i + j) & 1) != 0) acc[a][j][i] = __builtin_nanf("");
+#pragma unroll
+      for (int j = 0; j < VD; j += 4)
+        *reinterpret_cast<float4*>(o + j) = make_float4(acc[a][j][i], acc[a][j + 1][i], acc[a][j + 2][i], acc[a][j + 3][i]);
+    }
+    const float l = swap_sum(st[a].l);
+    if (j4 == 0) {
+      const float mu = st[a].m == NEG_INF ? 0.f : st[a].m;
+      L.m[wave][row] = st[a].m, L.l[wave][row] = l;
+      L.x[wave][row] = st[a].ar == NEG_INF ? NEG_INF : (st[a].ar - mu) + (st[a].ax - 7.f);
+    }
+  }
+  __syncthreads();
+  for (int o = tid; o < u.nv * (D / 4); o += NT) {
+    const int row = o / (D / 4), d = o % (D / 4) * 4;
+    float m[NWAVE], M = NEG_INF, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) m[w] = L.m[w][row], M = fmaxf(M, m[w]);
+    const float mu = M == NEG_INF ? 0.f : M;
+    f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) {
+      const float mw = m[w] == NEG_INF ? 0.f : m[w];
+      l += L.l[w][row] * fexp2(m[w] - mu);
+      a += *reinterpret_cast<const f32x4_t*>(&L.acc[w][row][d]) * fexp2((mw - mu) + L.x[w][row]);
+    }
+    store4(p, u, h, row, virtual_row(p, u, h, row), d, D, a, M, l);
+  }
+}
+
+// ---- Many rows: the four wavefronts hold 32 rows each and read the same pages, fp16 in LDS, two at a time: while one is
+// multiplied the next one's codes are on their way and converted, once for all rows. 32 x 32 products: K as it lies in
+// LDS, V by transposing reads. Chunks of 16 bytes are placed so that neither reads nor writes conflict: K chunk c of
+// row r at c ^ r, V's at c ^ 4 (r % 4) (64 dims: r / 2 in both).
+template <int D>
+struct Many {
+  uint8_t k[2][BLK * D * 2], v[2][BLK * D * 2];
+  uint32_t nan[2][BLK][4];  // of a cut page: a bit a dim (64 dims: 16 bits of each)
+  Reach reach[NWAVE];
+};
+
+template <int D, bool I8, bool MOD>
+__device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u, int h, Many<D>& L) {
+  constexpr int KS = D / 16, ND = D / 32, NC = D / 64;  // steps of a score product; dim tiles; 16-byte loads a thread
+  constexpr uint32_t ROW = 2 * D, PAGE = BLK * ROW;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
+  const int c32 = lane & 31, half = lane >> 5;
+  PageList<1> list(p, u, h, 0, u.n);
+  const uint8_t* kb = p.k + h * p.k_sh;
+  const uint8_t* vb = p.v + h * p.v_sh;
+  auto rows_of = [&](int blk, int pg) { return pg >= 0 ? min(BLK, u.len - blk * BLK) : 0; };
+  // staging: thread t holds 16 NC codes of row t / 4
+  const uint32_t srow = tid >> 2, sc = 2 * NC * (tid & 3);  // its first 16-byte chunk in LDS
+  const uint32_t kso = srow * p.k_st + 16 * NC * (tid & 3), vso = srow * p.v_st + 16 * NC * (tid & 3);
+  const uint32_t kx = D == 128 ? srow & 15 : (srow >> 1) & 7, vx = D == 128 ? (srow & 3) << 2 : ((srow >> 1) & 1) << 2;
+  u32x4 kc[NC], vc[NC];
+  auto fetch = [&](int k) {
+    const int blk = k < u.n ? list.blk(k) : -1, pg = k < u.n ? list.pg(k) : -1, n = rows_of(blk, pg);
+    const rsrc_t rk = page_res<D>(kb, p.k_sb, p.k_st, pg, n), rv = page_res<D>(vb, p.v_sb, p.v_st, pg, n);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kc[c] = bload16(rk, kso + 16 * c, 0);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) vc[c] = bload16(rv, vso + 16 * c, 0);
+  };
+  auto widen16 = [&](const u32x4& x, uint8_t* row, uint32_t chunk, uint32_t swz) {
+    const u32x2 a = widen4<I8>(x[0]), b = widen4<I8>(x[1]), c = widen4<I8>(x[2]), d = widen4<I8>(x[3]);
+    *reinterpret_cast<u32x4*>(row + ((chunk ^ swz) << 4)) = u32x4{a.x, a.y, b.x, b.y};
+    *reinterpret_cast<u32x4*>(row + (((chunk + 1) ^ swz) << 4)) = u32x4{c.x, c.y, d.x, d.y};
+  };
+  auto stage = [&](int buf, bool cut) {
+    uint8_t* k = L.k[buf] + srow * ROW;
+    uint8_t* v = L.v[buf] + srow * ROW;
+    if constexpr (!I8)
+      if (cut) {  // uniform
+        uint32_t bits = 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w = vc[c][e];
+            bits |= four_bits(take_nan(w)) << (16 * c + 4 * e);
+            vc[c][e] = w;
+          }
+        L.nan[buf][srow][tid & 3] = bits;
+      }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) widen16(kc[c], k, sc + 2 * c, kx);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) widen16(vc[c], v, sc + 2 * c, vx);
+  };
+  fetch(0);
+
+  // ---- this wavefront's rows
+  const bool busy = 32 * wave < u.nv;
+  const Row r = virtual_row(p, u, h, 32 * wave + c32);
+  u32x4 qh[KS];
+  float qf;
+  {
+    const uint16_t* qp = p.q + r.n * p.q_sn + r.hq * p.q_sh + 8 * half;
+    float amax = 0.f, bad = 0.f, up;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) qh[x] = ld16(qp + 16 * x);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) q_extent(qh[x], amax, bad);
+    qf = q_factor(swap32_max(amax), swap32_sum(bad), up) * (MOD ? p.scale : p.scale * LOG2E);
+#pragma unroll
+    for (int x = 0; x < KS; ++x) qh[x] = q_half(qh[x], up);
+  }
+  const Sight see = sight(p, u, r);
+  const Reach re = reach(see);
+  const float slope = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
+  State st;
+  f32x16_t acc[ND];
+  uint32_t poison[ND] = {};  // accumulators that are NaN
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
+  // operand addresses: K chunk 2 x + half of row c32 (step x: ^ 32 x), V dims 32 j + .. of a group's rows (tile j: ^ 64 j)
+  const uint32_t ka = c32 * ROW + ((half ^ (D == 128 ? c32 & 15 : (c32 >> 1) & 7)) << 4);
+  const uint32_t vrow = 4 * half + ((lane & 15) >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t va = vrow * ROW + ((vch ^ (D == 128 ? (vrow & 3) << 2 : ((vrow >> 1) & 1) << 2)) << 4) + 8 * (lane & 1);
+
+  Reach all = re;
+  if constexpr (!I8) {  // of the whole tile
+    if (lane == 0) L.reach[wave] = re;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) all = both(all, L.reach[w]);
+  }
+  auto is_cut = [&](int k) { return !sees_keys(all, list.blk(k) * BLK, list.pg(k) >= 0 ? u.len : 0); };
+  stage(0, u.n > 0 && is_cut(0));
+  bool cut = u.n > 0 && is_cut(0);
+  if (u.n > 1) fetch(1);
+  __syncthreads();
+  for (int k = 0; k < u.n; ++k) {
+    const uint32_t buf = k & 1;
+    const float ks = list.ks(k), vs = list.vs(k);
+    const int blk = list.blk(k), pg = list.pg(k);
+    const int t0 = blk * BLK, len = pg >= 0 ? u.len : 0;
+    if (busy && !sees_none(re, t0, len)) {
+      const uint8_t* kl = L.k[buf];
+      const uint8_t* vl = L.v[buf];
+      float s[32];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        f32x16_t c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[i] = 0.f;
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(kl + ((ka ^ (32 * x)) + 32 * kt * ROW));
+          c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, qh[x]), c, 0, 0,
+                                                     0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[16 * kt + i] = c[i];
+      }
+      float f = qf * ks;
+      if constexpr (MOD) {
+        modify(s, f, p.softcap, p.slopes != nullptr, slope, static_cast<float>(see.hi - t0 - 4 * half),
+               [](int i) { return static_cast<float>(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4); });
+        f = 1.f;
+      } else if ((__float_as_int(ks) ^ __float_as_int(p.scale)) < 0) {
+        f = -f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s[i] = -s[i];
+      }
+      if (!sees_all(re, t0, len)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int t = t0 + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
+          s[i] = t < len && sees(see, t) ? s[i] * f : NEG_INF;
+        }
+        f = 1.f;
+      }
+      uint32_t w[16];
+      float alpha;
+      if (soften(s, f, vs, st, alpha, w, [](float x) { return swap32_max(x); }))
+#pragma unroll
+        for (int j = 0; j < ND; ++j) acc[j] *= alpha;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u32x4 pw = {w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]};
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          typedef __attribute__((address_space(3))) fp16x4_t lds_t;
+          const uint8_t* x = vl + ((va ^ (64 * j)) + 16 * g * ROW);
+          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(x)));
+          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(x + 8 * ROW)));
+          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, (u32x4{lo.x, lo.y, hi.x, hi.y})),
+                                                          __builtin_bit_cast(f16x8_t, pw), acc[j], 0, 0, 0);
+        }
+      }
+      if constexpr (!I8)
+        if (cut) {  // uniform
+          const u32x4 b = *reinterpret_cast<const u32x4*>(L.nan[buf][lane]);
+          for (uint64_t bad = __ballot((b.x | b.y | b.z | b.w) != 0); bad != 0; bad &= bad - 1) {
+            const int t = __builtin_ctzll(bad);
+            const bool seen = sees(see, t0 + t);
+#pragma unroll
+            for (int j = 0; j < ND; ++j) {
+              const uint32_t x = D == 128 ? L.nan[buf][t][j] : L.nan[buf][t][2 * j] | L.nan[buf][t][2 * j + 1] << 16;
+              poison[j] |= seen ? x >> (4 * half) : 0u;  // bit 8 (i / 4) + i % 4
+            }
+          }
+        }
+    }
+    // the list turns after its last read of a step, 64 steps at a time; step k + 2 may be of the next 64
+    list.advance(k);
+    if ((k & 63) == 63) list.turn(k);
+    if (k + 1 < u.n) {
+      cut = !I8 && is_cut(k + 1);
+      stage(buf ^ 1, cut);
+    }
+    if (k + 2 < u.n) {
+      if ((k & 63) == 62) {  // (its page is in nxt still)
+        Pages t = list.cur;
+        list.cur = list.nxt;
+        fetch(k + 2);
+        list.cur = t;
+      } else {
+        fetch(k + 2);
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- results: lane holds row c32's dims 32 j + 8 (i / 4) + 4 half + i % 4
+  const int i0 = 32 * wave + c32;
+  const float l = swap32_sum(st.l);
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (!I8 && (poison[j] >> (8 * (i / 4) + i % 4) & 1) != 0) acc[j][i] = __builtin_nanf("");
+  if (i0 < u.nv) {
+    const float mu = st.m == NEG_INF ? 0.f : st.m;
+    const float x = st.ar == NEG_INF ? 0.f : fexp2((st.ar - mu) + (st.ax - 7.f));
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        store4(p, u, h, i0, r, 32 * j + 2 * i + 4 * half, D,
+               f32x4_t{acc[j][i] * x, acc[j][i + 1] * x, acc[j][i + 2] * x, acc[j][i + 3] * x}, st.m, l);
+  }
+}
+
+// (two workgroups a CU with large tiles, else as many as attn_decode8.hip has)
+template <int D, bool I8, bool MOD, bool LARGE>
+__global__ void __launch_bounds__(NT, LARGE ? 2 : D == 64 ? 4 : 3) attend_kernel(const AttendP p) {
+  constexpr int NQ = LARGE ? TILE_FEW / 16 : 1;
+  __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D, NQ>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D, NQ>)
+                                                                                                        : sizeof(Many<D>)];
+  const int i = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
+  if (i >= p.head[H_UNITS]) return;
+  const AttendUnit u = p.units[i];
+  if constexpr (LARGE) {
+    if (u.kind & 1) {
+      many_rows<D, I8, MOD>(p, u, h, *reinterpret_cast<Many<D>*>(raw));
+      return;
+    }
+  }
+  few_rows<D, NQ, I8, MOD>(p, u, h, *reinterpret_cast<Few<D, NQ>*>(raw));
+}
+
+// The join: workgroup (joined tile, KV head, run of 8 of its virtual rows); a wavefront finds the weights of two rows, then a
+// thread adds up four dims of a row. Rows that no request brings are cleared by the workgroups in turn.
+template <int D>
+__global__ void __launch_bounds__(NT) join_kernel(const AttendP p) {
+  constexpr int RW = 8, MOST = 2 * MAX_TILE_UNITS;
+  __shared__ float sW[RW][MOST];
+  __shared__ float sM[RW], sL[RW];
+  const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+  const int first = p.head[H_FIRST], last = p.head[H_LAST], n_out = p.n_rows - (last - first);
+  for (int i = blockIdx.x; i < n_out; i += gridDim.x) {
+    const int64_t n = i < first ? i : i - first + last;
+    for (int x = tid; x < p.Hq * (D / 8); x += NT) *reinterpret_cast<u32x4*>(p.out + n * p.Hq * D + 8 * x) = u32x4{0, 0, 0, 0};
+    for (int x = tid; x < p.Hq; x += NT) p.lse[n * p.Hq + x] = NEG_INF;
+  }
+  const int run = blockIdx.x % p.chunks, bh = blockIdx.x / p.chunks, h = bh % p.Hkv, j = bh / p.Hkv;
+  if (j >= p.head[H_JOINS]) return;
+  const AttendJoin o = p.joins[j];
+  const int v0 = run * RW, n = min(RW, o.nv - v0);
+  if (n <= 0) return;
+  struct Source {
+    int own, ns, more, step, n;  // partial rows own + s nv of its own pages, then more + s step of the prefix's
+  };
+  auto source = [&](int i) {
+    Source x{o.part + i, o.ns, 0, 0, o.ns};
+    if (o.sv0 >= 0) {
+      const int v = o.sv0 + i, t = o.tile0 + v / o.height;
+      const AttendTile y = p.tiles[t];
+      x.step = y.nv;
+      x.more = y.part + v % o.height;
+      x.n += y.ns;
+    }
+    return x;
+  };
+  auto row_at = [&](const Source& x, int s) { return static_cast<int64_t>(s < x.ns ? x.own + s * o.nv : x.more + (s - x.ns) * x.step); };
+#pragma unroll
+  for (int g = 0; g < RW / NWAVE; ++g) {
+    const int i = wave + NWAVE * g;
+    if (i < n) {  // uniform
+      const Source x = source(v0 + i);
+      float m[MOST / WAVE], l[MOST / WAVE], M = NEG_INF, L = 0.f;
+#pragma unroll
+      for (int e = 0; e < MOST / WAVE; ++e) {
+        const int s = lane + WAVE * e;
+        m[e] = NEG_INF, l[e] = 0.f;
+        if (s < x.n) {
+          const float2 t = *reinterpret_cast<const float2*>(p.part_ml + (row_at(x, s) * p.Hkv + h) * 2);
+          m[e] = t.x, l[e] = t.y;
+        }
+        M = fmaxf(M, m[e]);
+      }
+      M = wave_max(M);
+      const float mu = M == NEG_INF ? 0.f : M;
+#pragma unroll
+      for (int e = 0; e < MOST / WAVE; ++e) {
+        const int s = lane + WAVE * e;
+        const float w = l[e] == 0.f ? 0.f : fexp2(m[e] - mu);
+        L += l[e] * w;
+        if (s < x.n) sW[i][s] = l[e] == 0.f ? -1.f : w;  // (an empty partial counts for nothing, a NaN counts)
+      }
+      L = wave_sum(L);
+      if (lane == 0) sM[i] = M, sL[i] = L;
+    }
+  }
+  __syncthreads();
+  constexpr int TR = D / 4;  // threads of a row
+  for (int e = tid; e < n * TR; e += NT) {
+    const int i = e / TR, d = e % TR * 4;
+    const Source x = source(v0 + i);
+    f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < x.n; ++s) {
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p.part_acc + (row_at(x, s) * p.Hkv + h) * D + d);
+      const float w = sW[i][s];
+      if (w != -1.f) a += y * w;
+    }
+    const int v = o.v0 + v0 + i, r = v / p.G;
+    AttendUnit u{};
+    u.part = -1;
+    store4(p, u, h, 0, Row{o.row0 + r, h * p.G + (v - r * p.G), 0, 0}, d, D, a, sM[i], sL[i]);
+  }
+}
+
+template <int D, bool I8>
+hipError_t launch_d(const AttendP& p, const AttendSizes& z, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>(z.units * p.Hkv)), nt(NT);
+  const bool mod = p.softcap > 0.f || p.slopes != nullptr;
+  if (z.large) {
+    if (mod)
+      hipLaunchKernelGGL((attend_kernel<D, I8, true, true>), grid, nt, 0, s, p);
+    else
+      hipLaunchKernelGGL((attend_kernel<D, I8, false, true>), grid, nt, 0, s, p);
+  } else {
+    if (mod)
+      hipLaunchKernelGGL((attend_kernel<D, I8, true, false>), grid, nt, 0, s, p);
+    else
+      hipLaunchKernelGGL((attend_kernel<D, I8, false, false>), grid, nt, 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attend(const kvskip_attend_args& a, const AttendSizes& z, hipStream_t s) {
+  AttendP p;
+  p.q = static_cast<const uint16_t*>(a.q), p.q_sn = a.q_sn, p.q_sh = a.q_sh;
+  p.k = static_cast<const uint8_t*>(a.k), p.k_sb = a.k_sb, p.k_sh = a.k_sh, p.k_st = static_cast<uint32_t>(a.k_st);
+  p.v = static_cast<const uint8_t*>(a.v), p.v_sb = a.v_sb, p.v_sh = a.v_sh, p.v_st = static_cast<uint32_t>(a.v_st);
+  p.k_scale = a.k_scale, p.ks_sb = a.ks_sb, p.ks_sh = a.ks_sh;
+  p.v_scale = a.v_scale, p.vs_sb = a.vs_sb, p.vs_sh = a.vs_sh;
+  p.block_table = a.block_table, p.bt_stride = a.bt_stride;
+  p.shared_table = a.shared_table, p.st_stride = a.st_stride;
+  p.slopes = a.slopes;
+  p.out = static_cast<uint16_t*>(a.out), p.lse = a.lse, p.part_acc = a.part_acc, p.part_ml = a.part_ml;
+  const int* work = a.plan.work;
+  p.head = work;
+  p.units = reinterpret_cast<const AttendUnit*>(work + z.at_units);
+  p.joins = reinterpret_cast<const AttendJoin*>(work + z.at_joins);
+  p.tiles = reinterpret_cast<const AttendTile*>(work + z.at_tiles);
+  p.rows = reinterpret_cast<const AttendRow*>(work + z.at_rows);
+  p.n_rows = a.plan.rows, p.Hq = a.plan.Hq, p.Hkv = a.plan.Hkv, p.G = a.plan.Hq / a.plan.Hkv;
+  p.num_pages = a.num_pages, p.window = a.plan.window < (1 << 30) ? a.plan.window : 1 << 30;
+  p.scale = a.scale, p.softcap = a.softcap;
+  const int tall = z.large ? z.many : z.few;
+  p.chunks = (tall + 7) / 8;
+  const bool i8 = a.format == KVSKIP_INT8;
+  const hipError_t e = a.D == 128 ? (i8 ? launch_d<128, true>(p, z, s) : launch_d<128, false>(p, z, s))
+                                  : (i8 ? launch_d<64, true>(p, z, s) : launch_d<64, false>(p, z, s));
+  if (e != hipSuccess) return e;
+  const dim3 grid(static_cast<uint32_t>(z.own * p.Hkv * p.chunks));
+  if (a.D == 128)
+    hipLaunchKernelGGL(join_kernel<128>, grid, dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL(join_kernel<64>, grid, dim3(NT), 0, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace kvs

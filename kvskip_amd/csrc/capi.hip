@@ -7,6 +7,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "attend.hpp"
 #include "internal.hpp"
 
 namespace {
@@ -134,6 +135,9 @@ int kvskip_struct_size(int which) {
     case 5: return static_cast<int>(sizeof(kvskip_cache8_args));
     case 6: return static_cast<int>(sizeof(kvskip_page_args));
     case 7: return static_cast<int>(sizeof(kvskip_write_args));
+    case 8: return static_cast<int>(sizeof(kvskip_attend_plan_args));
+    case 9: return static_cast<int>(sizeof(kvskip_attend_args));
+    case 10: return static_cast<int>(sizeof(kvskip_rope_args));
     default: return -1;
   }
 }
@@ -642,6 +646,107 @@ int kvskip_cache_write(const kvskip_write_args* p, void* stream) {
   if (p->kp_st < p->D || p->vp_st < p->D) return fail(KVSKIP_E_INVALID, "cache_write: pool rows must not overlap");
   if (p->N == 0) return ok();
   return launched(kvs::launch_cache_write(*p, static_cast<hipStream_t>(stream)), "kvskip_cache_write");
+}
+
+// The sizes of a plan; `pointers`: its arrays too.
+static int check_attend_plan(const kvskip_attend_plan_args* p, bool pointers) {
+  if (p == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
+  if (p->B < 1 || p->rows < 1 || p->Hq < 1 || p->Hkv < 1 || p->T < 1)
+    return fail(KVSKIP_E_INVALID, "attend: sizes must be positive (B=%d rows=%d Hq=%d Hkv=%d T=%d)", p->B, p->rows, p->Hq, p->Hkv,
+                p->T);
+  if (p->Hq % p->Hkv != 0) return fail(KVSKIP_E_INVALID, "Hq must be a multiple of Hkv");
+  if (p->B > kvs::MAX_ATTEND_B) return fail(KVSKIP_E_UNSUPPORTED, "attend: B <= %d (got %d)", kvs::MAX_ATTEND_B, p->B);
+  if (p->shared < 0 || p->shared > kvs::MAX_SHARED)
+    return fail(KVSKIP_E_UNSUPPORTED, "attend: at most %d shared prefixes (got %d)", kvs::MAX_SHARED, p->shared);
+  if (p->shared > 0 && p->shared_T < 1) return fail(KVSKIP_E_INVALID, "attend: shared_T >= 1 with shared prefixes");
+  if (p->T > (1 << 27) || (p->shared > 0 && p->shared_T > (1 << 27)) || p->rows > (1 << 21) || p->Hq > 1024 ||
+      static_cast<int64_t>(p->rows) * p->Hq > (1 << 26) || static_cast<int64_t>(p->B) * p->Hkv > (1 << 17))
+    return fail(KVSKIP_E_UNSUPPORTED, "attend: T and shared_T up to 2^27, rows to 2^21, Hq to 1024, rows * Hq to 2^26, B * Hkv "
+                                      "to 2^17");
+  if (p->max_rows < 0 || p->window < 0) return fail(KVSKIP_E_INVALID, "attend: max_rows >= 0, window >= 0");
+  if (!pointers) return KVSKIP_OK;
+  if (p->work == nullptr || !aligned16(p->work)) return fail(KVSKIP_E_INVALID, "attend: work must be 16-byte aligned");
+  if (p->starts == nullptr || p->seq_lens == nullptr || p->positions == nullptr ||
+      (p->shared > 0 && (p->shared_lens == nullptr || p->shared_of == nullptr)))
+    return fail(KVSKIP_E_INVALID, "attend_plan: null tensor");
+  return KVSKIP_OK;
+}
+
+int64_t kvskip_attend_work_ints(const kvskip_attend_plan_args* p) {
+  return check_attend_plan(p, false) != KVSKIP_OK ? -1 : kvs::attend_sizes(*p).total;
+}
+
+int64_t kvskip_attend_part_rows(const kvskip_attend_plan_args* p) {
+  return check_attend_plan(p, false) != KVSKIP_OK ? -1 : kvs::attend_sizes(*p).part_rows;
+}
+
+int kvskip_attend_plan(const kvskip_attend_plan_args* p, void* stream) {
+  const int rc = check_attend_plan(p, true);
+  if (rc != KVSKIP_OK) return rc;
+  return launched(kvs::launch_attend_plan(*p, kvs::attend_sizes(*p), static_cast<hipStream_t>(stream)), "kvskip_attend_plan");
+}
+
+int kvskip_attend(const kvskip_attend_args* a, void* stream) {
+  if (a == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
+  const kvskip_attend_plan_args& p = a->plan;
+  const int rc = check_attend_plan(&p, false);
+  if (rc != KVSKIP_OK) return rc;
+  if (p.work == nullptr || !aligned16(p.work)) return fail(KVSKIP_E_INVALID, "attend: work must be 16-byte aligned");
+  if (a->D != 64 && a->D != 128) return fail(KVSKIP_E_UNSUPPORTED, "attend: D in {64, 128} (D=%d)", a->D);
+  if (a->format != KVSKIP_E4M3 && a->format != KVSKIP_INT8)
+    return fail(KVSKIP_E_INVALID, "attend: format e4m3 or int8 (got %d)", a->format);
+  if (a->q == nullptr || a->q_sn % 8 != 0 || a->q_sh % 8 != 0 || !aligned16(a->q))
+    return fail(KVSKIP_E_INVALID, "q rows must be 16-byte aligned");
+  const void* kv[2] = {a->k, a->v};
+  const int64_t st[2][3] = {{a->k_sb, a->k_sh, a->k_st}, {a->v_sb, a->v_sh, a->v_st}};
+  for (int i = 0; i < 2; ++i) {
+    const char* n = i == 0 ? "k" : "v";
+    if (kv[i] == nullptr || !aligned16(kv[i])) return fail(KVSKIP_E_INVALID, "%s must be 16-byte aligned", n);
+    if (st[i][0] % 16 != 0 || st[i][1] % 16 != 0 || st[i][2] % 16 != 0)
+      return fail(KVSKIP_E_INVALID, "%s strides must be multiples of 16 elements (16-byte rows)", n);
+    if (st[i][2] < 0 || st[i][2] >= (int64_t(1) << 24))
+      return fail(KVSKIP_E_UNSUPPORTED, "%s: token stride in [0, 2^24)", n);
+  }
+  if (a->k_scale == nullptr || a->v_scale == nullptr) return fail(KVSKIP_E_INVALID, "attend: k_scale and v_scale");
+  if (a->num_pages < 1) return fail(KVSKIP_E_INVALID, "attend: num_pages >= 1");
+  if (a->block_table == nullptr || a->bt_stride < (p.T + KVSKIP_BLOCK - 1) / KVSKIP_BLOCK)
+    return fail(KVSKIP_E_INVALID, "attend: block_table rows of ceil(T / 64) pages");
+  if (p.shared > 0 && (a->shared_table == nullptr || a->st_stride < (p.shared_T + KVSKIP_BLOCK - 1) / KVSKIP_BLOCK))
+    return fail(KVSKIP_E_INVALID, "attend: shared_table rows of ceil(shared_T / 64) pages");
+  if (a->out == nullptr || a->lse == nullptr || a->part_acc == nullptr || a->part_ml == nullptr)
+    return fail(KVSKIP_E_INVALID, "attend: null tensor");
+  if (!aligned16(a->out) || !aligned16(a->part_acc) || !aligned16(a->part_ml))
+    return fail(KVSKIP_E_INVALID, "attend: out, part_acc, part_ml must be 16-byte aligned");
+  if (!(a->softcap >= 0.f) || std::isinf(a->softcap)) return fail(KVSKIP_E_INVALID, "attend: softcap finite and >= 0");
+  return launched(kvs::launch_attend(*a, kvs::attend_sizes(p), static_cast<hipStream_t>(stream)), "kvskip_attend");
+}
+
+int kvskip_norm_rope(const kvskip_rope_args* p, void* stream) {
+  if (p == nullptr) return fail(KVSKIP_E_INVALID, "null argument block");
+  if (p->rows < 0 || p->Hq < 1 || p->Hkv < 0) return fail(KVSKIP_E_INVALID, "norm_rope: sizes must be positive");
+  if (p->D < 8 || p->D > 256 || p->D % 8 != 0) return fail(KVSKIP_E_UNSUPPORTED, "norm_rope: D a multiple of 8 up to 256 (D=%d)", p->D);
+  if (p->rot < 0 || p->rot > p->D || p->rot % 8 != 0)
+    return fail(KVSKIP_E_UNSUPPORTED, "norm_rope: rotated elements a multiple of 8 up to D (got %d)", p->rot);
+  if (p->Hq > 1024 || p->Hkv > 1024 || p->rows > (1 << 23))
+    return fail(KVSKIP_E_UNSUPPORTED, "norm_rope: Hq and Hkv up to 1024, rows to 2^23");
+  if (p->axes < 1 || p->axes > 4) return fail(KVSKIP_E_INVALID, "norm_rope: 1 to 4 axes (got %d)", p->axes);
+  int sum = 0;
+  for (int i = 0; i < p->axes; ++i) {
+    if (p->sections[i] < 0 || p->sections[i] > p->rot / 2) return fail(KVSKIP_E_INVALID, "norm_rope: sections of rot / 2 pairs in all");
+    sum += p->sections[i];
+  }
+  if (sum != p->rot / 2) return fail(KVSKIP_E_INVALID, "norm_rope: sections of rot / 2 pairs in all");
+  if (!(p->eps >= 0.f)) return fail(KVSKIP_E_INVALID, "norm_rope: eps >= 0");
+  if (p->rows == 0) return ok();
+  if (p->q == nullptr || p->q_out == nullptr || (p->Hkv > 0 && (p->k == nullptr || p->k_out == nullptr)) ||
+      (p->rot > 0 && (p->positions == nullptr || p->inv_freq == nullptr)))
+    return fail(KVSKIP_E_INVALID, "norm_rope: null tensor");
+  const void* t[4] = {p->q, p->q_out, p->k, p->k_out};
+  const int64_t st[8] = {p->q_sn, p->q_sh, p->qo_sn, p->qo_sh, p->k_sn, p->k_sh, p->ko_sn, p->ko_sh};
+  for (int i = 0; i < (p->Hkv > 0 ? 4 : 2); ++i)
+    if ((reinterpret_cast<uintptr_t>(t[i]) & 7u) != 0 || st[2 * i] % 4 != 0 || st[2 * i + 1] % 4 != 0)
+      return fail(KVSKIP_E_INVALID, "norm_rope: q, k and outputs in rows of whole 8 bytes");
+  return launched(kvs::launch_norm_rope(*p, static_cast<hipStream_t>(stream)), "kvskip_norm_rope");
 }
 
 }  // extern "C"

@@ -20,6 +20,7 @@
 #include <cstring>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "kvskip_amd.h"
@@ -48,6 +49,11 @@ struct Api {
   int (*page_map)(const kvskip_page_args*, void*);
   int64_t (*page_work_ints)(int32_t, int32_t);
   int (*cache_write)(const kvskip_write_args*, void*);
+  int (*attend_plan)(const kvskip_attend_plan_args*, void*);
+  int64_t (*attend_work_ints)(const kvskip_attend_plan_args*);
+  int64_t (*attend_part_rows)(const kvskip_attend_plan_args*);
+  int (*attend)(const kvskip_attend_args*, void*);
+  int (*norm_rope)(const kvskip_rope_args*, void*);
   const char* (*last_error)();
 };
 constexpr int N_API = sizeof(Api) / sizeof(void*);
@@ -999,6 +1005,219 @@ PyObject* cache_write(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
+// ---- attention of a step's rows over pages
+[[noreturn]] void fail_api() {
+  const char* m = api.last_error();
+  fail(m != nullptr && m[0] != '\0' ? std::string(m) : "kvskip_amd: invalid arguments");
+}
+
+// A plan's sizes, from its tables.
+void plan_sizes(kvskip_attend_plan_args& p, const at::Tensor& bt, const at::Tensor* st, int64_t rows, PyObject* Hq, PyObject* Hkv,
+                PyObject* max_rows, PyObject* window) {
+  std::memset(&p, 0, sizeof(p));
+  for (const at::Tensor* t : {&bt, st})
+    require(t == nullptr || (t->is_cuda() && t->scalar_type() == at::kInt && t->dim() == 2 && t->size(0) > 0 && t->size(1) > 0 &&
+                             (t->size(1) == 1 || t->stride(1) == 1)),
+            "block_table, shared_table: int32 [requests or prefixes, pages] on the device, rows contiguous");
+  require(bt.size(1) <= (1 << 21) && (st == nullptr || st->size(1) <= (1 << 21)), "attend: tables of up to 2^21 pages a row");
+  require(rows >= 0 && rows <= INT32_MAX && bt.size(0) <= INT32_MAX && (st == nullptr || st->size(0) <= INT32_MAX),
+          "attend: sizes out of range");
+  p.B = static_cast<int32_t>(bt.size(0)), p.T = static_cast<int32_t>(bt.size(1) * TILE);
+  if (st != nullptr) p.shared = static_cast<int32_t>(st->size(0)), p.shared_T = static_cast<int32_t>(st->size(1) * TILE);
+  p.rows = static_cast<int32_t>(rows), p.Hq = int32(Hq), p.Hkv = int32(Hkv);
+  p.max_rows = int32(max_rows), p.window = int32(window);
+}
+
+// attend_plan(starts, seq_lens, rows, block_table, Hq, Hkv, max_rows, window, prefix_lens, shared_table, shared_lens,
+//             shared_of): [work, positions]
+PyObject* attend_plan(PyObject* const* a) {
+  const at::Tensor &starts = tensor(a[0], "starts"), &lens = tensor(a[1], "seq_lens"), &bt = tensor(a[3], "block_table");
+  const at::Tensor *pre = opt_tensor(a[8], "prefix_lens"), *st = opt_tensor(a[9], "shared_table"),
+                   *sl = opt_tensor(a[10], "shared_lens"), *so = opt_tensor(a[11], "shared_of");
+  kvskip_attend_plan_args p;
+  plan_sizes(p, bt, st, integer(a[2]), a[4], a[5], a[6], a[7]);
+  require((st != nullptr) == (sl != nullptr) && (st != nullptr) == (so != nullptr),
+          "shared_table, shared_lens and shared_of belong together");
+  auto ints = [&](const at::Tensor* t, int64_t n, const char* name) -> const int32_t* {
+    if (t == nullptr) return nullptr;
+    if (!(t->is_cuda() && is(*t, at::kInt) && t->numel() == n))
+      fail(std::string("attend_plan: ") + name + ": contiguous int32 of " + std::to_string(n) + " on the device");
+    return static_cast<const int32_t*>(t->data_ptr());
+  };
+  p.starts = ints(&starts, int64_t(p.B) + 1, "starts"), p.seq_lens = ints(&lens, p.B, "seq_lens");
+  p.prefix_lens = ints(pre, p.B, "prefix_lens");
+  p.shared_lens = ints(sl, p.shared, "shared_lens"), p.shared_of = ints(so, p.B, "shared_of");
+  same_device(bt, {&starts, &lens, pre, st, sl, so}, "attend_plan: tensors on one device");
+  const at::Device dev = bt.device();
+  at::Tensor work, pos = empty({p.rows}, at::kInt, dev);
+  if (p.rows > 0) {
+    const int64_t n = api.attend_work_ints(&p);
+    if (n < 0) fail_api();
+    work = empty({n}, at::kInt, dev);
+    p.work = static_cast<int32_t*>(work.data_ptr()), p.positions = static_cast<int32_t*>(pos.data_ptr());
+    launch(dev, [&](void* s) { return api.attend_plan(&p, s); });
+  } else {
+    work = empty({0}, at::kInt, dev);
+  }
+  return list_of({work, pos});
+}
+
+// attend(q, k, v, k_scale, v_scale, scale, work, block_table, shared_table, rows, Hq, Hkv, max_rows, window, softcap, slopes):
+// [out, lse]
+PyObject* attend(PyObject* const* a) {
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &ks = tensor(a[3], "k_scale"),
+                   &vs = tensor(a[4], "v_scale"), &work = tensor(a[6], "work"), &bt = tensor(a[7], "block_table");
+  const at::Tensor *st = opt_tensor(a[8], "shared_table"), *slopes = opt_tensor(a[15], "slopes");
+  kvskip_attend_args c;
+  std::memset(&c, 0, sizeof(c));
+  require(is_bf16_cuda(q) && q.dim() == 3, "q must be CUDA bf16 [rows, Hq, D]");
+  plan_sizes(c.plan, bt, st, integer(a[9]), a[10], a[11], a[12], a[13]);
+  const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = c.plan.Hkv;
+  require(N == c.plan.rows && Hq == c.plan.Hq, "attend: q [rows, Hq, D] of the plan's rows and heads");
+  require(D <= 1024 && q.stride(2) == 1 && q.stride(1) % 8 == 0 && (N <= 1 || q.stride(0) % 8 == 0) && (N == 0 || aligned16(q)),
+          "q rows must be 16-byte aligned");
+  c.format = cache_format(k, "k");
+  require(cache_format(v, "v") == c.format, "k and v must have one type");
+  for (const at::Tensor* t : {&k, &v}) {
+    require(t->dim() == 4 && t->size(0) == k.size(0) && t->size(1) == Hkv && t->size(2) == TILE && t->size(3) == D,
+            "attend: k, v must be page pools [num_pages, Hkv, 64, D] of the plan's heads");
+    require(t->stride(3) == 1 && t->stride(0) % 16 == 0 && t->stride(1) % 16 == 0 && t->stride(2) % 16 == 0 && aligned16(*t),
+            "k, v rows must be 16-byte aligned (strides multiples of 16 elements)");
+  }
+  require(k.size(0) >= 1 && k.size(0) <= INT32_MAX, "attend: 1 <= num_pages < 2^31");
+  for (const at::Tensor* t : {&ks, &vs})
+    require(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == k.size(0) && t->size(1) == Hkv,
+            "k_scale, v_scale: fp32 [num_pages, Hkv]");
+  require(slopes == nullptr || (is(*slopes, at::kFloat) && slopes->numel() == Hq), "slopes: contiguous fp32 [Hq]");
+  same_device(q, {&k, &v, &ks, &vs, &work, &bt, st, slopes}, "attend: tensors on one device");
+  const double cap = real(a[14]);
+  require(cap >= 0.0 && std::isfinite(cap), "attend: softcap finite and >= 0");
+  const at::Device dev = q.device();
+  at::Tensor out = empty({N, Hq, D}, at::kBFloat16, dev), lse = empty({N, Hq}, at::kFloat, dev), part;
+  if (N > 0) {
+    const int64_t n = api.attend_work_ints(&c.plan), rows = api.attend_part_rows(&c.plan);
+    if (n < 0 || rows < 0) fail_api();
+    require(is(work, at::kInt) && work.numel() >= n, "attend: the plan's work");
+    const int64_t acc = rows * Hkv * D;
+    part = empty({acc + rows * Hkv * 2}, at::kFloat, dev);
+    c.part_acc = static_cast<float*>(part.data_ptr()), c.part_ml = c.part_acc + acc;
+    c.plan.work = static_cast<int32_t*>(work.data_ptr());
+    c.q = q.data_ptr(), c.q_sn = N > 1 ? q.stride(0) : 0, c.q_sh = q.stride(1);
+    c.k = k.data_ptr(), c.k_sb = k.stride(0), c.k_sh = k.stride(1), c.k_st = k.stride(2);
+    c.v = v.data_ptr(), c.v_sb = v.stride(0), c.v_sh = v.stride(1), c.v_st = v.stride(2);
+    c.k_scale = static_cast<const float*>(ks.data_ptr()), c.ks_sb = ks.stride(0), c.ks_sh = ks.stride(1);
+    c.v_scale = static_cast<const float*>(vs.data_ptr()), c.vs_sb = vs.stride(0), c.vs_sh = vs.stride(1);
+    c.block_table = static_cast<const int32_t*>(bt.data_ptr()), c.bt_stride = c.plan.B == 1 ? bt.size(1) : bt.stride(0);
+    if (st != nullptr)
+      c.shared_table = static_cast<const int32_t*>(st->data_ptr()), c.st_stride = c.plan.shared == 1 ? st->size(1) : st->stride(0);
+    c.slopes = slopes == nullptr ? nullptr : static_cast<const float*>(slopes->data_ptr());
+    c.out = out.data_ptr(), c.lse = static_cast<float*>(lse.data_ptr());
+    c.scale = static_cast<float>(real(a[5])), c.softcap = static_cast<float>(cap);
+    c.D = static_cast<int32_t>(D), c.num_pages = static_cast<int32_t>(k.size(0));
+    launch(dev, [&](void* s) { return api.attend(&c, s); });
+  }
+  return list_of({out, lse});
+}
+
+// norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, sections, pairs, mscale, q_out, k_out): [q_out, k_out]
+PyObject* norm_rope(PyObject* const* a) {
+  const at::Tensor& q = tensor(a[0], "q");
+  const at::Tensor *k = opt_tensor(a[1], "k"), *pos = opt_tensor(a[2], "positions"), *fr = opt_tensor(a[3], "inv_freq"),
+                   *qw = opt_tensor(a[4], "q_weight"), *kw = opt_tensor(a[5], "k_weight");
+  auto rows_ok = [](const at::Tensor& t) {
+    return is_bf16_cuda(t) && t.dim() == 3 && (t.size(2) <= 1 || t.stride(2) == 1);
+  };
+  require(rows_ok(q), "norm_rope: q must be CUDA bf16 [rows, Hq, D] with a contiguous last dim");
+  require(k == nullptr || (rows_ok(*k) && k->size(0) == q.size(0) && k->size(2) == q.size(2)),
+          "norm_rope: k must be CUDA bf16 [rows, Hkv, D] with a contiguous last dim");
+  const int64_t N = q.size(0), D = q.size(2);
+  require(N < (int64_t(1) << 31) && q.size(1) < (1 << 20) && D < (1 << 20) && (k == nullptr || k->size(1) < (1 << 20)),
+          "norm_rope: sizes out of range");
+  kvskip_rope_args p;
+  std::memset(&p, 0, sizeof(p));
+  p.rows = static_cast<int32_t>(N), p.Hq = static_cast<int32_t>(q.size(1)), p.D = static_cast<int32_t>(D);
+  p.Hkv = k == nullptr ? 0 : static_cast<int32_t>(k->size(1));
+  require((pos == nullptr) == (fr == nullptr), "norm_rope: positions and inv_freq belong together");
+  p.axes = 1;
+  if (fr != nullptr) {
+    require(fr->is_cuda() && is(*fr, at::kFloat) && fr->dim() == 1 && fr->numel() <= D / 2,
+            "norm_rope: inv_freq: contiguous CUDA fp32, a frequency a pair");
+    require(pos->is_cuda() && pos->scalar_type() == at::kInt && (pos->dim() == 1 || pos->dim() == 2) &&
+                pos->size(-1) == N && (N <= 1 || pos->stride(-1) == 1),
+            "norm_rope: positions: int32 [rows] or [axes, rows], rows contiguous");
+    p.rot = static_cast<int32_t>(2 * fr->numel());
+    if (pos->dim() == 2) {
+      require(1 <= pos->size(0) && pos->size(0) <= 4, "norm_rope: 1 to 4 axes");
+      p.axes = static_cast<int32_t>(pos->size(0)), p.pos_stride = p.axes > 1 ? pos->stride(0) : 0;
+    }
+    p.positions = static_cast<const int32_t*>(pos->data_ptr()), p.inv_freq = static_cast<const float*>(fr->data_ptr());
+  }
+  if (a[7] == Py_None) {
+    require(p.axes == 1, "norm_rope: sections, the pairs of each axis");
+    p.sections[0] = p.rot / 2;
+  } else {
+    PyObject* t = PySequence_Tuple(a[7]);
+    if (t == nullptr) throw PyErr{};
+    const Py_ssize_t n = PyTuple_GET_SIZE(t);
+    bool fits = n == p.axes;
+    for (Py_ssize_t i = 0; fits && i < n; ++i) {
+      const int64_t x = PyLong_AsLongLong(PyTuple_GET_ITEM(t, i));
+      if (x == -1 && PyErr_Occurred()) {
+        Py_DECREF(t);
+        throw PyErr{};
+      }
+      fits = 0 <= x && x <= p.rot / 2;
+      if (fits) p.sections[i] = static_cast<int32_t>(x);
+    }
+    Py_DECREF(t);
+    require(fits, "norm_rope: sections: the pairs of each axis, rot / 2 in all");
+  }
+  auto weight = [&](const at::Tensor* w, const char* name, const void*& at, int32_t& f32) {
+    if (w == nullptr) return;
+    const bool f = w->scalar_type() == at::kFloat;
+    if (!(w->is_cuda() && (f || w->scalar_type() == at::kBFloat16) && w->is_contiguous() && w->dim() == 1 && w->numel() == D))
+      fail(std::string("norm_rope: ") + name + ": contiguous bf16 or fp32 [D] on the device");
+    at = w->data_ptr(), f32 = f;
+  };
+  weight(qw, "q_weight", p.q_weight, p.q_weight_f32);
+  weight(kw, "k_weight", p.k_weight, p.k_weight_f32);
+  require(kw == nullptr || k != nullptr, "norm_rope: k_weight without k");
+  const at::Device dev = q.device();
+  auto out = [&](PyObject* o, const at::Tensor& like, const char* name) {
+    const at::Tensor* given = opt_tensor(o, name);
+    if (given == nullptr) return empty(like.sizes(), at::kBFloat16, dev);
+    if (!(rows_ok(*given) && given->sizes() == like.sizes())) fail(std::string("norm_rope: ") + name + ": bf16 of its input's shape");
+    // (in place, or apart: heads are written while others are read)
+    auto span = [](const at::Tensor& t) {
+      int64_t lo = 0, hi = 1;
+      for (int64_t i = 0; i < 3; ++i) (t.stride(i) < 0 ? lo : hi) += (t.size(i) - 1) * t.stride(i);
+      const char* b = static_cast<const char*>(t.data_ptr());
+      return std::make_pair(b + 2 * lo, b + 2 * hi);
+    };
+    if (like.numel() > 0 && !(given->data_ptr() == like.data_ptr() && given->strides() == like.strides())) {
+      const auto x = span(*given), y = span(like);
+      require(x.second <= y.first || y.second <= x.first, "norm_rope: an output is its input or does not overlap it");
+    }
+    return *given;
+  };
+  at::Tensor qo = out(a[10], q, "q_out"), ko;
+  if (k != nullptr) ko = out(a[11], *k, "k_out");
+  else require(a[11] == Py_None, "norm_rope: k_out without k");
+  same_device(q, {k, pos, fr, qw, kw, &qo, k != nullptr ? &ko : nullptr}, "norm_rope: tensors on one device");
+  auto strides = [&](const at::Tensor& t, int64_t& sn, int64_t& sh) {
+    sn = N > 1 ? t.stride(0) : 0, sh = t.size(1) > 1 ? t.stride(1) : 0;
+  };
+  p.q = q.data_ptr(), p.q_out = qo.data_ptr();
+  strides(q, p.q_sn, p.q_sh), strides(qo, p.qo_sn, p.qo_sh);
+  if (k != nullptr) {
+    p.k = k->data_ptr(), p.k_out = ko.data_ptr();
+    strides(*k, p.k_sn, p.k_sh), strides(ko, p.ko_sn, p.ko_sh);
+  }
+  p.pairs = truth(a[8]), p.eps = static_cast<float>(real(a[6])), p.mscale = static_cast<float>(real(a[9]));
+  launch(dev, [&](void* s) { return api.norm_rope(&p, s); });
+  return list_of({qo, ko});
+}
+
 // num_splits(bh, n_tiles, slots, max_splits, min_tiles): split_rule. In Python the scan took 45 us of a
 // decode call at 32k (63.8 us a call, 27 of them kernels) and 80 us of a planner layer-step.
 PyObject* num_splits(PyObject* const* a) {
@@ -1085,7 +1304,8 @@ PyMethodDef methods[] = {
     KVS_FN(attn_block, 20), KVS_FN(vskip1, 13), KVS_FN(select, 10), KVS_FN(pv, 9), KVS_FN(pv_select, 13),
     KVS_FN(plan_block, 33), KVS_FN(update_block, 24), KVS_FN(plan, 2), KVS_FN(merge_update, 3), KVS_FN(plan_scores, 2),
     KVS_FN(update, 2), KVS_FN(num_splits, 5), KVS_FN(zeroed, 2),
-    KVS_FN(decode8, 17), KVS_FN(page_map, 12), KVS_FN(cache_write, 7),
+    KVS_FN(decode8, 17), KVS_FN(page_map, 12), KVS_FN(cache_write, 7), KVS_FN(attend_plan, 12), KVS_FN(attend, 16),
+    KVS_FN(norm_rope, 12),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -19,6 +19,7 @@ The checks, allocations and launches of most operators are native (csrc/host.cpp
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
@@ -156,6 +157,60 @@ def cache_write(k, v, slot_map, k_pool, v_pool, k_scale=None, v_scale=None):
     k_scale, v_scale fp32 [num_pages, Hkv], which grow by powers of two as rows need it (a page whose row 0 is written
     starts anew). The rows of a page must lie next to each other in the map, as page_map's do."""
     _host().cache_write(k, v, slot_map, k_pool, v_pool, k_scale, v_scale)
+
+
+@dataclass(frozen=True)
+class AttendPlan:
+    """What attend() of a step's rows needs to know of them (attend_plan): the cut of its work, for all layers. positions:
+    int32 [rows], each row's (-1 for a row that no request brings), as norm_rope takes them."""
+    work: torch.Tensor
+    positions: torch.Tensor
+    block_table: torch.Tensor
+    shared_table: torch.Tensor | None
+    rows: int
+    Hq: int
+    Hkv: int
+    max_rows: int
+    window: int
+
+
+def attend_plan(starts, seq_lens, rows, block_table, Hq, Hkv, max_rows=0, window=0, prefix_lens=None, shared_table=None,
+                shared_lens=None, shared_of=None) -> AttendPlan:
+    """The plan of attend() over `rows` rows (kvskip_attend_plan; not in kvskip_ext), in one launch: request b brings rows
+    starts[b] .. starts[b + 1] - 1 (int32 [B + 1], rising; else no row belongs to any), the last of its seq_lens[b] tokens
+    (int32 [B], its tokens after the step), which lie in the pages of block_table[b] (int32 [B, pages]).
+
+    A row sees the keys of its request up to its own, with window > 0 the last `window` of them only, and besides the first
+    prefix_lens[b] keys (int32 [B]) wherever they lie. shared_table (int32 [P, pages]), shared_lens (int32 [P]), shared_of
+    (int32 [B]): the tokens of prefix shared_of[b] (none where it is not in 0 .. P - 1) come before request b's own; each
+    prefix is read once for all rows behind it. max_rows: the most rows that one request is expected to bring (0: all of
+    them), which chooses the tiles; more are served too, slower. Nothing here is read again after the launch but the tables,
+    by attend()."""
+    work, pos = _host().attend_plan(starts, seq_lens, rows, block_table, Hq, Hkv, max_rows, window, prefix_lens, shared_table,
+                                    shared_lens, shared_of)
+    return AttendPlan(work, pos, block_table, shared_table, int(rows), int(Hq), int(Hkv), int(max_rows), int(window))
+
+
+def attend(q, k, v, k_scale, v_scale, scale, plan: AttendPlan, softcap=0.0, slopes=None):
+    """Attention of a step's rows over 8-bit pages (kvskip_attend; not in kvskip_ext): q bf16 [rows, Hq, D], k, v pools
+    [num_pages, Hkv, 64, D] (float8_e4m3fn or int8) with fp32 scales [num_pages, Hkv]. Scores scale * k_scale * q.k; with
+    softcap > 0 softcap * tanh(s / softcap); with slopes (fp32 [Hq]) less slopes[head] times the distance of the key. Returns
+    [out bf16 [rows, Hq, D], lse fp32 [rows, Hq]], zeros and -inf for a row that sees no key or that no request brings."""
+    return _host().attend(q, k, v, k_scale, v_scale, scale, plan.work, plan.block_table, plan.shared_table, plan.rows, plan.Hq,
+                          plan.Hkv, plan.max_rows, plan.window, softcap, slopes)
+
+
+def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, sections=None, pairs=False, mscale=1.0,
+              q_out=None, k_out=None):
+    """Norms of queries and keys for each head and their rotation, in one pass (kvskip_norm_rope; not in kvskip_ext): q bf16
+    [rows, Hq, D], k bf16 [rows, Hkv, D] or None, any strides of rows and heads in multiples of 4 elements (slices of a
+    fused projection). With q_weight / k_weight (bf16 or fp32 [D]) a head is divided by the root of its mean square plus
+    eps and multiplied by the weight. Pair i of inv_freq (fp32 [rot / 2], rot a multiple of 8 up to D) is elements i and
+    i + rot / 2, or with pairs 2 i and 2 i + 1, and turns by positions * inv_freq[i]; elements from rot on do not turn, and
+    positions = inv_freq = None turns none. positions: int32 [rows], or [axes, rows] with up to 4 axes, of which axis 0 turns
+    the first sections[0] pairs, axis 1 the next sections[1], and so on. mscale multiplies what is turned. Returns
+    [q_out, k_out], new ones or those given, which may be the inputs (else must not overlap them)."""
+    return _host().norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, sections, pairs, mscale, q_out, k_out)
 
 
 class DecodeOp:

@@ -167,6 +167,25 @@ def _decode8(q, k, v, k_scale, v_scale, scale, plan, stats, num_splits, out_f32,
     return res
 
 
+def attend_plan(starts, seq_lens, rows: int, block_table, Hq: int, Hkv: int, max_rows: int = 0, window: int = 0,
+                prefix_lens=None, shared_table=None, shared_lens=None, shared_of=None):
+    """The plan of attend() for a step's rows (not in the reference; ext.attend_plan), made once for all layers:
+
+        plan = attend_plan(starts, seq_lens, rows, block_table, Hq, Hkv)   # on the device, no synchronisation
+        r = attend(q, k_pool, v_pool, scale, plan, k_scale, v_scale)       # each layer
+    """
+    return ext().attend_plan(starts, seq_lens, rows, block_table, Hq, Hkv, max_rows, window, prefix_lens, shared_table,
+                             shared_lens, shared_of)
+
+
+def attend(q, k, v, scale: float, plan, k_scale, v_scale, softcap: float = 0.0, slopes=None) -> dict:
+    """Attention of a step's rows over 8-bit pages (not in the reference; ext.attend): prompts, chunks of prompts and single
+    tokens in one call, q [rows, Hq, D]. Returns out [rows, Hq, D] bf16 and lse [rows, Hq]. decode() is the faster call for
+    one plain query a request: its K pass holds scores exactly and takes block lists and statistics."""
+    out, lse = ext().attend(q, k, v, k_scale, v_scale, scale, plan, softcap, slopes)
+    return {"out": out, "lse": lse}
+
+
 def block_weights(blk_max: torch.Tensor, blk_sum: torch.Tensor) -> torch.Tensor:
     """Each block's share of its query head's softmax mass [B, Hq, nb], from the statistics
     (kernels/kvskip.py:116-119)."""
