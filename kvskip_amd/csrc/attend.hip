@@ -35,9 +35,8 @@ struct AttendP {
   const int* head;
   const AttendUnit* units;
   const AttendJoin* joins;
-  const AttendTile* tiles;
   const AttendRow* rows;
-  int n_rows, Hq, Hkv, G, num_pages, window, chunks;
+  int n_rows, Hq, Hkv, G, num_pages, window;
   float scale, softcap;
 };
 
@@ -54,6 +53,8 @@ __device__ __forceinline__ float swap32_sum(float v) {
   const u32x2 r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
   return __uint_as_float(r.x) + __uint_as_float(r.y);
 }
+
+constexpr int JOIN_GRID = 2048;  // workgroups of the join: eight a CU
 
 // A virtual row: its row of q and out, query head, position, prefix.
 struct Row {
@@ -73,63 +74,60 @@ __device__ __forceinline__ Row virtual_row(const AttendP& p, const AttendUnit& u
   return x;
 }
 
-// What a row sees of the unit's keys, as indices: t < pre or lo < t <= hi (and t < the unit's len).
+// What a row sees of the unit's keys, as indices: from <= t < end, or t < pre (both ends at most the unit's len).
 struct Sight {
-  int lo, hi, pre;
+  int from, end, pre;
 };
 __device__ __forceinline__ Sight sight(const AttendP& p, const AttendUnit& u, const Row& r) {
   Sight s;
-  s.hi = r.pos - u.base;
-  s.lo = p.window > 0 ? s.hi - p.window : INT32_MIN;
-  s.pre = r.pre - u.base;
+  s.end = min(r.pos - u.base + 1, u.len);
+  s.from = p.window > 0 ? max(r.pos - u.base + 1 - p.window, 0) : 0;
+  s.pre = min(r.pre - u.base, u.len);
   return s;
 }
-__device__ __forceinline__ bool sees(const Sight& s, int t) { return t < s.pre || (t <= s.hi && t > s.lo); }
+__device__ __forceinline__ bool sees(const Sight& s, int t) { return ((t >= s.from) & (t < s.end)) | (t < s.pre); }
 
-template <int W>  // over all lanes
 __device__ __forceinline__ int wave_min_int(int v) {
 #pragma unroll
-  for (int m = 1; m < W; m *= 2) v = min(v, __shfl_xor(v, m, WAVE));
+  for (int m = 1; m < WAVE; m *= 2) v = min(v, __shfl_xor(v, m, WAVE));
   return __builtin_amdgcn_readfirstlane(v);
 }
+__device__ __forceinline__ int wave_max_int(int v) { return ~wave_min_int(~v); }
 
-// The rows of a wavefront together: a page of keys [t0, t0 + 64) is whole (every row sees all of it), cut, or empty.
+// The rows of a wavefront (or tile) together.
 struct Reach {
-  int hi_min, hi_max, lo_min, lo_max, pre_min, pre_max;
+  int from_min, from_max, end_min, end_max, pre_min, pre_max;
 };
 __device__ __forceinline__ Reach reach(const Sight& s) {
-  Reach r;
-  r.hi_min = wave_min_int<WAVE>(s.hi), r.hi_max = -wave_min_int<WAVE>(-s.hi);
-  r.lo_min = wave_min_int<WAVE>(s.lo);
-  r.lo_max = ~wave_min_int<WAVE>(~s.lo);
-  r.pre_min = wave_min_int<WAVE>(s.pre), r.pre_max = -wave_min_int<WAVE>(-s.pre);
-  return r;
+  return Reach{wave_min_int(s.from), wave_max_int(s.from), wave_min_int(s.end), wave_max_int(s.end), wave_min_int(s.pre),
+               wave_max_int(s.pre)};
 }
 __device__ __forceinline__ Reach both(const Reach& a, const Reach& b) {
-  return Reach{min(a.hi_min, b.hi_min), max(a.hi_max, b.hi_max), min(a.lo_min, b.lo_min), max(a.lo_max, b.lo_max),
-               min(a.pre_min, b.pre_min), max(a.pre_max, b.pre_max)};
+  return Reach{min(a.from_min, b.from_min), max(a.from_max, b.from_max), min(a.end_min, b.end_min),
+               max(a.end_max, b.end_max),   min(a.pre_min, b.pre_min),   max(a.pre_max, b.pre_max)};
 }
-// Every row sees all of a page's keys (there are none from len on, where its rows read as zeros).
+// Every row sees all of a page's keys, those of [t0, t0 + 64) before len (from len on its rows read as zeros); all 64 of them;
+// no row sees any.
 __device__ __forceinline__ bool sees_keys(const Reach& r, int t0, int len) {
-  const int t1 = min(t0 + BLK, len) - 1;
-  return t1 < r.pre_min || (t1 <= r.hi_min && t0 > r.lo_max);
+  const int t1 = min(t0 + BLK, len);
+  return t1 <= r.pre_min || (t1 <= r.end_min && t0 >= r.from_max);
 }
 __device__ __forceinline__ bool sees_all(const Reach& r, int t0, int len) { return t0 + BLK <= len && sees_keys(r, t0, len); }
-__device__ __forceinline__ bool sees_none(const Reach& r, int t0, int len) {
-  const int t1 = t0 + BLK - 1;
-  return t0 >= len || (t0 >= r.pre_max && (t0 > r.hi_max || t1 <= r.lo_min));
+__device__ __forceinline__ bool sees_none(const Reach& r, int t0) {
+  return t0 >= r.pre_max && (t0 >= r.end_max || t0 + BLK <= r.from_min);
 }
 
 // A NaN among V's codes (e4m3's 0x7f and 0xff) must reach the rows that see its key and no others, but a weight of 0 times NaN
-// is NaN. So where a page is cut, its NaN codes are made zeros before the product and put into the accumulators of the
-// rows that see them after it. Returns the bytes with a NaN as 0x80, and clears them.
-__device__ __forceinline__ uint32_t take_nan(uint32_t& w) {
-  const uint32_t z = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-  w &= ~((z >> 7) * 0xffu);
-  return z;
+// is NaN. So where a page is cut, its NaN codes are made zeros before the product; a unit that had any looks through its cut
+// pages again at the end and puts them into the accumulators of the rows that see them. (Put in page by page instead, the
+// registers that this takes in the loop cost 20 to 30 % of every pass over e4m3.)
+// Bytes of w that are NaN, as 0x80.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& any) {
+  const uint32_t z = nan_bytes(w);
+  any |= z;
+  return w & ~((z >> 7) * 0xffu);
 }
-// 0x80 of four bytes as four bits.
-__device__ __forceinline__ uint32_t four_bits(uint32_t z) { return ((z >> 7) * 0x01020408u) >> 24; }
 
 // Running state of a row: maximum and sum (log2 units; the sum is this lane's part), and the accumulators' reference ar + ax.
 struct State {
@@ -323,43 +321,6 @@ struct Few {
   float m[NWAVE][16 * NQ], l[NWAVE][16 * NQ], x[NWAVE][16 * NQ];
 };
 
-// The NaNs of a page's V in registers: cleared, noted in LDS as a bit a dim (D / 8 bytes a key), and the keys that have any.
-template <int D>
-__device__ __forceinline__ uint64_t nan_of_page(u32x2 (&vr)[Lay8<D>::VN], uint8_t* nan, int lane) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < Lay8<D>::VN; ++i)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint32_t w = vr[i][e];
-      any |= take_nan(w);
-    }
-  if (__ballot(any != 0) == 0) return 0;
-  const int j4 = lane >> 4, c16 = lane & 15;
-#pragma unroll
-  for (int i = 0; i < Lay8<D>::VN; ++i) {
-    const int t = D == 128 ? mf_tok(i / 4, i % 4, j4) : mf_tok(i / 2, 2 * (i % 2), j4) + (c16 >> 3);
-    uint32_t lo = vr[i].x, hi = vr[i].y;
-    const uint32_t b = four_bits(take_nan(lo)) | four_bits(take_nan(hi)) << 4;
-    nan[t * (D / 8) + c16 % (D / 8)] = static_cast<uint8_t>(b);
-    vr[i] = u32x2{lo, hi};
-  }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  uint32_t of = 0;
-#pragma unroll
-  for (int e = 0; e < D / 32; ++e) of |= *reinterpret_cast<const uint32_t*>(nan + lane * (D / 8) + 4 * e);
-  return __ballot(of != 0);
-}
-// Bit 8 i + x: a NaN of key t at dim mf_vdim(4 j4 + i) + x.
-template <int D>
-__device__ __forceinline__ uint32_t nan_bits(const uint8_t* nan, int t, int j4) {
-  const uint32_t* b = reinterpret_cast<const uint32_t*>(nan + t * (D / 8));
-  if constexpr (D == 128) return b[j4];
-  return b[j4 & 1] >> (j4 >= 2 ? 4 : 0) & 0x0f0f0f0fu;
-}
-
 template <int D, int NQ, bool I8, bool MOD>
 __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, int h, Few<D, NQ>& L) {
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
@@ -384,6 +345,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
   u32x4 qh[NQ][KS];
   float qf[NQ], slope[NQ];
   Sight see[NQ];
+  int at[NQ];  // the row's own index, less the lane's first token
   State st[NQ];
   Reach re;
 #pragma unroll
@@ -399,11 +361,11 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qh[a][ks] = q_half(qh[a][ks], up);
     see[a] = sight(p, u, r);
+    at[a] = r.pos - u.base - 4 * j4;
     slope[a] = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
     re = a == 0 ? reach(see[a]) : both(re, reach(see[a]));
   }
-  uint8_t* nan = reinterpret_cast<uint8_t*>(L.acc[wave]);  // (free until the loop's end)
-  uint32_t poison[NQ] = {};                                // accumulators that are NaN
+  bool nan = false;  // a cut page held one
   f32x4_t acc[NQ][VD];
 #pragma unroll
   for (int a = 0; a < NQ; ++a)
@@ -440,17 +402,21 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
     load_k8<D>(kr, res(kb, p.k_sb, p.k_st, blk_n, pg_n), koff, p.k_st);
     __builtin_amdgcn_sched_barrier(0);
 
-    const int t0 = blk * BLK, len = pg >= 0 ? u.len : 0;
-    const bool whole = sees_all(re, t0, len);
-    uint64_t bad = 0;  // keys of a cut page with a NaN in V
+    const int t0 = blk * BLK;
+    const bool whole = sees_all(re, t0, u.len);
     if constexpr (!I8)
-      if (!sees_keys(re, t0, len)) bad = nan_of_page<D>(vr, nan, lane);
+      if (!sees_keys(re, t0, u.len)) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < VN; ++i) vr[i] = u32x2{without_nan(vr[i].x, any), without_nan(vr[i].y, any)};
+        nan |= __ballot(any != 0) != 0;
+      }
     uint32_t w[NQ][8];
 #pragma unroll
     for (int a = 0; a < NQ; ++a) {
       float f = qf[a] * ks;
       if constexpr (MOD) {
-        modify(s[a], f, p.softcap, p.slopes != nullptr, slope[a], static_cast<float>(see[a].hi - t0 - 4 * j4),
+        modify(s[a], f, p.softcap, p.slopes != nullptr, slope[a], static_cast<float>(at[a] - t0),
                [](int i) { return static_cast<float>(16 * (i / 4) + i % 4); });
         f = 1.f;
       } else if ((__float_as_int(ks) ^ __float_as_int(p.scale)) < 0) {  // uniform: f made positive
@@ -458,11 +424,11 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[a][i] = -s[a][i];
       }
-      if (!whole) {  // uniform
+      if (!whole || pg < 0) {  // uniform
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = t0 + mf_tok(i / 4, i % 4, j4);
-          s[a][i] = t < len && sees(see[a], t) ? s[a][i] * f : NEG_INF;
+          s[a][i] = sees(see[a], t) & (pg >= 0) ? s[a][i] * f : NEG_INF;
         }
         f = 1.f;
       }
@@ -495,15 +461,29 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
       }
     __builtin_amdgcn_sched_barrier(0);
     load_v8<D>(vr, res(vb, p.v_sb, p.v_st, blk_n, pg_n), voff, p.v_st);
-    if constexpr (!I8)
-      for (; bad != 0; bad &= bad - 1) {  // uniform
-        const int t = __builtin_ctzll(bad);
-#pragma unroll
-        for (int a = 0; a < NQ; ++a) poison[a] |= sees(see[a], t0 + t) ? nan_bits<D>(nan, t, j4) : 0u;
-      }
     blk = blk_n;
     pg = pg_n;
   }
+
+  if (!I8 && nan)
+    for (int k = 0; k < nw; ++k) {
+      const int i0 = u.i0 + wave + NWAVE * k, b = i0 < u.a1 ? i0 : i0 - u.a1 + u.b0, g = list.table[b];
+      if (g < 0 || g >= p.num_pages || sees_keys(re, b * BLK, u.len)) continue;
+      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(vb + g * p.v_sb + (t - b * BLK) * p.v_st + mf_vdim<D>(4 * j4 + i));
+#pragma unroll
+          for (int j = 0; j < VD; j += 4) {
+            const uint32_t z = nan_bytes(w[j / 4]);
+#pragma unroll
+            for (int a = 0; a < NQ; ++a)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (sees(see[a], t) && (z >> (8 * e + 7) & 1) != 0) acc[a][j + e][i] = __builtin_nanf("");
+          }
+        }
+    }
 
   // ---- the four states joined: lane (c16, j4) holds row c16's dims mf_vdim(4 j4 + i) + j
 #pragma unroll
@@ -512,9 +492,6 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float* o = L.acc[wave][row] + mf_vdim<D>(4 * j4 + i);
-#pragma unroll
-      for (int j = 0; j < VD; ++j)
-        if (!I8 && (poison[a] >> (8 * i + j) & 1) != 0) acc[a][j][i] = __builtin_nanf("");
 #pragma unroll
       for (int j = 0; j < VD; j += 4)
         *reinterpret_cast<float4*>(o + j) = make_float4(acc[a][j][i], acc[a][j + 1][i], acc[a][j + 2][i], acc[a][j + 3][i]);
@@ -551,8 +528,8 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 template <int D>
 struct Many {
   uint8_t k[2][BLK * D * 2], v[2][BLK * D * 2];
-  uint32_t nan[2][BLK][4];  // of a cut page: a bit a dim (64 dims: 16 bits of each)
   Reach reach[NWAVE];
+  int nan;  // a cut page held one
 };
 
 template <int D, bool I8, bool MOD>
@@ -588,16 +565,12 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
     uint8_t* v = L.v[buf] + srow * ROW;
     if constexpr (!I8)
       if (cut) {  // uniform
-        uint32_t bits = 0;
+        uint32_t any = 0;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w = vc[c][e];
-            bits |= four_bits(take_nan(w)) << (16 * c + 4 * e);
-            vc[c][e] = w;
-          }
-        L.nan[buf][srow][tid & 3] = bits;
+          for (int e = 0; e < 4; ++e) vc[c][e] = without_nan(vc[c][e], any);
+        if (any != 0) L.nan = 1;
       }
 #pragma unroll
     for (int c = 0; c < NC; ++c) widen16(kc[c], k, sc + 2 * c, kx);
@@ -624,10 +597,10 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   }
   const Sight see = sight(p, u, r);
   const Reach re = reach(see);
+  const int at = r.pos - u.base - 4 * half;
   const float slope = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
   State st;
   f32x16_t acc[ND];
-  uint32_t poison[ND] = {};  // accumulators that are NaN
 #pragma unroll
   for (int j = 0; j < ND; ++j)
 #pragma unroll
@@ -640,21 +613,21 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   Reach all = re;
   if constexpr (!I8) {  // of the whole tile
     if (lane == 0) L.reach[wave] = re;
+    if (tid == 0) L.nan = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NWAVE; ++w) all = both(all, L.reach[w]);
   }
-  auto is_cut = [&](int k) { return !sees_keys(all, list.blk(k) * BLK, list.pg(k) >= 0 ? u.len : 0); };
-  stage(0, u.n > 0 && is_cut(0));
-  bool cut = u.n > 0 && is_cut(0);
+  auto is_cut = [&](int k) { return !sees_keys(all, list.blk(k) * BLK, u.len); };
+  stage(0, !I8 && u.n > 0 && is_cut(0));
   if (u.n > 1) fetch(1);
   __syncthreads();
   for (int k = 0; k < u.n; ++k) {
     const uint32_t buf = k & 1;
     const float ks = list.ks(k), vs = list.vs(k);
     const int blk = list.blk(k), pg = list.pg(k);
-    const int t0 = blk * BLK, len = pg >= 0 ? u.len : 0;
-    if (busy && !sees_none(re, t0, len)) {
+    const int t0 = blk * BLK;
+    if (busy && pg >= 0 && !sees_none(re, t0)) {
       const uint8_t* kl = L.k[buf];
       const uint8_t* vl = L.v[buf];
       float s[32];
@@ -674,7 +647,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
       }
       float f = qf * ks;
       if constexpr (MOD) {
-        modify(s, f, p.softcap, p.slopes != nullptr, slope, static_cast<float>(see.hi - t0 - 4 * half),
+        modify(s, f, p.softcap, p.slopes != nullptr, slope, static_cast<float>(at - t0),
                [](int i) { return static_cast<float>(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4); });
         f = 1.f;
       } else if ((__float_as_int(ks) ^ __float_as_int(p.scale)) < 0) {
@@ -682,11 +655,11 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
 #pragma unroll
         for (int i = 0; i < 32; ++i) s[i] = -s[i];
       }
-      if (!sees_all(re, t0, len)) {
+      if (!sees_all(re, t0, u.len)) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const int t = t0 + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
-          s[i] = t < len && sees(see, t) ? s[i] * f : NEG_INF;
+          s[i] = sees(see, t) ? s[i] * f : NEG_INF;
         }
         f = 1.f;
       }
@@ -708,27 +681,11 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
                                                           __builtin_bit_cast(f16x8_t, pw), acc[j], 0, 0, 0);
         }
       }
-      if constexpr (!I8)
-        if (cut) {  // uniform
-          const u32x4 b = *reinterpret_cast<const u32x4*>(L.nan[buf][lane]);
-          for (uint64_t bad = __ballot((b.x | b.y | b.z | b.w) != 0); bad != 0; bad &= bad - 1) {
-            const int t = __builtin_ctzll(bad);
-            const bool seen = sees(see, t0 + t);
-#pragma unroll
-            for (int j = 0; j < ND; ++j) {
-              const uint32_t x = D == 128 ? L.nan[buf][t][j] : L.nan[buf][t][2 * j] | L.nan[buf][t][2 * j + 1] << 16;
-              poison[j] |= seen ? x >> (4 * half) : 0u;  // bit 8 (i / 4) + i % 4
-            }
-          }
-        }
     }
     // the list turns after its last read of a step, 64 steps at a time; step k + 2 may be of the next 64
     list.advance(k);
     if ((k & 63) == 63) list.turn(k);
-    if (k + 1 < u.n) {
-      cut = !I8 && is_cut(k + 1);
-      stage(buf ^ 1, cut);
-    }
+    if (k + 1 < u.n) stage(buf ^ 1, !I8 && is_cut(k + 1));
     if (k + 2 < u.n) {
       if ((k & 63) == 62) {  // (its page is in nxt still)
         Pages t = list.cur;
@@ -742,14 +699,27 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
     __syncthreads();
   }
 
+  if (!I8 && busy && L.nan != 0)
+    for (int k = 0; k < u.n; ++k) {
+      const int i = u.i0 + k, b = i < u.a1 ? i : i - u.a1 + u.b0, g = list.table[b];
+      if (g < 0 || g >= p.num_pages || sees_keys(all, b * BLK, u.len)) continue;
+      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(vb + g * p.v_sb + (t - b * BLK) * p.v_st + 4 * half);
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const uint32_t z = nan_bytes(w[8 * j + i / 2]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (sees(see, t) && (z >> (8 * e + 7) & 1) != 0) acc[j][i + e] = __builtin_nanf("");
+          }
+      }
+    }
+
   // ---- results: lane holds row c32's dims 32 j + 8 (i / 4) + 4 half + i % 4
   const int i0 = 32 * wave + c32;
   const float l = swap32_sum(st.l);
-#pragma unroll
-  for (int j = 0; j < ND; ++j)
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (!I8 && (poison[j] >> (8 * (i / 4) + i % 4) & 1) != 0) acc[j][i] = __builtin_nanf("");
   if (i0 < u.nv) {
     const float mu = st.m == NEG_INF ? 0.f : st.m;
     const float x = st.ar == NEG_INF ? 0.f : fexp2((st.ar - mu) + (st.ax - 7.f));
@@ -762,15 +732,15 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   }
 }
 
-// (two workgroups a CU with large tiles, else as many as attn_decode8.hip has)
+// (two workgroups a CU: with three, 128 dims spill 40 registers, 24 tokens behind a window of 4096 63.7 us for 47.2)
 template <int D, bool I8, bool MOD, bool LARGE>
-__global__ void __launch_bounds__(NT, LARGE ? 2 : D == 64 ? 4 : 3) attend_kernel(const AttendP p) {
+__global__ void __launch_bounds__(NT, LARGE || D == 128 ? 2 : 3) attend_kernel(const AttendP p) {
   constexpr int NQ = LARGE ? TILE_FEW / 16 : 1;
   __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D, NQ>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D, NQ>)
                                                                                                         : sizeof(Many<D>)];
   const int i = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
+  const AttendUnit u = p.units[i];  // (the grid is as long as the array: not waited for twice)
   if (i >= p.head[H_UNITS]) return;
-  const AttendUnit u = p.units[i];
   if constexpr (LARGE) {
     if (u.kind & 1) {
       many_rows<D, I8, MOD>(p, u, h, *reinterpret_cast<Many<D>*>(raw));
@@ -780,13 +750,15 @@ __global__ void __launch_bounds__(NT, LARGE ? 2 : D == 64 ? 4 : 3) attend_kernel
   few_rows<D, NQ, I8, MOD>(p, u, h, *reinterpret_cast<Few<D, NQ>*>(raw));
 }
 
-// The join: workgroup (joined tile, KV head, run of 8 of its virtual rows); a wavefront finds the weights of two rows, then a
-// thread adds up four dims of a row. Rows that no request brings are cleared by the workgroups in turn.
+// The join: a workgroup takes runs of up to 8 virtual rows of a joined tile and KV head, a thread four dims of a row and a class
+// of its partial results; their first accumulators are asked for before the weights are found. Rows that no request brings are
+// cleared by the workgroups in turn.
 template <int D>
 __global__ void __launch_bounds__(NT) join_kernel(const AttendP p) {
-  constexpr int RW = 8, MOST = 2 * MAX_TILE_UNITS;
+  constexpr int RW = JOIN_ROWS, MOST = 2 * MAX_TILE_UNITS, TR = D / 4, U = 4;
   __shared__ float sW[RW][MOST];
   __shared__ float sM[RW], sL[RW];
+  __shared__ __attribute__((aligned(16))) f32x4_t sA[NT];
   const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
   const int first = p.head[H_FIRST], last = p.head[H_LAST], n_out = p.n_rows - (last - first);
   for (int i = blockIdx.x; i < n_out; i += gridDim.x) {
@@ -794,71 +766,77 @@ __global__ void __launch_bounds__(NT) join_kernel(const AttendP p) {
     for (int x = tid; x < p.Hq * (D / 8); x += NT) *reinterpret_cast<u32x4*>(p.out + n * p.Hq * D + 8 * x) = u32x4{0, 0, 0, 0};
     for (int x = tid; x < p.Hq; x += NT) p.lse[n * p.Hq + x] = NEG_INF;
   }
-  const int run = blockIdx.x % p.chunks, bh = blockIdx.x / p.chunks, h = bh % p.Hkv, j = bh / p.Hkv;
-  if (j >= p.head[H_JOINS]) return;
-  const AttendJoin o = p.joins[j];
-  const int v0 = run * RW, n = min(RW, o.nv - v0);
-  if (n <= 0) return;
-  struct Source {
-    int own, ns, more, step, n;  // partial rows own + s nv of its own pages, then more + s step of the prefix's
-  };
-  auto source = [&](int i) {
-    Source x{o.part + i, o.ns, 0, 0, o.ns};
-    if (o.sv0 >= 0) {
-      const int v = o.sv0 + i, t = o.tile0 + v / o.height;
-      const AttendTile y = p.tiles[t];
-      x.step = y.nv;
-      x.more = y.part + v % o.height;
-      x.n += y.ns;
-    }
-    return x;
-  };
-  auto row_at = [&](const Source& x, int s) { return static_cast<int64_t>(s < x.ns ? x.own + s * o.nv : x.more + (s - x.ns) * x.step); };
+  const int total = p.head[H_JOINS] * p.Hkv;
+  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    const int h = w % p.Hkv;
+    const AttendJoin o = p.joins[w / p.Hkv];
+    // partial result s of row i: own pages' first, then the prefix's
+    const int np = o.ns + o.more_ns;
+    auto at = [&](int i, int s) {
+      const int r = s < o.ns ? o.part + i + s * o.step : o.more + i + (s - o.ns) * o.more_step;
+      return static_cast<int64_t>(r) * p.Hkv + h;
+    };
+    const int R = o.n > 4 ? 8 : o.n > 2 ? 4 : o.n;      // rows side by side, NC classes of partials
+    const int NC = NT / TR / R, i = tid / TR % R, cls = tid / TR / R, d = tid % TR * 4;
+    const bool row = i < o.n;
+    auto load = [&](int s) {
+      return row && s < np ? *reinterpret_cast<const f32x4_t*>(p.part_acc + at(i, s) * D + d) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    };
+    f32x4_t x[U];
 #pragma unroll
-  for (int g = 0; g < RW / NWAVE; ++g) {
-    const int i = wave + NWAVE * g;
-    if (i < n) {  // uniform
-      const Source x = source(v0 + i);
-      float m[MOST / WAVE], l[MOST / WAVE], M = NEG_INF, L = 0.f;
+    for (int e = 0; e < U; ++e) x[e] = load(cls + NC * e);
 #pragma unroll
-      for (int e = 0; e < MOST / WAVE; ++e) {
-        const int s = lane + WAVE * e;
-        m[e] = NEG_INF, l[e] = 0.f;
-        if (s < x.n) {
-          const float2 t = *reinterpret_cast<const float2*>(p.part_ml + (row_at(x, s) * p.Hkv + h) * 2);
-          m[e] = t.x, l[e] = t.y;
+    for (int g = 0; g < RW / NWAVE; ++g) {
+      const int j = wave + NWAVE * g;
+      if (j < o.n) {  // uniform
+        float m[MOST / WAVE], l[MOST / WAVE], M = NEG_INF, L = 0.f;
+#pragma unroll
+        for (int e = 0; e < MOST / WAVE; ++e) {
+          const int s = lane + WAVE * e;
+          m[e] = NEG_INF, l[e] = 0.f;
+          if (s < np) {
+            const float2 t = *reinterpret_cast<const float2*>(p.part_ml + at(j, s) * 2);
+            m[e] = t.x, l[e] = t.y;
+          }
+          M = fmaxf(M, m[e]);
         }
-        M = fmaxf(M, m[e]);
-      }
-      M = wave_max(M);
-      const float mu = M == NEG_INF ? 0.f : M;
+        M = wave_max(M);
+        const float mu = M == NEG_INF ? 0.f : M;
 #pragma unroll
-      for (int e = 0; e < MOST / WAVE; ++e) {
-        const int s = lane + WAVE * e;
-        const float w = l[e] == 0.f ? 0.f : fexp2(m[e] - mu);
-        L += l[e] * w;
-        if (s < x.n) sW[i][s] = l[e] == 0.f ? -1.f : w;  // (an empty partial counts for nothing, a NaN counts)
+        for (int e = 0; e < MOST / WAVE; ++e) {
+          const int s = lane + WAVE * e;
+          const float v = l[e] == 0.f ? 0.f : fexp2(m[e] - mu);
+          L += l[e] * v;
+          if (s < np) sW[j][s] = l[e] == 0.f ? -1.f : v;  // (an empty partial counts for nothing, a NaN counts)
+        }
+        L = wave_sum(L);
+        if (lane == 0) sM[j] = M, sL[j] = L;
       }
-      L = wave_sum(L);
-      if (lane == 0) sM[i] = M, sL[i] = L;
     }
-  }
-  __syncthreads();
-  constexpr int TR = D / 4;  // threads of a row
-  for (int e = tid; e < n * TR; e += NT) {
-    const int i = e / TR, d = e % TR * 4;
-    const Source x = source(v0 + i);
+    __syncthreads();
     f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < x.n; ++s) {
-      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p.part_acc + (row_at(x, s) * p.Hkv + h) * D + d);
-      const float w = sW[i][s];
-      if (w != -1.f) a += y * w;
+    for (int s0 = cls; s0 < np; s0 += NC * U) {
+      f32x4_t y[U];  // the next round's, asked for before this one's are added
+#pragma unroll
+      for (int e = 0; e < U; ++e) y[e] = load(s0 + NC * (U + e));
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const float v = row && s0 + NC * e < np ? sW[i][s0 + NC * e] : -1.f;
+        if (v != -1.f) a += x[e] * v;
+      }
+#pragma unroll
+      for (int e = 0; e < U; ++e) x[e] = y[e];
     }
-    const int v = o.v0 + v0 + i, r = v / p.G;
-    AttendUnit u{};
-    u.part = -1;
-    store4(p, u, h, 0, Row{o.row0 + r, h * p.G + (v - r * p.G), 0, 0}, d, D, a, sM[i], sL[i]);
+    sA[tid] = a;
+    __syncthreads();
+    if (cls == 0 && row) {
+      for (int c = 1; c < NC; ++c) a += sA[tid + c * R * TR];
+      const int v = o.v0 + i, r = v / p.G;
+      AttendUnit u{};
+      u.part = -1;
+      store4(p, u, h, 0, Row{o.row0 + r, h * p.G + (v - r * p.G), 0, 0}, d, D, a, sM[i], sL[i]);
+    }
+    __syncthreads();
   }
 }
 
@@ -897,18 +875,16 @@ hipError_t launch_attend(const kvskip_attend_args& a, const AttendSizes& z, hipS
   p.head = work;
   p.units = reinterpret_cast<const AttendUnit*>(work + z.at_units);
   p.joins = reinterpret_cast<const AttendJoin*>(work + z.at_joins);
-  p.tiles = reinterpret_cast<const AttendTile*>(work + z.at_tiles);
   p.rows = reinterpret_cast<const AttendRow*>(work + z.at_rows);
   p.n_rows = a.plan.rows, p.Hq = a.plan.Hq, p.Hkv = a.plan.Hkv, p.G = a.plan.Hq / a.plan.Hkv;
   p.num_pages = a.num_pages, p.window = a.plan.window < (1 << 30) ? a.plan.window : 1 << 30;
   p.scale = a.scale, p.softcap = a.softcap;
-  const int tall = z.large ? z.many : z.few;
-  p.chunks = (tall + 7) / 8;
   const bool i8 = a.format == KVSKIP_INT8;
   const hipError_t e = a.D == 128 ? (i8 ? launch_d<128, true>(p, z, s) : launch_d<128, false>(p, z, s))
                                   : (i8 ? launch_d<64, true>(p, z, s) : launch_d<64, false>(p, z, s));
   if (e != hipSuccess) return e;
-  const dim3 grid(static_cast<uint32_t>(z.own * p.Hkv * p.chunks));
+  const int64_t joins = z.joins * p.Hkv;
+  const dim3 grid(static_cast<uint32_t>(joins < JOIN_GRID ? joins : JOIN_GRID));
   if (a.D == 128)
     hipLaunchKernelGGL(join_kernel<128>, grid, dim3(NT), 0, s, p);
   else

@@ -35,17 +35,19 @@ struct alignas(16) AttendUnit {
 };
 static_assert(sizeof(AttendUnit) == 64, "a unit is one line");
 
-struct alignas(16) AttendJoin {
-  int row0, v0, nv;
-  int part, ns;      // partial results of the request's own pages: ns times nv rows
-  int sv0;           // the first virtual row's place among those of its shared prefix, -1: none
-  int tile0, height; // the prefix's first tile, and a tile's rows
+
+constexpr int JOIN_ROWS = 8;
+struct alignas(16) AttendJoin {  // a run of virtual rows whose partial results are added up
+  int row0, v0, n;               // first row of the request; virtual rows [v0, v0 + n)
+  int part, ns, step;            // partial rows part + i + s step of row v0 + i, s < ns: over its own pages
+  int more, more_ns, more_step;  // and over its shared prefix's
+  int spare[3];
 };
 
 struct AttendRow {  // a row behind a shared prefix
   int row, pos, pre, spare;
 };
-struct alignas(16) AttendTile {  // scratch of the plan; those over a shared prefix are read by the join
+struct alignas(16) AttendTile {  // scratch of the plan
   int who, v0, pages, part;
   int nv, ns, spare[2];
 };
@@ -54,7 +56,7 @@ struct alignas(16) AttendTile {  // scratch of the plan; those over a shared pre
 struct AttendSizes {  // (host)
   bool large;        // large tiles occur
   int few, many;     // heights
-  int64_t tiles, own, units, part_rows;
+  int64_t tiles, joins, units, part_rows;
   int64_t at_units, at_joins, at_tiles, at_rows, total;
 };
 

@@ -4,7 +4,7 @@
 //   1. a request's tiles are counted and summed (LDS holds every request's first tile), a shared prefix's rows listed;
 //   2. every tile finds its pages: [0, a1) that prefix_lens shows it and [b0, ...) up to its last row, from its first
 //      row's window on; the pages' sum gives the chunk that a unit takes;
-//   3. partial rows, joins and units are counted in tile order, so that results never depend on when a workgroup ran;
+//   3. partial rows and the runs of rows to join are counted in tile order, so that results never depend on when a workgroup ran;
 //   4. units are written longest first, by a counting sort over 32 classes of length (their order inside a class is
 //      whatever the atomics gave: it decides when a unit starts and nothing else).
 // Every record lies inside its array by attend_sizes' bounds: a row belongs to one request, so tiles are at most the rows' share
@@ -20,9 +20,11 @@ namespace {
 constexpr int PT = 1024;  // threads
 constexpr int CLASSES = 32;
 
-// Units that fill the GPU: two workgroups a CU, and twice as many again so that those that end early make room.
-constexpr int TARGET_UNITS = 1024;
-constexpr int LEAST_PAGES = 4;  // of a unit: its four wavefronts take a page each
+// Workgroups that run at once: two a CU. (Units for one round of them, 24 tokens of up to 20011 behind a window of 4096: 47.1 us
+// with 1024 units in about two rounds, 39.0; 16 tokens of up to 32000 54.3, 47.4; one of 32768 33.9, 24.0.)
+constexpr int SLOTS = 512;
+constexpr int TARGET_UNITS = 2 * SLOTS;  // units of a queued plan: those that end early take another
+constexpr int LEAST_PAGES = 4;           // of a unit: its four wavefronts take a page each
 
 struct PlanP {
   kvskip_attend_plan_args a;
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
   __shared__ Group sGr[MAX_SHARED];
   __shared__ int sW[PT / WAVE];
   __shared__ int sClass[CLASSES];
-  __shared__ int sMost;
+  __shared__ int sMost, sFit;
   const int tid = threadIdx.x, G = p.a.Hq / p.a.Hkv, window = p.a.window;
   int* work = p.a.work;
   AttendUnit* units = reinterpret_cast<AttendUnit*>(work + p.at_units);
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
 
   // ---- 1. requests (starts that do not rise would give rows to two of them: then no row belongs to any)
   if (tid < CLASSES) sClass[tid] = 0;
-  if (tid == 0) sMost = 1;
+  if (tid == 0) sMost = 1, sFit = INT32_MAX;
   bool fall = false;
   for (int b = tid; b < p.a.B; b += PT) fall |= p.a.starts[b + 1] < p.a.starts[b];
   const int B = __syncthreads_or(fall) ? 0 : p.a.B;
@@ -202,24 +204,34 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
   __syncthreads();
   atomicAdd(&sSum, static_cast<unsigned long long>(sum));
   __syncthreads();
-  const int64_t work_pages = static_cast<int64_t>(sSum) * p.a.Hkv;
-  const int chunk = static_cast<int>(max(static_cast<int64_t>(LEAST_PAGES), (work_pages + TARGET_UNITS - 1) / TARGET_UNITS));
+  // the shortest of 16 chunks whose units all run at once, or where there is none a queue's
+  const int64_t all_pages = static_cast<int64_t>(sSum);
+  const int room = max(SLOTS / p.a.Hkv, 1);
+  if (n_tiles <= room) {  // uniform
+    const int wave = tid / WAVE, c0 = static_cast<int>(max(static_cast<int64_t>(LEAST_PAGES), (all_pages + room - 1) / room));
+    const int c = c0 + (c0 * wave + PT / WAVE - 1) / (PT / WAVE);
+    int n = 0;
+    for (int t = tid % WAVE; t < n_tiles; t += WAVE) n += (tiles[t].pages + c - 1) / c;
+    if (wave_sum_int(n) <= room && tid % WAVE == 0) atomicMin(&sFit, c);
+  }
+  __syncthreads();
+  const int queued = static_cast<int>(max(static_cast<int64_t>(LEAST_PAGES), (all_pages * p.a.Hkv + TARGET_UNITS - 1) / TARGET_UNITS));
+  const int chunk = sFit != INT32_MAX ? sFit : queued;
   auto cut = [&](int pages) { return min(max((pages + chunk - 1) / chunk, 1), MAX_TILE_UNITS); };
 
-  // ---- 3. partial rows and joins in tile order; the longest unit
-  int parts = 0, n_joins = 0;
+  // ---- 3. partial rows in tile order; the longest unit
+  int parts = 0;
   for (int t0 = 0; t0 < n_tiles; t0 += PT) {
     const int t = t0 + tid;
-    int nv = 0, ns = 0, group = -1;
-    Request r{};
-    AttendTile x{};
+    int nv = 0, ns = 0;
     bool partial = false;
     if (t < n_tiles) {
-      x = tiles[t];
+      const AttendTile x = tiles[t];
+      int virt, group;
       if (x.who >= 0) {
-        r = request(p, x.who);
-        group = r.group;
-        nv = min(height(p, r.n * G), r.n * G - x.v0);
+        const Request r = request(p, x.who);
+        virt = r.n * G, group = r.group;
+        nv = min(height(p, virt), virt - x.v0);
       } else {
         group = ~x.who;
         nv = min(sGr[group].height, sGr[group].rows * G - x.v0);
@@ -231,21 +243,44 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
     int total;
     const int at = parts + block_scan(partial ? nv * ns : 0, sW, total);
     parts += total;
-    const bool join = partial && x.who >= 0;
-    const int j = n_joins + block_scan(join ? 1 : 0, sW, total);
-    n_joins += total;
     if (t < n_tiles) tiles[t].part = partial ? at : -1, tiles[t].nv = nv, tiles[t].ns = ns;
-    if (join) {
-      AttendJoin o{r.first, x.v0, nv, at, ns, -1, 0, 1};
-      if (group >= 0) {
-        o.sv0 = sPlace[x.who] * G + x.v0;
-        o.tile0 = sGr[group].tile0;
-        o.height = sGr[group].height;
-      }
-      joins[j] = o;
-    }
   }
-  __syncthreads();
+  __syncthreads();  // (the joins read the tiles of a prefix, other threads')
+  // runs of rows to join: up to JOIN_ROWS of a tile, of one tile of the prefix
+  int n_joins = 0;
+  for (int t0 = 0; t0 < own; t0 += PT) {
+    const int t = t0 + tid;
+    AttendTile x{};
+    int group = -1, place = 0, runs = 0;
+    Request r{};
+    if (t < own) {
+      x = tiles[t];
+      if (x.part >= 0) {
+        r = request(p, x.who);
+        group = r.group;
+        place = group >= 0 ? sPlace[x.who] * G + x.v0 : 0;
+      }
+    }
+    auto run = [&](int i) {  // length of the one at row i
+      const int n = min(x.nv - i, JOIN_ROWS);
+      return group >= 0 ? min(n, sGr[group].height - (place + i) % sGr[group].height) : n;
+    };
+    if (x.part >= 0 && t < own)
+      for (int i = 0; i < x.nv; i += run(i)) ++runs;
+    int total;
+    int j = n_joins + block_scan(runs, sW, total);
+    n_joins += total;
+    if (runs > 0)
+      for (int i = 0; i < x.nv; i += run(i), ++j) {
+        AttendJoin o{r.first, x.v0 + i, run(i), x.part + i, x.ns, x.nv, 0, 0, 0, {0, 0, 0}};
+        if (group >= 0) {
+          const int v = place + i, h = sGr[group].height;
+          const AttendTile y = tiles[sGr[group].tile0 + v / h];
+          o.more = y.part + v % h, o.more_ns = y.ns, o.more_step = y.nv;
+        }
+        joins[j] = o;
+      }
+  }
   // ---- 4. units, longest first
   const int most = sMost;
   auto cls = [&](int pages, int ns) {
@@ -320,8 +355,9 @@ AttendSizes attend_sizes(const kvskip_attend_plan_args& p) {
   z.many = z.large ? TILE_MANY : 0;
   // a small tile holds a whole request where large ones occur, so a batch has at most one short tile a request
   const int64_t h = z.large ? z.many : z.few;
-  z.own = virt / h + p.B;
-  z.tiles = z.own + (p.shared > 0 ? virt / h + p.shared : 0);
+  z.tiles = virt / h + p.B + (p.shared > 0 ? virt / h + p.shared : 0);
+  // a run a JOIN_ROWS rows, one more a tile, and one more where a tile of a prefix ends inside it
+  z.joins = virt / JOIN_ROWS + z.tiles;
   const int64_t cut = TARGET_UNITS / p.Hkv + 1;  // units beyond one a tile: the sum of floor(pages / chunk)
   z.units = z.tiles + cut;
   const int64_t tall = virt < h ? virt : h;
@@ -329,7 +365,7 @@ AttendSizes attend_sizes(const kvskip_attend_plan_args& p) {
   auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
   z.at_units = HEAD;
   z.at_joins = z.at_units + up(z.units * (sizeof(AttendUnit) / 4));
-  z.at_tiles = z.at_joins + up(z.tiles * (sizeof(AttendJoin) / 4));
+  z.at_tiles = z.at_joins + up(z.joins * (sizeof(AttendJoin) / 4));
   z.at_rows = z.at_tiles + up(z.tiles * (sizeof(AttendTile) / 4));
   z.total = z.at_rows + (p.shared > 0 ? up(static_cast<int64_t>(p.rows) * (sizeof(AttendRow) / 4)) : 0);
   return z;
