@@ -129,9 +129,30 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& any) {
   return w & ~((z >> 7) * 0xffu);
 }
 
-// Running state of a row: maximum and sum (log2 units; the sum is this lane's part), and the accumulators' reference ar + ax.
+// Running state of a row. m: a score in log2 units at most 2^4 below its largest so far, l: this lane's part of sum 2^(s - m).
+// ar + ax: the accumulators' reference, a score and the exponent of its page's vs (apart, since in one float a large score takes
+// the exponent's bits); p |vs| passes 2^(ar + ax) by at most 2^7. c and d: 7 - ax - ar and ar + ax - 7 - m. All of it but l
+// changes only where a page's largest score passes what it may.
 struct State {
-  float m = NEG_INF, l = 0.f, ar = NEG_INF, ax = 0.f;
+  float m = NEG_INF, l = 0.f, ar = NEG_INF, ax = 0.f, c = 0.f, d = 0.f;
+};
+// What a wavefront's rows share: the largest exponent of vs so far; a reference has passed 2^10.
+struct Common {
+  int top = -1000;
+  bool odd = false;
+};
+// A page's vs. plain: a positive number of middling size, and not 2^40 below another one.
+struct Weight {
+  float vs, lv, ev;
+  bool plain;
+  __device__ Weight(float v, Common& w) : vs(v) {
+    const int e = static_cast<int>(__float_as_uint(v) >> 23);  // (a negative one from 256 on)
+    const int x = max((e & 0xff) - 127, -100);
+    w.top = max(w.top, x);
+    plain = e >= 27 && e <= 227 && x >= w.top - 40 && !w.odd;
+    lv = flog2(v);
+    ev = static_cast<float>(x);
+  }
 };
 
 // Capped and biased scores, in log2 units, of raw products s times f (a score in natural units): tanh y as
@@ -168,46 +189,76 @@ __device__ __forceinline__ void modify(float (&s)[N], float f, float cap, bool b
   }
 }
 
-// One page of a row: s in, e = weights relative to the reference out (as fp16 pairs, tokens in order). f >= 0: s f is the
-// score in log2 units. The row's maximum is taken over `swap`'s lanes. Returns the factor of the accumulators.
-template <int N, class F>
-__device__ __forceinline__ bool soften(float (&s)[N], float f, float vs, State& st, float& alpha, uint32_t (&w)[N / 2], F&& swap) {
+// (v_maximum3_f32: half the instructions of fmaxf, which makes each operand canonical first)
+template <int N>
+__device__ __forceinline__ float most_of(const float (&s)[N]) {
   float x = s[0];
 #pragma unroll
-  for (int i = 1; i < N; ++i) x = fmaxf(x, s[i]);
-  const float mt = swap(x) * f;
-  const float mtu = mt == NEG_INF ? 0.f : mt;
-  // (scores so large that mt's rounding would show in s f - mt: rounded alike)
-  if (__ballot(fabsf(mtu) > 0x1p17f) != 0) {
+  for (int i = 1; i < N; ++i) x = __builtin_elementwise_maximum(x, s[i]);
+  return x;
+}
+template <int N>
+__device__ __forceinline__ float least_of(const float (&s)[N]) {
+  float x = s[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] *= f;
-    f = 1.f;
-  }
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    s[i] = fexp2(fmaf(s[i], f, -mtu));
-    sum[i % 4] += s[i];
-  }
-  const float m_new = fmaxf(st.m, mt);
-  const float mu = m_new == NEG_INF ? 0.f : m_new;
-  const float cf = mt == NEG_INF ? 0.f : fexp2(mt - mu);
-  st.l = st.l * fexp2(st.m - mu) + ((sum[0] + sum[1]) + (sum[2] + sum[3])) * cf;
-  st.m = m_new;
-  const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(vs) >> 23 & 0xffu) - 127, -100));
-  const float past = (mt - st.ar) + (ev - st.ax);  // (NaN, which passes nothing, where nothing came yet)
-  const bool move = __ballot(past > 7.f) != 0;
+  for (int i = 1; i < N; ++i) x = __builtin_elementwise_minimum(x, s[i]);
+  return x;
+}
+
+// One page of a row: s in, w = 2^7 p vs / 2^(ar + ax) as fp16 pairs out, tokens in order; s f is the score in log2 units (neg: f <
+// 0), its maximum over `swap`'s lanes the row's. alpha: the factor of the accumulators, true if it is not 1 for all.
+//   The plain way takes 2^(s f + c + log2 vs) at once, from which l is found too: an fma, an exponential, a sum and half a
+// conversion a score. Its one rounding more, of c + log2 vs, is 2^-14 at most where no reference passes 2^10; and no weight that
+// l could feel is below 2^-126: a page's largest score that is at most 2^60 below m lies at most 2^64 below ar, and vs at
+// most 2^40 below 2^ax. Elsewhere weights are taken relative to the page's largest score and multiplied by their factor.
+template <int N, class F>
+__device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const Weight& v, State& st, Common& com, float& alpha,
+                                       uint32_t (&w)[N / 2], F&& swap) {
+  const float mt = neg ? swap(-least_of(s)) * -f : swap(most_of(s)) * f;
+  const float past = (mt - st.ar) + (v.ev - st.ax);  // (NaN, which passes nothing, where nothing came yet)
+  const bool move = __ballot((past > 7.f) | (mt > st.m + 4.f)) != 0;
   alpha = 1.f;
   if (move) {
     const bool on = past > 0.f;
     alpha = on ? fexp2(-past) : 1.f;
     st.ar = on ? mt : st.ar;
-    st.ax = on ? ev : st.ax;
+    st.ax = on ? v.ev : st.ax;
+    const float m = fmaxf(st.m, mt), mu = m == NEG_INF ? 0.f : m;
+    st.l *= fexp2(st.m - mu);
+    st.m = m;
+    const bool none = st.ar == NEG_INF;
+    st.c = none ? 0.f : (7.f - st.ax) - st.ar;
+    st.d = none ? 0.f : ((st.ar - mu) + st.ax) - 7.f;
+    com.odd |= __ballot(!none & (fabsf(st.ar) > 0x1p10f)) != 0;
   }
-  // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
-  const float fv = mt == NEG_INF ? 0.f : vs * fexp2((mt - st.ar) - st.ax) * 0x1p7f;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (v.plain & !com.odd) {  // uniform
+    const float c = st.c + v.lv;
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) w[i] = pack_h(s[2 * i] * fv, s[2 * i + 1] * fv);
+    for (int i = 0; i < N; i += 2) {
+      const float x = fexp2(fmaf(s[i], f, c)), y = fexp2(fmaf(s[i + 1], f, c));
+      sum[i % 4] += x, sum[i % 4 + 1] += y;
+      w[i / 2] = pack_h(x, y);
+    }
+    st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), fexp2(st.d - v.lv), st.l);
+  } else {
+    const float mtu = mt == NEG_INF ? 0.f : mt;
+    // (scores so large that mt's rounding would show in s f - mt: rounded alike)
+    if (__ballot(fabsf(mtu) > 0x1p17f) != 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] *= f;
+      f = 1.f;
+    }
+    // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
+    const float fv = mt == NEG_INF ? 0.f : v.vs * fexp2((mt - st.ar) - st.ax) * 0x1p7f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float x = fexp2(fmaf(s[i], f, -mtu)), y = fexp2(fmaf(s[i + 1], f, -mtu));
+      sum[i % 4] += x, sum[i % 4 + 1] += y;
+      w[i / 2] = pack_h(x * fv, y * fv);
+    }
+    st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), mt == NEG_INF ? 0.f : fexp2(mt - st.m), st.l);
+  }
   return move;
 }
 
@@ -313,6 +364,17 @@ __device__ __forceinline__ void store4(const AttendP& p, const AttendUnit& u, in
   if (d == 0) p.lse[at] = l == 0.f ? NEG_INF : (m + flog2(l)) * LN2;
 }
 
+// NaN over those of a stored row's four dims that have 0x80 in z.
+__device__ __forceinline__ void store_nan(const AttendP& p, const AttendUnit& u, int h, int i, const Row& r, int d, int D, uint32_t z) {
+  for (int e = 0; e < 4; ++e)
+    if (z >> (8 * e + 7) & 1) {
+      if (u.part >= 0)
+        p.part_acc[(static_cast<int64_t>(u.part + i) * p.Hkv + h) * D + d + e] = __builtin_nanf("");
+      else
+        p.out[(static_cast<int64_t>(r.n) * p.Hq + r.hq) * D + d + e] = 0x7fc0;
+    }
+}
+
 // ---- Few rows: four independent wavefronts, a page a step each, no barrier but the one before their states are joined. Keys
 // come from memory as operands and become fp16 in registers (the layouts of attn_decode8.hip), 16 rows a product.
 template <int D, int NQ>
@@ -347,6 +409,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
   Sight see[NQ];
   int at[NQ];  // the row's own index, less the lane's first token
   State st[NQ];
+  Common com;
   Reach re;
 #pragma unroll
   for (int a = 0; a < NQ; ++a) {
@@ -411,18 +474,17 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
         for (int i = 0; i < VN; ++i) vr[i] = u32x2{without_nan(vr[i].x, any), without_nan(vr[i].y, any)};
         nan |= __ballot(any != 0) != 0;
       }
+    const Weight wt(vs, com);
     uint32_t w[NQ][8];
 #pragma unroll
     for (int a = 0; a < NQ; ++a) {
       float f = qf[a] * ks;
+      bool neg = (__float_as_int(ks) ^ __float_as_int(p.scale)) < 0;  // uniform
       if constexpr (MOD) {
         modify(s[a], f, p.softcap, p.slopes != nullptr, slope[a], static_cast<float>(at[a] - t0),
                [](int i) { return static_cast<float>(16 * (i / 4) + i % 4); });
         f = 1.f;
-      } else if ((__float_as_int(ks) ^ __float_as_int(p.scale)) < 0) {  // uniform: f made positive
-        f = -f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[a][i] = -s[a][i];
+        neg = false;
       }
       if (!whole || pg < 0) {  // uniform
 #pragma unroll
@@ -430,10 +492,10 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
           const int t = t0 + mf_tok(i / 4, i % 4, j4);
           s[a][i] = sees(see[a], t) & (pg >= 0) ? s[a][i] * f : NEG_INF;
         }
-        f = 1.f;
+        f = 1.f, neg = false;
       }
       float alpha;
-      if (soften(s[a], f, vs, st[a], alpha, w[a], [](float x) { return swap_max(x); }))
+      if (soften(s[a], f, neg, wt, st[a], com, alpha, w[a], [](float x) { return swap_max(x); }))
 #pragma unroll
         for (int j = 0; j < VD; ++j) acc[a][j] *= alpha;
     }
@@ -465,26 +527,6 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
     pg = pg_n;
   }
 
-  if (!I8 && nan)
-    for (int k = 0; k < nw; ++k) {
-      const int i0 = u.i0 + wave + NWAVE * k, b = i0 < u.a1 ? i0 : i0 - u.a1 + u.b0, g = list.table[b];
-      if (g < 0 || g >= p.num_pages || sees_keys(re, b * BLK, u.len)) continue;
-      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(vb + g * p.v_sb + (t - b * BLK) * p.v_st + mf_vdim<D>(4 * j4 + i));
-#pragma unroll
-          for (int j = 0; j < VD; j += 4) {
-            const uint32_t z = nan_bytes(w[j / 4]);
-#pragma unroll
-            for (int a = 0; a < NQ; ++a)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (sees(see[a], t) && (z >> (8 * e + 7) & 1) != 0) acc[a][j + e][i] = __builtin_nanf("");
-          }
-        }
-    }
-
   // ---- the four states joined: lane (c16, j4) holds row c16's dims mf_vdim(4 j4 + i) + j
 #pragma unroll
   for (int a = 0; a < NQ; ++a) {
@@ -503,6 +545,19 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
       L.x[wave][row] = st[a].ar == NEG_INF ? NEG_INF : (st[a].ar - mu) + (st[a].ax - 7.f);
     }
   }
+  if (!I8 && nan)  // NaN of cut pages
+    for (int k = 0; k < nw; ++k) {
+      const int i0 = u.i0 + wave + NWAVE * k, b = i0 < u.a1 ? i0 : i0 - u.a1 + u.b0, g = list.table[b];
+      if (g < 0 || g >= p.num_pages || sees_keys(re, b * BLK, u.len)) continue;
+      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t)
+        for (int d = 4 * j4; d < D; d += 16) {
+          const uint32_t z = nan_bytes(*reinterpret_cast<const uint32_t*>(vb + g * p.v_sb + (t - b * BLK) * p.v_st + d));
+#pragma unroll
+          for (int a = 0; a < NQ; ++a)
+            for (int e = 0; e < 4; ++e)
+              if (sees(see[a], t) && (z >> (8 * e + 7) & 1) != 0) L.acc[wave][16 * a + c16][d + e] = __builtin_nanf("");
+        }
+    }
   __syncthreads();
   for (int o = tid; o < u.nv * (D / 4); o += NT) {
     const int row = o / (D / 4), d = o % (D / 4) * 4;
@@ -524,7 +579,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 // ---- Many rows: the four wavefronts hold 32 rows each and read the same pages, fp16 in LDS, two at a time: while one is
 // multiplied the next one's codes are on their way and converted, once for all rows. 32 x 32 products: K as it lies in
 // LDS, V by transposing reads. Chunks of 16 bytes are placed so that neither reads nor writes conflict: K chunk c of
-// row r at c ^ r, V's at c ^ 4 (r % 4) (64 dims: r / 2 in both).
+// row r at c ^ r, V's at c ^ 5 (r % 4) (64 dims: r / 2 in both).
 template <int D>
 struct Many {
   uint8_t k[2][BLK * D * 2], v[2][BLK * D * 2];
@@ -545,7 +600,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   // staging: thread t holds 16 NC codes of row t / 4
   const uint32_t srow = tid >> 2, sc = 2 * NC * (tid & 3);  // its first 16-byte chunk in LDS
   const uint32_t kso = srow * p.k_st + 16 * NC * (tid & 3), vso = srow * p.v_st + 16 * NC * (tid & 3);
-  const uint32_t kx = D == 128 ? srow & 15 : (srow >> 1) & 7, vx = D == 128 ? (srow & 3) << 2 : ((srow >> 1) & 1) << 2;
+  const uint32_t kx = D == 128 ? srow & 15 : (srow >> 1) & 7, vx = 5 * (D == 128 ? srow & 3 : (srow >> 1) & 1);
   u32x4 kc[NC], vc[NC];
   auto fetch = [&](int k) {
     const int blk = k < u.n ? list.blk(k) : -1, pg = k < u.n ? list.pg(k) : -1, n = rows_of(blk, pg);
@@ -600,6 +655,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   const int at = r.pos - u.base - 4 * half;
   const float slope = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
   State st;
+  Common com;
   f32x16_t acc[ND];
 #pragma unroll
   for (int j = 0; j < ND; ++j)
@@ -608,7 +664,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   // operand addresses: K chunk 2 x + half of row c32 (step x: ^ 32 x), V dims 32 j + .. of a group's rows (tile j: ^ 64 j)
   const uint32_t ka = c32 * ROW + ((half ^ (D == 128 ? c32 & 15 : (c32 >> 1) & 7)) << 4);
   const uint32_t vrow = 4 * half + ((lane & 15) >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const uint32_t va = vrow * ROW + ((vch ^ (D == 128 ? (vrow & 3) << 2 : ((vrow >> 1) & 1) << 2)) << 4) + 8 * (lane & 1);
+  const uint32_t va = vrow * ROW + ((vch ^ 5 * (D == 128 ? vrow & 3 : (vrow >> 1) & 1)) << 4) + 8 * (lane & 1);
 
   Reach all = re;
   if constexpr (!I8) {  // of the whole tile
@@ -617,6 +673,8 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NWAVE; ++w) all = both(all, L.reach[w]);
+    for (int* x : {&all.from_min, &all.from_max, &all.end_min, &all.end_max, &all.pre_min, &all.pre_max})
+      *x = __builtin_amdgcn_readfirstlane(*x);
   }
   auto is_cut = [&](int k) { return !sees_keys(all, list.blk(k) * BLK, u.len); };
   stage(0, !I8 && u.n > 0 && is_cut(0));
@@ -646,14 +704,11 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
         for (int i = 0; i < 16; ++i) s[16 * kt + i] = c[i];
       }
       float f = qf * ks;
+      bool neg = (__float_as_int(ks) ^ __float_as_int(p.scale)) < 0;  // uniform
       if constexpr (MOD) {
         modify(s, f, p.softcap, p.slopes != nullptr, slope, static_cast<float>(at - t0),
                [](int i) { return static_cast<float>(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4); });
-        f = 1.f;
-      } else if ((__float_as_int(ks) ^ __float_as_int(p.scale)) < 0) {
-        f = -f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) s[i] = -s[i];
+        f = 1.f, neg = false;
       }
       if (!sees_all(re, t0, u.len)) {
 #pragma unroll
@@ -661,11 +716,11 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
           const int t = t0 + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
           s[i] = sees(see, t) ? s[i] * f : NEG_INF;
         }
-        f = 1.f;
+        f = 1.f, neg = false;
       }
       uint32_t w[16];
       float alpha;
-      if (soften(s, f, vs, st, alpha, w, [](float x) { return swap32_max(x); }))
+      if (soften(s, f, neg, Weight(vs, com), st, com, alpha, w, [](float x) { return swap32_max(x); }))
 #pragma unroll
         for (int j = 0; j < ND; ++j) acc[j] *= alpha;
 #pragma unroll
@@ -699,43 +754,35 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
     __syncthreads();
   }
 
-  if (!I8 && busy && L.nan != 0)
-    for (int k = 0; k < u.n; ++k) {
-      const int i = u.i0 + k, b = i < u.a1 ? i : i - u.a1 + u.b0, g = list.table[b];
-      if (g < 0 || g >= p.num_pages || sees_keys(all, b * BLK, u.len)) continue;
-      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(vb + g * p.v_sb + (t - b * BLK) * p.v_st + 4 * half);
-#pragma unroll
-        for (int j = 0; j < ND; ++j)
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const uint32_t z = nan_bytes(w[8 * j + i / 2]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (sees(see, t) && (z >> (8 * e + 7) & 1) != 0) acc[j][i + e] = __builtin_nanf("");
-          }
-      }
-    }
-
   // ---- results: lane holds row c32's dims 32 j + 8 (i / 4) + 4 half + i % 4
   const int i0 = 32 * wave + c32;
   const float l = swap32_sum(st.l);
-  if (i0 < u.nv) {
-    const float mu = st.m == NEG_INF ? 0.f : st.m;
-    const float x = st.ar == NEG_INF ? 0.f : fexp2((st.ar - mu) + (st.ax - 7.f));
+  if (i0 >= u.nv) return;
+  const float mu = st.m == NEG_INF ? 0.f : st.m;
+  const float x = st.ar == NEG_INF ? 0.f : fexp2((st.ar - mu) + (st.ax - 7.f));
 #pragma unroll
-    for (int j = 0; j < ND; ++j)
+  for (int j = 0; j < ND; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        store4(p, u, h, i0, r, 32 * j + 2 * i + 4 * half, D,
-               f32x4_t{acc[j][i] * x, acc[j][i + 1] * x, acc[j][i + 2] * x, acc[j][i + 3] * x}, st.m, l);
+    for (int i = 0; i < 16; i += 4)
+      store4(p, u, h, i0, r, 32 * j + 2 * i + 4 * half, D,
+             f32x4_t{acc[j][i] * x, acc[j][i + 1] * x, acc[j][i + 2] * x, acc[j][i + 3] * x}, st.m, l);
+  if (I8 || L.nan == 0) return;
+  // NaN of cut pages over what was stored
+  for (int k = 0; k < u.n; ++k) {
+    const int i = u.i0 + k, b = i < u.a1 ? i : i - u.a1 + u.b0, g = list.table[b];
+    if (g < 0 || g >= p.num_pages || sees_keys(all, b * BLK, u.len)) continue;
+    for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t) {
+      if (!sees(see, t)) continue;
+      const uint8_t* row = vb + g * p.v_sb + (t - b * BLK) * p.v_st;
+      for (int d = 4 * half; d < D; d += 8) store_nan(p, u, h, i0, r, d, D, nan_bytes(*reinterpret_cast<const uint32_t*>(row + d)));
+    }
   }
 }
 
 // (two workgroups a CU: with three, 128 dims spill 40 registers, 24 tokens behind a window of 4096 63.7 us for 47.2)
 template <int D, bool I8, bool MOD, bool LARGE>
 __global__ void __launch_bounds__(NT, LARGE || D == 128 ? 2 : 3) attend_kernel(const AttendP p) {
-  constexpr int NQ = LARGE ? TILE_FEW / 16 : 1;
+  constexpr int NQ = TILE_FEW / 16;
   __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D, NQ>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D, NQ>)
                                                                                                         : sizeof(Many<D>)];
   const int i = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;

@@ -14,9 +14,8 @@
 
 namespace kvs {
 
-constexpr int TILE_ONE = 16;    // virtual rows of a tile where no request brings more (the pass for single tokens)
-constexpr int TILE_FEW = 32;    // of a small tile beside large ones
-constexpr int TILE_MANY = 128;  // of a large tile
+constexpr int TILE_FEW = 16;    // virtual rows of a small tile
+constexpr int TILE_MANY = 128;  // of a large one
 constexpr int MAX_ATTEND_B = 2048, MAX_SHARED = 64, MAX_TILE_UNITS = 128;
 
 struct alignas(16) AttendUnit {
@@ -55,7 +54,7 @@ struct alignas(16) AttendTile {  // scratch of the plan
 // Sizes of a plan and where its parts lie in the workspace (int32 elements).
 struct AttendSizes {  // (host)
   bool large;        // large tiles occur
-  int few, many;     // heights
+  int few, many;     // heights (many 0: small tiles only)
   int64_t tiles, joins, units, part_rows;
   int64_t at_units, at_joins, at_tiles, at_rows, total;
 };

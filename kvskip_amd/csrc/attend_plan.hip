@@ -350,8 +350,8 @@ AttendSizes attend_sizes(const kvskip_attend_plan_args& p) {
   AttendSizes z{};
   const int64_t G = p.Hq / p.Hkv, virt = static_cast<int64_t>(p.rows) * G;
   const int64_t most = p.max_rows > 0 && p.max_rows < p.rows ? p.max_rows : p.rows;
-  z.large = most * G > TILE_ONE || (p.shared > 0 && virt > TILE_ONE);
-  z.few = z.large ? TILE_FEW : TILE_ONE;
+  z.large = most * G > TILE_FEW || (p.shared > 0 && virt > TILE_FEW);
+  z.few = TILE_FEW;
   z.many = z.large ? TILE_MANY : 0;
   // a small tile holds a whole request where large ones occur, so a batch has at most one short tile a request
   const int64_t h = z.large ? z.many : z.few;
