@@ -11,6 +11,8 @@
 #include "codes8.hpp"
 #include "attend.hpp"
 
+#include <type_traits>
+
 namespace kvs {
 namespace {
 
@@ -129,12 +131,12 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& any) {
   return w & ~((z >> 7) * 0xffu);
 }
 
-// Running state of a row. m: a score in log2 units at most 2^4 below its largest so far, l: this lane's part of sum 2^(s - m).
-// ar + ax: the accumulators' reference, a score and the exponent of its page's vs (apart, since in one float a large score takes
-// the exponent's bits); p |vs| passes 2^(ar + ax) by at most 2^7. c and d: 7 - ax - ar and ar + ax - 7 - m. All of it but l
-// changes only where a page's largest score passes what it may.
+// Running state of a row. m: a score in log2 units, the row's largest when the state was last looked at; l: this lane's part of
+// sum 2^(s - m). ar + ax: the accumulators' reference, a score and the exponent of its page's vs (apart, since in one float a large
+// score takes the exponent's bits). c and d: 7 - ax - ar (while the row has seen nothing: infinite, or 0) and ar + ax - 7 - m.
 struct State {
-  float m = NEG_INF, l = 0.f, ar = NEG_INF, ax = 0.f, c = 0.f, d = 0.f;
+  float m = NEG_INF, l = 0.f, ar = NEG_INF, ax = 0.f, c, d = 0.f;
+  __device__ explicit State(bool blind) : c(blind ? -NEG_INF : 0.f) {}
 };
 // What a wavefront's rows share: the largest exponent of vs so far; a reference has passed 2^10.
 struct Common {
@@ -206,18 +208,39 @@ __device__ __forceinline__ float least_of(const float (&s)[N]) {
 }
 
 // One page of a row: s in, w = 2^7 p vs / 2^(ar + ax) as fp16 pairs out, tokens in order; s f is the score in log2 units (neg: f <
-// 0), its maximum over `swap`'s lanes the row's. alpha: the factor of the accumulators, true if it is not 1 for all.
+// 0). alpha: the factor of the accumulators, true if it is not 1 for all.
 //   The plain way takes 2^(s f + c + log2 vs) at once, from which l is found too: an fma, an exponential, a sum and half a
 // conversion a score. Its one rounding more, of c + log2 vs, is 2^-14 at most where no reference passes 2^10; and no weight that
-// l could feel is below 2^-126: a page's largest score that is at most 2^60 below m lies at most 2^64 below ar, and vs at
-// most 2^40 below 2^ax. Elsewhere weights are taken relative to the page's largest score and multiplied by their factor.
-template <int N, class F>
+// l could feel is below 2^-126: a score at most 2^60 below the row's largest lies at most 2^64 below ar, and vs at most 2^40
+// below 2^ax. It holds while no weight leaves fp16. BLIND: taken without the page's largest score, and taken back where a lane's
+// sum passes 2^15 (or is NaN: a row's first keys, whose c is infinite, and masked ones before them); else only after the
+// reference has been moved to where no weight passes 2^14.
+//   Elsewhere weights are taken relative to the page's largest score and multiplied by their factor.
+template <bool BLIND, int N, class F>
 __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const Weight& v, State& st, Common& com, float& alpha,
                                        uint32_t (&w)[N / 2], F&& swap) {
+  alpha = 1.f;
+  auto plain = [&]() {
+    float sum[4];
+    const float c = st.c + v.lv;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float x = fexp2(fmaf(s[i], f, c)), y = fexp2(fmaf(s[i + 1], f, c));
+      sum[i % 4] = i < 4 ? x : sum[i % 4] + x, sum[i % 4 + 1] = i < 4 ? y : sum[i % 4 + 1] + y;
+      w[i / 2] = pack_h(x, y);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  };
+  if (BLIND && v.plain && !com.odd) {  // uniform
+    const float all = plain();
+    if (__ballot(!(all <= 0x1p15f)) == 0) {
+      st.l = fmaf(all, fexp2(st.d - v.lv), st.l);
+      return false;
+    }
+  }
   const float mt = neg ? swap(-least_of(s)) * -f : swap(most_of(s)) * f;
   const float past = (mt - st.ar) + (v.ev - st.ax);  // (NaN, which passes nothing, where nothing came yet)
-  const bool move = __ballot((past > 7.f) | (mt > st.m + 4.f)) != 0;
-  alpha = 1.f;
+  const bool move = BLIND || __ballot((past > 7.f) | (mt > st.m + 4.f)) != 0;
   if (move) {
     const bool on = past > 0.f;
     alpha = on ? fexp2(-past) : 1.f;
@@ -227,38 +250,31 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
     st.l *= fexp2(st.m - mu);
     st.m = m;
     const bool none = st.ar == NEG_INF;
-    st.c = none ? 0.f : (7.f - st.ax) - st.ar;
+    st.c = none ? (BLIND ? -NEG_INF : 0.f) : (7.f - st.ax) - st.ar;
     st.d = none ? 0.f : ((st.ar - mu) + st.ax) - 7.f;
     com.odd |= __ballot(!none & (fabsf(st.ar) > 0x1p10f)) != 0;
   }
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (v.plain & !com.odd) {  // uniform
-    const float c = st.c + v.lv;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float x = fexp2(fmaf(s[i], f, c)), y = fexp2(fmaf(s[i + 1], f, c));
-      sum[i % 4] += x, sum[i % 4 + 1] += y;
-      w[i / 2] = pack_h(x, y);
-    }
-    st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), fexp2(st.d - v.lv), st.l);
-  } else {
-    const float mtu = mt == NEG_INF ? 0.f : mt;
-    // (scores so large that mt's rounding would show in s f - mt: rounded alike)
-    if (__ballot(fabsf(mtu) > 0x1p17f) != 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) s[i] *= f;
-      f = 1.f;
-    }
-    // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
-    const float fv = mt == NEG_INF ? 0.f : v.vs * fexp2((mt - st.ar) - st.ax) * 0x1p7f;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float x = fexp2(fmaf(s[i], f, -mtu)), y = fexp2(fmaf(s[i + 1], f, -mtu));
-      sum[i % 4] += x, sum[i % 4 + 1] += y;
-      w[i / 2] = pack_h(x * fv, y * fv);
-    }
-    st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), mt == NEG_INF ? 0.f : fexp2(mt - st.m), st.l);
+  if (!BLIND && v.plain && !com.odd) {  // uniform
+    st.l = fmaf(plain(), fexp2(st.d - v.lv), st.l);
+    return move;
   }
+  const float mtu = mt == NEG_INF ? 0.f : mt;
+  // (scores so large that mt's rounding would show in s f - mt: rounded alike)
+  if (__ballot(fabsf(mtu) > 0x1p17f) != 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] *= f;
+    f = 1.f;
+  }
+  // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
+  const float fv = mt == NEG_INF ? 0.f : v.vs * fexp2((mt - st.ar) - st.ax) * 0x1p7f;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float x = fexp2(fmaf(s[i], f, -mtu)), y = fexp2(fmaf(s[i + 1], f, -mtu));
+    sum[i % 4] += x, sum[i % 4 + 1] += y;
+    w[i / 2] = pack_h(x * fv, y * fv);
+  }
+  st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), mt == NEG_INF ? 0.f : fexp2(mt - st.m), st.l);
   return move;
 }
 
@@ -290,7 +306,6 @@ struct Pages {
   int blk, pg;
   float ks, vs;
 };
-template <int STRIDE>
 struct PageList {
   const AttendP& p;
   const AttendUnit& u;
@@ -307,7 +322,7 @@ struct PageList {
     const int k = k0 + static_cast<int>(threadIdx.x % WAVE);
     x.blk = -1;
     if (k < n) {
-      const int i = u.i0 + first + STRIDE * k;
+      const int i = u.i0 + first + NWAVE * k;
       x.blk = i < u.a1 ? i : i - u.a1 + u.b0;
     }
   }
@@ -385,11 +400,12 @@ struct Few {
 
 template <int D, int NQ, bool I8, bool MOD>
 __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, int h, Few<D, NQ>& L) {
+  static_assert(NQ == 1);
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
   const int j4 = lane >> 4, c16 = lane & 15;
   const int nw = u.n > wave ? (u.n - wave + NWAVE - 1) / NWAVE : 0;
-  PageList<NWAVE> list(p, u, h, wave, nw);
+  PageList list(p, u, h, wave, nw);
   const uint32_t koff = c16 * p.k_st + 16 * j4;
   const uint32_t voff = D == 128 ? 4 * j4 * p.v_st + 8 * c16 : (4 * j4 + (c16 >> 3)) * p.v_st + 8 * (c16 & 7);
   const bool up_half = (lane & 8) != 0;
@@ -408,7 +424,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
   float qf[NQ], slope[NQ];
   Sight see[NQ];
   int at[NQ];  // the row's own index, less the lane's first token
-  State st[NQ];
+  State st[NQ] = {State(false)};
   Common com;
   Reach re;
 #pragma unroll
@@ -490,12 +506,12 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = t0 + mf_tok(i / 4, i % 4, j4);
-          s[a][i] = sees(see[a], t) & (pg >= 0) ? s[a][i] * f : NEG_INF;
+          s[a][i] = (sees(see[a], t) & (pg >= 0)) ? s[a][i] * f : NEG_INF;
         }
         f = 1.f, neg = false;
       }
       float alpha;
-      if (soften(s[a], f, neg, wt, st[a], com, alpha, w[a], [](float x) { return swap_max(x); }))
+      if (soften<false>(s[a], f, neg, wt, st[a], com, alpha, w[a], [](float x) { return swap_max(x); }))
 #pragma unroll
         for (int j = 0; j < VD; ++j) acc[a][j] *= alpha;
     }
@@ -580,6 +596,11 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 // multiplied the next one's codes are on their way and converted, once for all rows. 32 x 32 products: K as it lies in
 // LDS, V by transposing reads. Chunks of 16 bytes are placed so that neither reads nor writes conflict: K chunk c of
 // row r at c ^ r, V's at c ^ 5 (r % 4) (64 dims: r / 2 in both).
+//   Vector instructions bound it: beside products, which take the matrix unit 1024 clocks a page of 128 dims and wavefront,
+// vector instructions run at half their rate or so, and two wavefronts a SIMD take turns at best. So: operands asked for four
+// products ahead (read and waited for one by one, prompts of 8192 took 1850 us, for 1780), addresses that a page's turn
+// does not change (two pages a turn, 1745 to 1737), maxima only where they are needed (1650), and nothing in the loop that waits for
+// the codes asked for last (the page list in groups).
 template <int D>
 struct Many {
   uint8_t k[2][BLK * D * 2], v[2][BLK * D * 2];
@@ -590,21 +611,47 @@ struct Many {
 template <int D, bool I8, bool MOD>
 __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u, int h, Many<D>& L) {
   constexpr int KS = D / 16, ND = D / 32, NC = D / 64;  // steps of a score product; dim tiles; 16-byte loads a thread
-  constexpr uint32_t ROW = 2 * D, PAGE = BLK * ROW;
+  constexpr int AHEAD = 4;  // operands are read that many products before theirs
+  constexpr uint32_t ROW = 2 * D;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
   const int c32 = lane & 31, half = lane >> 5;
-  PageList<1> list(p, u, h, 0, u.n);
+  const int n = u.n;
   const uint8_t* kb = p.k + h * p.k_sh;
   const uint8_t* vb = p.v + h * p.v_sh;
-  auto rows_of = [&](int blk, int pg) { return pg >= 0 ? min(BLK, u.len - blk * BLK) : 0; };
+  const int* table = (u.kind & 2) ? p.shared_table + u.table * p.st_stride : p.block_table + u.table * p.bt_stride;
+  // the pages of 64 steps from g0 on, one a lane, of which the loop takes GROUP before it asks again: it looks up to two ahead
+  constexpr int GROUP = 60;
+  int g0 = 0, what;            // table entry (-1: no page)
+  uint32_t k_lo, v_lo, kv_hi;  // addresses, 48 bits each
+  float k_sc, v_sc;
+  auto gather = [&](int first) {
+    g0 = first;
+    const int j = first + lane, i = u.i0 + j, b = i < u.a1 ? i : i - u.a1 + u.b0;
+    int pg = j < n ? table[b] : -1;
+    if (pg >= p.num_pages) pg = -1;
+    what = pg >= 0 ? b : -1;
+    const int at = max(pg, 0);
+    const uint64_t ka = reinterpret_cast<uint64_t>(kb) + at * p.k_sb, va = reinterpret_cast<uint64_t>(vb) + at * p.v_sb;
+    k_lo = static_cast<uint32_t>(ka), v_lo = static_cast<uint32_t>(va);
+    kv_hi = (static_cast<uint32_t>(ka >> 32) & 0xffffu) | static_cast<uint32_t>(va >> 32) << 16;
+    k_sc = pg >= 0 ? p.k_scale[pg * p.ks_sb + h * p.ks_sh] : 0.f;
+    v_sc = pg >= 0 ? p.v_scale[pg * p.vs_sb + h * p.vs_sh] : 0.f;
+    // (waited for here: first used in the loop, they would be waited for there at each turn, with the codes asked for last)
+    asm volatile("" : "+v"(k_sc), "+v"(v_sc));
+  };
+  auto entry = [&](int k) { return static_cast<int>(lane_u32(static_cast<uint32_t>(what), k - g0)); };
+  auto of_step = [&](uint32_t lo, int shift, uint32_t st, int k) {  // rows past the sequence's last read zeros
+    const uint64_t at = static_cast<uint64_t>(lane_u32(kv_hi, k - g0) >> shift & 0xffffu) << 32 | lane_u32(lo, k - g0);
+    const int b = entry(k);
+    return make_rsrc(reinterpret_cast<const void*>(at), b >= 0 ? (min(BLK, u.len - b * BLK) - 1) * st + D : 0u);
+  };
   // staging: thread t holds 16 NC codes of row t / 4
   const uint32_t srow = tid >> 2, sc = 2 * NC * (tid & 3);  // its first 16-byte chunk in LDS
   const uint32_t kso = srow * p.k_st + 16 * NC * (tid & 3), vso = srow * p.v_st + 16 * NC * (tid & 3);
   const uint32_t kx = D == 128 ? srow & 15 : (srow >> 1) & 7, vx = 5 * (D == 128 ? srow & 3 : (srow >> 1) & 1);
   u32x4 kc[NC], vc[NC];
   auto fetch = [&](int k) {
-    const int blk = k < u.n ? list.blk(k) : -1, pg = k < u.n ? list.pg(k) : -1, n = rows_of(blk, pg);
-    const rsrc_t rk = page_res<D>(kb, p.k_sb, p.k_st, pg, n), rv = page_res<D>(vb, p.v_sb, p.v_st, pg, n);
+    const rsrc_t rk = of_step(k_lo, 0, p.k_st, k), rv = of_step(v_lo, 16, p.v_st, k);
 #pragma unroll
     for (int c = 0; c < NC; ++c) kc[c] = bload16(rk, kso + 16 * c, 0);
 #pragma unroll
@@ -615,7 +662,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
     *reinterpret_cast<u32x4*>(row + ((chunk ^ swz) << 4)) = u32x4{a.x, a.y, b.x, b.y};
     *reinterpret_cast<u32x4*>(row + (((chunk + 1) ^ swz) << 4)) = u32x4{c.x, c.y, d.x, d.y};
   };
-  auto stage = [&](int buf, bool cut) {
+  auto stage = [&](auto buf, bool cut) {
     uint8_t* k = L.k[buf] + srow * ROW;
     uint8_t* v = L.v[buf] + srow * ROW;
     if constexpr (!I8)
@@ -632,6 +679,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
 #pragma unroll
     for (int c = 0; c < NC; ++c) widen16(vc[c], v, sc + 2 * c, vx);
   };
+  gather(0);
   fetch(0);
 
   // ---- this wavefront's rows
@@ -654,7 +702,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   const Reach re = reach(see);
   const int at = r.pos - u.base - 4 * half;
   const float slope = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
-  State st;
+  State st(!MOD);
   Common com;
   f32x16_t acc[ND];
 #pragma unroll
@@ -676,19 +724,26 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
     for (int* x : {&all.from_min, &all.from_max, &all.end_min, &all.end_max, &all.pre_min, &all.pre_max})
       *x = __builtin_amdgcn_readfirstlane(*x);
   }
-  auto is_cut = [&](int k) { return !sees_keys(all, list.blk(k) * BLK, u.len); };
-  stage(0, !I8 && u.n > 0 && is_cut(0));
-  if (u.n > 1) fetch(1);
+  auto is_cut = [&](int k) {
+    const int b = entry(k);
+    return b >= 0 && !sees_keys(all, b * BLK, u.len);
+  };
+  stage(std::integral_constant<int, 0>{}, !I8 && is_cut(0));
+  fetch(1);
   __syncthreads();
-  for (int k = 0; k < u.n; ++k) {
-    const uint32_t buf = k & 1;
-    const float ks = list.ks(k), vs = list.vs(k);
-    const int blk = list.blk(k), pg = list.pg(k);
-    const int t0 = blk * BLK;
-    if (busy && pg >= 0 && !sees_none(re, t0)) {
+  auto step = [&](int k, auto buf) {
+    const float ks = lane_value(k_sc, k - g0), vs = lane_value(v_sc, k - g0);
+    const int blk = entry(k), t0 = blk * BLK;
+    if (busy && blk >= 0 && !sees_none(re, t0)) {
       const uint8_t* kl = L.k[buf];
       const uint8_t* vl = L.v[buf];
       float s[32];
+      u32x4 a[2 * KS];  // operands, read a few products ahead
+      auto read_k = [&](int x) {
+        if (x < 2 * KS) a[x] = *reinterpret_cast<const u32x4*>(kl + ((ka ^ (32 * (x % KS))) + 32 * (x / KS) * ROW));
+      };
+#pragma unroll
+      for (int x = 0; x < AHEAD; ++x) read_k(x);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         f32x16_t c;
@@ -696,13 +751,24 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
         for (int i = 0; i < 16; ++i) c[i] = 0.f;
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(kl + ((ka ^ (32 * x)) + 32 * kt * ROW));
-          c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, qh[x]), c, 0, 0,
-                                                     0);
+          read_k(kt * KS + x + AHEAD);
+          __builtin_amdgcn_sched_barrier(0);
+          c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a[kt * KS + x]),
+                                                     __builtin_bit_cast(f16x8_t, qh[x]), c, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[16 * kt + i] = c[i];
       }
+      u32x4 b[4 * ND];
+      auto read_v = [&](int y) {
+        if (y < 4 * ND) {
+          typedef __attribute__((address_space(3))) fp16x4_t lds_t;
+          const uint8_t* x = vl + ((va ^ (64 * (y % ND))) + 16 * (y / ND) * ROW);
+          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(x)));
+          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(x + 8 * ROW)));
+          b[y] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+      };
       float f = qf * ks;
       bool neg = (__float_as_int(ks) ^ __float_as_int(p.scale)) < 0;  // uniform
       if constexpr (MOD) {
@@ -720,38 +786,36 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
       }
       uint32_t w[16];
       float alpha;
-      if (soften(s, f, neg, Weight(vs, com), st, com, alpha, w, [](float x) { return swap32_max(x); }))
+      if (soften<!MOD>(s, f, neg, Weight(vs, com), st, com, alpha, w, [](float x) { return swap32_max(x); }))
 #pragma unroll
         for (int j = 0; j < ND; ++j) acc[j] *= alpha;
+#pragma unroll
+      for (int y = 0; y < AHEAD; ++y) read_v(y);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const u32x4 pw = {w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]};
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
-          typedef __attribute__((address_space(3))) fp16x4_t lds_t;
-          const uint8_t* x = vl + ((va ^ (64 * j)) + 16 * g * ROW);
-          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(x)));
-          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_t*)(x + 8 * ROW)));
-          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, (u32x4{lo.x, lo.y, hi.x, hi.y})),
+          read_v(g * ND + j + AHEAD);
+          __builtin_amdgcn_sched_barrier(0);
+          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, b[g * ND + j]),
                                                           __builtin_bit_cast(f16x8_t, pw), acc[j], 0, 0, 0);
         }
       }
     }
-    // the list turns after its last read of a step, 64 steps at a time; step k + 2 may be of the next 64
-    list.advance(k);
-    if ((k & 63) == 63) list.turn(k);
-    if (k + 1 < u.n) stage(buf ^ 1, !I8 && is_cut(k + 1));
-    if (k + 2 < u.n) {
-      if ((k & 63) == 62) {  // (its page is in nxt still)
-        Pages t = list.cur;
-        list.cur = list.nxt;
-        fetch(k + 2);
-        list.cur = t;
-      } else {
-        fetch(k + 2);
-      }
+    if (k + 1 < n) {
+      stage(std::integral_constant<int, buf ^ 1>{}, !I8 && is_cut(k + 1));
+      fetch(k + 2);
     }
     __syncthreads();
+  };
+  for (int first = 0; first < n; first += GROUP) {
+    if (first > 0) gather(first);
+    const int end = min(first + GROUP, n);
+    for (int k = first; k < end; k += 2) {
+      step(k, std::integral_constant<int, 0>{});
+      if (k + 1 < end) step(k + 1, std::integral_constant<int, 1>{});
+    }
   }
 
   // ---- results: lane holds row c32's dims 32 j + 8 (i / 4) + 4 half + i % 4
@@ -768,8 +832,8 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
              f32x4_t{acc[j][i] * x, acc[j][i + 1] * x, acc[j][i + 2] * x, acc[j][i + 3] * x}, st.m, l);
   if (I8 || L.nan == 0) return;
   // NaN of cut pages over what was stored
-  for (int k = 0; k < u.n; ++k) {
-    const int i = u.i0 + k, b = i < u.a1 ? i : i - u.a1 + u.b0, g = list.table[b];
+  for (int k = 0; k < n; ++k) {
+    const int i = u.i0 + k, b = i < u.a1 ? i : i - u.a1 + u.b0, g = table[b];
     if (g < 0 || g >= p.num_pages || sees_keys(all, b * BLK, u.len)) continue;
     for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t) {
       if (!sees(see, t)) continue;
@@ -779,9 +843,10 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   }
 }
 
-// (two workgroups a CU: with three, 128 dims spill 40 registers, 24 tokens behind a window of 4096 63.7 us for 47.2)
+// Workgroups a CU: two for 128 dims (with three they spill 40 registers, 24 tokens behind a window of 4096 63.7 us for 47.2), three for
+// 64 (two: prompts of 2111 behind a prefix 174 us for 154).
 template <int D, bool I8, bool MOD, bool LARGE>
-__global__ void __launch_bounds__(NT, LARGE || D == 128 ? 2 : 3) attend_kernel(const AttendP p) {
+__global__ void __launch_bounds__(NT, D == 128 ? 2 : 3) attend_kernel(const AttendP p) {
   constexpr int NQ = TILE_FEW / 16;
   __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D, NQ>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D, NQ>)
                                                                                                         : sizeof(Many<D>)];
