@@ -511,7 +511,7 @@ typedef struct kvskip_attend_plan_args {
   const int32_t* shared_of;    /* [B] */
   int32_t* work;               /* kvskip_attend_work_ints int32, 16-byte aligned */
   int32_t* positions;          /* [rows] out */
-  int32_t B, rows, Hq, Hkv, T; /* B <= 2048, rows <= 2^21, rows * Hq < 2^28, T <= 2^27 */
+  int32_t B, rows, Hq, Hkv, T; /* B <= 2048, rows <= 2^21, Hq <= 1024, rows * Hq <= 2^26, B * Hkv <= 2^17, T <= 2^27 */
   int32_t shared, shared_T;    /* shared prefixes (0: none; at most 64) and the capacity of one, <= 2^27 */
   int32_t max_rows, window;
 } kvskip_attend_plan_args;
@@ -562,7 +562,7 @@ int kvskip_attend(const kvskip_attend_args* a, void* stream);
  *   angle = positions[axis(i), n] * inv_freq[i], the product in 64 bits;
  *   (a, b) -> mscale * (a cos - b sin, b cos + a sin); elements from rot on stay y.
  * axis(i): the first sections[0] pairs belong to axis 0, the next sections[1] to axis 1, ... (their sum is rot / 2).
- * Outputs may be the inputs themselves (same pointer and strides), and must not overlap them otherwise. D a multiple of 8 up
+ * Outputs may be their inputs (same pointer and strides), and must overlap neither input nor each other otherwise. D a multiple of 8 up
  * to 256, rot a multiple of 8 up to D (0: no rotation); strides multiples of 4 elements, bases 8-byte aligned. Hkv 0: no k. */
 typedef struct kvskip_rope_args {
   const void* q;

@@ -20,7 +20,6 @@
 #include <cstring>
 #include <stdexcept>
 #include <string>
-#include <utility>
 #include <vector>
 
 #include "kvskip_amd.h"
@@ -1119,6 +1118,27 @@ PyObject* attend(PyObject* const* a) {
   return list_of({out, lse});
 }
 
+// Of [rows, heads, D] tensors with a contiguous last dim: the elements from one row's first to its last.
+int64_t row_extent(const at::Tensor& t) { return (t.size(1) - 1) * t.stride(1) + t.size(2); }
+// No element twice: heads apart in a row and rows apart, or the other way round.
+bool once(const at::Tensor& t) {
+  const int64_t n = t.size(0), h = t.size(1), D = t.size(2);
+  if (t.numel() == 0) return true;
+  if ((h <= 1 || t.stride(1) >= D) && (n <= 1 || t.stride(0) >= row_extent(t))) return true;
+  return (n <= 1 || t.stride(0) >= D) && (h <= 1 || t.stride(1) >= (n - 1) * t.stride(0) + D);
+}
+// No element of both: one behind the other, or slices of rows of one width.
+bool apart(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return true;
+  const int64_t n = x.size(0), a = reinterpret_cast<intptr_t>(x.data_ptr()), b = reinterpret_cast<intptr_t>(y.data_ptr());
+  const int64_t ex = 2 * ((n - 1) * x.stride(0) + row_extent(x)), ey = 2 * ((n - 1) * y.stride(0) + row_extent(y));
+  if (a + ex <= b || b + ey <= a) return true;
+  const int64_t w = 2 * x.stride(0);
+  if (n <= 1 || x.stride(0) != y.stride(0) || 2 * row_extent(x) > w || 2 * row_extent(y) > w) return false;
+  const int64_t d = ((b - a) % w + w) % w;
+  return 2 * row_extent(x) <= d && d + 2 * row_extent(y) <= w;
+}
+
 // norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, sections, pairs, mscale, q_out, k_out): [q_out, k_out]
 PyObject* norm_rope(PyObject* const* a) {
   const at::Tensor& q = tensor(a[0], "q");
@@ -1187,22 +1207,19 @@ PyObject* norm_rope(PyObject* const* a) {
     const at::Tensor* given = opt_tensor(o, name);
     if (given == nullptr) return empty(like.sizes(), at::kBFloat16, dev);
     if (!(rows_ok(*given) && given->sizes() == like.sizes())) fail(std::string("norm_rope: ") + name + ": bf16 of its input's shape");
-    // (in place, or apart: heads are written while others are read)
-    auto span = [](const at::Tensor& t) {
-      int64_t lo = 0, hi = 1;
-      for (int64_t i = 0; i < 3; ++i) (t.stride(i) < 0 ? lo : hi) += (t.size(i) - 1) * t.stride(i);
-      const char* b = static_cast<const char*>(t.data_ptr());
-      return std::make_pair(b + 2 * lo, b + 2 * hi);
-    };
-    if (like.numel() > 0 && !(given->data_ptr() == like.data_ptr() && given->strides() == like.strides())) {
-      const auto x = span(*given), y = span(like);
-      require(x.second <= y.first || y.second <= x.first, "norm_rope: an output is its input or does not overlap it");
-    }
     return *given;
   };
   at::Tensor qo = out(a[10], q, "q_out"), ko;
   if (k != nullptr) ko = out(a[11], *k, "k_out");
   else require(a[11] == Py_None, "norm_rope: k_out without k");
+  // An output is its input, or apart from both inputs (heads are written while others are read); the outputs are apart.
+  auto in_place = [](const at::Tensor& x, const at::Tensor& y) {
+    return x.data_ptr() == y.data_ptr() && x.strides() == y.strides();
+  };
+  require(once(qo) && (k == nullptr || once(ko)), "norm_rope: an output's elements must not overlap each other");
+  require((in_place(qo, q) || apart(qo, q)) && (k == nullptr || (apart(qo, *k) && apart(ko, q) && apart(qo, ko) &&
+                                                                 (in_place(ko, *k) || apart(ko, *k)))),
+          "norm_rope: an output is its input or does not overlap the inputs and the other output");
   same_device(q, {k, pos, fr, qw, kw, &qo, k != nullptr ? &ko : nullptr}, "norm_rope: tensors on one device");
   auto strides = [&](const at::Tensor& t, int64_t& sn, int64_t& sh) {
     sn = N > 1 ? t.stride(0) : 0, sh = t.size(1) > 1 ? t.stride(1) : 0;

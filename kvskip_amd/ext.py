@@ -209,7 +209,7 @@ def norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
     i + rot / 2, or with pairs 2 i and 2 i + 1, and turns by positions * inv_freq[i]; elements from rot on do not turn, and
     positions = inv_freq = None turns none. positions: int32 [rows], or [axes, rows] with up to 4 axes, of which axis 0 turns
     the first sections[0] pairs, axis 1 the next sections[1], and so on. mscale multiplies what is turned. Returns
-    [q_out, k_out], new ones or those given, which may be the inputs (else must not overlap them)."""
+    [q_out, k_out], new ones or those given: each its own input, or apart from both inputs and the other one."""
     return _host().norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, sections, pairs, mscale, q_out, k_out)
 
 

@@ -98,8 +98,8 @@ class PagedCache:
         K.ext().cache_write(k, v, self.slot_map[:k.shape[0]], *self.pools[layer], *self.scales[layer])
 
     def decode(self, layer: int, q: torch.Tensor, scale: float, **kw) -> dict:
-        """kvskip.decode of one query a request [requests, Hq, D] over its tokens. An empty request's row is
-        zeros (lse -inf)."""
+        """kvskip.decode of one query a request [requests, Hq, D] over its own tokens; attend() is the call
+        for requests behind shared prefixes. An empty request's row is zeros (lse -inf)."""
         k, v = self.pools[layer]
         ks, vs = self.scales[layer]
         return K.decode(q, k, v, scale, seq_lens=self.lens, block_table=self.block_table, T=self.T, k_scale=ks, v_scale=vs,

@@ -214,6 +214,21 @@ def test_scales_of_any_size(gpu, Hq, Hkv, D):
     check(s.call(s.plan()), s.exact(), D)
 
 
+@pytest.mark.parametrize("signed", [False, True])
+@pytest.mark.parametrize("rising", [True, False])
+@pytest.mark.parametrize("fmt,D", [("int8", 128), ("e4m3", 64)])
+def test_scores_that_rise(gpu, fmt, D, rising, signed):
+    """Scores that grow, or fall, by half a power of two a page, V's scales the other way: references that every page
+    passes, and ones that no later page does."""
+    s = Step([(64 * 14 + 9, 260), (64 * 14, 1)], 8, 2, D, fmt, 23, signed=signed)
+    for b in range(2):
+        for i in range(14):
+            x = 2.0 ** ((i if rising else 13 - i) / 2 - 9)
+            s.ks[s.table[b, i]] = s.ks[s.table[b, i]].sign() * x
+            s.vs[s.table[b, i]] = s.vs[s.table[b, i]].sign() * 2.0 ** -12 / x
+    check(s.call(s.plan()), s.exact(), D)
+
+
 def test_strides(gpu):
     """q as a slice of a fused projection, pools and scales as views, tables of more columns than needed."""
     s = Step([(90, 60), (130, 1)], 8, 2, 128, "e4m3", 22, width=9)

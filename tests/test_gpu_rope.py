@@ -118,3 +118,25 @@ def test_captured(gpu):
         torch.cuda.synchronize()
         got = [o.clone() for o in outs]
         assert all(torch.equal(x, y) for x, y in zip(got, run()))
+
+
+def test_outputs_that_overlap(gpu):
+    """Slices of one buffer that share no element are served; an output over the other input, the other output or itself is not."""
+    q, k, pos, freq, w = make(5, 4, 2, 64, 64, 1, 9)
+    args = pos[0].cuda(), freq.cuda(), w[0].cuda(), w[1].cuda()
+    want = ext.norm_rope(q.cuda(), k.cuda(), *args)
+    qkv = torch.cat([q, k, k, q], 1).cuda()                    # [5, 12, 64]
+    a, b = qkv[:, :4], qkv[:, 4:6]
+    ext.norm_rope(a, b, *args, q_out=qkv[:, 8:], k_out=qkv[:, 6:8])
+    assert torch.equal(qkv[:, 8:], want[0]) and torch.equal(qkv[:, 6:8], want[1])
+    assert torch.equal(qkv[:, :4], q.cuda()) and torch.equal(qkv[:, 4:6], k.cuda())
+    both = torch.zeros(4 + 2, 5, 64, dtype=torch.bfloat16, device="cuda")
+    ext.norm_rope(a, b, *args, q_out=both[:4].transpose(0, 1), k_out=both[4:].transpose(0, 1))
+    assert torch.equal(both[:4].transpose(0, 1), want[0]) and torch.equal(both[4:].transpose(0, 1), want[1])
+    kept = qkv.clone()
+    for kw in (dict(q_out=qkv[:, 3:7]), dict(q_out=qkv[:, 1:5]), dict(k_out=qkv[:, 3:5]), dict(k_out=qkv[:, 5:7]),
+               dict(q_out=qkv[:, 6:10], k_out=qkv[:, 8:10]), dict(q_out=a[:1].expand(5, 4, 64)),
+               dict(k_out=both[:1].transpose(0, 1).expand(5, 2, 64))):
+        with pytest.raises(RuntimeError, match="norm_rope: an output"):
+            ext.norm_rope(a, b, *args, **kw)
+    assert torch.equal(qkv, kept)
