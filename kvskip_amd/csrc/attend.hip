@@ -6,8 +6,8 @@
 // own registers and one or two lane swaps, and its weights are already the operand of O^T = V^T P^T (any order of the
 // keys will do inside a product, as long as V's operand has the same). Codes become fp16, which holds them exactly; q is
 // fp16 times a power of two of its row (2^14 <= largest < 2^15: exact, but for what lies below 2^-39 of that); weights
-// are one fp16 part, 2^-12 of each, taken relative to a reference that is within 2^7 of the largest weight times |vs|
-// so far (as in attn_decode8.hip: accumulators are rescaled only when a page passes it); sums and statistics are fp32.
+// are one fp16 part, 2^-12 of each, taken relative to a reference that the largest weight times |vs| so far passes by 2^8 at
+// most (accumulators are rescaled only when a page passes that); sums and statistics are fp32.
 #include "codes8.hpp"
 #include "attend.hpp"
 
