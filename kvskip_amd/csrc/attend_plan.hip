@@ -25,6 +25,10 @@ constexpr int CLASSES = 32;
 constexpr int SLOTS = 512;
 constexpr int TARGET_UNITS = 2 * SLOTS;  // units of a queued plan: those that end early take another
 constexpr int LEAST_PAGES = 4;           // of a unit: its four wavefronts take a page each
+// Of a unit of a queued plan: partial results cost more than a shorter last round saves. (Least 4, 16 and 32, us: 9 prompts of up to
+// 763 behind bidirectional prefixes 86.5, 63.5, 63.3; 7 of up to 1412 in a window of 234 72, 43, 43; 64 tokens behind a prefix
+// of 8192 46.8, 42, 61.)
+constexpr int LEAST_QUEUED = 16;
 
 struct PlanP {
   kvskip_attend_plan_args a;
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
     if (wave_sum_int(n) <= room && tid % WAVE == 0) atomicMin(&sFit, c);
   }
   __syncthreads();
-  const int queued = static_cast<int>(max(static_cast<int64_t>(LEAST_PAGES), (all_pages * p.a.Hkv + TARGET_UNITS - 1) / TARGET_UNITS));
+  const int queued = static_cast<int>(max(static_cast<int64_t>(LEAST_QUEUED), (all_pages * p.a.Hkv + TARGET_UNITS - 1) / TARGET_UNITS));
   const int chunk = sFit != INT32_MAX ? sFit : queued;
   auto cut = [&](int pages) { return min(max((pages + chunk - 1) / chunk, 1), MAX_TILE_UNITS); };
 
