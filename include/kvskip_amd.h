@@ -529,7 +529,7 @@ int64_t kvskip_attend_part_rows(const kvskip_attend_plan_args* p);
  * 0 and -inf for a row that sees nothing and for rows that no request brings. q: bf16 [rows, Hq, D] (strides multiples of 8,
  * 16-byte aligned). Pools [num_pages, Hkv, 64, D] of codes (strides multiples of 16, 16-byte aligned, token strides below
  * 2^24), scales [num_pages, Hkv]; a page outside [0, num_pages) holds no keys. D in {64, 128}, any Hq / Hkv. q is exact to
- * 2^-39 of its row's largest element, a weight holds 11 bits, scores and sums are fp32. Keys that a row does not see do not
+ * 2^-39 of its row's largest element, a weight holds 22 bits, scores and sums are fp32. Keys that a row does not see do not
  * reach it, whatever they hold. part_acc [part_rows, Hkv, D] and part_ml [part_rows, Hkv, 2] fp32, 16-byte aligned. */
 typedef struct kvskip_attend_args {
   kvskip_attend_plan_args plan;  /* sizes and work; its other pointers are not read */

@@ -6,8 +6,11 @@
 // own registers and one or two lane swaps, and its weights are already the operand of O^T = V^T P^T (any order of the
 // keys will do inside a product, as long as V's operand has the same). Codes become fp16, which holds them exactly; q is
 // fp16 times a power of two of its row (2^14 <= largest < 2^15: exact, but for what lies below 2^-39 of that); weights
-// are one fp16 part, 2^-12 of each, taken relative to a reference that the largest weight times |vs| so far passes by 2^8 at
-// most (accumulators are rescaled only when a page passes that); sums and statistics are fp32.
+// are two fp16 parts, 2^-23 of each, taken relative to a reference that the largest weight times |vs| so far passes by 2^8 at
+// most (accumulators are rescaled only when a page passes that); sums and statistics are fp32. (One part, 2^-12, shows beside
+// bf16 results, more where values cancel: 2^-10 of a result in the norm from a softmax in fp32, for 2^-14. The second one
+// costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2210 us for 1665, 64 tokens behind a prefix of 8192 48.5 for
+// 42.2. Its order among the products makes no difference.)
 #include "codes8.hpp"
 #include "attend.hpp"
 
@@ -207,10 +210,16 @@ __device__ __forceinline__ float least_of(const float (&s)[N]) {
   return x;
 }
 
-// One page of a row: s in, w = 2^7 p vs / 2^(ar + ax) as fp16 pairs out, tokens in order; s f is the score in log2 units (neg: f <
+// A pair of weights in two parts of fp16, the second what the first leaves: 22 bits.
+__device__ __forceinline__ void two_parts(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_h(x, y);
+  lo = mix_h(x, y, 1.f, -__builtin_bit_cast(f16x2_t, hi));
+}
+
+// One page of a row: s in, w + wl = 2^7 p vs / 2^(ar + ax) as fp16 pairs out, tokens in order; s f is the score in log2 units (neg: f <
 // 0). alpha: the factor of the accumulators, true if it is not 1 for all.
-//   The plain way takes 2^(s f + c + log2 vs) at once, from which l is found too: an fma, an exponential, a sum and half a
-// conversion a score. Its one rounding more, of c + log2 vs, is 2^-14 at most where no reference passes 2^10; and no weight that
+//   The plain way takes 2^(s f + c + log2 vs) at once, from which l is found too: an fma, an exponential, a sum and one and a
+// half conversions a score. Its one rounding more, of c + log2 vs, is 2^-14 at most where no reference passes 2^10; and no weight that
 // l could feel is below 2^-126: a score at most 2^60 below the row's largest lies at most 2^64 below ar, and vs at most 2^40
 // below 2^ax. It holds while no weight leaves fp16. BLIND: taken without the page's largest score, and taken back where a lane's
 // sum passes 2^15 (or is NaN: a row's first keys, whose c is infinite, and masked ones before them); else only after the
@@ -218,7 +227,7 @@ __device__ __forceinline__ float least_of(const float (&s)[N]) {
 //   Elsewhere weights are taken relative to the page's largest score and multiplied by their factor.
 template <bool BLIND, int N, class F>
 __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const Weight& v, State& st, Common& com, float& alpha,
-                                       uint32_t (&w)[N / 2], F&& swap) {
+                                       uint32_t (&w)[N / 2], uint32_t (&wl)[N / 2], F&& swap) {
   alpha = 1.f;
   auto plain = [&]() {
     float sum[4];
@@ -227,7 +236,7 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
     for (int i = 0; i < N; i += 2) {
       const float x = fexp2(fmaf(s[i], f, c)), y = fexp2(fmaf(s[i + 1], f, c));
       sum[i % 4] = i < 4 ? x : sum[i % 4] + x, sum[i % 4 + 1] = i < 4 ? y : sum[i % 4 + 1] + y;
-      w[i / 2] = pack_h(x, y);
+      two_parts(x, y, w[i / 2], wl[i / 2]);
     }
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
@@ -272,7 +281,7 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
   for (int i = 0; i < N; i += 2) {
     const float x = fexp2(fmaf(s[i], f, -mtu)), y = fexp2(fmaf(s[i + 1], f, -mtu));
     sum[i % 4] += x, sum[i % 4 + 1] += y;
-    w[i / 2] = pack_h(x * fv, y * fv);
+    two_parts(x * fv, y * fv, w[i / 2], wl[i / 2]);
   }
   st.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), mt == NEG_INF ? 0.f : fexp2(mt - st.m), st.l);
   return move;
@@ -491,7 +500,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
         nan |= __ballot(any != 0) != 0;
       }
     const Weight wt(vs, com);
-    uint32_t w[NQ][8];
+    uint32_t w[NQ][8], wl[NQ][8];
 #pragma unroll
     for (int a = 0; a < NQ; ++a) {
       float f = qf[a] * ks;
@@ -511,7 +520,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
         f = 1.f, neg = false;
       }
       float alpha;
-      if (soften<false>(s[a], f, neg, wt, st[a], com, alpha, w[a], [](float x) { return swap_max(x); }))
+      if (soften<false>(s[a], f, neg, wt, st[a], com, alpha, w[a], wl[a], [](float x) { return swap_max(x); }))
 #pragma unroll
         for (int j = 0; j < VD; ++j) acc[a][j] *= alpha;
     }
@@ -531,10 +540,15 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
         for (int a = 0; a < NQ; ++a) {
           const u32x4 pw = {w[a][4 * q], w[a][4 * q + 1], w[a][4 * q + 2], w[a][4 * q + 3]};
+          const u32x4 pl = {wl[a][4 * q], wl[a][4 * q + 1], wl[a][4 * q + 2], wl[a][4 * q + 3]};
 #pragma unroll
           for (int y = 0; y < 4; ++y)
             acc[a][4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                 __builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pw), acc[a][4 * d + y], 0, 0, 0);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            acc[a][4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                __builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pl), acc[a][4 * d + y], 0, 0, 0);
         }
       }
     __builtin_amdgcn_sched_barrier(0);
@@ -784,9 +798,9 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
         }
         f = 1.f, neg = false;
       }
-      uint32_t w[16];
+      uint32_t w[16], wl[16];
       float alpha;
-      if (soften<!MOD>(s, f, neg, Weight(vs, com), st, com, alpha, w, [](float x) { return swap32_max(x); }))
+      if (soften<!MOD>(s, f, neg, Weight(vs, com), st, com, alpha, w, wl, [](float x) { return swap32_max(x); }))
 #pragma unroll
         for (int j = 0; j < ND; ++j) acc[j] *= alpha;
 #pragma unroll
@@ -794,12 +808,15 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const u32x4 pw = {w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]};
+        const u32x4 pl = {wl[4 * g], wl[4 * g + 1], wl[4 * g + 2], wl[4 * g + 3]};
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
           read_v(g * ND + j + AHEAD);
           __builtin_amdgcn_sched_barrier(0);
           acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, b[g * ND + j]),
                                                           __builtin_bit_cast(f16x8_t, pw), acc[j], 0, 0, 0);
+          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, b[g * ND + j]),
+                                                          __builtin_bit_cast(f16x8_t, pl), acc[j], 0, 0, 0);
         }
       }
     }
