@@ -490,8 +490,9 @@ int kvskip_cache_write(const kvskip_write_args* p, void* stream);
 
 /* ---- Attention of the rows that a step brings, over 8-bit pages (none of it in the reference).
  *
- * Request b brings the rows [starts[b], starts[b + 1]) of the call's `rows` rows (clamped to them), the last of its
- * seq_lens[b] tokens (clamped to [0, T]); its tokens lie in the pages of its block table row, T / 64 of them at most. Where
+ * Request b brings the rows [starts[b], starts[b + 1]), the last of its seq_lens[b] tokens (clamped to [0, T]): row
+ * starts[b + 1] - 1 is its last token, whether or not the row is among the call's `rows`, and those that are not are left out
+ * (a start past 2^28 counts as 2^28). Its tokens lie in the pages of its block table row, T / 64 of them at most. Where
  * shared_of[b] is in [0, shared), the shared_lens[shared_of[b]] tokens (clamped to [0, shared_T]) of that prefix come before
  * them, in the pages of the prefix's own table row. Position 0 is the first token of all. A row at position p sees the key at
  * position j of its request where

@@ -41,14 +41,16 @@ struct Group {
 };
 
 struct Request {
-  int first, n, len, base, pre, group;  // group -1: behind no prefix
-  __device__ int pos0() const { return base + len - n; }
+  int first, n, end, len, base, pre, group;  // its rows among the call's; the row after its last; group -1: behind no prefix
+  __device__ int pos0() const { return base + len - (end - first); }
 };
+constexpr int MOST_END = 1 << 28;  // (no request has more tokens and rows before them: positions stay in 32 bits)
 
 __device__ __forceinline__ Request request(const PlanP& p, int b) {
   Request r;
   r.first = min(max(p.a.starts[b], 0), p.a.rows);
-  r.n = min(max(p.a.starts[b + 1], r.first), p.a.rows) - r.first;
+  r.end = min(p.a.starts[b + 1], MOST_END);
+  r.n = min(max(r.end, r.first), p.a.rows) - r.first;
   r.len = min(max(p.a.seq_lens[b], 0), p.a.T);
   r.group = p.a.shared > 0 ? p.a.shared_of[b] : -1;
   if (r.group < 0 || r.group >= p.a.shared) r.group = -1;
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
     int count = 0;
     for (int b0 = 0; b0 < B; b0 += PT) {
       const int b = b0 + tid;
-      Request r{0, 0, 0, 0, 0, -1};
+      Request r{0, 0, 0, 0, 0, 0, -1};
       if (b < B) r = request(p, b);
       const bool in = r.group == g && r.n > 0;
       int total;

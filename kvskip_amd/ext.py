@@ -178,7 +178,8 @@ def attend_plan(starts, seq_lens, rows, block_table, Hq, Hkv, max_rows=0, window
                 shared_lens=None, shared_of=None) -> AttendPlan:
     """The plan of attend() over `rows` rows (kvskip_attend_plan; not in kvskip_ext), in one launch: request b brings rows
     starts[b] .. starts[b + 1] - 1 (int32 [B + 1], rising; else no row belongs to any), the last of its seq_lens[b] tokens
-    (int32 [B], its tokens after the step), which lie in the pages of block_table[b] (int32 [B, pages]).
+    (int32 [B], its tokens after the step), which lie in the pages of block_table[b] (int32 [B, pages]). Rows of starts outside
+    0 .. rows - 1 are left out; the others' positions do not depend on that.
 
     A row sees the keys of its request up to its own, with window > 0 the last `window` of them only, and besides the first
     prefix_lens[b] keys (int32 [B]) wherever they lie. shared_table (int32 [P, pages]), shared_lens (int32 [P]), shared_of

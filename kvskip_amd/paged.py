@@ -107,7 +107,8 @@ class PagedCache:
 
     def plan(self, rows: int, Hq: int, max_rows: int = 0, window: int = 0, prefix_lens: torch.Tensor | None = None):
         """The plan of attend() for the last step's rows (kvskip.attend_plan), once for all layers that share a window; rows:
-        those of the q that attend() will be given. Rows past the step's come back as zeros; what those of a request that the
+        those of the q that attend() will be given. Rows past the step's come back as zeros, and of a step with more only the
+        first `rows` are attended; what those of a request that the
         step did not serve come back as means nothing. max_rows: the most rows that one request is expected to bring (0: all)."""
         return K.attend_plan(self.starts, self.lens, rows, self.block_table, Hq, self.Hkv, max_rows, window, prefix_lens,
                              self.shared_table, self.shared_lens, self.shared_of)

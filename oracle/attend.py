@@ -11,14 +11,14 @@ PAGE = 64
 
 
 def positions(starts, lens, rows, shared_lens=None, shared_of=None):
-    """Each row's position, -1 of a row that no request brings."""
+    """Each row's position, -1 of a row that no request brings: a request's last token is in row starts[b + 1] - 1, there or not."""
     pos = [-1] * rows
     if all(a <= b for a, b in zip(starts, starts[1:])):
         for b, n in enumerate(lens):
             s0, s1 = (min(max(x, 0), rows) for x in starts[b:b + 2])
             base = _base(shared_lens, shared_of, b)
             for i in range(s0, s1):
-                pos[i] = base + max(n, 0) - (s1 - s0) + i - s0
+                pos[i] = base + max(n, 0) - min(starts[b + 1], 1 << 28) + i
     return pos
 
 
