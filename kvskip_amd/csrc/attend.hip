@@ -148,11 +148,12 @@ struct Common {
 };
 // A page's vs. plain: a positive number of middling size, and not 2^40 below another one.
 struct Weight {
-  float vs, lv, ev;
+  float part, lv, ev;  // vs = part 2^ev
   bool plain;
-  __device__ Weight(float v, Common& w) : vs(v) {
+  __device__ Weight(float v, Common& w) {
     const int e = static_cast<int>(__float_as_uint(v) >> 23);  // (a negative one from 256 on)
-    const int x = max((e & 0xff) - 127, -100);
+    const int x = max((e & 0xff) - 127, -126);
+    part = ldexpf(v, -x);
     w.top = max(w.top, x);
     plain = e >= 27 && e <= 227 && x >= w.top - 40 && !w.odd;
     lv = flog2(v);
@@ -275,7 +276,7 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
     f = 1.f;
   }
   // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
-  const float fv = mt == NEG_INF ? 0.f : v.vs * fexp2((mt - st.ar) - st.ax) * 0x1p7f;
+  const float fv = mt == NEG_INF ? 0.f : v.part * fexp2(((mt - st.ar) + (v.ev - st.ax)) + 7.f);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
@@ -599,8 +600,9 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
     for (int w = 0; w < NWAVE; ++w) {
       const float mw = m[w] == NEG_INF ? 0.f : m[w];
+      const float x = fexp2(0.5f * ((mw - mu) + L.x[w][row]));  // (twice: with vs near 2^-126 the whole is below what is held)
       l += L.l[w][row] * fexp2(m[w] - mu);
-      a += *reinterpret_cast<const f32x4_t*>(&L.acc[w][row][d]) * fexp2((mw - mu) + L.x[w][row]);
+      a += *reinterpret_cast<const f32x4_t*>(&L.acc[w][row][d]) * x * x;
     }
     store4(p, u, h, row, virtual_row(p, u, h, row), d, D, a, M, l);
   }
@@ -840,13 +842,13 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   const float l = swap32_sum(st.l);
   if (i0 >= u.nv) return;
   const float mu = st.m == NEG_INF ? 0.f : st.m;
-  const float x = st.ar == NEG_INF ? 0.f : fexp2((st.ar - mu) + (st.ax - 7.f));
+  const float x = st.ar == NEG_INF ? 0.f : fexp2(0.5f * ((st.ar - mu) + (st.ax - 7.f)));  // (twice, as in small tiles)
 #pragma unroll
   for (int j = 0; j < ND; ++j)
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
       store4(p, u, h, i0, r, 32 * j + 2 * i + 4 * half, D,
-             f32x4_t{acc[j][i] * x, acc[j][i + 1] * x, acc[j][i + 2] * x, acc[j][i + 3] * x}, st.m, l);
+             f32x4_t{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]} * x * x, st.m, l);
   if (I8 || L.nan == 0) return;
   // NaN of cut pages over what was stored
   for (int k = 0; k < n; ++k) {

@@ -1,0 +1,36 @@
+"""GPU: attention over a step's rows at the ends of what its scales can be."""
+
+import pytest
+import torch
+
+from attend_side import Step, check
+
+pytestmark = pytest.mark.gpu
+
+
+def check_any_size(r, ref, D, what):
+    """attend_side.check, for results of any size. Its bound has half a step of a bf16 as 2^-8 of the value, which holds from 2^-126 on:
+    below, bf16's step is 2^-133 whatever the value, so a result rounded right is off by up to 2^-134."""
+    out, lse, mass, reach, grain = ref
+    ds = (D + 8) * 2.0 ** -23 * reach
+    got = r["out"].double().cpu()
+    tol = (2 * ds[..., None] + 2.0 ** -11 + 2.0 ** -16) * mass + 2.0 ** -32 * grain + 2.0 ** -8 * out.abs() + 2.0 ** -134
+    bad = ~((got - out).abs() <= tol)
+    assert not bad.any(), (what, bad.sum().item(), bad.nonzero()[:4].tolist())
+    check(dict(out=ref[0], lse=r["lse"]), ref, D, what)          # (places and lse)
+
+
+@pytest.mark.parametrize("fmt,Hq,Hkv,D", [("int8", 8, 2, 128), ("e4m3", 8, 2, 64)])
+@pytest.mark.parametrize("exps", [(-126, -126), (-121, -101), (-130, -126), (-126, 20), (100, 118)])
+def test_value_scales_of_any_size(gpu, exps, fmt, Hq, Hkv, D):
+    """V's scales from the smallest that rows are written with (and below, where fp32 holds fewer bits) to the largest: as exact
+    as others."""
+    for most, reqs in ((0, [(64 * 9, 150), (64 * 3 + 5, 1)]), (1, [(64 * 9, 1), (64 * 30 + 5, 1)])):
+        s = Step(reqs, Hq, Hkv, D, fmt, 41)
+        g = torch.Generator().manual_seed(42)
+        e = torch.randint(exps[0], exps[1] + 1, s.vs.shape, generator=g)
+        s.vs = torch.ldexp(torch.ones(s.vs.shape, dtype=torch.float64), e).float()
+        s.q *= 4                                              # weights far apart
+        ref = s.exact()
+        assert (s.vs > 0).all() and ref[0].isfinite().all() and (ref[2] > 0).any()
+        check_any_size(s.call(s.plan(max_rows=most)), ref, D, (exps, most))
