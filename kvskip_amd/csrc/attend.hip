@@ -1009,7 +1009,10 @@ hipError_t launch_attend(const kvskip_attend_args& a, const AttendSizes& z, hipS
   p.rows = reinterpret_cast<const AttendRow*>(work + z.at_rows);
   p.n_rows = a.plan.rows, p.Hq = a.plan.Hq, p.Hkv = a.plan.Hkv, p.G = a.plan.Hq / a.plan.Hkv;
   p.num_pages = a.num_pages, p.window = a.plan.window < (1 << 30) ? a.plan.window : 1 << 30;
-  p.scale = a.scale, p.softcap = a.softcap;
+  p.scale = a.scale;
+  // (scores over the cap stay in fp32's range: below 2^-64 capped scores are all alike, and those that feel one above 2^96
+  // leave one key any weight)
+  p.softcap = a.softcap > 0.f ? fminf(fmaxf(a.softcap, 0x1p-64f), 0x1p96f) : 0.f;
   const bool i8 = a.format == KVSKIP_INT8;
   const hipError_t e = a.D == 128 ? (i8 ? launch_d<128, true>(p, z, s) : launch_d<128, false>(p, z, s))
                                   : (i8 ? launch_d<64, true>(p, z, s) : launch_d<64, false>(p, z, s));

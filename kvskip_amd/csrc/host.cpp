@@ -1111,7 +1111,7 @@ PyObject* attend(PyObject* const* a) {
       c.shared_table = static_cast<const int32_t*>(st->data_ptr()), c.st_stride = c.plan.shared == 1 ? st->size(1) : st->stride(0);
     c.slopes = slopes == nullptr ? nullptr : static_cast<const float*>(slopes->data_ptr());
     c.out = out.data_ptr(), c.lse = static_cast<float*>(lse.data_ptr());
-    c.scale = static_cast<float>(real(a[5])), c.softcap = static_cast<float>(cap);
+    c.scale = static_cast<float>(real(a[5])), c.softcap = static_cast<float>(cap > 0.0 ? std::max(cap, 0x1p-126) : 0.0);
     c.D = static_cast<int32_t>(D), c.num_pages = static_cast<int32_t>(k.size(0));
     launch(dev, [&](void* s) { return api.attend(&c, s); });
   }

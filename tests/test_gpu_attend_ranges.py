@@ -34,3 +34,20 @@ def test_value_scales_of_any_size(gpu, exps, fmt, Hq, Hkv, D):
         ref = s.exact()
         assert (s.vs > 0).all() and ref[0].isfinite().all() and (ref[2] > 0).any()
         check_any_size(s.call(s.plan(max_rows=most)), ref, D, (exps, most))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,most", [(8, 2, 128, 0), (8, 2, 64, 0), (8, 2, 128, 1)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_caps_of_any_size(gpu, Hq, Hkv, D, most, slopes):
+    """A cap far above every score changes none of them: 2^-60 of a score or less; one far below makes all of them equal."""
+    s = Step([(200, 1), (300, 300 if most == 0 else 1)], Hq, Hkv, D, "e4m3", 43)
+    s.k[:, :, 3] = 0.0                                        # scores of exactly 0 too
+    s.k[:, :, 9] = 0.0
+    sl = torch.linspace(0.01, 0.1, Hq) if slopes else None
+    plan = s.plan(max_rows=most)
+    for cap in (1e30, 1e37, 3.4e38):
+        check(s.call(plan, cap, sl), s.exact(0, 0.0, sl), D, cap)
+    for cap in (1e-50, 1e-45, 1e-38, 1e-37, 1e-30, 1e-15):
+        ref = s.exact(0, cap, sl)
+        check(s.call(plan, cap, sl), ref, D, cap, softcap=cap)
+        assert slopes or (ref[1].exp() - ref[1].exp().round()).abs().max() < 1e-9       # (as many keys as are seen)
