@@ -402,15 +402,15 @@ __device__ __forceinline__ void store_nan(const AttendP& p, const AttendUnit& u,
 
 // ---- Few rows: four independent wavefronts, a page a step each, no barrier but the one before their states are joined. Keys
 // come from memory as operands and become fp16 in registers (the layouts of attn_decode8.hip), 16 rows a product.
-template <int D, int NQ>
+template <int D>
 struct Few {
-  float acc[NWAVE][16 * NQ][D];
-  float m[NWAVE][16 * NQ], l[NWAVE][16 * NQ], x[NWAVE][16 * NQ];
+  float acc[NWAVE][TILE_FEW][D];
+  float m[NWAVE][TILE_FEW], l[NWAVE][TILE_FEW], x[NWAVE][TILE_FEW];
 };
 
-template <int D, int NQ, bool I8, bool MOD>
-__device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, int h, Few<D, NQ>& L) {
-  static_assert(NQ == 1);
+template <int D, bool I8, bool MOD>
+__device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, int h, Few<D>& L) {
+  static_assert(TILE_FEW == 16, "rows of a product");
   constexpr int KC = Lay8<D>::KC, KS = Lay8<D>::KS, VN = Lay8<D>::VN, VD = Lay8<D>::VD;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
   const int j4 = lane >> 4, c16 = lane & 15;
@@ -430,36 +430,30 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
   load_k8<D>(kr, res(kb, p.k_sb, p.k_st, blk, pg), koff, p.k_st);
   load_v8<D>(vr, res(vb, p.v_sb, p.v_st, blk, pg), voff, p.v_st);
 
-  u32x4 qh[NQ][KS];
-  float qf[NQ], slope[NQ];
-  Sight see[NQ];
-  int at[NQ];  // the row's own index, less the lane's first token
-  State st[NQ] = {State(false)};
-  Common com;
-  Reach re;
-#pragma unroll
-  for (int a = 0; a < NQ; ++a) {
-    const Row r = virtual_row(p, u, h, 16 * a + c16);
+  const Row r = virtual_row(p, u, h, c16);
+  u32x4 qh[KS];
+  float qf;
+  {
     const uint16_t* qp = p.q + r.n * p.q_sn + r.hq * p.q_sh + 16 * j4;
     float amax = 0.f, bad = 0.f, up;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qh[a][ks] = ld16(qp + 64 * (ks / 2) + 8 * (ks % 2));
+    for (int x = 0; x < KS; ++x) qh[x] = ld16(qp + 64 * (x / 2) + 8 * (x % 2));
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) q_extent(qh[a][ks], amax, bad);
-    qf[a] = q_factor(swap_max(amax), swap_sum(bad), up) * (MOD ? p.scale : p.scale * LOG2E);
+    for (int x = 0; x < KS; ++x) q_extent(qh[x], amax, bad);
+    qf = q_factor(swap_max(amax), swap_sum(bad), up) * (MOD ? p.scale : p.scale * LOG2E);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qh[a][ks] = q_half(qh[a][ks], up);
-    see[a] = sight(p, u, r);
-    at[a] = r.pos - u.base - 4 * j4;
-    slope[a] = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
-    re = a == 0 ? reach(see[a]) : both(re, reach(see[a]));
+    for (int x = 0; x < KS; ++x) qh[x] = q_half(qh[x], up);
   }
+  const Sight see = sight(p, u, r);
+  const Reach re = reach(see);
+  const int at = r.pos - u.base - 4 * j4;  // the row's own index, less the lane's first token
+  const float slope = MOD && p.slopes != nullptr ? p.slopes[r.hq] : 0.f;
+  State st(false);
+  Common com;
   bool nan = false;  // a cut page held one
-  f32x4_t acc[NQ][VD];
+  f32x4_t acc[VD];
 #pragma unroll
-  for (int a = 0; a < NQ; ++a)
-#pragma unroll
-    for (int j = 0; j < VD; ++j) acc[a][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < VD; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
   for (int k = 0; k < nw; ++k) {
     list.advance(k);
@@ -467,25 +461,18 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
     list.turn(k);
     int blk_n = -1, pg_n = -1;
     if (k + 1 < nw) blk_n = list.blk(k + 1), pg_n = list.pg(k + 1);
-    float s[NQ][16];
+    float s[16];
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
-      u32x4 w[KS];
+      f32x4_t c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int x = 0; x < KS; ++x) {
         const u32x2 w0 = widen4<I8>(kr[nt][x / 2][2 * (x % 2)]), w1 = widen4<I8>(kr[nt][x / 2][2 * (x % 2) + 1]);
-        w[x] = u32x4{w0.x, w0.y, w1.x, w1.y};
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, u32x4{w0.x, w0.y, w1.x, w1.y}),
+                                                   __builtin_bit_cast(f16x8_t, qh[x]), c, 0, 0, 0);
       }
 #pragma unroll
-      for (int a = 0; a < NQ; ++a) {
-        f32x4_t c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int x = 0; x < KS; ++x)
-          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[x]), __builtin_bit_cast(f16x8_t, qh[a][x]), c,
-                                                     0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[a][4 * nt + i] = c[i];
-      }
+      for (int i = 0; i < 4; ++i) s[4 * nt + i] = c[i];
     }
     __builtin_amdgcn_sched_barrier(0);
     load_k8<D>(kr, res(kb, p.k_sb, p.k_st, blk_n, pg_n), koff, p.k_st);
@@ -500,31 +487,26 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
         for (int i = 0; i < VN; ++i) vr[i] = u32x2{without_nan(vr[i].x, any), without_nan(vr[i].y, any)};
         nan |= __ballot(any != 0) != 0;
       }
-    const Weight wt(vs, com);
-    uint32_t w[NQ][8], wl[NQ][8];
-#pragma unroll
-    for (int a = 0; a < NQ; ++a) {
-      float f = qf[a] * ks;
-      bool neg = (__float_as_int(ks) ^ __float_as_int(p.scale)) < 0;  // uniform
-      if constexpr (MOD) {
-        modify(s[a], f, p.softcap, p.slopes != nullptr, slope[a], static_cast<float>(at[a] - t0),
-               [](int i) { return static_cast<float>(16 * (i / 4) + i % 4); });
-        f = 1.f;
-        neg = false;
-      }
-      if (!whole || pg < 0) {  // uniform
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = t0 + mf_tok(i / 4, i % 4, j4);
-          s[a][i] = (sees(see[a], t) & (pg >= 0)) ? s[a][i] * f : NEG_INF;
-        }
-        f = 1.f, neg = false;
-      }
-      float alpha;
-      if (soften<false>(s[a], f, neg, wt, st[a], com, alpha, w[a], wl[a], [](float x) { return swap_max(x); }))
-#pragma unroll
-        for (int j = 0; j < VD; ++j) acc[a][j] *= alpha;
+    float f = qf * ks;
+    bool neg = (__float_as_int(ks) ^ __float_as_int(p.scale)) < 0;  // uniform
+    if constexpr (MOD) {
+      modify(s, f, p.softcap, p.slopes != nullptr, slope, static_cast<float>(at - t0),
+             [](int i) { return static_cast<float>(16 * (i / 4) + i % 4); });
+      f = 1.f, neg = false;
     }
+    if (!whole || pg < 0) {  // uniform
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = t0 + mf_tok(i / 4, i % 4, j4);
+        s[i] = (sees(see, t) & (pg >= 0)) ? s[i] * f : NEG_INF;
+      }
+      f = 1.f, neg = false;
+    }
+    uint32_t w[8], wl[8];
+    float alpha;
+    if (soften<false>(s, f, neg, Weight(vs, com), st, com, alpha, w, wl, [](float x) { return swap_max(x); }))
+#pragma unroll
+      for (int j = 0; j < VD; ++j) acc[j] *= alpha;
 #pragma unroll
     for (int d = 0; d < VD / 4; ++d)
 #pragma unroll
@@ -538,19 +520,16 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
           const u32x2 w23 = widen4<I8>(__builtin_amdgcn_perm(c, a, 0x07030602u));
           x[0][y] = w01.x, x[1][y] = w01.y, x[2][y] = w23.x, x[3][y] = w23.y;
         }
+        const u32x4 pw = {w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
+        const u32x4 pl = {wl[4 * q], wl[4 * q + 1], wl[4 * q + 2], wl[4 * q + 3]};
 #pragma unroll
-        for (int a = 0; a < NQ; ++a) {
-          const u32x4 pw = {w[a][4 * q], w[a][4 * q + 1], w[a][4 * q + 2], w[a][4 * q + 3]};
-          const u32x4 pl = {wl[a][4 * q], wl[a][4 * q + 1], wl[a][4 * q + 2], wl[a][4 * q + 3]};
+        for (int y = 0; y < 4; ++y)
+          acc[4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pw),
+                                                                  acc[4 * d + y], 0, 0, 0);
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-            acc[a][4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                __builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pw), acc[a][4 * d + y], 0, 0, 0);
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            acc[a][4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                __builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pl), acc[a][4 * d + y], 0, 0, 0);
-        }
+        for (int y = 0; y < 4; ++y)
+          acc[4 * d + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, x[y]), __builtin_bit_cast(f16x8_t, pl),
+                                                                  acc[4 * d + y], 0, 0, 0);
       }
     __builtin_amdgcn_sched_barrier(0);
     load_v8<D>(vr, res(vb, p.v_sb, p.v_st, blk_n, pg_n), voff, p.v_st);
@@ -560,34 +539,30 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 
   // ---- the four states joined: lane (c16, j4) holds row c16's dims mf_vdim(4 j4 + i) + j
 #pragma unroll
-  for (int a = 0; a < NQ; ++a) {
-    const int row = 16 * a + c16;
+  for (int i = 0; i < 4; ++i) {
+    float* o = L.acc[wave][c16] + mf_vdim<D>(4 * j4 + i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float* o = L.acc[wave][row] + mf_vdim<D>(4 * j4 + i);
-#pragma unroll
-      for (int j = 0; j < VD; j += 4)
-        *reinterpret_cast<float4*>(o + j) = make_float4(acc[a][j][i], acc[a][j + 1][i], acc[a][j + 2][i], acc[a][j + 3][i]);
-    }
-    const float l = swap_sum(st[a].l);
-    if (j4 == 0) {
-      const float mu = st[a].m == NEG_INF ? 0.f : st[a].m;
-      L.m[wave][row] = st[a].m, L.l[wave][row] = l;
-      L.x[wave][row] = st[a].ar == NEG_INF ? NEG_INF : (st[a].ar - mu) + (st[a].ax - 7.f);
-    }
+    for (int j = 0; j < VD; j += 4)
+      *reinterpret_cast<float4*>(o + j) = make_float4(acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]);
+  }
+  const float sum = swap_sum(st.l);
+  if (j4 == 0) {
+    const float mu = st.m == NEG_INF ? 0.f : st.m;
+    L.m[wave][c16] = st.m, L.l[wave][c16] = sum;
+    L.x[wave][c16] = st.ar == NEG_INF ? NEG_INF : (st.ar - mu) + (st.ax - 7.f);
   }
   if (!I8 && nan)  // NaN of cut pages
     for (int k = 0; k < nw; ++k) {
       const int i0 = u.i0 + wave + NWAVE * k, b = i0 < u.a1 ? i0 : i0 - u.a1 + u.b0, g = list.table[b];
       if (g < 0 || g >= p.num_pages || sees_keys(re, b * BLK, u.len)) continue;
-      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t)
+      for (int t = b * BLK; t < min(b * BLK + BLK, u.len); ++t) {
+        if (!sees(see, t)) continue;
         for (int d = 4 * j4; d < D; d += 16) {
           const uint32_t z = nan_bytes(*reinterpret_cast<const uint32_t*>(vb + g * p.v_sb + (t - b * BLK) * p.v_st + d));
-#pragma unroll
-          for (int a = 0; a < NQ; ++a)
-            for (int e = 0; e < 4; ++e)
-              if (sees(see[a], t) && (z >> (8 * e + 7) & 1) != 0) L.acc[wave][16 * a + c16][d + e] = __builtin_nanf("");
+          for (int e = 0; e < 4; ++e)
+            if ((z >> (8 * e + 7) & 1) != 0) L.acc[wave][c16][d + e] = __builtin_nanf("");
         }
+      }
     }
   __syncthreads();
   for (int o = tid; o < u.nv * (D / 4); o += NT) {
@@ -866,9 +841,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
 // 64 (two: prompts of 2111 behind a prefix 174 us for 154).
 template <int D, bool I8, bool MOD, bool LARGE>
 __global__ void __launch_bounds__(NT, D == 128 ? 2 : 3) attend_kernel(const AttendP p) {
-  constexpr int NQ = TILE_FEW / 16;
-  __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D, NQ>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D, NQ>)
-                                                                                                        : sizeof(Many<D>)];
+  __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D>) : sizeof(Many<D>)];
   const int i = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   const AttendUnit u = p.units[i];  // (the grid is as long as the array: not waited for twice)
   if (i >= p.head[H_UNITS]) return;
@@ -878,7 +851,7 @@ __global__ void __launch_bounds__(NT, D == 128 ? 2 : 3) attend_kernel(const Atte
       return;
     }
   }
-  few_rows<D, NQ, I8, MOD>(p, u, h, *reinterpret_cast<Few<D, NQ>*>(raw));
+  few_rows<D, I8, MOD>(p, u, h, *reinterpret_cast<Few<D>*>(raw));
 }
 
 // The join: a workgroup takes runs of up to 8 virtual rows of a joined tile and KV head, a thread four dims of a row and a class

@@ -34,7 +34,6 @@ struct alignas(16) AttendUnit {
 };
 static_assert(sizeof(AttendUnit) == 64, "a unit is one line");
 
-
 constexpr int JOIN_ROWS = 8;
 struct alignas(16) AttendJoin {  // a run of virtual rows whose partial results are added up
   int row0, v0, n;               // first row of the request; virtual rows [v0, v0 + n)
@@ -59,9 +58,9 @@ struct AttendSizes {  // (host)
   int64_t at_units, at_joins, at_tiles, at_rows, total;
 };
 
-// The workspace's first elements: units, joins, the requests' first row and the one after their last, pages of a unit.
+// The workspace's first elements: units, joins, the requests' first row and the one after their last.
 constexpr int HEAD = 16;
-enum { H_UNITS = 0, H_JOINS = 1, H_FIRST = 2, H_LAST = 3, H_CHUNK = 4 };
+enum { H_UNITS = 0, H_JOINS = 1, H_FIRST = 2, H_LAST = 3 };
 
 AttendSizes attend_sizes(const kvskip_attend_plan_args& p);
 

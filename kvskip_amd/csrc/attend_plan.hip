@@ -309,7 +309,6 @@ __global__ void __launch_bounds__(PT) attend_plan_kernel(const PlanP p) {
     work[H_JOINS] = n_joins;
     work[H_FIRST] = first;
     work[H_LAST] = last;
-    work[H_CHUNK] = chunk;
   }
   __syncthreads();
   for (int t = tid; t < n_tiles; t += PT) {
