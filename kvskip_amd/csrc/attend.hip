@@ -9,8 +9,8 @@
 // are two fp16 parts, 2^-23 of each, taken relative to a reference that the largest weight times |vs| so far passes by 2^8 at
 // most (accumulators are rescaled only when a page passes that); sums and statistics are fp32. (One part, 2^-12, shows beside
 // bf16 results, more where values cancel: 2^-10 of a result in the norm from a softmax in fp32, for 2^-14. The second one
-// costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2210 us for 1665, 64 tokens behind a prefix of 8192 48.5 for
-// 42.2. Its order among the products makes no difference.)
+// costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2258 us for 1717, 64 tokens behind a prefix of 8192 48.5 for
+// 43.0. Its order among the products makes no difference.)
 #include "codes8.hpp"
 #include "attend.hpp"
 
@@ -587,11 +587,12 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 // multiplied the next one's codes are on their way and converted, once for all rows. 32 x 32 products: K as it lies in
 // LDS, V by transposing reads. Chunks of 16 bytes are placed so that neither reads nor writes conflict: K chunk c of
 // row r at c ^ r, V's at c ^ 5 (r % 4) (64 dims: r / 2 in both).
-//   Vector instructions bound it: beside products, which take the matrix unit 1024 clocks a page of 128 dims and wavefront,
-// vector instructions run at half their rate or so, and two wavefronts a SIMD take turns at best. So: operands asked for four
-// products ahead (read and waited for one by one, prompts of 8192 took 1850 us, for 1780), addresses that a page's turn
-// does not change (two pages a turn, 1745 to 1737), maxima only where they are needed (1650), and nothing in the loop that waits for
-// the codes asked for last (the page list in groups).
+//   Products and vector instructions bound it together: products take the matrix unit 1536 clocks a page of 128 dims and wavefront,
+// beside them vector instructions run at half their rate or so, and two wavefronts a SIMD take turns at best (prompts of 8192:
+// 2258 us, the matrix units busy for half of the clocks). So: operands asked for four products ahead (read and waited for one by one,
+// prompts took 1850 us with one part a weight, for 1780), addresses that a page's turn does not change (two pages a turn,
+// 1745 to 1737), maxima only where they are needed (1650), and nothing in the loop that waits for the codes asked for last (the
+// page list in groups).
 template <int D>
 struct Many {
   uint8_t k[2][BLK * D * 2], v[2][BLK * D * 2];
@@ -838,7 +839,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
 }
 
 // Workgroups a CU: two for 128 dims (with three they spill 40 registers, 24 tokens behind a window of 4096 63.7 us for 47.2), three for
-// 64 (two: prompts of 2111 behind a prefix 174 us for 154).
+// 64 (two, with one part a weight: prompts of 2111 behind a prefix 174 us for 154; with two parts large tiles spill 6 registers).
 template <int D, bool I8, bool MOD, bool LARGE>
 __global__ void __launch_bounds__(NT, D == 128 ? 2 : 3) attend_kernel(const AttendP p) {
   __shared__ __attribute__((aligned(16))) uint8_t raw[sizeof(Few<D>) > (LARGE ? sizeof(Many<D>) : 0) ? sizeof(Few<D>) : sizeof(Many<D>)];

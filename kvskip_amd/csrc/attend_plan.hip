@@ -24,10 +24,10 @@ constexpr int CLASSES = 32;
 // with 1024 units in about two rounds, 39.0; 16 tokens of up to 32000 54.3, 47.4; one of 32768 33.9, 24.0.)
 constexpr int SLOTS = 512;
 constexpr int TARGET_UNITS = 2 * SLOTS;  // units of a queued plan: those that end early take another
-constexpr int LEAST_PAGES = 4;           // of a unit: its four wavefronts take a page each
-// Of a unit of a queued plan: partial results cost more than a shorter last round saves. (Least 4, 16 and 32, us: 9 prompts of up to
-// 763 behind bidirectional prefixes 86.5, 63.5, 63.3; 7 of up to 1412 in a window of 234 72, 43, 43; 64 tokens behind a prefix
-// of 8192 46.8, 42, 61.)
+constexpr int LEAST_PAGES = 4;           // of a chunk: a unit's four wavefronts take a page each
+// Of a chunk of a queued plan: partial results cost more than a shorter last round saves. (Least 4, 16 and 32, us, with one part a
+// weight: 9 prompts of up to 763 behind bidirectional prefixes 86.5, 63.5, 63.3; 7 of up to 1412 in a window of 234 72, 43, 43; 64
+// tokens behind a prefix of 8192 46.8, 42, 61.) A tile is cut evenly into ceil(pages / chunk) units, which hold half a chunk or more.
 constexpr int LEAST_QUEUED = 16;
 
 struct PlanP {

@@ -23,7 +23,10 @@ Prefixes that requests share (an instruction, a document) are held once, in page
     cache.shared_of.zero_()                      # int32 [requests]: the prefix that each request is behind, -1 none
 
 Nothing synchronises: a step can be captured in a HIP graph and replayed. What is allocated after the construction comes from
-torch's allocator: decode's outputs and split partials, and in a step of more than 4096 rows page_map's workspace. cache.short
+torch's allocator: decode's outputs and split partials, in a step of more than 4096 rows page_map's workspace, a plan's
+workspace (50 KB for 256 single tokens, 1 to 3 MB for 32768 rows), and attend's outputs and partial results: up to 137 MB at 128
+dims, and in a cache with shared prefixes 8 * rows * Hq * D bytes more (1.1 GB at 32768 rows of 32 heads of 128 dims), whether
+or not a request is behind one. cache.short
 (int32 [1], on the device) counts the requests that the last step had no pages or rows for: their rows are not written, they
 keep the tokens they had, and a caller that admits requests without counting pages reads it now and then."""
 
@@ -118,7 +121,8 @@ class PagedCache:
         return K.attend(q, *self.pools[layer], scale, plan, *self.scales[layer], **kw)
 
     def plan_prefix(self, prefix: int, n: int, Hq: int, window: int = 0):
-        """Shared prefix `prefix` has n tokens from now on; the plan of attend() for its own n rows, from position 0 on."""
+        """Shared prefix `prefix` has n tokens from now on; the plan of attend() for its own n rows, from position 0 on: all of a
+        prefix in one call."""
         if not (0 <= prefix < len(self.shared) and 1 <= n <= self.shared[prefix]):
             raise ValueError(f"prefix in 0..{len(self.shared) - 1}, n in 1..its capacity (got {prefix}, {n})")
         self.shared_lens[prefix].fill_(n)
