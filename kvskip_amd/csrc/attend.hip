@@ -6,8 +6,8 @@
 // own registers and one or two lane swaps, and its weights are already the operand of O^T = V^T P^T (any order of the
 // keys will do inside a product, as long as V's operand has the same). Codes become fp16, which holds them exactly; q is
 // fp16 times a power of two of its row (2^14 <= largest < 2^15: exact, but for what lies below 2^-39 of that); weights
-// are two fp16 parts, 2^-23 of each, taken relative to a reference that the largest weight times |vs| so far passes by 2^8 at
-// most (accumulators are rescaled only when a page passes that); sums and statistics are fp32. (One part, 2^-12, shows beside
+// are two fp16 parts, 2^-23 of each but for what lies below 2^-35 of the row's largest weight times |vs|, taken relative to a
+// reference that this passes by 2^6 at most (accumulators are rescaled only when a page passes that); sums and statistics are fp32. (One part, 2^-12, shows beside
 // bf16 results, more where values cancel: 2^-10 of a result in the norm from a softmax in fp32, for 2^-14. The second one
 // costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2258 us for 1717, 64 tokens behind a prefix of 8192 48.5 for
 // 43.0. Its order among the products makes no difference.)
@@ -136,7 +136,10 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& any) {
 
 // Running state of a row. m: a score in log2 units, the row's largest when the state was last looked at; l: this lane's part of
 // sum 2^(s - m). ar + ax: the accumulators' reference, a score and the exponent of its page's vs (apart, since in one float a large
-// score takes the exponent's bits). c and d: 7 - ax - ar (while the row has seen nothing: infinite, or 0) and ar + ax - 7 - m.
+// score takes the exponent's bits). c and d: LIFT - ax - ar (while the row has seen nothing: infinite, or 0) and ar + ax - LIFT - m.
+//   LIFT: the exponent in fp16, whose finest is 2^-24, of a weight at the reference. (7 and 10 take the same time within 1 %; beside a key
+// of value 0 with most of a row's weight, weights 2^-26 below it are off by 2^-6 each with 7 at worst, by 2^-9 with 10.)
+constexpr int LIFT = 10;
 struct State {
   float m = NEG_INF, l = 0.f, ar = NEG_INF, ax = 0.f, c, d = 0.f;
   __device__ explicit State(bool blind) : c(blind ? -NEG_INF : 0.f) {}
@@ -217,14 +220,14 @@ __device__ __forceinline__ void two_parts(float x, float y, uint32_t& hi, uint32
   lo = mix_h(x, y, 1.f, -__builtin_bit_cast(f16x2_t, hi));
 }
 
-// One page of a row: s in, w + wl = 2^7 p vs / 2^(ar + ax) as fp16 pairs out, tokens in order; s f is the score in log2 units (neg: f <
+// One page of a row: s in, w + wl = 2^LIFT p vs / 2^(ar + ax) as fp16 pairs out, tokens in order; s f is the score in log2 units (neg: f <
 // 0). alpha: the factor of the accumulators, true if it is not 1 for all.
 //   The plain way takes 2^(s f + c + log2 vs) at once, from which l is found too: an fma, an exponential, a sum and one and a
 // half conversions a score. Its one rounding more, of c + log2 vs, is 2^-14 at most where no reference passes 2^10; and no weight that
 // l could feel is below 2^-126: a score at most 2^60 below the row's largest lies at most 2^64 below ar, and vs at most 2^40
 // below 2^ax. It holds while no weight leaves fp16. BLIND: taken without the page's largest score, and taken back where a lane's
-// sum passes 2^15 (or is NaN: a row's first keys, whose c is infinite, and masked ones before them); else only after the
-// reference has been moved to where no weight passes 2^14.
+// sum passes fp16's largest (or is NaN: a row's first keys, whose c is infinite, and masked ones before them); else only after the
+// reference has been moved to where no weight passes 2^15.
 //   Elsewhere weights are taken relative to the page's largest score and multiplied by their factor.
 template <bool BLIND, int N, class F>
 __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const Weight& v, State& st, Common& com, float& alpha,
@@ -243,14 +246,14 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
   };
   if (BLIND && v.plain && !com.odd) {  // uniform
     const float all = plain();
-    if (__ballot(!(all <= 0x1p15f)) == 0) {
+    if (__ballot(!(all <= 65504.f)) == 0) {
       st.l = fmaf(all, fexp2(st.d - v.lv), st.l);
       return false;
     }
   }
   const float mt = neg ? swap(-least_of(s)) * -f : swap(most_of(s)) * f;
   const float past = (mt - st.ar) + (v.ev - st.ax);  // (NaN, which passes nothing, where nothing came yet)
-  const bool move = BLIND || __ballot((past > 7.f) | (mt > st.m + 4.f)) != 0;
+  const bool move = BLIND || __ballot((past > 14.f - LIFT) | (mt > st.m + 4.f)) != 0;
   if (move) {
     const bool on = past > 0.f;
     alpha = on ? fexp2(-past) : 1.f;
@@ -260,8 +263,8 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
     st.l *= fexp2(st.m - mu);
     st.m = m;
     const bool none = st.ar == NEG_INF;
-    st.c = none ? (BLIND ? -NEG_INF : 0.f) : (7.f - st.ax) - st.ar;
-    st.d = none ? 0.f : ((st.ar - mu) + st.ax) - 7.f;
+    st.c = none ? (BLIND ? -NEG_INF : 0.f) : (LIFT - st.ax) - st.ar;
+    st.d = none ? 0.f : ((st.ar - mu) + st.ax) - LIFT;
     com.odd |= __ballot(!none & (fabsf(st.ar) > 0x1p10f)) != 0;
   }
   if (!BLIND && v.plain && !com.odd) {  // uniform
@@ -276,7 +279,7 @@ __device__ __forceinline__ bool soften(float (&s)[N], float f, bool neg, const W
     f = 1.f;
   }
   // below 2^15 (none for a row that sees nothing of the page, whatever vs is)
-  const float fv = mt == NEG_INF ? 0.f : v.part * fexp2(((mt - st.ar) + (v.ev - st.ax)) + 7.f);
+  const float fv = mt == NEG_INF ? 0.f : v.part * fexp2(((mt - st.ar) + (v.ev - st.ax)) + LIFT);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
@@ -549,7 +552,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
   if (j4 == 0) {
     const float mu = st.m == NEG_INF ? 0.f : st.m;
     L.m[wave][c16] = st.m, L.l[wave][c16] = sum;
-    L.x[wave][c16] = st.ar == NEG_INF ? NEG_INF : (st.ar - mu) + (st.ax - 7.f);
+    L.x[wave][c16] = st.ar == NEG_INF ? NEG_INF : (st.ar - mu) + (st.ax - LIFT);
   }
   if (!I8 && nan)  // NaN of cut pages
     for (int k = 0; k < nw; ++k) {
@@ -818,7 +821,7 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   const float l = swap32_sum(st.l);
   if (i0 >= u.nv) return;
   const float mu = st.m == NEG_INF ? 0.f : st.m;
-  const float x = st.ar == NEG_INF ? 0.f : fexp2(0.5f * ((st.ar - mu) + (st.ax - 7.f)));  // (twice, as in small tiles)
+  const float x = st.ar == NEG_INF ? 0.f : fexp2(0.5f * ((st.ar - mu) + (st.ax - LIFT)));  // (twice, as in small tiles)
 #pragma unroll
   for (int j = 0; j < ND; ++j)
 #pragma unroll
