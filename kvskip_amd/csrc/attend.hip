@@ -578,9 +578,9 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 #pragma unroll
     for (int w = 0; w < NWAVE; ++w) {
       const float mw = m[w] == NEG_INF ? 0.f : m[w];
-      const float x = fexp2(0.5f * ((mw - mu) + L.x[w][row]));  // (twice: with vs near 2^-126 the whole is below what is held)
+      const Pow2 x((mw - mu) + L.x[w][row]);
       l += L.l[w][row] * fexp2(m[w] - mu);
-      a += *reinterpret_cast<const f32x4_t*>(&L.acc[w][row][d]) * x * x;
+      a += *reinterpret_cast<const f32x4_t*>(&L.acc[w][row][d]) * x.a * x.b;
     }
     store4(p, u, h, row, virtual_row(p, u, h, row), d, D, a, M, l);
   }
@@ -821,13 +821,13 @@ __device__ __forceinline__ void many_rows(const AttendP& p, const AttendUnit& u,
   const float l = swap32_sum(st.l);
   if (i0 >= u.nv) return;
   const float mu = st.m == NEG_INF ? 0.f : st.m;
-  const float x = st.ar == NEG_INF ? 0.f : fexp2(0.5f * ((st.ar - mu) + (st.ax - LIFT)));  // (twice, as in small tiles)
+  const Pow2 x(st.ar == NEG_INF ? NEG_INF : (st.ar - mu) + (st.ax - LIFT));
 #pragma unroll
   for (int j = 0; j < ND; ++j)
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
       store4(p, u, h, i0, r, 32 * j + 2 * i + 4 * half, D,
-             f32x4_t{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]} * x * x, st.m, l);
+             f32x4_t{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]} * x.a * x.b, st.m, l);
   if (I8 || L.nan == 0) return;
   // NaN of cut pages over what was stored
   for (int k = 0; k < n; ++k) {

@@ -73,6 +73,16 @@ __device__ __forceinline__ void v_pair8(const u32x2 (&vr)[Lay8<D>::VN], int nt, 
   }
 }
 
+// 2^y in two factors, for y of which the whole may lie below or above what fp32 holds (2^-133 where a scale is 2^-126). The second
+// is a whole power of two, so whole y stay exact.
+struct Pow2 {
+  float a, b;
+  __device__ __forceinline__ explicit Pow2(float y) {
+    const float k = fmaxf(rintf(0.5f * y), -1000.f);  // (y may be -infinity)
+    a = fexp2(y - k), b = fexp2(k);
+  }
+};
+
 // Two values as fp16, to nearest even, the first in the low half.
 __device__ __forceinline__ uint32_t pack_h(float a, float b) {
   typedef float f32x2_t __attribute__((ext_vector_type(2)));

@@ -51,3 +51,26 @@ def test_caps_of_any_size(gpu, Hq, Hkv, D, most, slopes):
         ref = s.exact(0, cap, sl)
         check(s.call(plan, cap, sl), ref, D, cap, softcap=cap)
         assert slopes or (ref[1].exp() - ref[1].exp().round()).abs().max() < 1e-9       # (as many keys as are seen)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_every_code_is_exact(gpu, fmt, D):
+    """One key with scores 0 and a scale that is a power of two, whole or odd: the result is the value itself, which bf16 holds."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    codes = codes[(codes & 127) != 127] if fmt == "e4m3" else codes
+    n = codes.numel()
+    for rows, most in ((1, 1), (64, 0)):
+        for e in (-2, -1, 0, 5, -101):
+            s = Step([(64, rows)], 4, 1, D, fmt, 45)
+            s.lens, s.starts, s.rows = [1] * n, list(range(n + 1)), n
+            if rows > 1:                                          # (large tiles: each request brings rows that see nothing, and one)
+                s.starts, s.rows = list(range(0, 33 * n + 1, 33)), 33 * n
+            s.q = torch.randn(s.rows, 4, D, generator=torch.Generator().manual_seed(46)).to(torch.bfloat16)
+            s.k = torch.zeros(n, 1, 64, D, dtype=torch.uint8).view(s.k.dtype)
+            s.v = codes.view(n, 1, 1, 1).expand(n, 1, 64, D).contiguous().view(s.v.dtype)
+            s.ks, s.vs = torch.ones(n, 1), torch.full((n, 1), 2.0 ** e)
+            s.table = torch.arange(n, dtype=torch.int32).view(n, 1)
+            out = s.call(s.plan(max_rows=most))["out"].double().cpu().view(n, -1, 4, D)
+            want = s.v[:, 0, 0].double()[:, None] * 2.0 ** e
+            assert torch.equal(out[:, -1], want.expand(n, 4, D)) and not out[:, :-1].any(), (fmt, D, rows, e)
