@@ -174,7 +174,8 @@ __device__ __forceinline__ void finish8(const Attn8P& p, int b, int h, int split
       Ls += l[w] * fexp2(m[w] - mu);
       f32x4_t x = *reinterpret_cast<const f32x4_t*>(L.acc + (w * NP * GP + g) * D + d);
       if constexpr (NP == 2) x -= *reinterpret_cast<const f32x4_t*>(L.acc + ((w * NP + 1) * GP + g) * D + d);
-      A += x * fexp2((r[w] - mu) + (rx[w] - 7.f));
+      const Pow2 f((r[w] - mu) + (rx[w] - 7.f));
+      A += x * f.a * f.b;
     }
     const int64_t hq = hq0 + g;
     if (whole) {
@@ -457,7 +458,8 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
       mr = m_new;
       // the accumulators' reference: mt + log2 |vs| (its whole part) of the largest block so far, left where it is for as
       // long as a block passes it by at most 2^7
-      const float ev = static_cast<float>(max(static_cast<int>(__float_as_uint(vs) >> 23 & 0xffu) - 127, -100));
+      const int ex = max(static_cast<int>(__float_as_uint(vs) >> 23 & 0xffu) - 127, -126);
+      const float ev = static_cast<float>(ex);
       const float past = (mt - ar) + (ev - ax);  // (NaN, which passes nothing, where nothing came yet)
       if (__ballot(past > 7.f) != 0) {
         const bool on = past > 0.f;
@@ -465,7 +467,8 @@ __global__ void __launch_bounds__(NT, (WG8<D, GP>)) decode8_kernel(const Attn8P 
         ar = on ? mt : ar;
         ax = on ? ev : ax;
       }
-      const float fv = vs * fexp2((mt - (ar == NEG_INF ? 0.f : ar)) - ax) * 0x1p7f;  // below 2^15
+      // below 2^15 (vs by its own part and one power of two: with vs near either end of fp32 no other order stays inside)
+      const float fv = ldexpf(vs, -ex) * fexp2(((mt - (ar == NEG_INF ? 0.f : ar)) + (ev - ax)) + 7.f);
       if constexpr (STATS) {
         const uint32_t blk4 = 4u * static_cast<uint32_t>(max(blk, 0));
         const uint32_t at = blk >= 0 ? v_stat : OOB;
