@@ -9,8 +9,8 @@
 // are two fp16 parts, 2^-23 of each but for what lies below 2^-35 of the row's largest weight times |vs|, taken relative to a
 // reference that this passes by 2^6 at most (accumulators are rescaled only when a page passes that); sums and statistics are fp32. (One part, 2^-12, shows beside
 // bf16 results, more where values cancel: 2^-10 of a result in the norm from a softmax in fp32, for 2^-14. The second one
-// costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2258 us for 1717, 64 tokens behind a prefix of 8192 48.5 for
-// 43.0. Its order among the products makes no difference.)
+// costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2293 us for 1712, 64 tokens behind a prefix of 8192 49.8 for
+// 43.2. Its order among the products makes no difference.)
 #include "codes8.hpp"
 #include "attend.hpp"
 
@@ -592,7 +592,7 @@ __device__ __forceinline__ void few_rows(const AttendP& p, const AttendUnit& u, 
 // row r at c ^ r, V's at c ^ 5 (r % 4) (64 dims: r / 2 in both).
 //   Products and vector instructions bound it together: products take the matrix unit 1536 clocks a page of 128 dims and wavefront,
 // beside them vector instructions run at half their rate or so, and two wavefronts a SIMD take turns at best (prompts of 8192:
-// 2258 us, the matrix units busy for half of the clocks). So: operands asked for four products ahead (read and waited for one by one,
+// 2293 us, the matrix units busy for half of the clocks). So: operands asked for four products ahead (read and waited for one by one,
 // prompts took 1850 us with one part a weight, for 1780), addresses that a page's turn does not change (two pages a turn,
 // 1745 to 1737), maxima only where they are needed (1650), and nothing in the loop that waits for the codes asked for last (the
 // page list in groups).
