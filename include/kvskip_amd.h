@@ -530,9 +530,9 @@ int64_t kvskip_attend_part_rows(const kvskip_attend_plan_args* p);
  * 0 and -inf for a row that sees nothing and for rows that no request brings. q: bf16 [rows, Hq, D] (strides multiples of 8,
  * 16-byte aligned). Pools [num_pages, Hkv, 64, D] of codes (strides multiples of 16, 16-byte aligned, token strides below
  * 2^24), scales [num_pages, Hkv]; a page outside [0, num_pages) holds no keys. D in {64, 128}, any Hq / Hkv. q is exact to
- * 2^-39 of its row's largest element, a weight holds 22 bits but for what lies below 2^-35 of its row's heaviest weight times |v_scale|, scores and sums are
- * fp32. A cap counts as one of 2^-64 .. 2^96, beyond which results do not change. Keys that a row does not see do not reach it,
- * whatever they hold. part_acc [part_rows, Hkv, D] and part_ml [part_rows, Hkv, 2] fp32, 16-byte aligned; part_rows is at most
+ * 2^-39 of its row's largest element, a weight holds 22 bits but for what lies below 2^-35 of its row's heaviest weight times
+ * |v_scale|, scores and sums are fp32. A cap counts as one of 2^-64 .. 2^96, beyond which results do not change. Keys that a row
+ * does not see do not reach it, whatever they hold. part_acc [part_rows, Hkv, D] and part_ml [part_rows, Hkv, 2] fp32, 16-byte aligned; part_rows is at most
  * 2 (1024 / Hkv + 1) times the rows of a tile (128, or as many as rows Hq / Hkv), and with shared > 0 2 rows Hq / Hkv more,
  * whether or not a request is behind a prefix. */
 typedef struct kvskip_attend_args {

@@ -7,10 +7,10 @@
 // keys will do inside a product, as long as V's operand has the same). Codes become fp16, which holds them exactly; q is
 // fp16 times a power of two of its row (2^14 <= largest < 2^15: exact, but for what lies below 2^-39 of that); weights
 // are two fp16 parts, 2^-23 of each but for what lies below 2^-35 of the row's largest weight times |vs|, taken relative to a
-// reference that this passes by 2^6 at most (accumulators are rescaled only when a page passes that); sums and statistics are fp32. (One part, 2^-12, shows beside
-// bf16 results, more where values cancel: 2^-10 of a result in the norm from a softmax in fp32, for 2^-14. The second one
-// costs small tiles 1 to 3 %, large ones 10 to 33: prompts of 8192 2293 us for 1712, 64 tokens behind a prefix of 8192 49.8 for
-// 43.2. Its order among the products makes no difference.)
+// reference that this passes by 2^6 at most (accumulators are rescaled only when a page passes that); sums and statistics are
+// fp32. (One part, 2^-12, shows beside bf16 results, more where values cancel: 2^-10 of a result in the norm from a softmax in
+// fp32, for 2^-13. The second one costs small tiles 1 to 4 %, large ones 8 to 34: prompts of 8192 2293 us for 1712, 64 tokens
+// behind a prefix of 8192 49.8 for 43.2. Its order among the products makes no difference.)
 #include "codes8.hpp"
 #include "attend.hpp"
 
